@@ -246,6 +246,56 @@ int ob200_bias_gelu(const void* x, void* y, const float* bias, long long rows, i
 int ob200_adamw_f32(float* p, const float* g, float* m, float* v, long long n, float lr, float beta1, float beta2, float eps,
                     float weight_decay, int step, int num_ctas, void* stream);
 
+/* y = residual + dropout(act(x . w^T + bias)) in one launch (bfloat16; float32 accumulation, rounded once): x [M, K] rows ldx apart,
+ * w [N, K] rows ldw apart, y and residual [M, N] contiguous; K, ldx, ldw multiples of 8, pointers 16-byte aligned (residual and bias:
+ * any), N any.  bias [N] float32 (bias_f32) or bfloat16, or NULL; residual may be NULL; act 0 none, 1 ReLU, 2 GELU (erf).
+ * Dropout with probability p (0: none), rounded to a multiple of 2^-16: an element is kept, and scaled by the exact reciprocal of the
+ * kept share, where 16 bits of Philox4x32-10 (Salmon et al., SC'11) are at least round(65536 p); element i of the flattened y takes half
+ * i % 8 of the four words at counter (low 32 bits of i / 8, bits 32..47 of i / 8 | bits 32..47 of step << 16, low 32 bits of step, site)
+ * under the key seed.  rng points to (seed, step) in device memory, read when the kernel runs, so that a captured graph draws a new
+ * mask when the step moves on; `site` tells the calls of one step apart.  pre (NULL: not wanted), rows ld_pre apart (a multiple of 8):
+ * x . w^T + bias in bfloat16, which the backward pass of an activation needs.  workspace: the bytes that
+ * ob200_linear_act_workspace names (0: none), any contents, the call's own until it has run.
+ * Returns -1 for bad arguments, -2 for misaligned pointers or strides, -3 for a workspace that is too small, -4 when a TMA descriptor
+ * cannot be built.  Stands for the sgemm, bias, GELU, fused_dropout_kernel_vec and add rows of the reference's
+ * benchmarking/model_kernels/bert_8_fb1 (src/scheduler/utils_sched.cpp:490-501; src/cuda_capture/intercept_temp.cpp:418-458). */
+int ob200_linear_act_bf16(const void* x, const void* w, void* y, void* pre, const void* bias, int bias_f32, const void* residual, int act,
+                          float p, const long long* rng, int site, int M, int N, int K, long long ldx, long long ldw, long long ld_pre,
+                          void* workspace, long long workspace_bytes, int num_ctas, void* stream);
+long long ob200_linear_act_workspace(int M, int N, int K);
+/* Its gradients: dz = dropout(dy) * act'(pre), dbias = column sums of dz (in a fixed order, in the bias's type), dx = dz . w,
+ * dw = dz^T . x; dy [M, N], dx [M, K], dw [N, K] contiguous, 16-byte aligned; dx, dw, dbias may be NULL (not wanted); pre only with an
+ * activation.  The residual's gradient is dy. */
+int ob200_linear_act_backward_bf16(const void* dy, const void* pre, const void* x, const void* w, void* dx, void* dw, void* dbias,
+                                   int bias_f32, int act, float p, const long long* rng, int site, int M, int N, int K, long long ldx,
+                                   long long ldw, long long ld_pre, void* workspace, long long workspace_bytes, int num_ctas, void* stream);
+long long ob200_linear_act_backward_workspace(int M, int N, int K, int act, float p, int want_dx, int want_dw, int want_dbias);
+
+/* y = dropout(x) [+ residual] over n contiguous elements with the mask above (dtype 0 float32, 1 bfloat16; residual may be NULL; y may
+ * be x): the gradient is the same call on dy.  Stands for fused_dropout_kernel_vec and its masked-scale backward kernel (reference
+ * benchmarking/model_kernels/bert_8_fb1), without the stored mask. */
+int ob200_dropout(const void* x, const void* residual, void* y, long long n, float p, const long long* rng, int site, int dtype,
+                  int num_ctas, void* stream);
+
+/* Softmax cross-entropy of the logits x . w^T over a vocabulary of V, without the logits (bfloat16 x [rows, H] and w [V, H], rows ldx / ldw
+ * apart; H, ldx, ldw multiples of 8, 16-byte aligned; V any): loss[row] = lse[row] - logit of target[row], lse[row] = logsumexp; 0 for
+ * a row whose target is ignore_index, not a number for any other target outside the vocabulary.  total (NULL: not wanted) receives
+ * the sum of the losses, or with `mean` their mean over the rows that count (0 where none does), count their number (at least 1).  The
+ * results do not depend on num_ctas.  Stands where the reference's clients launch the vocabulary projection's sgemm and the softmax /
+ * nll_loss kernels (reference benchmarking/model_kernels/bert_8_fb1). */
+int ob200_linear_cross_entropy_forward(const void* x, const void* w, const long long* target, float* loss, float* lse, float* total,
+                                       float* count, int rows, int V, int H, long long ldx, long long ldw, long long ignore_index, int mean,
+                                       void* workspace, long long workspace_bytes, int num_ctas, void* stream);
+long long ob200_linear_cross_entropy_workspace(int rows, int V);
+/* Its gradients in pieces of the vocabulary, dx [rows, H] and dw [V, H] contiguous bfloat16 (either may be NULL): logits of a piece are
+ * computed again.  grad: the upstream gradient, one value or one per row (grad_per_row), divided by *count where count is given (the
+ * mean).  Rows that do not count contribute nothing, whatever x holds there. */
+int ob200_linear_cross_entropy_backward(const void* x, const void* w, const long long* target, const float* lse, const float* grad,
+                                        int grad_per_row, const float* count, void* dx, void* dw, int rows, int V, int H, long long ldx,
+                                        long long ldw, long long ignore_index, void* workspace, long long workspace_bytes, int num_ctas,
+                                        void* stream);
+long long ob200_linear_cross_entropy_backward_workspace(int rows, int V, int H, int want_dx, int want_dw);
+
 /* Device status word of the current device (synchronises the device): 0, or the code of
  * the bounded wait a kernel gave up on.  Clears the word; after a non-zero status it also clears the split-K arrival
  * counters of every stream of the device, which the kernel that gave up may have left above zero.  No counterpart in the

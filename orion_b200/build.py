@@ -19,7 +19,7 @@ BIN = os.path.join(HERE, "bin")
 ROOT = os.path.dirname(HERE)
 
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
-              "-Xcompiler", "-fPIC", "--cudart", "shared"]
+              "-Xcompiler", "-fPIC", "--cudart", "shared", "--threads", "0"]
 CXX_FLAGS = ["-O2", "-std=c++17", "-fPIC", "-Wall", "-pthread"]
 
 

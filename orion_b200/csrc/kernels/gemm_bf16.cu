@@ -35,6 +35,9 @@
 #include <string.h>
 
 #include "elastic.h"
+#include "fast_gelu.cuh"
+#include "gemm_call.h"
+#include "philox.cuh"
 #include "sm100_primitives.cuh"
 
 namespace ob200 {
@@ -73,9 +76,11 @@ struct GemmParams {
                              // 2 = A[m, k] is zero for k > m (reduction stops behind the tile's last row),
                              // 3 = A[m, k] is zero for k < m (reduction starts at the tile's first row)
     float alpha;
+    GemmEpi e;               // of the epilogues other than GM_EPI_PLAIN
     alignas(64) unsigned char tmap_a[128];
     alignas(64) unsigned char tmap_b[128];
     alignas(64) unsigned char tmap_c[128];
+    alignas(64) unsigned char tmap_pre[128];
 };
 
 struct GemmCtl {
@@ -111,7 +116,9 @@ __device__ __forceinline__ bool gm_tile_skipped(const GemmParams& p, int tm, int
     return p.tri == 1 && tn * BN > tm * GM_BM + GM_BM - 1;
 }
 
-template <int BN, int CG>
+#include "gemm_epilogue.cuh"
+
+template <int BN, int CG, int EPI>
 __global__ void __launch_bounds__(GM_THREADS, 1) gemm_bf16_kernel(const __grid_constant__ GemmParams p) {
     using C = GemmCfg<BN, CG>;
     extern __shared__ uint8_t smem_raw[];
@@ -292,6 +299,10 @@ __global__ void __launch_bounds__(GM_THREADS, 1) gemm_bf16_kernel(const __grid_c
             const int m = (tm * CG + (int)rank) * GM_BM + r;
             const int n0 = tn * BN;
             const uint32_t t_row = tmem_base + ((uint32_t)(q * 32) << 16) + ab * BN;
+            if constexpr (EPI == GM_EPI_ACT) gm_epilogue_act<BN>(p, t_row, m, (tm * CG + (int)rank) * GM_BM + q * 32, n0, sp, lane, epi_smem + (warp - 2) * 8192, slab_i);
+            else if constexpr (EPI == GM_EPI_LSE) gm_epilogue_lse<BN>(p, t_row, m, n0);
+            else if constexpr (EPI == GM_EPI_DLOGITS) gm_epilogue_dlogits<BN>(p, t_row, m, (tm * CG + (int)rank) * GM_BM + q * 32, n0, lane, epi_smem + (warp - 2) * 8192, slab_i);
+            else {
             const bool to_slab = p.splits > 1;
             const bool row_ok = m < p.M;
             float* srow = to_slab ? p.slabs + (((long long)sp * p.batch + b) * p.M + m) * p.N : nullptr;
@@ -351,6 +362,17 @@ __global__ void __launch_bounds__(GM_THREADS, 1) gemm_bf16_kernel(const __grid_c
 #pragma unroll
                         for (int j = 0; j < 32; j++)
                             if (n + j < p.N) f[j] += __bfloat162float(res[j]);
+                    }
+                }
+                if constexpr (EPI == GM_EPI_ACC) {
+                    if (row_ok) {   // N a multiple of 4: no column of a vector is past the edge alone
+                        const float* add = p.e.addend + (long long)m * p.N + n;
+#pragma unroll
+                        for (int j = 0; j < 32; j += 4)
+                            if (full || n + j < p.N) {
+                                const float4 a = *reinterpret_cast<const float4*>(add + j);
+                                f[j] += a.x; f[j + 1] += a.y; f[j + 2] += a.z; f[j + 3] += a.w;
+                            }
                     }
                 }
                 if (by_tma) {
@@ -424,6 +446,7 @@ __global__ void __launch_bounds__(GM_THREADS, 1) gemm_bf16_kernel(const __grid_c
                     }
                 }
             }
+            }
             tc_fence_before_sync();
             __syncwarp();
             if (lane == 0) {
@@ -445,10 +468,10 @@ __global__ void __launch_bounds__(GM_THREADS, 1) gemm_bf16_kernel(const __grid_c
 }
 
 // Sums the split-K partial matrices in split order, applies alpha and the bias, writes C.
-__global__ void __launch_bounds__(256) gemm_splitk_finish_kernel(const float* __restrict__ slabs, void* __restrict__ c,
+__global__ void __launch_bounds__(256) gemm_splitk_finish_kernel(const float* __restrict__ slabs, void* c,
                                                                  const float* __restrict__ bias,
                                                                  const __nv_bfloat16* __restrict__ bias_bf16,
-                                                                 const __nv_bfloat16* __restrict__ residual, int splits, int batch, int nb_inner,
+                                                                 const __nv_bfloat16* __restrict__ residual, const float* addend, int splits, int batch, int nb_inner,
                                                                  int M, int N, long long ldc, long long c_si, long long c_so,
                                                                  int out_f32, float alpha) {
     const long long per_split = (long long)batch * M * N;
@@ -461,8 +484,69 @@ __global__ void __launch_bounds__(256) gemm_splitk_finish_kernel(const float* __
         acc = acc * alpha + (bias ? bias[n] : 0.f) + (bias_bf16 ? __bfloat162float(bias_bf16[n]) : 0.f);
         const long long off = (long long)(b / nb_inner) * c_so + (long long)(b % nb_inner) * c_si + (long long)m * ldc + n;
         if (residual) acc += __bfloat162float(residual[off]);
+        if (addend) acc += addend[i];   // may be C itself
         if (out_f32) reinterpret_cast<float*>(c)[off] = acc;
         else reinterpret_cast<__nv_bfloat16*>(c)[off] = __float2bfloat16_rn(acc);
+    }
+}
+
+// The same for GM_EPI_ACT: bias, activation, dropout and residual behind the sum.  A thread takes eight elements of the flattened
+// output, the unit of the dropout's counter; partial matrices lie elems apart, so they are read in vectors where that allows it.
+__global__ void __launch_bounds__(256) gemm_splitk_act_kernel(const float* __restrict__ slabs, __nv_bfloat16* __restrict__ c,
+                                                              const float* __restrict__ bias, const __nv_bfloat16* __restrict__ bias_bf16,
+                                                              const __nv_bfloat16* __restrict__ residual, int splits, int M, int N, GemmEpi e) {
+    pdl_wait();
+    pdl_launch_dependents();
+    const long long elems = (long long)M * N, groups = (elems + 7) / 8;
+    const bool vec = elems % 4 == 0;
+    DropKey key = {};
+    if (e.drop_threshold) key = drop_key(e.rng, e.site);
+    for (long long g = (long long)blockIdx.x * blockDim.x + threadIdx.x; g < groups; g += (long long)gridDim.x * blockDim.x) {
+        float f[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) f[j] = 0.f;
+        const long long i0 = g * 8;
+        const int n = elems - i0 < 8 ? (int)(elems - i0) : 8;
+        if (vec && n == 8) {
+            for (int s = 0; s < splits; s++) {
+                const float4* src = reinterpret_cast<const float4*>(slabs + s * elems + i0);
+                const float4 a = src[0], b = src[1];
+                f[0] += a.x; f[1] += a.y; f[2] += a.z; f[3] += a.w;
+                f[4] += b.x; f[5] += b.y; f[6] += b.z; f[7] += b.w;
+            }
+        } else {
+            for (int s = 0; s < splits; s++)
+#pragma unroll
+                for (int j = 0; j < 8; j++)
+                    if (j < n) f[j] += slabs[s * elems + i0 + j];
+        }
+        uint32_t mask = 0;
+        if (e.drop_threshold) mask = drop_group_mask(key, (unsigned long long)g, e.drop_threshold);
+        long long m = i0 / N;
+        int col = (int)(i0 - m * N);
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            if (j < n) {
+                float a = f[j];
+                if (bias) a += bias[col];
+                if (bias_bf16) a += __bfloat162float(bias_bf16[col]);
+                if (e.pre) e.pre[m * e.ld_pre + col] = __float2bfloat16_rn(a);
+                a = gm_activate(a, e.act);
+                if (e.drop_threshold) a = mask >> j & 1u ? a * e.drop_scale : 0.f;
+                if (residual) a += __bfloat162float(residual[i0 + j]);
+                f[j] = a;
+            }
+            if (++col == N) { col = 0; m++; }
+        }
+        if (n == 8) {
+            uint4 pk;
+            pk.x = gm_pack(f[0], f[1]); pk.y = gm_pack(f[2], f[3]); pk.z = gm_pack(f[4], f[5]); pk.w = gm_pack(f[6], f[7]);
+            *reinterpret_cast<uint4*>(c + i0) = pk;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                if (j < n) c[i0 + j] = __float2bfloat16_rn(f[j]);
+        }
     }
 }
 
@@ -496,6 +580,18 @@ static bool gm_make_map(unsigned char* out, const void* base, long long inner, l
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// Tensor map of a bfloat16 output [M, N] that is stored 32 rows x 32 columns at a time (64-byte rows, swizzled).
+static bool gm_make_store_map(unsigned char* out, const void* base, int M, int N, long long ld) {
+    GmEncodeTiledFn enc = gm_encode_fn();
+    if (!enc) return false;
+    cuuint64_t dims[2] = {(cuuint64_t)N, (cuuint64_t)M};
+    cuuint64_t strides[1] = {(cuuint64_t)ld * 2};
+    cuuint32_t box[2] = {32, 32}, steps[2] = {1, 1};
+    return enc(reinterpret_cast<CUtensorMap*>(out), CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, box, steps,
+               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 // Tile width, CTAs per tile and split factor of a problem.
 //
 // The smallest modelled time in microseconds: rounds of tiles, each as long as its k-blocks or as a tile's way out of tensor
@@ -515,12 +611,12 @@ static bool gm_make_map(unsigned char* out, const void* base, long long inner, l
 // work a pair's k-block gains 7 % more on a single CTA's than on the full device (seven CTAs, 8192 x 1024 x 1024: 201 us in six, 212).
 struct GemmPlan { int bn, cg, splits, grid; };
 struct GemmTile { int bn, cg; double kblock_us, tile_us, tail_us, launch_us; };
-static GemmPlan gm_plan(int M, int N, int K, long long batch, int tri, int device_sms, int num_ctas) {
+static GemmPlan gm_plan(int M, int N, int K, long long batch, int tri, int device_sms, int num_ctas, bool splittable = true) {
     static const GemmTile kNarrow = {64, 1, 0.44, 2.15, 1.0, 0.0};   // outputs of at most 64 columns
     static const GemmTile kTiles[] = {{128, 1, 0.44, 2.15, 1.0, 0.0}, {256, 1, 0.51, 3.0, 2.0, 0.0},
                                       {128, 2, 0.32, 2.15, 1.0, 1.3}, {256, 2, 0.45, 3.0, 2.0, 1.3}};
-    const GemmTile* list = N <= 64 ? &kNarrow : kTiles;
-    const int count = N <= 64 ? 1 : 4;
+    const GemmTile* list = N <= 64 && splittable ? &kNarrow : kTiles;
+    const int count = N <= 64 && splittable ? 1 : 4;
     const long long kblocks = (K + GM_BK - 1) / GM_BK;
     auto tiles_of = [&](int bn, int cg) { return batch * (((long long)M + cg * GM_BM - 1) / (cg * GM_BM)) * (((long long)N + bn - 1) / bn); };
     auto fits = [&](const GemmTile& t) { return !((t.bn == 256 && N < 256) || (t.cg == 2 && (M <= GM_BM || tri != 0))); };
@@ -530,7 +626,7 @@ static GemmPlan gm_plan(int M, int N, int K, long long batch, int tri, int devic
         const double us = t.launch_us + rounds * (depth > t.tile_us ? depth : t.tile_us) + t.tail_us;
         return splits > 1 ? us + 6.0 + (double)splits * batch * M * N * 8.0 / 6e6 : us;
     };
-    const bool may_split = tiles_of(list[0].bn, 1) * 2 <= device_sms && kblocks >= 8 && tri == 0;
+    const bool may_split = tiles_of(list[0].bn, 1) * 2 <= device_sms && kblocks >= 8 && tri == 0 && splittable;
     GemmPlan pl = {0, 1, 1, 1};
     double best = 0.0;
     for (int i = 0; i < count; i++) {
@@ -561,17 +657,17 @@ static GemmPlan gm_plan(int M, int N, int K, long long batch, int tri, int devic
     return pl;
 }
 
-template <int BN, int CG>
+template <int BN, int CG, int EPI>
 static int gm_launch(const GemmParams& p, int grid, cudaStream_t stream) {
     static bool attr_set[64] = {};
     int dev = 0;
     cudaGetDevice(&dev);
     if (dev < 64 && !attr_set[dev]) {
-        cudaError_t e = cudaFuncSetAttribute(gemm_bf16_kernel<BN, CG>, cudaFuncAttributeMaxDynamicSharedMemorySize, GemmCfg<BN, CG>::SMEM);
+        cudaError_t e = cudaFuncSetAttribute(gemm_bf16_kernel<BN, CG, EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, GemmCfg<BN, CG>::SMEM);
         if (e != cudaSuccess) return (int)e;
         attr_set[dev] = true;
     }
-    OB200_ELASTIC((gemm_bf16_kernel<BN, CG>), 1);
+    OB200_ELASTIC((gemm_bf16_kernel<BN, CG, EPI>), 1);
     // Programmatic dependent launch: the kernel's set-up (barriers, tensor memory, descriptor prefetch) may overlap the tail of
     // the kernel before it in the stream; it reads and writes global memory only behind its griddepcontrol.wait.
     static const bool pdl = [] {   // ORION_PDL=0: plain stream order between consecutive kernels
@@ -599,7 +695,7 @@ static int gm_launch(const GemmParams& p, int grid, cudaStream_t stream) {
     }
     cfg.attrs = attr;
     cfg.numAttrs = (unsigned)n;
-    return (int)cudaLaunchKernelEx(&cfg, gemm_bf16_kernel<BN, CG>, p);
+    return (int)cudaLaunchKernelEx(&cfg, gemm_bf16_kernel<BN, CG, EPI>, p);
 }
 
 }  // namespace ob200
@@ -620,36 +716,40 @@ extern "C" int ob200_plan_gemm_bf16(int M, int N, int K, long long batch, int tr
     return 0;
 }
 
-// See include/orion_kernels.h.  Returns 0, -1 (unsupported sizes), -2 (misaligned pointers or strides), -4 (no TMA descriptor).
-extern "C" int ob200_gemm_bf16_ex(const void* a, const void* b, void* c, const float* bias, const void* bias_bf16, const void* residual,
-                                  int M, int N, int K, int a_mn, int b_mn, long long lda, long long ldb, long long ldc, int batch_inner,
-                                  int batch_outer, long long a_si, long long a_so, long long b_si, long long b_so, long long c_si,
-                                  long long c_so, float alpha, int out_f32, int tri, int num_ctas, void* stream);
+namespace ob200 {
 
-extern "C" int ob200_gemm_bf16(const void* a, const void* b, void* c, const float* bias, int M, int N, int K, int a_mn, int b_mn,
-                               long long lda, long long ldb, long long ldc, int batch_inner, int batch_outer, long long a_si,
-                               long long a_so, long long b_si, long long b_so, long long c_si, long long c_so, float alpha, int out_f32,
-                               int num_ctas, void* stream) {
-    return ob200_gemm_bf16_ex(a, b, c, bias, nullptr, nullptr, M, N, K, a_mn, b_mn, lda, ldb, ldc, batch_inner, batch_outer, a_si, a_so,
-                              b_si, b_so, c_si, c_so, alpha, out_f32, 0, num_ctas, stream);
+size_t gemm_bf16_slab_bytes(int M, int N, int K) {
+    const int sms = ob200_plan_sm_count();
+    const GemmPlan pl = gm_plan(M, N, K, 1, 0, sms, sms);
+    return pl.splits > 1 ? (size_t)pl.splits * M * N * sizeof(float) : 0;
 }
 
-extern "C" int ob200_gemm_bf16_ex(const void* a, const void* b, void* c, const float* bias, const void* bias_bf16, const void* residual,
-                                  int M, int N, int K, int a_mn, int b_mn, long long lda, long long ldb, long long ldc, int batch_inner,
-                                  int batch_outer, long long a_si, long long a_so, long long b_si, long long b_so, long long c_si,
-                                  long long c_so, float alpha, int out_f32, int tri, int num_ctas, void* stream) {
-    using namespace ob200;
+template <int EPI>
+static int gm_launch_tile(const GemmParams& p, int bn, int cg, int grid, cudaStream_t st) {
+    if (cg == 2) return bn == 256 ? gm_launch<256, 2, EPI>(p, grid, st) : gm_launch<128, 2, EPI>(p, grid, st);
+    if (bn == 256) return gm_launch<256, 1, EPI>(p, grid, st);
+    if constexpr (EPI == GM_EPI_PLAIN || EPI == GM_EPI_ACC || EPI == GM_EPI_ACT)
+        if (bn == 64) return gm_launch<64, 1, EPI>(p, grid, st);
+    return gm_launch<128, 1, EPI>(p, grid, st);
+}
+
+int gemm_bf16_run(const GemmCall& g) {
+    const int M = g.M, N = g.N, K = g.K, a_mn = g.a_mn, b_mn = g.b_mn, batch_inner = g.batch_inner, batch_outer = g.batch_outer;
+    const int out_f32 = g.out_f32, tri = g.tri, num_ctas = g.num_ctas, epi = g.epi;
+    const long long lda = g.lda, ldb = g.ldb, ldc = g.ldc, c_si = g.c_si, c_so = g.c_so;
+    const void *a = g.a, *b = g.b, *residual = g.residual;
+    void* c = g.c;
     if (tri < 0 || tri > 3) return -1;
     if (M < 0 || N < 0 || K <= 0 || batch_inner < 0 || batch_outer < 0 || num_ctas <= 0 || lda <= 0 || ldb <= 0 || ldc < N) return -1;
     if (M == 0 || N == 0 || batch_inner == 0 || batch_outer == 0) return 0;
     if (((uintptr_t)a | (uintptr_t)b) % 16 || (lda | ldb) % 8) return -2;
-    if ((batch_inner > 1 && ((a_si | b_si) % 8)) || (batch_outer > 1 && ((a_so | b_so) % 8))) return -2;
+    if ((batch_inner > 1 && ((g.a_si | g.b_si) % 8)) || (batch_outer > 1 && ((g.a_so | g.b_so) % 8))) return -2;
     const long long batch_ll = (long long)batch_inner * batch_outer;
     if (batch_ll > 0x7fffffffLL) return -1;
     GemmParams p;
     memset(&p, 0, sizeof p);
-    p.c = c; p.bias = bias;
-    p.bias_bf16 = reinterpret_cast<const __nv_bfloat16*>(bias_bf16);
+    p.c = c; p.bias = g.bias;
+    p.bias_bf16 = reinterpret_cast<const __nv_bfloat16*>(g.bias_bf16);
     p.residual = reinterpret_cast<const __nv_bfloat16*>(residual);
     p.status = ob200_status_word_for_current_device();
     p.M = M; p.N = N; p.K = K;
@@ -657,13 +757,14 @@ extern "C" int ob200_gemm_bf16_ex(const void* a, const void* b, void* c, const f
     p.ldc = ldc; p.c_si = c_si; p.c_so = c_so;
     p.out_f32 = out_f32 ? 1 : 0;
     p.a_mn = a_mn ? 1 : 0; p.b_mn = b_mn ? 1 : 0;
-    p.alpha = alpha;
+    p.alpha = g.alpha;
     p.tri = tri;
+    p.e = g.e;
     const int cal = out_f32 ? 4 : 8;   // elements per 16 bytes of C
     p.vec_ok = ((uintptr_t)c % 16 == 0) && ((uintptr_t)residual % 16 == 0) && (!residual || !out_f32) && (ldc % cal == 0) && (batch_inner == 1 || c_si % cal == 0) && (batch_outer == 1 || c_so % cal == 0);
     const int plan = ob200_plan_sm_count();
     p.kblocks = (K + GM_BK - 1) / GM_BK;
-    const GemmPlan pl = gm_plan(M, N, K, batch_ll, tri, plan, num_ctas);
+    const GemmPlan pl = gm_plan(M, N, K, batch_ll, tri, plan, num_ctas, epi != GM_EPI_LSE && epi != GM_EPI_DLOGITS);
     const int bn = pl.bn, cg = pl.cg;
     int splits = pl.splits;
     p.tiles_m = (M + cg * GM_BM - 1) / (cg * GM_BM);
@@ -671,8 +772,8 @@ extern "C" int ob200_gemm_bf16_ex(const void* a, const void* b, void* c, const f
     const long long tiles = batch_ll * p.tiles_m * p.tiles_n;
     if (tiles > 0x7fffffffLL) return -1;
     if (splits > 1) {
-        size_t slab_bytes = 0;
-        float* slabs = ob200_stream_slabs(stream, &slab_bytes);
+        size_t slab_bytes = g.slab_bytes;
+        float* slabs = g.stream_slabs ? ob200_stream_slabs(g.stream, &slab_bytes) : g.slabs;
         const size_t per_split = (size_t)batch_ll * M * N * sizeof(float);
         if (!slabs || per_split == 0) splits = 1;
         else if ((size_t)splits * per_split > slab_bytes) splits = (int)(slab_bytes / per_split);
@@ -682,10 +783,10 @@ extern "C" int ob200_gemm_bf16_ex(const void* a, const void* b, void* c, const f
     p.kb_per_split = (p.kblocks + splits - 1) / splits;
     p.splits = (p.kblocks + p.kb_per_split - 1) / p.kb_per_split;   // every split owns at least one k-block
     if (p.splits <= 1) { p.splits = 1; p.slabs = nullptr; p.kb_per_split = p.kblocks; }
-    const bool ok_a = a_mn ? gm_make_map(p.tmap_a, a, M, K, lda, batch_inner, a_si, batch_outer, a_so, 64, GM_BK)
-                           : gm_make_map(p.tmap_a, a, K, M, lda, batch_inner, a_si, batch_outer, a_so, GM_BK, GM_BM);
-    const bool ok_b = b_mn ? gm_make_map(p.tmap_b, b, N, K, ldb, batch_inner, b_si, batch_outer, b_so, 64, GM_BK)
-                           : gm_make_map(p.tmap_b, b, K, N, ldb, batch_inner, b_si, batch_outer, b_so, GM_BK, bn / cg);
+    const bool ok_a = a_mn ? gm_make_map(p.tmap_a, a, M, K, lda, batch_inner, g.a_si, batch_outer, g.a_so, 64, GM_BK)
+                           : gm_make_map(p.tmap_a, a, K, M, lda, batch_inner, g.a_si, batch_outer, g.a_so, GM_BK, GM_BM);
+    const bool ok_b = b_mn ? gm_make_map(p.tmap_b, b, N, K, ldb, batch_inner, g.b_si, batch_outer, g.b_so, 64, GM_BK)
+                           : gm_make_map(p.tmap_b, b, K, N, ldb, batch_inner, g.b_si, batch_outer, g.b_so, GM_BK, bn / cg);
     if (!ok_a || !ok_b) return -4;
     // C by TMA stores when its rows and batch offsets are 16-byte multiples (always true for the layouts of the clients)
     {
@@ -693,7 +794,11 @@ extern "C" int ob200_gemm_bf16_ex(const void* a, const void* b, void* c, const f
         const bool aligned = ((uintptr_t)c % 16 == 0) && (ldc * es) % 16 == 0 && (batch_inner == 1 || (c_si * es) % 16 == 0) &&
                              (batch_outer == 1 || (c_so * es) % 16 == 0);
         static const bool tma_off = [] { const char* e = getenv("ORION_GEMM_TMA_STORE"); return e && e[0] == '0'; }();
-        if (aligned && !tma_off && p.splits == 1) {
+        if (epi == GM_EPI_ACT || epi == GM_EPI_DLOGITS) {   // 32 rows x 32 columns a store
+            if (aligned && p.splits == 1) p.c_tma = gm_make_store_map(p.tmap_c, c, M, N, ldc) ? 1 : 0;
+            if (epi == GM_EPI_DLOGITS && !p.c_tma) return -4;
+            if (g.e.pre && p.splits == 1 && !gm_make_store_map(p.tmap_pre, g.e.pre, M, N, g.e.ld_pre)) return -4;
+        } else if (epi != GM_EPI_LSE && aligned && !tma_off && p.splits == 1) {
             GmEncodeTiledFn enc = gm_encode_fn();
             const long long si = batch_inner > 1 ? c_si : ldc * M, so = batch_outer > 1 ? c_so : si * (batch_inner > 1 ? batch_inner : 1);
             cuuint64_t dims[4] = {(cuuint64_t)N, (cuuint64_t)M, (cuuint64_t)batch_inner, (cuuint64_t)batch_outer};
@@ -714,22 +819,63 @@ extern "C" int ob200_gemm_bf16_ex(const void* a, const void* b, void* c, const f
     static const int tiles_per_cta = [] { const char* e = getenv("ORION_GEMM_TILES_PER_CTA"); return e ? atoi(e) : 0; }();
     if (tiles_per_cta > 0) {
         const long long want = (units + tiles_per_cta - 1) / tiles_per_cta * cg;
-        if (want > grid) grid = want > 0x7fffffffLL ? 0x7fffffff : (int)want;
+        if (want > grid) grid = want > 0x7fffffff ? 0x7fffffff : (int)want;
     }
     {
         const double flop = 2.0 * batch_ll * M * (double)N * K;
         const double bytes = 2.0 * batch_ll * ((double)M * K + (double)N * K) + (out_f32 ? 4.0 : 2.0) * batch_ll * (double)M * N;
         annotate_launch(flop / bytes > ai_threshold(1) ? 1 : 0, flop, bytes);
     }
-    cudaStream_t st = (cudaStream_t)stream;
-    int rc = cg == 2 ? (bn == 256 ? gm_launch<256, 2>(p, grid, st) : gm_launch<128, 2>(p, grid, st))
-             : bn == 256 ? gm_launch<256, 1>(p, grid, st) : bn == 128 ? gm_launch<128, 1>(p, grid, st) : gm_launch<64, 1>(p, grid, st);
+    cudaStream_t st = (cudaStream_t)g.stream;
+    int rc;
+    switch (epi) {
+        case GM_EPI_ACC: rc = gm_launch_tile<GM_EPI_ACC>(p, bn, cg, grid, st); break;
+        case GM_EPI_ACT: rc = gm_launch_tile<GM_EPI_ACT>(p, bn, cg, grid, st); break;
+        case GM_EPI_LSE: return gm_launch_tile<GM_EPI_LSE>(p, bn, cg, grid, st);
+        case GM_EPI_DLOGITS: return gm_launch_tile<GM_EPI_DLOGITS>(p, bn, cg, grid, st);
+        default: rc = gm_launch_tile<GM_EPI_PLAIN>(p, bn, cg, grid, st);
+    }
     if (rc != 0 || p.splits == 1) return rc;
     const long long elems = batch_ll * M * N;
+    if (epi == GM_EPI_ACT) {
+        long long blocks = ((elems + 7) / 8 + 255) / 256;
+        if (blocks > 8LL * num_ctas) blocks = 8LL * num_ctas;
+        OB200_ELASTIC_HBM(gemm_splitk_act_kernel, 8);
+        return launch_pdl(gemm_splitk_act_kernel, (unsigned)blocks, 256u, st, (const float*)p.slabs, (__nv_bfloat16*)c, p.bias, p.bias_bf16, p.residual,
+                          p.splits, M, N, p.e);
+    }
     long long blocks = (elems + 255) / 256;
     if (blocks > 4LL * num_ctas) blocks = 4LL * num_ctas;
     OB200_ELASTIC_HBM(gemm_splitk_finish_kernel, 4);
-    gemm_splitk_finish_kernel<<<(int)blocks, 256, 0, (cudaStream_t)stream>>>(p.slabs, c, bias, p.bias_bf16, p.residual, p.splits, p.batch, p.nb_inner, M, N, ldc, c_si,
-                                                                            c_so, p.out_f32, alpha);
+    gemm_splitk_finish_kernel<<<(int)blocks, 256, 0, st>>>(p.slabs, c, g.bias, p.bias_bf16, p.residual, epi == GM_EPI_ACC ? p.e.addend : nullptr, p.splits, p.batch,
+                                                           p.nb_inner, M, N, ldc, c_si, c_so, p.out_f32, g.alpha);
     return (int)cudaGetLastError();
+}
+
+}  // namespace ob200
+
+// See include/orion_kernels.h.  Returns 0, -1 (unsupported sizes), -2 (misaligned pointers or strides), -4 (no TMA descriptor).
+extern "C" int ob200_gemm_bf16_ex(const void* a, const void* b, void* c, const float* bias, const void* bias_bf16, const void* residual,
+                                  int M, int N, int K, int a_mn, int b_mn, long long lda, long long ldb, long long ldc, int batch_inner,
+                                  int batch_outer, long long a_si, long long a_so, long long b_si, long long b_so, long long c_si,
+                                  long long c_so, float alpha, int out_f32, int tri, int num_ctas, void* stream) {
+    ob200::GemmCall g;
+    g.a = a; g.b = b; g.c = c;
+    g.bias = bias; g.bias_bf16 = bias_bf16; g.residual = residual;
+    g.M = M; g.N = N; g.K = K; g.a_mn = a_mn; g.b_mn = b_mn;
+    g.lda = lda; g.ldb = ldb; g.ldc = ldc;
+    g.batch_inner = batch_inner; g.batch_outer = batch_outer;
+    g.a_si = a_si; g.a_so = a_so; g.b_si = b_si; g.b_so = b_so; g.c_si = c_si; g.c_so = c_so;
+    g.alpha = alpha; g.out_f32 = out_f32; g.tri = tri;
+    g.stream_slabs = true;
+    g.num_ctas = num_ctas; g.stream = stream;
+    return ob200::gemm_bf16_run(g);
+}
+
+extern "C" int ob200_gemm_bf16(const void* a, const void* b, void* c, const float* bias, int M, int N, int K, int a_mn, int b_mn,
+                               long long lda, long long ldb, long long ldc, int batch_inner, int batch_outer, long long a_si,
+                               long long a_so, long long b_si, long long b_so, long long c_si, long long c_so, float alpha, int out_f32,
+                               int num_ctas, void* stream) {
+    return ob200_gemm_bf16_ex(a, b, c, bias, nullptr, nullptr, M, N, K, a_mn, b_mn, lda, ldb, ldc, batch_inner, batch_outer, a_si, a_so,
+                              b_si, b_so, c_si, c_so, alpha, out_f32, 0, num_ctas, stream);
 }

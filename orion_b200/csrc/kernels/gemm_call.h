@@ -1,0 +1,64 @@
+// The bfloat16 GEMM (gemm_bf16.cu) as the other kernels of the library call it: one problem with one of several epilogues.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+
+namespace ob200 {
+
+enum : int {
+    GM_EPI_PLAIN = 0,    // C = alpha * A.B^T (+ bias) (+ bfloat16 residual)
+    GM_EPI_ACC = 1,      // the same plus a float32 addend (which may be C itself)
+    GM_EPI_ACT = 2,      // C = residual + dropout(act(A.B^T + bias)), optionally A.B^T + bias beside it
+    GM_EPI_LSE = 3,      // no C: per row and 128 columns the maximum and the sum of exponentials, and the label's column
+    GM_EPI_DLOGITS = 4,  // C = (exp(A.B^T - lse) - onehot(label)) * coefficient
+};
+
+struct GemmEpi {
+    // GM_EPI_ACC
+    const float* addend;            // [M, N], rows N apart
+    // GM_EPI_ACT
+    int act;                        // 0 none, 1 ReLU, 2 GELU
+    uint32_t drop_threshold;        // 0: no dropout
+    float drop_scale;
+    const long long* rng;           // (seed, step), in device memory
+    uint32_t site;
+    __nv_bfloat16* pre;             // optional: A.B^T + bias, rows ld_pre apart (a multiple of 8)
+    long long ld_pre;
+    // GM_EPI_LSE, GM_EPI_DLOGITS
+    const long long* target;        // label of every row
+    long long col0;                 // column of the vocabulary that column 0 of this product is
+    float2* part;                   // GM_EPI_LSE: [ceil(N / 128)][M] (maximum, sum of exp(x - maximum)) of 128 columns
+    float* label_logit;             // GM_EPI_LSE: [M], written where the label is one of the columns
+    const float2* row;              // GM_EPI_DLOGITS: [M] (lse * log2(e), coefficient); a coefficient of zero gives zeros whatever else the row holds
+};
+
+struct GemmCall {
+    const void* a = nullptr;
+    const void* b = nullptr;
+    void* c = nullptr;
+    const float* bias = nullptr;
+    const void* bias_bf16 = nullptr;
+    const void* residual = nullptr;
+    int M = 0, N = 0, K = 0, a_mn = 0, b_mn = 0;
+    long long lda = 0, ldb = 0, ldc = 0;
+    int batch_inner = 1, batch_outer = 1;
+    long long a_si = 0, a_so = 0, b_si = 0, b_so = 0, c_si = 0, c_so = 0;
+    float alpha = 1.0f;
+    int out_f32 = 0, tri = 0;
+    int epi = GM_EPI_PLAIN;
+    GemmEpi e = {};
+    bool stream_slabs = false;      // split-K partial matrices in the stream's own scratch; otherwise in `slabs` (none: no split)
+    float* slabs = nullptr;
+    size_t slab_bytes = 0;
+    int num_ctas = 0;
+    void* stream = nullptr;
+};
+
+// 0, a cudaError_t, -1 (sizes), -2 (alignment), -4 (no TMA descriptor).
+int gemm_bf16_run(const GemmCall& call);
+// Bytes of partial matrices that the split of such a product (plain or with GM_EPI_ACT) wants; 0 where it is not split.
+size_t gemm_bf16_slab_bytes(int M, int N, int K);
+
+}  // namespace ob200

@@ -1,0 +1,284 @@
+// Softmax cross-entropy of logits x . w^T over a large vocabulary, and its gradients, without the logits:
+//
+//   loss[t] = lse[t] - l[t, target[t]],   l = x . w^T,   lse[t] = log sum_v exp(l[t, v])
+//   dl = (exp(l - lse) - onehot(target)) * c[t];   dx = dl . w;   dw = dl^T . x       c[t] = upstream gradient (/ rows that count)
+//
+// Forward: one GEMM whose epilogue keeps, of every row and 128 columns, the maximum and the sum of exponentials (gemm_bf16.cu,
+// GM_EPI_LSE), and a kernel that joins them: 2 T V H operations and V / 16 bytes a row instead of 2 V.  Backward, in pieces of the
+// vocabulary: the logits of a piece are computed again and leave the epilogue as dl in bfloat16 (GM_EPI_DLOGITS), which the two gradient
+// products read.  Computing a logit again costs 2 H operations, 1.5 ps on a B200 at H = 1024; keeping it in float32 would cost 4 bytes
+// written and 4 read, 1.2 ps, and the memory.  dl is rounded to bfloat16 because the tensor cores take it so: an error of at most
+// 2^-9 of each term of dx and dw, as large as that of the rounded result.  dx adds up over the pieces in float32.
+// It stands where the reference's clients launch the vocabulary projection's sgemm and the softmax / nll_loss rows behind it
+// (reference benchmarking/model_kernels/bert_8_fb1; src/scheduler/utils_sched.cpp:490-501).
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include "elastic.h"
+#include "gemm_call.h"
+#include "pdl.cuh"
+
+namespace ob200 {
+
+constexpr int CE_THREADS = 256;
+constexpr float CE_LOG2E = 1.4426950408889634f;
+
+// lse and loss of every row from its parts.  32 rows a CTA; group g of 8 joins parts g, g + 8, ..., then the groups are joined in order.
+__global__ void __launch_bounds__(CE_THREADS) ce_rows_kernel(const float2* __restrict__ part, const float* __restrict__ label_logit,
+                                                             const long long* __restrict__ target, float* __restrict__ loss,
+                                                             float* __restrict__ lse, int rows, int parts, int V, long long ignore_index) {
+    pdl_wait();
+    pdl_launch_dependents();
+    __shared__ float2 sh[8][32];
+    const int c = threadIdx.x & 31, g = threadIdx.x >> 5;
+    for (int r0 = blockIdx.x * 32; r0 < rows; r0 += gridDim.x * 32) {
+        const int r = r0 + c;
+        float top = -INFINITY, sum = 0.f;
+        auto join = [&](float2 q) {
+            const float now = fmaxf(top, q.x);
+            if (now == -INFINITY) {   // nothing above minus infinity yet; a sum that is not a number stays one
+                sum += q.y;
+                return;
+            }
+            sum = (top == -INFINITY ? sum : sum * exp2f((top - now) * CE_LOG2E)) + (q.x == -INFINITY ? q.y : q.y * exp2f((q.x - now) * CE_LOG2E));
+            top = now;
+        };
+        if (r < rows) {
+#pragma unroll 8
+            for (int t = g; t < parts; t += 8) join(part[(long long)t * rows + r]);
+        }
+        sh[g][c] = make_float2(top, sum);
+        __syncthreads();
+        if (g == 0 && r < rows) {
+#pragma unroll
+            for (int k = 1; k < 8; k++) join(sh[k][c]);
+            const float l = top + logf(sum);
+            const long long t = target[r];
+            lse[r] = l;
+            loss[r] = t == ignore_index ? 0.f : t >= 0 && t < V ? l - label_logit[r] : NAN;
+        }
+        __syncthreads();
+    }
+}
+
+// Sum or mean of the losses, and the number of rows that count, at least 1: one CTA, in a fixed order.
+__global__ void __launch_bounds__(1024) ce_total_kernel(const float* __restrict__ loss, const long long* __restrict__ target,
+                                                        float* __restrict__ total, float* __restrict__ count, long long rows,
+                                                        long long ignore_index, int mean) {
+    pdl_wait();
+    pdl_launch_dependents();
+    __shared__ double sh_sum[32];
+    __shared__ long long sh_count[32];
+    double s = 0.0;
+    long long n = 0;
+    for (long long r = threadIdx.x; r < rows; r += 1024) {
+        s += loss[r];
+        n += target[r] != ignore_index;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        s += __shfl_xor_sync(0xffffffffu, s, o);
+        n += __shfl_xor_sync(0xffffffffu, n, o);
+    }
+    if ((threadIdx.x & 31) == 0) {
+        sh_sum[threadIdx.x >> 5] = s;
+        sh_count[threadIdx.x >> 5] = n;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        s = 0.0;
+        n = 0;
+        for (int w = 0; w < 32; w++) {
+            s += sh_sum[w];
+            n += sh_count[w];
+        }
+        if (n < 1) n = 1;   // no row counts: the loss is 0
+        *total = (float)(mean ? s / (double)n : s);
+        *count = (float)n;
+    }
+}
+
+// Per row (lse * log2(e), coefficient) for the epilogue, and a copy of x without the rows that do not count, whatever they hold (0 times
+// infinity would reach dw).  One warp a row.  A label outside the vocabulary makes the coefficient, and so the gradients, not a number.
+__global__ void __launch_bounds__(CE_THREADS) ce_prepare_kernel(const __nv_bfloat16* __restrict__ x, long long ldx, __nv_bfloat16* __restrict__ kept,
+                                                                const float* __restrict__ lse, const long long* __restrict__ target,
+                                                                const float* __restrict__ grad, int grad_per_row, const float* __restrict__ count,
+                                                                float2* __restrict__ row, long long rows, int V, int H, long long ignore_index) {
+    pdl_wait();
+    pdl_launch_dependents();
+    const int lane = threadIdx.x & 31;
+    for (long long r = (long long)blockIdx.x * (CE_THREADS / 32) + (threadIdx.x >> 5); r < rows; r += (long long)gridDim.x * (CE_THREADS / 32)) {
+        const long long t = target[r];
+        const float g = (grad_per_row ? grad[r] : grad[0]) / (count ? *count : 1.f);
+        const float c = t == ignore_index ? 0.f : t >= 0 && t < V ? g : NAN;
+        if (lane == 0) row[r] = make_float2(lse[r] * CE_LOG2E, c);
+        if (kept) {
+            const uint4* src = reinterpret_cast<const uint4*>(x + r * ldx);
+            uint4* dst = reinterpret_cast<uint4*>(kept + r * H);
+            for (int i = lane; i < H / 8; i += 32) dst[i] = c == 0.f ? make_uint4(0, 0, 0, 0) : src[i];
+        }
+    }
+}
+
+// Columns of the vocabulary a piece of the backward pass has: dl of a piece is about as large as the L2 cache, and no piece so narrow
+// that its products are small.
+static int ce_piece(long long rows, int V) {
+    long long v = (128LL << 20) / (2 * rows) / 256 * 256;
+    if (v < 2048) v = 2048;
+    const long long all = ((long long)V + 7) / 8 * 8;
+    if (v >= all) return (int)all;
+    const long long pieces = (V + v - 1) / v;
+    return (int)(((V + pieces - 1) / pieces + 255) / 256 * 256);
+}
+constexpr int CE_ROW_BLOCK = 65536;   // rows a forward pass has in its workspace at a time
+static size_t ce_round(size_t bytes) { return (bytes + 255) & ~(size_t)255; }
+
+struct CeBackwardSpace {
+    size_t row, kept, dl, acc, slabs, total;
+    int piece;
+    CeBackwardSpace(long long rows, int V, int H, bool want_dx, bool want_dw) {
+        piece = ce_piece(rows, V);
+        row = ce_round((size_t)rows * sizeof(float2));
+        kept = want_dw ? ce_round((size_t)rows * H * 2) : 0;
+        dl = ce_round((size_t)rows * piece * 2);
+        acc = want_dx && piece < V ? ce_round((size_t)rows * H * sizeof(float)) : 0;
+        slabs = 0;
+        const int last = V - (V - 1) / piece * piece;   // columns of the last piece
+        for (int v : {piece < V ? piece : V, last}) {
+            const size_t a = want_dx ? gemm_bf16_slab_bytes((int)rows, H, v) : 0, b = want_dw ? gemm_bf16_slab_bytes(v, H, (int)rows) : 0;
+            if (a > slabs) slabs = a;
+            if (b > slabs) slabs = b;
+        }
+        slabs = ce_round(slabs);
+        total = row + kept + dl + acc + slabs;
+    }
+};
+
+}  // namespace ob200
+
+using namespace ob200;
+
+extern "C" long long ob200_linear_cross_entropy_workspace(int rows, int V) {
+    if (rows <= 0 || V <= 0) return 0;
+    const long long block = rows < CE_ROW_BLOCK ? rows : CE_ROW_BLOCK;
+    return (long long)ce_round((size_t)block * ((V + 127) / 128) * sizeof(float2)) + block * (long long)sizeof(float);
+}
+
+// See include/orion_kernels.h.  -1: sizes or arguments, -2: alignment, -3: workspace too small, -4: no TMA descriptor.
+extern "C" int ob200_linear_cross_entropy_forward(const void* x, const void* w, const long long* target, float* loss, float* lse, float* total, float* count,
+                                                  int rows, int V, int H, long long ldx, long long ldw, long long ignore_index, int mean, void* workspace,
+                                                  long long workspace_bytes, int num_ctas, void* stream) {
+    if (rows < 0 || V <= 0 || H <= 0 || ldx < H || ldw < H || num_ctas <= 0) return -1;
+    if ((rows > 0 && (!x || !w || !target || !loss || !lse)) || (total && !count)) return -1;
+    if (((uintptr_t)x | (uintptr_t)w | (uintptr_t)workspace) % 16 || (ldx | ldw) % 8) return -2;
+    if (workspace_bytes < ob200_linear_cross_entropy_workspace(rows, V) || (!workspace && rows > 0)) return -3;
+    cudaStream_t st = (cudaStream_t)stream;
+    const int block = rows < CE_ROW_BLOCK ? rows : CE_ROW_BLOCK, parts = (V + 127) / 128;
+    float2* part = (float2*)workspace;
+    float* label_logit = (float*)((char*)workspace + ce_round((size_t)block * parts * sizeof(float2)));
+    for (int r0 = 0; r0 < rows; r0 += CE_ROW_BLOCK) {
+        const int n = rows - r0 < CE_ROW_BLOCK ? rows - r0 : CE_ROW_BLOCK;
+        GemmCall g;
+        g.a = (const __nv_bfloat16*)x + (long long)r0 * ldx;
+        g.b = w;
+        g.M = n; g.N = V; g.K = H;
+        g.lda = ldx; g.ldb = ldw; g.ldc = V;
+        g.epi = GM_EPI_LSE;
+        g.e.target = target + r0;
+        g.e.part = part;
+        g.e.label_logit = label_logit;
+        g.num_ctas = num_ctas;
+        g.stream = stream;
+        int rc = gemm_bf16_run(g);
+        if (rc) return rc;
+        const int want = (n + 31) / 32, cap = num_ctas * 8;
+        OB200_ELASTIC_HBM(ce_rows_kernel, 8);
+        rc = launch_pdl(ce_rows_kernel, (unsigned)(want < cap ? want : cap), (unsigned)CE_THREADS, st, (const float2*)part, (const float*)label_logit,
+                        target + r0, loss + r0, lse + r0, n, parts, V, ignore_index);
+        if (rc) return rc;
+    }
+    if (!total) return 0;
+    OB200_HBM_BOUND();
+    return launch_pdl(ce_total_kernel, 1u, 1024u, st, (const float*)loss, target, total, count, (long long)rows, ignore_index, mean);
+}
+
+extern "C" long long ob200_linear_cross_entropy_backward_workspace(int rows, int V, int H, int want_dx, int want_dw) {
+    if (rows <= 0 || V <= 0 || H <= 0) return 0;
+    return (long long)CeBackwardSpace(rows, V, H, want_dx, want_dw).total;
+}
+
+extern "C" int ob200_linear_cross_entropy_backward(const void* x, const void* w, const long long* target, const float* lse, const float* grad,
+                                                   int grad_per_row, const float* count, void* dx, void* dw, int rows, int V, int H, long long ldx,
+                                                   long long ldw, long long ignore_index, void* workspace, long long workspace_bytes, int num_ctas,
+                                                   void* stream) {
+    if (rows < 0 || V <= 0 || H <= 0 || ldx < H || ldw < H || num_ctas <= 0) return -1;
+    if (rows == 0) return dw ? (int)cudaMemsetAsync(dw, 0, (size_t)V * H * 2, (cudaStream_t)stream) : 0;
+    if (!x || !w || !target || !lse || !grad) return -1;
+    if (((uintptr_t)x | (uintptr_t)w | (uintptr_t)dx | (uintptr_t)dw | (uintptr_t)workspace) % 16 || (ldx | ldw) % 8 || H % 8) return -2;
+    if (!dx && !dw) return 0;
+    const CeBackwardSpace space(rows, V, H, dx != nullptr, dw != nullptr);
+    if (workspace_bytes < (long long)space.total || !workspace) return -3;
+    cudaStream_t st = (cudaStream_t)stream;
+    char* at = (char*)workspace;
+    float2* row = (float2*)at;
+    at += space.row;
+    __nv_bfloat16* kept = dw ? (__nv_bfloat16*)at : nullptr;
+    at += space.kept;
+    __nv_bfloat16* dl = (__nv_bfloat16*)at;
+    at += space.dl;
+    float* acc = (float*)at;
+    at += space.acc;
+    {
+        const long long want = ((long long)rows + CE_THREADS / 32 - 1) / (CE_THREADS / 32), cap = (long long)num_ctas * 8;
+        OB200_ELASTIC_HBM(ce_prepare_kernel, 8);
+        const int rc = launch_pdl(ce_prepare_kernel, (unsigned)(want < cap ? want : cap), (unsigned)CE_THREADS, st, (const __nv_bfloat16*)x, ldx, kept, lse,
+                                  target, grad, grad_per_row, count, row, (long long)rows, V, H, ignore_index);
+        if (rc) return rc;
+    }
+    for (int v0 = 0; v0 < V; v0 += space.piece) {
+        const int nv = V - v0 < space.piece ? V - v0 : space.piece;
+        const bool first = v0 == 0, last = v0 + nv == V;
+        const __nv_bfloat16* wp = (const __nv_bfloat16*)w + (long long)v0 * ldw;
+        GemmCall g;
+        g.num_ctas = num_ctas;
+        g.stream = stream;
+        g.a = x; g.b = wp; g.c = dl;
+        g.M = rows; g.N = nv; g.K = H;
+        g.lda = ldx; g.ldb = ldw; g.ldc = space.piece;
+        g.epi = GM_EPI_DLOGITS;
+        g.e.target = target;
+        g.e.col0 = v0;
+        g.e.row = row;
+        int rc = gemm_bf16_run(g);
+        if (rc) return rc;
+        g.slabs = (float*)at;
+        g.slab_bytes = space.slabs;
+        g.a = dl; g.lda = space.piece;
+        g.b_mn = 1;
+        g.N = H;
+        g.ldc = H;
+        if (dx) {   // dx[t, h] += sum_v dl[t, v] w[v, h]
+            g.b = wp; g.ldb = ldw;
+            g.M = rows; g.K = nv;
+            g.epi = first ? GM_EPI_PLAIN : GM_EPI_ACC;
+            g.e.addend = first ? nullptr : acc;
+            g.out_f32 = last ? 0 : 1;
+            g.c = last ? dx : (void*)acc;
+            rc = gemm_bf16_run(g);
+            if (rc) return rc;
+        }
+        if (dw) {   // dw[v, h] = sum_t dl[t, v] x[t, h]
+            g.a_mn = 1;
+            g.b = kept; g.ldb = H;
+            g.M = nv; g.K = rows;
+            g.epi = GM_EPI_PLAIN;
+            g.out_f32 = 0;
+            g.c = (__nv_bfloat16*)dw + (long long)v0 * H;
+            rc = gemm_bf16_run(g);
+            if (rc) return rc;
+        }
+    }
+    return 0;
+}

@@ -20,6 +20,7 @@
 // SM budget its scheduler stream was given).
 #include <ATen/ATen.h>
 #include <ATen/NativeFunctions.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/autograd.h>
 #include <torch/library.h>
@@ -95,6 +96,25 @@ int ob200_cross_entropy_backward(const void* logits, const long long* target, co
                                  long long rows, int V, int dtype, void* stream);
 int ob200_adamw_multi(void* const* p, const void* const* g, void* const* m, void* const* v, const long long* n, int count, float lr,
                       float beta1, float beta2, float eps, float weight_decay, int step, int dtype, int num_ctas, void* stream);
+int ob200_linear_act_bf16(const void* x, const void* w, void* y, void* pre, const void* bias, int bias_f32, const void* residual, int act,
+                          float p, const long long* rng, int site, int M, int N, int K, long long ldx, long long ldw, long long ld_pre,
+                          void* workspace, long long workspace_bytes, int num_ctas, void* stream);
+long long ob200_linear_act_workspace(int M, int N, int K);
+int ob200_linear_act_backward_bf16(const void* dy, const void* pre, const void* x, const void* w, void* dx, void* dw, void* dbias,
+                                   int bias_f32, int act, float p, const long long* rng, int site, int M, int N, int K, long long ldx,
+                                   long long ldw, long long ld_pre, void* workspace, long long workspace_bytes, int num_ctas, void* stream);
+long long ob200_linear_act_backward_workspace(int M, int N, int K, int act, float p, int want_dx, int want_dw, int want_dbias);
+int ob200_dropout(const void* x, const void* residual, void* y, long long n, float p, const long long* rng, int site, int dtype,
+                  int num_ctas, void* stream);
+int ob200_linear_cross_entropy_forward(const void* x, const void* w, const long long* target, float* loss, float* lse, float* total,
+                                       float* count, int rows, int V, int H, long long ldx, long long ldw, long long ignore_index, int mean,
+                                       void* workspace, long long workspace_bytes, int num_ctas, void* stream);
+long long ob200_linear_cross_entropy_workspace(int rows, int V);
+int ob200_linear_cross_entropy_backward(const void* x, const void* w, const long long* target, const float* lse, const float* grad,
+                                        int grad_per_row, const float* count, void* dx, void* dw, int rows, int V, int H, long long ldx,
+                                        long long ldw, long long ignore_index, void* workspace, long long workspace_bytes, int num_ctas,
+                                        void* stream);
+long long ob200_linear_cross_entropy_backward_workspace(int rows, int V, int H, int want_dx, int want_dw);
 int ob200_maxpool_backward_nhwc_f32(const float* dy, const float* x, float* dx, int Nb, int H, int W, int C, int k, int stride,
                                     int pad, int num_ctas, void* stream);
 int ob200_sgd_momentum_multi_f32(float* const* p, const float* const* g, float* const* m, const long long* n, int count, float lr,
@@ -798,6 +818,265 @@ at::Tensor linear_train_op(const at::Tensor& x, const at::Tensor& w, const c10::
     return LinearTrain::apply(x, w, bias, residual);
 }
 
+// ------------------------------------------------------------------ fused linear layer, dropout, loss without logits
+// `t` as rows of its last dimension: a view where the rows lie a multiple of 8 elements apart and 16-byte aligned (what a TMA copy
+// needs), else a copy.
+at::Tensor as_rows(const at::Tensor& t) {
+    at::Tensor r = t.dim() == 2 ? t : t.reshape({-1, t.size(-1)});
+    const bool fits = r.stride(1) == 1 && r.stride(0) >= r.size(1) && r.stride(0) % 8 == 0 && (uintptr_t)r.data_ptr() % 16 == 0;
+    return fits || r.numel() == 0 ? r : r.clone(at::MemoryFormat::Contiguous);
+}
+// Contiguous and 16-byte aligned.
+at::Tensor as_dense(const at::Tensor& t) {
+    at::Tensor r = t.contiguous();
+    return (uintptr_t)r.data_ptr() % 16 == 0 ? r : r.clone(at::MemoryFormat::Contiguous);
+}
+at::Tensor workspace(int64_t bytes, const at::Tensor& like) { return at::empty({bytes}, like.options().dtype(at::kByte)); }
+bool given(const c10::optional<at::Tensor>& t) { return t.has_value() && t->defined(); }
+// The gradients are plain results, not functions of the inputs: a second derivative would silently be missing a term.
+void refuse_double_backward(const char* op) {
+    TORCH_CHECK(!at::GradMode::is_enabled(), op, " cannot be differentiated twice (create_graph=True)");
+}
+
+void check_dropout(const char* op, const at::Tensor& x, double p, const c10::optional<at::Tensor>& rng, int64_t site) {
+    TORCH_CHECK(p >= 0.0 && p <= 1.0, op, ": a probability p between 0 and 1 expected, got ", p);
+    TORCH_CHECK(site >= 0 && site <= 0x7fffffff, op, ": a site between 0 and 2^31 - 1 expected, got ", site);
+    if (p > 0.0)
+        TORCH_CHECK(given(rng) && rng->device() == x.device() && rng->scalar_type() == at::kLong && rng->numel() == 2 && rng->is_contiguous(),
+                    op, ": dropout needs rng, a contiguous int64 tensor (seed, step) on the input's device");
+}
+const long long* rng_ptr(const c10::optional<at::Tensor>& rng, double p) {
+    return p > 0.0 ? (const long long*)rng->data_ptr<int64_t>() : nullptr;
+}
+
+// y = residual + dropout(act(x . w^T + bias)) and its gradients, see ob200_linear_act_bf16.  Scratch is the call's own tensor, never
+// a buffer of the stream: two captured graphs may replay side by side.
+struct LinearAct : public torch::autograd::Function<LinearAct> {
+    static int act_code(c10::string_view act) {
+        const int code = act == "none" ? 0 : act == "relu" ? 1 : act == "gelu" ? 2 : -1;
+        TORCH_CHECK(code >= 0, "orion::linear_act: act has to be none, relu or gelu, got ", act);
+        return code;
+    }
+    static void check_args(const at::Tensor& x, const at::Tensor& w, const c10::optional<at::Tensor>& bias, const c10::optional<at::Tensor>& residual,
+                           double p, const c10::optional<at::Tensor>& rng, int64_t site) {
+        TORCH_CHECK(x.is_cuda() && x.scalar_type() == at::kBFloat16 && w.scalar_type() == at::kBFloat16 && w.device() == x.device() &&
+                        x.dim() >= 2 && w.dim() == 2 && x.size(-1) == w.size(1) && w.size(1) > 0 && w.size(1) % 8 == 0,
+                    "orion::linear_act: bfloat16 CUDA tensors [..., K] x [N, K] with K a multiple of 8 expected");
+        const int64_t N = w.size(0), M = x.numel() / w.size(1);
+        TORCH_CHECK(M <= 0x7fffffff && N <= 0x7fffffff && w.size(1) <= 0x7fffffff, "orion::linear_act: sizes beyond 2^31 - 1");
+        if (given(bias))
+            TORCH_CHECK(dtype_code(*bias) >= 0 && bias->dim() == 1 && bias->numel() == N && bias->is_contiguous() && bias->device() == x.device(),
+                        "orion::linear_act: bias has to be contiguous [N], bfloat16 or float32");
+        if (given(residual)) {
+            auto shape = x.sizes().vec();
+            shape.back() = N;
+            TORCH_CHECK(residual->scalar_type() == at::kBFloat16 && residual->sizes() == at::IntArrayRef(shape) && residual->device() == x.device(),
+                        "orion::linear_act: the residual must be bfloat16 and have the output's shape");
+        }
+        check_dropout("orion::linear_act", x, p, rng, site);
+    }
+    // The output, and with `want_pre` the pre-activation in rows padded to a multiple of 8.
+    static at::Tensor run(const at::Tensor& x, const at::Tensor& w, const c10::optional<at::Tensor>& bias, const c10::optional<at::Tensor>& residual,
+                          int act, double p, const c10::optional<at::Tensor>& rng, int64_t site, bool want_pre, at::Tensor* pre) {
+        c10::cuda::CUDAGuard guard(x.device());
+        const int64_t K = w.size(1), N = w.size(0);
+        auto shape = x.sizes().vec();
+        shape.back() = N;
+        at::Tensor y = at::empty(shape, x.options().memory_format(at::MemoryFormat::Contiguous));
+        if (y.numel() == 0) return y;
+        const at::Tensor xr = as_rows(x), wr = as_rows(w);
+        const int64_t M = xr.size(0);
+        const at::Tensor res = given(residual) ? residual->contiguous() : at::Tensor();
+        if (want_pre) *pre = at::empty({M, (N + 7) / 8 * 8}, x.options());
+        const long long bytes = ob200_linear_act_workspace((int)M, (int)N, (int)K);
+        const at::Tensor space = bytes ? workspace(bytes, x) : at::Tensor();
+        check(ob200_linear_act_bf16(xr.data_ptr(), wr.data_ptr(), y.data_ptr(), want_pre ? pre->data_ptr() : nullptr,
+                                    given(bias) ? bias->data_ptr() : nullptr, given(bias) && bias->scalar_type() == at::kFloat ? 1 : 0,
+                                    res.defined() ? res.data_ptr() : nullptr, act, (float)p, rng_ptr(rng, p), (int)site, (int)M, (int)N, (int)K,
+                                    xr.stride(0), wr.stride(0), want_pre ? pre->size(1) : 0, bytes ? space.data_ptr() : nullptr, bytes, quota(),
+                                    cur_stream()),
+              "ob200_linear_act_bf16");
+        return y;
+    }
+    static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w, const c10::optional<at::Tensor>& bias,
+                              const c10::optional<at::Tensor>& residual, int64_t act, double p, const c10::optional<at::Tensor>& rng, int64_t site) {
+        at::Tensor pre;
+        at::Tensor y = run(x, w, bias, residual, (int)act, p, rng, site, act != 0, &pre);
+        ctx->save_for_backward({x, w, pre, p > 0.0 ? *rng : at::Tensor()});
+        ctx->saved_data["act"] = act;
+        ctx->saved_data["p"] = p;
+        ctx->saved_data["site"] = site;
+        ctx->saved_data["bias"] = given(bias) ? (int64_t)(bias->scalar_type() == at::kFloat ? 2 : 1) : (int64_t)0;
+        ctx->saved_data["residual"] = given(residual);
+        return y;
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+        refuse_double_backward("orion::linear_act");
+        auto saved = ctx->get_saved_variables();
+        const at::Tensor &x = saved[0], &w = saved[1], &pre = saved[2], &rng = saved[3];
+        c10::cuda::CUDAGuard guard(x.device());
+        const int act = (int)ctx->saved_data["act"].toInt(), bias = (int)ctx->saved_data["bias"].toInt();
+        const double p = ctx->saved_data["p"].toDouble();
+        const bool has_res = ctx->saved_data["residual"].toBool();
+        const int64_t K = w.size(1), N = w.size(0), M = x.numel() / K;
+        // an argument that was not given has no place among the edges
+        const bool want_dx = ctx->needs_input_grad(0), want_dw = ctx->needs_input_grad(1), want_db = bias && ctx->needs_input_grad(2);
+        at::Tensor dx, dw, db, dres;
+        const auto dense = x.options().memory_format(at::MemoryFormat::Contiguous);
+        if (want_dx) dx = at::empty(x.sizes(), dense);
+        if (want_dw) dw = at::empty(w.sizes(), dense);
+        if (want_db) db = at::empty({N}, x.options().dtype(bias == 2 ? at::kFloat : at::kBFloat16));
+        if (has_res) dres = grads[0];
+        if (M == 0 || N == 0) {
+            for (at::Tensor* t : {&dx, &dw, &db})
+                if (t->defined()) t->zero_();
+        } else if (want_dx || want_dw || want_db) {
+            const at::Tensor dy = as_dense(grads[0]), xr = as_rows(x), wr = as_rows(w);
+            const long long bytes = ob200_linear_act_backward_workspace((int)M, (int)N, (int)K, act, (float)p, want_dx, want_dw, want_db);
+            const at::Tensor space = bytes ? workspace(bytes, x) : at::Tensor();
+            check(ob200_linear_act_backward_bf16(dy.data_ptr(), act ? pre.data_ptr() : nullptr, xr.data_ptr(), wr.data_ptr(),
+                                                 want_dx ? dx.data_ptr() : nullptr, want_dw ? dw.data_ptr() : nullptr, want_db ? db.data_ptr() : nullptr,
+                                                 bias == 2 ? 1 : 0, act, (float)p, p > 0.0 ? (const long long*)rng.data_ptr<int64_t>() : nullptr,
+                                                 (int)ctx->saved_data["site"].toInt(), (int)M, (int)N, (int)K, xr.stride(0), wr.stride(0),
+                                                 act ? pre.size(1) : 0, bytes ? space.data_ptr() : nullptr, bytes, quota(), cur_stream()),
+                  "ob200_linear_act_backward_bf16");
+            g_own_launches.fetch_add((want_dx ? 1 : 0) + (want_dw ? 1 : 0) + (want_db ? 1 : 0), std::memory_order_relaxed);
+        }
+        return {dx, dw, db, dres, at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+    }
+};
+at::Tensor linear_act_op(const at::Tensor& x, const at::Tensor& w, const c10::optional<at::Tensor>& bias, const c10::optional<at::Tensor>& residual,
+                         c10::string_view act, double p, const c10::optional<at::Tensor>& rng, int64_t site) {
+    const int code = LinearAct::act_code(act);
+    LinearAct::check_args(x, w, bias, residual, p, rng, site);
+    return LinearAct::run(x, w, bias, residual, code, p, rng, site, false, nullptr);
+}
+at::Tensor linear_act_autograd(const at::Tensor& x, const at::Tensor& w, const c10::optional<at::Tensor>& bias, const c10::optional<at::Tensor>& residual,
+                               c10::string_view act, double p, const c10::optional<at::Tensor>& rng, int64_t site) {
+    const bool grad = at::GradMode::is_enabled() &&
+                      (x.requires_grad() || w.requires_grad() || (given(bias) && bias->requires_grad()) || (given(residual) && residual->requires_grad()));
+    if (!grad) return linear_act_op(x, w, bias, residual, act, p, rng, site);
+    const int code = LinearAct::act_code(act);
+    LinearAct::check_args(x, w, bias, residual, p, rng, site);
+    return LinearAct::apply(x, w, bias, residual, code, p, rng, site);
+}
+
+// y = dropout(x) [+ residual]; the gradient is the same kernel on dy, with the mask drawn again.
+struct Dropout : public torch::autograd::Function<Dropout> {
+    static void check_args(const at::Tensor& x, double p, const c10::optional<at::Tensor>& rng, int64_t site, const c10::optional<at::Tensor>& residual) {
+        TORCH_CHECK(x.is_cuda() && dtype_code(x) >= 0, "orion::dropout: float32/bfloat16 CUDA tensor expected");
+        if (given(residual))
+            TORCH_CHECK(residual->scalar_type() == x.scalar_type() && residual->sizes() == x.sizes() && residual->device() == x.device(),
+                        "orion::dropout: the residual must have the input's type and shape");
+        check_dropout("orion::dropout", x, p, rng, site);
+    }
+    static at::Tensor run(const at::Tensor& x, double p, const c10::optional<at::Tensor>& rng, int64_t site, const c10::optional<at::Tensor>& residual) {
+        c10::cuda::CUDAGuard guard(x.device());
+        const at::Tensor xc = x.contiguous(), res = given(residual) ? residual->contiguous() : at::Tensor();
+        at::Tensor y = at::empty(x.sizes(), x.options().memory_format(at::MemoryFormat::Contiguous));
+        if (y.numel() == 0) return y;
+        check(ob200_dropout(xc.data_ptr(), res.defined() ? res.data_ptr() : nullptr, y.data_ptr(), y.numel(), (float)p, rng_ptr(rng, p), (int)site,
+                            dtype_code(x), quota(), cur_stream()),
+              "ob200_dropout");
+        return y;
+    }
+    static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, double p, const c10::optional<at::Tensor>& rng, int64_t site,
+                              const c10::optional<at::Tensor>& residual) {
+        ctx->save_for_backward({p > 0.0 ? *rng : at::Tensor()});
+        ctx->saved_data["p"] = p;
+        ctx->saved_data["site"] = site;
+        ctx->saved_data["residual"] = given(residual);
+        return run(x, p, rng, site, residual);
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+        refuse_double_backward("orion::dropout");
+        const double p = ctx->saved_data["p"].toDouble();
+        at::Tensor dx;
+        if (ctx->needs_input_grad(0)) dx = run(grads[0], p, ctx->get_saved_variables()[0], ctx->saved_data["site"].toInt(), c10::nullopt);
+        return {dx, at::Tensor(), at::Tensor(), at::Tensor(), ctx->saved_data["residual"].toBool() ? grads[0] : at::Tensor()};
+    }
+};
+at::Tensor dropout_op(const at::Tensor& x, double p, const c10::optional<at::Tensor>& rng, int64_t site, const c10::optional<at::Tensor>& residual) {
+    Dropout::check_args(x, p, rng, site, residual);
+    return Dropout::run(x, p, rng, site, residual);
+}
+at::Tensor dropout_autograd(const at::Tensor& x, double p, const c10::optional<at::Tensor>& rng, int64_t site, const c10::optional<at::Tensor>& residual) {
+    Dropout::check_args(x, p, rng, site, residual);
+    return Dropout::apply(x, p, rng, site, residual);
+}
+
+// Cross-entropy of x . w^T without the logits, see ob200_linear_cross_entropy_forward.  reduction: 0 none, 1 sum, 2 mean.
+struct LinearCrossEntropy : public torch::autograd::Function<LinearCrossEntropy> {
+    static int check_args(const at::Tensor& x, const at::Tensor& w, const at::Tensor& target, c10::string_view reduction) {
+        TORCH_CHECK(x.is_cuda() && x.scalar_type() == at::kBFloat16 && w.scalar_type() == at::kBFloat16 && w.device() == x.device() &&
+                        x.dim() >= 2 && w.dim() == 2 && x.size(-1) == w.size(1) && w.size(1) > 0 && w.size(1) % 8 == 0 && w.size(0) > 0,
+                    "orion::linear_cross_entropy: bfloat16 CUDA tensors [..., H] x [V, H] with H a multiple of 8 expected");
+        TORCH_CHECK(target.scalar_type() == at::kLong && target.device() == x.device() && target.sizes() == x.sizes().slice(0, x.dim() - 1),
+                    "orion::linear_cross_entropy: int64 targets of the input's shape without its last dimension expected");
+        TORCH_CHECK(target.numel() <= 0x7fffffff && w.size(0) <= 0x7fffffff && w.size(1) <= 0x7fffffff,
+                    "orion::linear_cross_entropy: sizes beyond 2^31 - 1");
+        const int code = reduction == "none" ? 0 : reduction == "sum" ? 1 : reduction == "mean" ? 2 : -1;
+        TORCH_CHECK(code >= 0, "orion::linear_cross_entropy: reduction has to be none, sum or mean, got ", reduction);
+        return code;
+    }
+    // (loss, lse, number of rows that count)
+    static std::vector<at::Tensor> run(const at::Tensor& x, const at::Tensor& w, const at::Tensor& target, int64_t ignore_index, int reduction) {
+        c10::cuda::CUDAGuard guard(x.device());
+        const at::Tensor xr = as_rows(x), wr = as_rows(w), tc = target.contiguous();
+        const int64_t rows = target.numel(), V = w.size(0), H = w.size(1);
+        const auto f32 = x.options().dtype(at::kFloat).memory_format(at::MemoryFormat::Contiguous);
+        at::Tensor loss = at::empty(target.sizes(), f32), lse = at::empty({rows}, f32);
+        at::Tensor total = reduction ? at::empty({}, f32) : at::Tensor(), count = reduction ? at::empty({}, f32) : at::Tensor();
+        const long long bytes = ob200_linear_cross_entropy_workspace((int)rows, (int)V);
+        const at::Tensor space = workspace(bytes, x);
+        check(ob200_linear_cross_entropy_forward(rows ? xr.data_ptr() : nullptr, wr.data_ptr(), (const long long*)tc.data_ptr<int64_t>(),
+                                                 loss.data_ptr<float>(), lse.data_ptr<float>(), reduction ? total.data_ptr<float>() : nullptr,
+                                                 reduction ? count.data_ptr<float>() : nullptr, (int)rows, (int)V, (int)H, rows ? xr.stride(0) : H,
+                                                 wr.stride(0), ignore_index, reduction == 2 ? 1 : 0, space.data_ptr(), bytes, quota(), cur_stream()),
+              "ob200_linear_cross_entropy_forward");
+        g_own_launches.fetch_add(reduction ? 2 : 1, std::memory_order_relaxed);
+        return {reduction ? total : loss, lse, count};
+    }
+    static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w, const at::Tensor& target,
+                              int64_t ignore_index, int64_t reduction) {
+        auto out = run(x, w, target, ignore_index, (int)reduction);
+        ctx->save_for_backward({x, w, target, out[1], reduction == 2 ? out[2] : at::Tensor()});
+        ctx->saved_data["ignore_index"] = ignore_index;
+        ctx->saved_data["reduction"] = reduction;
+        return out[0];
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+        refuse_double_backward("orion::linear_cross_entropy");
+        auto saved = ctx->get_saved_variables();
+        const at::Tensor &x = saved[0], &w = saved[1], &lse = saved[3], &count = saved[4];
+        c10::cuda::CUDAGuard guard(x.device());
+        const int64_t rows = saved[2].numel(), V = w.size(0), H = w.size(1);
+        const bool want_dx = ctx->needs_input_grad(0), want_dw = ctx->needs_input_grad(1);
+        const at::Tensor xr = as_rows(x), wr = as_rows(w), tc = saved[2].contiguous(), g = grads[0].to(at::kFloat).contiguous();
+        const auto dense = x.options().memory_format(at::MemoryFormat::Contiguous);
+        at::Tensor dx = want_dx ? at::empty(x.sizes(), dense) : at::Tensor(), dw = want_dw ? at::empty(w.sizes(), dense) : at::Tensor();
+        const long long bytes = ob200_linear_cross_entropy_backward_workspace((int)rows, (int)V, (int)H, want_dx, want_dw);
+        const at::Tensor space = workspace(bytes, x);
+        check(ob200_linear_cross_entropy_backward(rows ? xr.data_ptr() : nullptr, wr.data_ptr(), (const long long*)tc.data_ptr<int64_t>(),
+                                                  lse.data_ptr<float>(), g.data_ptr<float>(), ctx->saved_data["reduction"].toInt() == 0 ? 1 : 0,
+                                                  count.defined() ? count.data_ptr<float>() : nullptr, want_dx && rows ? dx.data_ptr() : nullptr,
+                                                  want_dw ? dw.data_ptr() : nullptr, (int)rows, (int)V, (int)H, rows ? xr.stride(0) : H, wr.stride(0),
+                                                  ctx->saved_data["ignore_index"].toInt(), space.data_ptr(), bytes, quota(), cur_stream()),
+              "ob200_linear_cross_entropy_backward");
+        g_own_launches.fetch_add(1 + (want_dx ? 1 : 0) + (want_dw ? 1 : 0), std::memory_order_relaxed);
+        return {dx, dw, at::Tensor(), at::Tensor(), at::Tensor()};
+    }
+};
+at::Tensor linear_cross_entropy_op(const at::Tensor& x, const at::Tensor& w, const at::Tensor& target, int64_t ignore_index, c10::string_view reduction) {
+    const int code = LinearCrossEntropy::check_args(x, w, target, reduction);
+    return LinearCrossEntropy::run(x, w, target, ignore_index, code)[0];
+}
+at::Tensor linear_cross_entropy_autograd(const at::Tensor& x, const at::Tensor& w, const at::Tensor& target, int64_t ignore_index,
+                                         c10::string_view reduction) {
+    const int code = LinearCrossEntropy::check_args(x, w, target, reduction);
+    return LinearCrossEntropy::apply(x, w, target, ignore_index, code);
+}
+
 // Self-attention for training, straight on the fused projection qkv [B, S, 3 * heads * d]: scores, softmax, context and all
 // five gradient products on ob200_gemm_bf16 (no re-laid-out copy of Q, K, V or of their gradients), softmax and its gradient on
 // the row kernels.  The probabilities are kept for the backward pass.  Causal attention computes only the score tiles that reach
@@ -1072,6 +1351,9 @@ TORCH_LIBRARY(orion, m) {
     m.def("bias_gelu_train(Tensor x, Tensor bias) -> Tensor");
     m.def("cross_entropy(Tensor logits, Tensor target) -> Tensor");
     m.def("linear_train(Tensor x, Tensor w, Tensor? bias, Tensor? residual=None) -> Tensor");
+    m.def("linear_act(Tensor x, Tensor w, Tensor? bias=None, Tensor? residual=None, str act='none', float p=0.0, Tensor? rng=None, int site=0) -> Tensor");
+    m.def("dropout(Tensor x, float p, Tensor? rng, int site=0, Tensor? residual=None) -> Tensor");
+    m.def("linear_cross_entropy(Tensor x, Tensor w, Tensor target, int ignore_index=-100, str reduction='mean') -> Tensor");
     m.def("attention_train(Tensor qkv, int heads, float scale, bool causal) -> Tensor");
     m.def("embedding_train(Tensor ids, Tensor word, Tensor pos, Tensor? typ=None) -> Tensor");
     m.def("adamw_step(Tensor(a!)[] params, Tensor[] grads, Tensor(b!)[] exp_avg, Tensor(c!)[] exp_avg_sq, float lr, float beta1, float beta2, float eps, float weight_decay, int step) -> ()");
@@ -1099,6 +1381,9 @@ TORCH_LIBRARY_IMPL(orion, CUDA, m) {
     m.impl("linear_batched", &linear_batched_op);
     m.impl("attention", &attention_op);
     m.impl("attention_long", &attention_long_op);
+    m.impl("linear_act", &linear_act_op);
+    m.impl("dropout", &dropout_op);
+    m.impl("linear_cross_entropy", &linear_cross_entropy_op);
     m.impl("plan_run", &plan_run);
     m.impl("sgd_step", &sgd_step_op);
     m.impl("adamw_step", &adamw_step_op);
@@ -1111,6 +1396,9 @@ TORCH_LIBRARY_IMPL(orion, Autograd, m) {
     m.impl("bias_gelu_train", &bias_gelu_train_op);
     m.impl("cross_entropy", &cross_entropy_op);
     m.impl("linear_train", &linear_train_op);
+    m.impl("linear_act", &linear_act_autograd);
+    m.impl("dropout", &dropout_autograd);
+    m.impl("linear_cross_entropy", &linear_cross_entropy_autograd);
     m.impl("attention_train", &attention_train_op);
     m.impl("embedding_train", &embedding_train_op);
 }

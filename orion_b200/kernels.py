@@ -73,6 +73,19 @@ def lib():
         L.ob200_tma_launch_count.restype = c_ll
         L.ob200_pad_channels.argtypes = [c_void_p, c_void_p, c_ll, c_int, c_int, c_int, c_int, c_void_p]
         L.ob200_pad_channels.restype = c_int
+        L.ob200_linear_act_bf16.argtypes = [c_void_p] * 5 + [c_int, c_void_p, c_int, c_float, c_void_p] + [c_int] * 4 + [c_ll] * 3 + [c_void_p, c_ll, c_int, c_void_p]
+        L.ob200_linear_act_workspace.argtypes = [c_int] * 3
+        L.ob200_linear_act_backward_bf16.argtypes = [c_void_p] * 7 + [c_int, c_int, c_float, c_void_p] + [c_int] * 4 + [c_ll] * 3 + [c_void_p, c_ll, c_int, c_void_p]
+        L.ob200_linear_act_backward_workspace.argtypes = [c_int] * 4 + [c_float] + [c_int] * 3
+        L.ob200_dropout.argtypes = [c_void_p] * 3 + [c_ll, c_float, c_void_p, c_int, c_int, c_int, c_void_p]
+        L.ob200_linear_cross_entropy_forward.argtypes = [c_void_p] * 7 + [c_int] * 3 + [c_ll] * 3 + [c_int, c_void_p, c_ll, c_int, c_void_p]
+        L.ob200_linear_cross_entropy_workspace.argtypes = [c_int] * 2
+        L.ob200_linear_cross_entropy_backward.argtypes = [c_void_p] * 5 + [c_int] + [c_void_p] * 3 + [c_int] * 3 + [c_ll] * 3 + [c_void_p, c_ll, c_int, c_void_p]
+        L.ob200_linear_cross_entropy_backward_workspace.argtypes = [c_int] * 5
+        for name in ("linear_act_bf16", "linear_act_backward_bf16", "dropout", "linear_cross_entropy_forward", "linear_cross_entropy_backward"):
+            getattr(L, "ob200_" + name).restype = c_int
+        for name in ("linear_act", "linear_act_backward", "linear_cross_entropy", "linear_cross_entropy_backward"):
+            getattr(L, "ob200_%s_workspace" % name).restype = c_ll
         _lib = L
     return _lib
 
@@ -421,6 +434,84 @@ def bias_gelu(x, bias=None, num_ctas=None):
 def adamw_(p, g, m, v, step, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, num_ctas=None):
     _check(lib().ob200_adamw_f32(_ptr(p), _ptr(g), _ptr(m), _ptr(v), p.numel(), lr, betas[0], betas[1], eps, weight_decay, step,
                                  num_ctas or sm_count(), _stream()), "ob200_adamw_f32")
+
+
+_ACTS = {"none": 0, "relu": 1, "gelu": 2}
+
+
+def _rows_ok(*tensors):
+    return all(t.dim() == 2 and t.stride(1) == 1 and t.dtype == torch.bfloat16 for t in tensors)
+
+
+def linear_act(x, w, bias=None, residual=None, act="none", p=0.0, rng=None, site=0, want_pre=False, num_ctas=None):
+    """residual + dropout(act(x . w^T + bias)) for bfloat16 x [M, K], w [N, K] (rows a multiple of 8 elements apart), bias bfloat16 or
+    float32; rng: int64 CUDA tensor (seed, step).  With `want_pre` also the pre-activation, in rows padded to a multiple of 8."""
+    assert _rows_ok(x, w) and x.shape[1] == w.shape[1] and (residual is None or residual.is_contiguous())
+    M, K = x.shape
+    N = w.shape[0]
+    y = torch.empty((M, N), device=x.device, dtype=x.dtype)
+    pre = torch.empty((M, (N + 7) // 8 * 8), device=x.device, dtype=x.dtype) if want_pre else None
+    n = lib().ob200_linear_act_workspace(M, N, K)
+    space = torch.empty(n, device=x.device, dtype=torch.uint8) if n else None
+    _check(lib().ob200_linear_act_bf16(_ptr(x), _ptr(w), _ptr(y), _ptr(pre), _ptr(bias), int(bias is not None and bias.dtype == torch.float32),
+                                       _ptr(residual), _ACTS[act], float(p), _ptr(rng), int(site), M, N, K, x.stride(0), w.stride(0),
+                                       pre.shape[1] if want_pre else 0, _ptr(space), n, num_ctas or sm_count(), _stream()),
+           "ob200_linear_act_bf16")
+    return (y, pre) if want_pre else y
+
+
+def linear_act_backward(dy, pre, x, w, bias_dtype=torch.bfloat16, act="none", p=0.0, rng=None, site=0, num_ctas=None):
+    """(dx, dw, dbias) of linear_act from dy [M, N] and what `want_pre` gave (None without an activation)."""
+    assert _rows_ok(x, w) and dy.is_contiguous() and dy.dtype == torch.bfloat16
+    M, K = x.shape
+    N = w.shape[0]
+    dx, dw = torch.empty((M, K), device=x.device, dtype=x.dtype), torch.empty((N, K), device=x.device, dtype=x.dtype)
+    db = torch.empty(N, device=x.device, dtype=bias_dtype)
+    n = lib().ob200_linear_act_backward_workspace(M, N, K, _ACTS[act], float(p), 1, 1, 1)
+    space = torch.empty(n, device=x.device, dtype=torch.uint8)
+    _check(lib().ob200_linear_act_backward_bf16(_ptr(dy), _ptr(pre), _ptr(x), _ptr(w), _ptr(dx), _ptr(dw), _ptr(db),
+                                                int(bias_dtype == torch.float32), _ACTS[act], float(p), _ptr(rng), int(site), M, N, K, x.stride(0),
+                                                w.stride(0), 0 if pre is None else pre.shape[1], _ptr(space), n, num_ctas or sm_count(), _stream()),
+           "ob200_linear_act_backward_bf16")
+    return dx, dw, db
+
+
+def dropout(x, p, rng=None, site=0, residual=None, num_ctas=None):
+    """dropout(x) [+ residual] with the mask that linear_act draws for an output of this shape; x contiguous float32 / bfloat16."""
+    assert x.is_contiguous() and (residual is None or residual.is_contiguous() and residual.dtype == x.dtype and residual.shape == x.shape)
+    y = torch.empty_like(x)
+    _check(lib().ob200_dropout(_ptr(x), _ptr(residual), _ptr(y), x.numel(), float(p), _ptr(rng), int(site), _dtype_code(x), num_ctas or sm_count(),
+                               _stream()), "ob200_dropout")
+    return y
+
+
+def linear_cross_entropy(x, w, target, ignore_index=-100, mean=True, num_ctas=None):
+    """(total, loss per row, lse per row, rows that count) of the cross-entropy of x . w^T, x [rows, H], w [V, H] bfloat16, int64 targets."""
+    assert _rows_ok(x, w) and x.shape[1] == w.shape[1] and target.dtype == torch.int64 and target.is_contiguous()
+    rows, H = x.shape
+    V = w.shape[0]
+    loss, lse = (torch.empty(rows, device=x.device, dtype=torch.float32) for _ in range(2))
+    total, count = (torch.empty((), device=x.device, dtype=torch.float32) for _ in range(2))
+    n = lib().ob200_linear_cross_entropy_workspace(rows, V)
+    space = torch.empty(n, device=x.device, dtype=torch.uint8)
+    _check(lib().ob200_linear_cross_entropy_forward(_ptr(x), _ptr(w), _ptr(target), _ptr(loss), _ptr(lse), _ptr(total), _ptr(count), rows, V, H,
+                                                    x.stride(0), w.stride(0), ignore_index, int(mean), _ptr(space), n, num_ctas or sm_count(),
+                                                    _stream()), "ob200_linear_cross_entropy_forward")
+    return total, loss, lse, count
+
+
+def linear_cross_entropy_backward(x, w, target, lse, grad, count=None, ignore_index=-100, num_ctas=None):
+    """(dx, dw) from what linear_cross_entropy gave; grad: one value, or one per row; count: rows that count (the mean) or None."""
+    assert _rows_ok(x, w) and grad.dtype == torch.float32 and grad.is_contiguous() and target.is_contiguous()
+    rows, H = x.shape
+    V = w.shape[0]
+    dx, dw = torch.empty((rows, H), device=x.device, dtype=x.dtype), torch.empty((V, H), device=x.device, dtype=x.dtype)
+    n = lib().ob200_linear_cross_entropy_backward_workspace(rows, V, H, 1, 1)
+    space = torch.empty(n, device=x.device, dtype=torch.uint8)
+    _check(lib().ob200_linear_cross_entropy_backward(_ptr(x), _ptr(w), _ptr(target), _ptr(lse), _ptr(grad), int(grad.dim() > 0), _ptr(count), _ptr(dx),
+                                                     _ptr(dw), rows, V, H, x.stride(0), w.stride(0), ignore_index, _ptr(space), n,
+                                                     num_ctas or sm_count(), _stream()), "ob200_linear_cross_entropy_backward")
+    return dx, dw
 
 
 def conv2d_wgrad_nhwc(x, dy, filter_rs, stride=(1, 1), padding=(0, 0), dilation=(1, 1), num_ctas=None, tf32=False):
