@@ -34,6 +34,8 @@
 #include <stdlib.h>
 #include <string.h>
 
+#include <type_traits>
+
 #include "elastic.h"
 #include "fast_gelu.cuh"
 #include "gemm_call.h"
@@ -44,16 +46,19 @@ namespace ob200 {
 
 constexpr int GM_BM = 128;
 constexpr int GM_BK = 64;
-constexpr int GM_THREADS = 192;          // warp 0: TMA, warp 1: MMA + tensor memory, warps 2-5: epilogue
+// Warp 0: TMA, warp 1: MMA + tensor memory, the others: epilogue.  Four of them, or sixteen (four for each 32 rows, each a share of the
+// columns) where a turn of the epilogue is a long chain of latencies: bias + GELU of 8192 x 4096 x 1024.
+__host__ __device__ constexpr int gm_epi_warps(int epi) { return epi == GM_EPI_ACT || epi == GM_EPI_ACT_ANY ? 16 : epi == GM_EPI_DLOGITS ? 8 : 4; }
+__host__ __device__ constexpr int gm_threads(int epi) { return 64 + 32 * gm_epi_warps(epi); }
 constexpr int GM_A_BYTES = GM_BM * 128;
 
 // CG CTAs (1, or a pair) share a tile of CG * 128 rows: each stages its 128 rows of A and BN / CG rows of B.
-template <int BN, int CG>
+template <int BN, int CG, int EPI>
 struct GemmCfg {
     static constexpr int STAGE_BYTES = GM_A_BYTES + BN / CG * 128;
-    static constexpr int STAGES = STAGE_BYTES == 49152 ? 4 : STAGE_BYTES == 32768 ? 6 : 8;
-    static constexpr int EPI_BYTES = 4 * 2 * 4096;   // per epilogue warp two slabs of 32 rows x 128 bytes for the TMA stores
-    static constexpr int SMEM = STAGES * STAGE_BYTES + EPI_BYTES + 1024 + 256;
+    static constexpr int STAGES = gm_epi_warps(EPI) == 16 ? (STAGE_BYTES == 49152 ? 3 : STAGE_BYTES == 32768 ? 5 : 6) : STAGE_BYTES == 49152 ? 4 : STAGE_BYTES == 32768 ? 6 : 8;
+    static constexpr int EPI_BYTES = gm_epi_warps(EPI) == 16 ? 16 * 4096 : 32768;   // per epilogue warp two slabs of 32 rows x 64 (x 128) bytes for the TMA stores
+    static constexpr int SMEM = STAGES * STAGE_BYTES + EPI_BYTES + 1024 + 512;   // + alignment, barriers
     static constexpr int TMEM_COLS = 2 * BN < 32 ? 32 : 2 * BN;
 };
 
@@ -81,13 +86,27 @@ struct GemmParams {
     alignas(64) unsigned char tmap_b[128];
     alignas(64) unsigned char tmap_c[128];
     alignas(64) unsigned char tmap_pre[128];
+    alignas(64) unsigned char tmap_res[128];
 };
+
+// The second product of a GM_EPI_DUAL launch; its tiles come behind the first one's.
+struct GemmSecond {
+    int M, N, kblocks, tiles_m, tiles_n, a_mn, b_mn, out_f32;
+    alignas(64) unsigned char tmap_a[128];
+    alignas(64) unsigned char tmap_b[128];
+    alignas(64) unsigned char tmap_c[128];
+};
+struct GemmParamsDual : GemmParams { GemmSecond second; };
+template <int EPI>
+using GemmParamsOf = std::conditional_t<EPI == GM_EPI_DUAL, GemmParamsDual, GemmParams>;
 
 struct GemmCtl {
     uint64_t full[8], empty[8], acc_full[2], acc_empty[2];
+    uint64_t res_full[16][2];   // GM_EPI_ACT: a warp's residual slabs
     uint32_t tmem_base;
     int abort_flag;
 };
+static_assert(sizeof(GemmCtl) <= 512, "the barriers have 512 bytes of shared memory");
 
 __device__ __forceinline__ uint64_t gm_desc_mn(uint32_t addr) {
     return (uint64_t)((addr & 0x3FFFF) >> 4) | ((uint64_t)(8192 >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) |
@@ -116,11 +135,39 @@ __device__ __forceinline__ bool gm_tile_skipped(const GemmParams& p, int tm, int
     return p.tri == 1 && tn * BN > tm * GM_BM + GM_BM - 1;
 }
 
+// Work unit u: output tile (tm, tn) of problem b (bi, bo), k-blocks [kb0, kb1), split sp; `second`: of a dual launch's second product.
+struct GemmUnit { int sp, bi, bo, tm, tn, kb0, kb1; bool skip, second; };
+template <int BN, int EPI>
+__device__ __forceinline__ GemmUnit gm_unit(const GemmParamsOf<EPI>& p, long long u, int tiles_per_problem) {
+    GemmUnit w;
+    w.second = false;
+    if constexpr (EPI == GM_EPI_DUAL) {
+        w.second = u >= tiles_per_problem;
+        const int t = (int)(w.second ? u - tiles_per_problem : u), tiles_n = w.second ? p.second.tiles_n : p.tiles_n;
+        w.sp = w.bi = w.bo = w.kb0 = 0;
+        w.tm = t / tiles_n;
+        w.tn = t - w.tm * tiles_n;
+        w.kb1 = w.second ? p.second.kblocks : p.kblocks;
+        w.skip = false;
+    } else {
+        w.sp = (int)(u % p.splits);
+        const int tile = (int)(u / p.splits);
+        const int b = tile / tiles_per_problem, t = gm_rotate(p, tile - b * tiles_per_problem, b, tiles_per_problem);
+        w.tm = t / p.tiles_n;
+        w.tn = t - w.tm * p.tiles_n;
+        w.bi = b % p.nb_inner;
+        w.bo = b / p.nb_inner;
+        w.skip = gm_tile_skipped<BN>(p, w.tm, w.tn);
+        gm_kb_range(p, w.sp, w.tm, w.kb0, w.kb1);
+    }
+    return w;
+}
+
 #include "gemm_epilogue.cuh"
 
 template <int BN, int CG, int EPI>
-__global__ void __launch_bounds__(GM_THREADS, 1) gemm_bf16_kernel(const __grid_constant__ GemmParams p) {
-    using C = GemmCfg<BN, CG>;
+__global__ void __launch_bounds__(gm_threads(EPI), 1) gemm_bf16_kernel(const __grid_constant__ GemmParamsOf<EPI> p) {
+    using C = GemmCfg<BN, CG, EPI>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     uint8_t* epi_smem = smem + C::STAGES * C::STAGE_BYTES;
@@ -135,8 +182,10 @@ __global__ void __launch_bounds__(GM_THREADS, 1) gemm_bf16_kernel(const __grid_c
         }
         for (int a = 0; a < 2; a++) {
             mbar_init(&ctl->acc_full[a], 1);
-            mbar_init(&ctl->acc_empty[a], 4 * CG);   // the epilogue warps of both CTAs
+            mbar_init(&ctl->acc_empty[a], gm_epi_warps(EPI) * CG);   // the epilogue warps of both CTAs
         }
+        if (EPI == GM_EPI_ACT)
+            for (int i = 0; i < 32; i++) mbar_init(&ctl->res_full[i >> 1][i & 1], 1);
         ctl->abort_flag = 0;
         fence_barrier_init();
     }
@@ -163,7 +212,8 @@ __global__ void __launch_bounds__(GM_THREADS, 1) gemm_bf16_kernel(const __grid_c
     const uint32_t tmem_base = ctl->tmem_base;
     volatile int* abort_flag = &ctl->abort_flag;
     const int tiles_per_problem = p.tiles_m * p.tiles_n;
-    const long long units = (long long)p.batch * tiles_per_problem * p.splits;
+    long long units = (long long)p.batch * tiles_per_problem * p.splits;
+    if constexpr (EPI == GM_EPI_DUAL) units += p.second.tiles_m * p.second.tiles_n;
 
     if (warp == 0) {
         // ------------------------------------------------------------ TMA producer (the warp as one, see elect_one)
@@ -171,16 +221,14 @@ __global__ void __launch_bounds__(GM_THREADS, 1) gemm_bf16_kernel(const __grid_c
         uint32_t ph = 0;
         bool dead = false;
         for (long long u = blockIdx.x / CG; u < units && !dead; u += gridDim.x / CG) {
-            const int sp = (int)(u % p.splits);
-            const int tile = (int)(u / p.splits);
-            const int b = tile / tiles_per_problem, t = gm_rotate(p, tile - b * tiles_per_problem, b, tiles_per_problem);
-            const int tm = t / p.tiles_n, tn = t - tm * p.tiles_n;
-            const int bi = b % p.nb_inner, bo = b / p.nb_inner;
-            if (gm_tile_skipped<BN>(p, tm, tn)) continue;
-            int kb0, kb1;
-            gm_kb_range(p, sp, tm, kb0, kb1);
-            const int m0 = (tm * CG + (int)rank) * GM_BM, nb0 = tn * BN + (int)rank * (BN / CG);
-            for (int kb = kb0; kb < kb1; kb++) {
+            const GemmUnit w = gm_unit<BN, EPI>(p, u, tiles_per_problem);
+            if (w.skip) continue;
+            const int m0 = (w.tm * CG + (int)rank) * GM_BM, nb0 = w.tn * BN + (int)rank * (BN / CG);
+            const unsigned char *map_a = p.tmap_a, *map_b = p.tmap_b;
+            int a_mn = p.a_mn, b_mn = p.b_mn;
+            if constexpr (EPI == GM_EPI_DUAL)
+                if (w.second) { map_a = p.second.tmap_a; map_b = p.second.tmap_b; a_mn = p.second.a_mn; b_mn = p.second.b_mn; }
+            for (int kb = w.kb0; kb < w.kb1; kb++) {
                 if (!mbar_wait_warp(&ctl->empty[s], ph ^ 1u, abort_flag)) {
                     if (!*abort_flag) { ctl->abort_flag = 1; if (p.status) atomicExch(p.status, OB200_ERR_WAIT_EMPTY); }
                     dead = true;
@@ -193,20 +241,20 @@ __global__ void __launch_bounds__(GM_THREADS, 1) gemm_bf16_kernel(const __grid_c
                     if (rank == 0) mbar_arrive_expect_tx(&ctl->full[s], (uint32_t)(CG * C::STAGE_BYTES));
                     const uint32_t bar = CG == 2 ? cluster_addr(smem_u32(&ctl->full[s]), 0) : 0;
                     auto load = [&](uint32_t dst, const void* map, int c0, int c1) {
-                        if (CG == 2) tma_load_tile_4d_pair(dst, map, bar, c0, c1, bi, bo);
-                        else tma_load_tile_4d(dst, map, &ctl->full[s], c0, c1, bi, bo);
+                        if (CG == 2) tma_load_tile_4d_pair(dst, map, bar, c0, c1, w.bi, w.bo);
+                        else tma_load_tile_4d(dst, map, &ctl->full[s], c0, c1, w.bi, w.bo);
                     };
-                    if (!p.a_mn) {
-                        load(a_dst, p.tmap_a, kb * GM_BK, m0);
+                    if (!a_mn) {
+                        load(a_dst, map_a, kb * GM_BK, m0);
                     } else {
 #pragma unroll
-                        for (int g = 0; g < GM_BM / 64; g++) load(a_dst + g * 8192, p.tmap_a, m0 + 64 * g, kb * GM_BK);
+                        for (int g = 0; g < GM_BM / 64; g++) load(a_dst + g * 8192, map_a, m0 + 64 * g, kb * GM_BK);
                     }
-                    if (!p.b_mn) {
-                        load(b_dst, p.tmap_b, kb * GM_BK, nb0);
+                    if (!b_mn) {
+                        load(b_dst, map_b, kb * GM_BK, nb0);
                     } else {
 #pragma unroll
-                        for (int g = 0; g < BN / CG / 64; g++) load(b_dst + g * 8192, p.tmap_b, nb0 + 64 * g, kb * GM_BK);
+                        for (int g = 0; g < BN / CG / 64; g++) load(b_dst + g * 8192, map_b, nb0 + 64 * g, kb * GM_BK);
                     }
                 }
                 __syncwarp();
@@ -222,23 +270,21 @@ __global__ void __launch_bounds__(GM_THREADS, 1) gemm_bf16_kernel(const __grid_c
     } else if (warp == 1) {
         // ------------------------------------------------------------ MMA issue (the warp as one)
         if (rank == 0) {
-            const uint32_t idesc = umma_idesc(1, CG * GM_BM, BN) | (p.a_mn ? UMMA_IDESC_A_MN : 0u) | (p.b_mn ? UMMA_IDESC_B_MN : 0u);
-            // descriptors above the address; 16 reduction indices further on: 32 bytes along a K-major row, two 8-row atoms of
-            // an MN-major tile
-            const uint64_t a_bits = p.a_mn ? gm_desc_mn(0) : umma_desc_sw128(0), b_bits = p.b_mn ? gm_desc_mn(0) : umma_desc_sw128(0);
-            const uint64_t a_step = p.a_mn ? 2048 >> 4 : 2, b_step = p.b_mn ? 2048 >> 4 : 2;
             int s = 0;
             uint32_t ph = 0;
             uint32_t local = 0;
             bool dead = false;
             for (long long u = blockIdx.x / CG; u < units && !dead; u += gridDim.x / CG) {
-                const int sp = (int)(u % p.splits);
-                const int tile = (int)(u / p.splits);
-                const int t = gm_rotate(p, tile % tiles_per_problem, tile / tiles_per_problem, tiles_per_problem);
-                const int tm = t / p.tiles_n, tn = t - tm * p.tiles_n;
-                if (gm_tile_skipped<BN>(p, tm, tn)) continue;
-                int kb0, kb1;
-                gm_kb_range(p, sp, tm, kb0, kb1);
+                const GemmUnit w = gm_unit<BN, EPI>(p, u, tiles_per_problem);
+                if (w.skip) continue;
+                int a_mn = p.a_mn, b_mn = p.b_mn;
+                if constexpr (EPI == GM_EPI_DUAL)
+                    if (w.second) { a_mn = p.second.a_mn; b_mn = p.second.b_mn; }
+                const uint32_t idesc = umma_idesc(1, CG * GM_BM, BN) | (a_mn ? UMMA_IDESC_A_MN : 0u) | (b_mn ? UMMA_IDESC_B_MN : 0u);
+                // descriptors above the address; 16 reduction indices further on: 32 bytes along a K-major row, two 8-row atoms of
+                // an MN-major tile
+                const uint64_t a_bits = a_mn ? gm_desc_mn(0) : umma_desc_sw128(0), b_bits = b_mn ? gm_desc_mn(0) : umma_desc_sw128(0);
+                const uint64_t a_step = a_mn ? 2048 >> 4 : 2, b_step = b_mn ? 2048 >> 4 : 2;
                 const uint32_t ab = local & 1u, use = local >> 1;
                 local++;
                 if (!mbar_wait_warp(&ctl->acc_empty[ab], (use & 1u) ^ 1u, abort_flag)) {
@@ -247,14 +293,14 @@ __global__ void __launch_bounds__(GM_THREADS, 1) gemm_bf16_kernel(const __grid_c
                 }
                 tc_fence_after_sync();
                 const uint32_t d = tmem_base + ab * BN;
-                for (int kb = kb0; kb < kb1; kb++) {
+                for (int kb = w.kb0; kb < w.kb1; kb++) {
                     if (!mbar_wait_warp(&ctl->full[s], ph, abort_flag)) {
                         if (!*abort_flag) { ctl->abort_flag = 1; if (p.status) atomicExch(p.status, OB200_ERR_WAIT_FULL); }
                         dead = true;
                         break;
                     }
                     tc_fence_after_sync();
-                    const uint32_t first = kb > kb0 ? 1u : 0u;   // 0: the tile's first product overwrites the accumulator
+                    const uint32_t first = kb > w.kb0 ? 1u : 0u;   // 0: the tile's first product overwrites the accumulator
                     if (elect_one()) {
                         const uint32_t a_base = smem_u32(smem + s * C::STAGE_BYTES);
                         const uint64_t ad = umma_desc_mn(a_bits, a_base), bd = umma_desc_mn(b_bits, a_base + GM_A_BYTES);
@@ -265,7 +311,7 @@ __global__ void __launch_bounds__(GM_THREADS, 1) gemm_bf16_kernel(const __grid_c
                         }
                         if (CG == 2) umma_commit_pair(&ctl->empty[s]);
                         else umma_commit(&ctl->empty[s]);
-                        if (kb + 1 == kb1) {
+                        if (kb + 1 == w.kb1) {
                             if (CG == 2) umma_commit_pair(&ctl->acc_full[ab]);
                             else umma_commit(&ctl->acc_full[ab]);
                         }
@@ -279,36 +325,49 @@ __global__ void __launch_bounds__(GM_THREADS, 1) gemm_bf16_kernel(const __grid_c
     } else {
         // ------------------------------------------------------------ epilogue: thread = output row
         const int q = warp & 3;                       // tensor-memory lane group this warp may read
-        const int r = q * 32 + lane;
         uint32_t local = 0;
         uint32_t slab_i = 0;
         for (long long u = blockIdx.x / CG; u < units; u += gridDim.x / CG) {
-            const int sp = (int)(u % p.splits);
-            const int tile = (int)(u / p.splits);
-            const int b = tile / tiles_per_problem, t = gm_rotate(p, tile - b * tiles_per_problem, b, tiles_per_problem);
-            const int tm = t / p.tiles_n, tn = t - tm * p.tiles_n;
-            const int bi = b % p.nb_inner, bo = b / p.nb_inner;
-            if (gm_tile_skipped<BN>(p, tm, tn)) continue;
+            const GemmUnit w = gm_unit<BN, EPI>(p, u, tiles_per_problem);
+            const int sp = w.sp, tm = w.tm, tn = w.tn, bi = w.bi, bo = w.bo;
+            if (w.skip) continue;
             const uint32_t ab = local & 1u, use = local >> 1;
             local++;
+            constexpr int kCols = BN * 4 / gm_epi_warps(EPI) < 32 ? 32 : BN * 4 / gm_epi_warps(EPI);   // columns of a tile that a warp takes
+            const int part = (warp - 2) >> 2;
+            const bool idle = part * kCols >= BN;   // a narrow tile has no columns for this warp
+            const int m0w = (tm * CG + (int)rank) * GM_BM + q * 32;      // first row of this warp's 32
+            bool ahead = false;
+            if constexpr (EPI == GM_EPI_ACT) if (!idle) ahead = gm_residual_ahead<kCols>(p, m0w, tn * BN + part * kCols, epi_smem + (warp - 2) * 4096, slab_i, ctl->res_full[warp - 2]);
             if (!mbar_wait_warp(&ctl->acc_full[ab], use & 1u, abort_flag)) {
                 if (!*abort_flag) { ctl->abort_flag = 1; if (p.status) atomicExch(p.status, OB200_ERR_WAIT_TMEM_FULL); }
+                if (ahead) {   // the residual's copy must have landed before the CTA leaves
+                    const uint32_t s = p.e.pre ? 0 : slab_i & 1;
+                    mbar_wait_landed(&ctl->res_full[warp - 2][s], p.e.pre ? slab_i & 1 : (slab_i >> 1) & 1, clock64());
+                }
                 break;
             }
             tc_fence_after_sync();
-            const int m = (tm * CG + (int)rank) * GM_BM + r;
+            const int m = m0w + lane;
             const int n0 = tn * BN;
             const uint32_t t_row = tmem_base + ((uint32_t)(q * 32) << 16) + ab * BN;
-            if constexpr (EPI == GM_EPI_ACT) gm_epilogue_act<BN>(p, t_row, m, (tm * CG + (int)rank) * GM_BM + q * 32, n0, sp, lane, epi_smem + (warp - 2) * 8192, slab_i);
+            if (idle) {
+            } else if constexpr (EPI == GM_EPI_ACT || EPI == GM_EPI_ACT_ANY) {
+                if (p.splits > 1) gm_epilogue_slab<kCols>(p, t_row + part * kCols, m, n0 + part * kCols, sp);
+                else if constexpr (EPI == GM_EPI_ACT_ANY) gm_epilogue_act_any<kCols>(p, t_row + part * kCols, m, m0w, n0 + part * kCols, lane, epi_smem + (warp - 2) * 4096);
+                else if (!gm_epilogue_act<kCols>(p, t_row + part * kCols, m, m0w, n0 + part * kCols, lane, epi_smem + (warp - 2) * 4096, slab_i, ctl->res_full[warp - 2], abort_flag)) {
+                    if (!*abort_flag) { ctl->abort_flag = 1; if (p.status) atomicExch(p.status, OB200_ERR_WAIT_FULL); }
+                    break;
+                }
+            } else if constexpr (EPI == GM_EPI_DUAL) gm_epilogue_dual<BN>(p, w.second, t_row, m, m0w, n0, lane, epi_smem + (warp - 2) * 8192, slab_i);
             else if constexpr (EPI == GM_EPI_LSE) gm_epilogue_lse<BN>(p, t_row, m, n0);
-            else if constexpr (EPI == GM_EPI_DLOGITS) gm_epilogue_dlogits<BN>(p, t_row, m, (tm * CG + (int)rank) * GM_BM + q * 32, n0, lane, epi_smem + (warp - 2) * 8192, slab_i);
+            else if constexpr (EPI == GM_EPI_DLOGITS) gm_epilogue_dlogits<kCols>(p, t_row + part * kCols, m, m0w, n0 + part * kCols, lane, epi_smem + (warp - 2) * 4096, slab_i);
             else {
             const bool to_slab = p.splits > 1;
             const bool row_ok = m < p.M;
-            float* srow = to_slab ? p.slabs + (((long long)sp * p.batch + b) * p.M + m) * p.N : nullptr;
+            float* srow = to_slab ? p.slabs + (((long long)sp * p.batch + bo * p.nb_inner + bi) * p.M + m) * p.N : nullptr;
             const long long c_off = (long long)bo * p.c_so + (long long)bi * p.c_si + (long long)m * p.ldc;
             const bool by_tma = p.c_tma && !to_slab;
-            const int m0w = (tm * CG + (int)rank) * GM_BM + q * 32;      // first row of this warp's 32
 #pragma unroll 1
             for (int c0 = 0; c0 < BN; c0 += 32) {
                 if (n0 + c0 >= p.N) break;            // warp-uniform
@@ -454,7 +513,7 @@ __global__ void __launch_bounds__(GM_THREADS, 1) gemm_bf16_kernel(const __grid_c
                 else mbar_arrive(&ctl->acc_empty[ab]);
             }
         }
-        if (lane == 0) bulk_wait_group<0>();   // the slabs must outlive the stores that read them
+        bulk_wait_group<0>();   // the slabs must outlive the stores that read them
     }
     tc_fence_before_sync();
     __syncthreads();
@@ -531,7 +590,7 @@ __global__ void __launch_bounds__(256) gemm_splitk_act_kernel(const float* __res
                 if (bias) a += bias[col];
                 if (bias_bf16) a += __bfloat162float(bias_bf16[col]);
                 if (e.pre) e.pre[m * e.ld_pre + col] = __float2bfloat16_rn(a);
-                a = gm_activate(a, e.act);
+                a = e.act == 2 ? a * gauss_cdf(a) : e.act == 1 ? fmaxf(a, 0.f) : a;
                 if (e.drop_threshold) a = mask >> j & 1u ? a * e.drop_scale : 0.f;
                 if (residual) a += __bfloat162float(residual[i0 + j]);
                 f[j] = a;
@@ -580,8 +639,8 @@ static bool gm_make_map(unsigned char* out, const void* base, long long inner, l
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// Tensor map of a bfloat16 output [M, N] that is stored 32 rows x 32 columns at a time (64-byte rows, swizzled).
-static bool gm_make_store_map(unsigned char* out, const void* base, int M, int N, long long ld) {
+// Tensor map of a bfloat16 matrix [M, N] that is copied 32 rows x 32 columns at a time (64-byte rows, swizzled).
+static bool gm_make_slab_map(unsigned char* out, const void* base, int M, int N, long long ld) {
     GmEncodeTiledFn enc = gm_encode_fn();
     if (!enc) return false;
     cuuint64_t dims[2] = {(cuuint64_t)N, (cuuint64_t)M};
@@ -658,12 +717,12 @@ static GemmPlan gm_plan(int M, int N, int K, long long batch, int tri, int devic
 }
 
 template <int BN, int CG, int EPI>
-static int gm_launch(const GemmParams& p, int grid, cudaStream_t stream) {
+static int gm_launch(const GemmParamsOf<EPI>& p, int grid, cudaStream_t stream) {
     static bool attr_set[64] = {};
     int dev = 0;
     cudaGetDevice(&dev);
     if (dev < 64 && !attr_set[dev]) {
-        cudaError_t e = cudaFuncSetAttribute(gemm_bf16_kernel<BN, CG, EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, GemmCfg<BN, CG>::SMEM);
+        cudaError_t e = cudaFuncSetAttribute(gemm_bf16_kernel<BN, CG, EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, (GemmCfg<BN, CG, EPI>::SMEM));
         if (e != cudaSuccess) return (int)e;
         attr_set[dev] = true;
     }
@@ -677,8 +736,8 @@ static int gm_launch(const GemmParams& p, int grid, cudaStream_t stream) {
     cudaLaunchConfig_t cfg;
     memset(&cfg, 0, sizeof cfg);
     cfg.gridDim = dim3((unsigned)grid);
-    cfg.blockDim = dim3(GM_THREADS);
-    cfg.dynamicSmemBytes = GemmCfg<BN, CG>::SMEM;
+    cfg.blockDim = dim3(gm_threads(EPI));
+    cfg.dynamicSmemBytes = (GemmCfg<BN, CG, EPI>::SMEM);
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
     int n = 0;
@@ -728,14 +787,15 @@ template <int EPI>
 static int gm_launch_tile(const GemmParams& p, int bn, int cg, int grid, cudaStream_t st) {
     if (cg == 2) return bn == 256 ? gm_launch<256, 2, EPI>(p, grid, st) : gm_launch<128, 2, EPI>(p, grid, st);
     if (bn == 256) return gm_launch<256, 1, EPI>(p, grid, st);
-    if constexpr (EPI == GM_EPI_PLAIN || EPI == GM_EPI_ACC || EPI == GM_EPI_ACT)
+    if constexpr (EPI != GM_EPI_LSE && EPI != GM_EPI_DLOGITS)
         if (bn == 64) return gm_launch<64, 1, EPI>(p, grid, st);
     return gm_launch<128, 1, EPI>(p, grid, st);
 }
 
 int gemm_bf16_run(const GemmCall& g) {
     const int M = g.M, N = g.N, K = g.K, a_mn = g.a_mn, b_mn = g.b_mn, batch_inner = g.batch_inner, batch_outer = g.batch_outer;
-    const int out_f32 = g.out_f32, tri = g.tri, num_ctas = g.num_ctas, epi = g.epi;
+    const int out_f32 = g.out_f32, tri = g.tri, num_ctas = g.num_ctas;
+    int epi = g.epi;
     const long long lda = g.lda, ldb = g.ldb, ldc = g.ldc, c_si = g.c_si, c_so = g.c_so;
     const void *a = g.a, *b = g.b, *residual = g.residual;
     void* c = g.c;
@@ -794,10 +854,12 @@ int gemm_bf16_run(const GemmCall& g) {
         const bool aligned = ((uintptr_t)c % 16 == 0) && (ldc * es) % 16 == 0 && (batch_inner == 1 || (c_si * es) % 16 == 0) &&
                              (batch_outer == 1 || (c_so * es) % 16 == 0);
         static const bool tma_off = [] { const char* e = getenv("ORION_GEMM_TMA_STORE"); return e && e[0] == '0'; }();
-        if (epi == GM_EPI_ACT || epi == GM_EPI_DLOGITS) {   // 32 rows x 32 columns a store
-            if (aligned && p.splits == 1) p.c_tma = gm_make_store_map(p.tmap_c, c, M, N, ldc) ? 1 : 0;
-            if (epi == GM_EPI_DLOGITS && !p.c_tma) return -4;
-            if (g.e.pre && p.splits == 1 && !gm_make_store_map(p.tmap_pre, g.e.pre, M, N, g.e.ld_pre)) return -4;
+        if (epi == GM_EPI_ACT || epi == GM_EPI_DLOGITS) {   // 32 rows x 32 columns a copy
+            if (epi == GM_EPI_ACT && (!aligned || g.bias || ((uintptr_t)g.bias_bf16 | (uintptr_t)residual) % 16)) epi = GM_EPI_ACT_ANY;
+            if (p.splits == 1 && ((epi != GM_EPI_ACT_ANY && !gm_make_slab_map(p.tmap_c, c, M, N, ldc)) ||
+                                  (epi == GM_EPI_ACT && residual && !gm_make_slab_map(p.tmap_res, residual, M, N, N)) ||
+                                  (g.e.pre && !gm_make_slab_map(p.tmap_pre, g.e.pre, M, N, g.e.ld_pre))))
+                return -4;
         } else if (epi != GM_EPI_LSE && aligned && !tma_off && p.splits == 1) {
             GmEncodeTiledFn enc = gm_encode_fn();
             const long long si = batch_inner > 1 ? c_si : ldc * M, so = batch_outer > 1 ? c_so : si * (batch_inner > 1 ? batch_inner : 1);
@@ -831,13 +893,14 @@ int gemm_bf16_run(const GemmCall& g) {
     switch (epi) {
         case GM_EPI_ACC: rc = gm_launch_tile<GM_EPI_ACC>(p, bn, cg, grid, st); break;
         case GM_EPI_ACT: rc = gm_launch_tile<GM_EPI_ACT>(p, bn, cg, grid, st); break;
+        case GM_EPI_ACT_ANY: rc = gm_launch_tile<GM_EPI_ACT_ANY>(p, bn, cg, grid, st); break;
         case GM_EPI_LSE: return gm_launch_tile<GM_EPI_LSE>(p, bn, cg, grid, st);
         case GM_EPI_DLOGITS: return gm_launch_tile<GM_EPI_DLOGITS>(p, bn, cg, grid, st);
         default: rc = gm_launch_tile<GM_EPI_PLAIN>(p, bn, cg, grid, st);
     }
     if (rc != 0 || p.splits == 1) return rc;
     const long long elems = batch_ll * M * N;
-    if (epi == GM_EPI_ACT) {
+    if (epi == GM_EPI_ACT || epi == GM_EPI_ACT_ANY) {
         long long blocks = ((elems + 7) / 8 + 255) / 256;
         if (blocks > 8LL * num_ctas) blocks = 8LL * num_ctas;
         OB200_ELASTIC_HBM(gemm_splitk_act_kernel, 8);
@@ -850,6 +913,59 @@ int gemm_bf16_run(const GemmCall& g) {
     gemm_splitk_finish_kernel<<<(int)blocks, 256, 0, st>>>(p.slabs, c, g.bias, p.bias_bf16, p.residual, epi == GM_EPI_ACC ? p.e.addend : nullptr, p.splits, p.batch,
                                                            p.nb_inner, M, N, ldc, c_si, c_so, p.out_f32, g.alpha);
     return (int)cudaGetLastError();
+}
+
+// Bfloat16 output, or float32 with its addend: 128 bytes x 32 rows a store.
+static bool gm_make_c_map(unsigned char* out, const GemmCall& g) {
+    GmEncodeTiledFn enc = gm_encode_fn();
+    const int es = g.out_f32 ? 4 : 2;
+    cuuint64_t dims[2] = {(cuuint64_t)g.N, (cuuint64_t)g.M};
+    cuuint64_t strides[1] = {(cuuint64_t)g.ldc * es};
+    cuuint32_t box[2] = {(cuuint32_t)(128 / es), 32}, steps[2] = {1, 1};
+    return enc && enc(reinterpret_cast<CUtensorMap*>(out), g.out_f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2,
+                      g.c, dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+bool gemm_bf16_dual_fits(const GemmCall& a, const GemmCall& b) {
+    for (const GemmCall* g : {&a, &b})
+        if (g->M <= GM_BM || g->N < 256 || g->N % 8 || gemm_bf16_slab_bytes(g->M, g->N, g->K) > 0) return false;
+    return a.num_ctas >= 2;
+}
+
+int gemm_bf16_run_dual(const GemmCall& a, const GemmCall& b) {
+    GemmParamsDual p;
+    memset(&p, 0, sizeof p);
+    p.status = ob200_status_word_for_current_device();
+    p.M = a.M; p.N = a.N; p.K = a.K;
+    p.batch = p.nb_inner = p.splits = 1;
+    p.out_f32 = a.out_f32 ? 1 : 0;
+    p.a_mn = a.a_mn; p.b_mn = a.b_mn;
+    p.alpha = 1.0f;
+    p.e = a.e;
+    p.kblocks = (a.K + GM_BK - 1) / GM_BK;
+    p.kb_per_split = p.kblocks;
+    p.tiles_m = (a.M + 2 * GM_BM - 1) / (2 * GM_BM);
+    p.tiles_n = (a.N + 255) / 256;
+    p.second.M = b.M; p.second.N = b.N;
+    p.second.out_f32 = b.out_f32 ? 1 : 0;
+    p.second.a_mn = b.a_mn; p.second.b_mn = b.b_mn;
+    p.second.kblocks = (b.K + GM_BK - 1) / GM_BK;
+    p.second.tiles_m = (b.M + 2 * GM_BM - 1) / (2 * GM_BM);
+    p.second.tiles_n = (b.N + 255) / 256;
+    auto operands = [](const GemmCall& g, unsigned char* ta, unsigned char* tb) {
+        return (g.a_mn ? gm_make_map(ta, g.a, g.M, g.K, g.lda, 1, 0, 1, 0, 64, GM_BK) : gm_make_map(ta, g.a, g.K, g.M, g.lda, 1, 0, 1, 0, GM_BK, GM_BM)) &&
+               (g.b_mn ? gm_make_map(tb, g.b, g.N, g.K, g.ldb, 1, 0, 1, 0, 64, GM_BK) : gm_make_map(tb, g.b, g.K, g.N, g.ldb, 1, 0, 1, 0, GM_BK, 128));
+    };
+    if (!operands(a, p.tmap_a, p.tmap_b) || !operands(b, p.second.tmap_a, p.second.tmap_b) || !gm_make_c_map(p.tmap_c, a) ||
+        !gm_make_c_map(p.second.tmap_c, b))
+        return -4;
+    p.c_tma = 1;
+    const long long tiles = (long long)p.tiles_m * p.tiles_n + (long long)p.second.tiles_m * p.second.tiles_n;
+    if (tiles > 0x3fffffffLL) return -1;
+    const long long most = a.num_ctas / 2;
+    annotate_launch(1, 2.0 * ((double)a.M * a.N * a.K + (double)b.M * b.N * b.K), 2.0 * ((double)a.M * a.K + (double)a.K * a.N + (double)b.M * b.K + (double)b.K * b.N));
+    return gm_launch<256, 2, GM_EPI_DUAL>(p, (int)(tiles < most ? tiles : most) * 2, (cudaStream_t)a.stream);
 }
 
 }  // namespace ob200

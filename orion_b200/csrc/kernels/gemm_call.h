@@ -11,8 +11,10 @@ enum : int {
     GM_EPI_PLAIN = 0,    // C = alpha * A.B^T (+ bias) (+ bfloat16 residual)
     GM_EPI_ACC = 1,      // the same plus a float32 addend (which may be C itself)
     GM_EPI_ACT = 2,      // C = residual + dropout(act(A.B^T + bias)), optionally A.B^T + bias beside it
-    GM_EPI_LSE = 3,      // no C: per row and 128 columns the maximum and the sum of exponentials, and the label's column
-    GM_EPI_DLOGITS = 4,  // C = (exp(A.B^T - lse) - onehot(label)) * coefficient
+    GM_EPI_ACT_ANY = 3,  // GM_EPI_ACT for widths, types and alignments that its vector accesses do not take (chosen by the launcher)
+    GM_EPI_LSE = 4,      // no C: per row and 128 columns the maximum and the sum of exponentials, and the label's column
+    GM_EPI_DLOGITS = 5,  // C = (exp(A.B^T - lse) - onehot(label)) * coefficient
+    GM_EPI_DUAL = 6,     // two products of one launch, each plain (the first one with GM_EPI_ACC's addend)
 };
 
 struct GemmEpi {
@@ -58,6 +60,10 @@ struct GemmCall {
 
 // 0, a cudaError_t, -1 (sizes), -2 (alignment), -4 (no TMA descriptor).
 int gemm_bf16_run(const GemmCall& call);
+// Two products in one launch of CTA pairs, so that the last round of tiles is one and not two: no batch, bias, residual or alpha; rows
+// of C 16-byte multiples.  `fits`: both are wide enough for 256 x 256 tiles and neither wants its reduction split.
+bool gemm_bf16_dual_fits(const GemmCall& first, const GemmCall& second);
+int gemm_bf16_run_dual(const GemmCall& first, const GemmCall& second);
 // Bytes of partial matrices that the split of such a product (plain or with GM_EPI_ACT) wants; 0 where it is not split.
 size_t gemm_bf16_slab_bytes(int M, int N, int K);
 

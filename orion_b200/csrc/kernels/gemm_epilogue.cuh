@@ -1,13 +1,12 @@
 // Epilogues of the bfloat16 GEMM (included by gemm_bf16.cu, inside its namespace): what a warp does with its 32 rows of a finished
 // tile in tensor memory, thread = row, 32 columns at a time.  Arithmetic is float32; an output is rounded to bfloat16 once, staged in
-// a swizzled slab of 32 rows x 64 bytes and written by a TMA store.  A warp has 8 KB of shared memory: two turns of two slabs (the
-// output, and the pre-activation beside it), so that a slab is filled while the stores of the turn before read theirs.
+// a swizzled slab of 32 rows x 64 bytes and written by a TMA store.  A warp has two such slabs: its turns alternate between them, or
+// the pre-activation has the second one and a turn waits until the stores of the turn before have read theirs.
 
 __device__ __forceinline__ uint32_t gm_pack(float a, float b) {
     const __nv_bfloat162 h2 = __floats2bfloat162_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&h2);
 }
-__device__ __forceinline__ float gm_activate(float a, int act) { return act == 2 ? a * gauss_cdf(a) : act == 1 ? fmaxf(a, 0.f) : a; }
 
 // 32 bfloat16 values of this thread's row into a slab of 64-byte rows, 64-byte swizzle (16-byte chunk index XOR (row / 2) % 4: eight
 // consecutive rows of one chunk fall into eight different bank groups).
@@ -23,6 +22,16 @@ __device__ __forceinline__ void gm_stage32(uint8_t* slab, int lane, const float 
     }
 }
 
+// f += eight bfloat16 values (the upper halves of float32 ones).
+__device__ __forceinline__ void gm_add8(float* f, uint4 v) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+        split_f32x2(add_f32x2(f32x2(f[e * 2], f[e * 2 + 1]), f32x2(__uint_as_float(w[e] << 16), __uint_as_float(w[e] & 0xFFFF0000u))), f[e * 2],
+                    f[e * 2 + 1]);
+}
+
+// (Never issued ahead of its wait: the compiler takes the registers for filled and may move them.)
 __device__ __forceinline__ void gm_load32(uint32_t t_addr, float (&f)[32]) {
     uint32_t v[32];
     tmem_ld_32x32(t_addr, v);
@@ -31,102 +40,169 @@ __device__ __forceinline__ void gm_load32(uint32_t t_addr, float (&f)[32]) {
     for (int j = 0; j < 32; j++) f[j] = __uint_as_float(v[j]);
 }
 
-// C = residual + dropout(act(A.B^T + bias)); the split-K partial matrices of such a product are written as they are.
-template <int BN>
-__device__ __forceinline__ void gm_epilogue_act(const GemmParams& p, uint32_t t_row, int m, int m0w, int n0, int sp, int lane, uint8_t* stage,
-                                                uint32_t& turn) {
-    const bool row_ok = m < p.M;
-    const bool aligned = p.c_tma;   // rows of C are 16-byte multiples: N is a multiple of 8
-    DropKey key = {};
-    if (p.e.drop_threshold && p.splits == 1) key = drop_key(p.e.rng, p.e.site);
+// Partial matrices of a product with split-K, as they are: the rest is gemm_splitk_act_kernel's.
+template <int COLS>
+__device__ __forceinline__ void gm_epilogue_slab(const GemmParams& p, uint32_t t_row, int m, int n0, int sp) {
 #pragma unroll 1
-    for (int c0 = 0; c0 < BN; c0 += 32) {
+    for (int c0 = 0; c0 < COLS; c0 += 32) {
+        const int n = n0 + c0;
+        if (n >= p.N) break;            // warp-uniform
+        uint32_t v[32];
+        tmem_ld_32x32(t_row + c0, v);
+        tmem_ld_wait();
+        if (m >= p.M) continue;
+        float* srow = p.slabs + ((long long)sp * p.M + m) * p.N + n;
+        if (n + 32 <= p.N && (p.N & 3) == 0) {
+#pragma unroll
+            for (int j = 0; j < 32; j += 4) *reinterpret_cast<uint4*>(srow + j) = make_uint4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 32; j++)
+                if (n + j < p.N) srow[j] = __uint_as_float(v[j]);
+        }
+    }
+}
+
+// C = residual + dropout(act(A.B^T + bias)): N a multiple of 8, all pointers 16-byte aligned, the bias bfloat16.
+//
+// What bounds it is latency (a warp's turn is a chain: tensor memory, arithmetic, slab, fence, store), so a turn has little in it beside
+// the arithmetic: no path for ragged widths, and the residual
+// brought into the slab that the output will leave from by a TMA load one turn ahead (read by the threads, each a row, it took 25 us of
+// 8192 x 4096; so 13).  The residual of the first turn is asked for before the accumulator is waited for (gm_residual_ahead).
+template <int COLS>
+__device__ __forceinline__ bool gm_residual_ahead(const GemmParams& p, int m0w, int n0, uint8_t* stage, uint32_t turn, uint64_t* bars) {
+    if (!p.residual || p.splits > 1 || n0 >= p.N) return false;
+    if (elect_one()) {
+        if (p.e.pre) bulk_wait_group_read<0>();
+        else bulk_wait_group_read<1>();
+        const uint32_t s = p.e.pre ? 0 : turn & 1;
+        mbar_arrive_expect_tx(&bars[s], 2048);
+        tma_load_tile_2d(smem_u32(stage + s * 2048), p.tmap_res, &bars[s], n0, m0w);
+    }
+    __syncwarp();
+    return true;
+}
+template <int COLS>
+__device__ __forceinline__ bool gm_epilogue_act(const GemmParams& p, uint32_t t_row, int m, int m0w, int n0, int lane, uint8_t* stage, uint32_t& turn,
+                                                uint64_t* bars, volatile int* abort_flag) {
+    if (n0 >= p.N) return true;
+    const bool has_pre = p.e.pre != nullptr, has_res = p.residual != nullptr;
+    const int cols = p.N - n0 < COLS ? p.N - n0 : COLS, act = p.e.act;
+    const uint32_t threshold = p.e.drop_threshold;
+    DropKey key = {};
+    if (threshold) key = drop_key(p.e.rng, p.e.site);
+    unsigned long long group = ((unsigned long long)m * p.N + n0) >> 3;
+    const __nv_bfloat16* bias = p.bias_bf16 ? p.bias_bf16 + n0 : nullptr;
+#pragma unroll 1
+    for (int c0 = 0; c0 < cols; c0 += 32) {
+        uint4 b[4];
+        if (bias) {
+#pragma unroll
+            for (int ch = 0; ch < 4; ch++)
+                if (c0 + ch * 8 < cols) b[ch] = __ldg(reinterpret_cast<const uint4*>(bias + c0 + ch * 8));
+        }
+        float f[32];
+        gm_load32(t_row + c0, f);
+        if (bias) {
+#pragma unroll
+            for (int ch = 0; ch < 4; ch++) gm_add8(f + ch * 8, b[ch]);
+        }
+        uint8_t* slab = has_pre ? stage : stage + (turn & 1) * 2048;
+        if (has_pre) {
+            if (elect_one()) bulk_wait_group_read<0>();
+            __syncwarp();
+            gm_stage32(stage + 2048, lane, f);
+        }
+        if (act == 2) {
+#pragma unroll
+            for (int j = 0; j < 32; j += 2) gelu_pair(f[j], f[j + 1]);
+        } else if (act == 1) {
+#pragma unroll
+            for (int j = 0; j < 32; j++) f[j] = fmaxf(f[j], 0.f);
+        }
+        if (threshold) {
+            drop_apply32(key, group, threshold, p.e.drop_scale, f);
+            group += 4;
+        }
+        if (has_res) {
+            const uint32_t s = has_pre ? 0 : turn & 1, ph = has_pre ? turn & 1 : (turn >> 1) & 1;
+            if (!mbar_wait_warp(&bars[s], ph, abort_flag)) return false;
+#pragma unroll
+            for (int ch = 0; ch < 4; ch++) gm_add8(f + ch * 8, *reinterpret_cast<const uint4*>(slab + lane * 64 + ((ch ^ ((lane >> 1) & 3)) << 4)));
+        } else if (!has_pre) {
+            if (elect_one()) bulk_wait_group_read<1>();   // the store of two turns ago has read this slab
+            __syncwarp();
+        }
+        gm_stage32(slab, lane, f);
+        fence_proxy_async_smem();
+        __syncwarp();
+        turn++;
+        if (elect_one()) {
+            if (m0w < p.M) {
+                tma_store_tile_2d(p.tmap_c, smem_u32(slab), n0 + c0, m0w);
+                if (has_pre) tma_store_tile_2d(p.tmap_pre, smem_u32(stage + 2048), n0 + c0, m0w);
+            }
+            bulk_commit_group();
+        }
+        __syncwarp();
+        if (c0 + 32 < cols) gm_residual_ahead<COLS>(p, m0w, n0 + c0 + 32, stage, turn, bars);
+    }
+    return true;
+}
+
+// The same for any width, alignment and type of the bias.
+template <int COLS>
+__device__ __forceinline__ void gm_epilogue_act_any(const GemmParams& p, uint32_t t_row, int m, int m0w, int n0, int lane, uint8_t* stage) {
+    const bool row_ok = m < p.M;
+    DropKey key = {};
+    if (p.e.drop_threshold) key = drop_key(p.e.rng, p.e.site);
+#pragma unroll 1
+    for (int c0 = 0; c0 < COLS; c0 += 32) {
         const int n = n0 + c0;
         if (n >= p.N) break;            // warp-uniform
         float f[32];
         gm_load32(t_row + c0, f);
-        const bool full = n + 32 <= p.N;
-        if (p.splits > 1) {
-            if (row_ok) {
-                float* srow = p.slabs + ((long long)sp * p.M + m) * p.N + n;
-                if (full && (p.N & 3) == 0) {
-#pragma unroll
-                    for (int j = 0; j < 32; j += 4) *reinterpret_cast<float4*>(srow + j) = make_float4(f[j], f[j + 1], f[j + 2], f[j + 3]);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 32; j++)
-                        if (n + j < p.N) srow[j] = f[j];
-                }
-            }
-            continue;
-        }
-        if (p.bias) {
+        const long long index = (long long)m * p.N + n;
+        if (p.bias || p.bias_bf16) {
 #pragma unroll
             for (int j = 0; j < 32; j++)
-                if (full || n + j < p.N) f[j] += __ldg(p.bias + n + j);
+                if (n + j < p.N) f[j] += p.bias ? __ldg(p.bias + n + j) : __bfloat162float(p.bias_bf16[n + j]);
         }
-        if (p.bias_bf16) {
-#pragma unroll
-            for (int j = 0; j < 32; j++)
-                if (full || n + j < p.N) f[j] += __bfloat162float(p.bias_bf16[n + j]);
-        }
-        uint8_t* slab = stage + (turn & 1) * 4096;
-        if (lane == 0) bulk_wait_group_read<1>();   // the stores of two turns ago have read their slabs
+        if (elect_one()) bulk_wait_group_read<0>();   // the pre-activations of the turn before have left
         __syncwarp();
-        turn++;
-        if (p.e.pre) gm_stage32(slab + 2048, lane, f);
+        if (p.e.pre) gm_stage32(stage + 2048, lane, f);
         if (p.e.act == 2) {
 #pragma unroll
-            for (int j = 0; j < 32; j++) f[j] *= gauss_cdf(f[j]);
+            for (int j = 0; j < 32; j += 2) gelu_pair(f[j], f[j + 1]);
         } else if (p.e.act == 1) {
 #pragma unroll
             for (int j = 0; j < 32; j++) f[j] = fmaxf(f[j], 0.f);
         }
         if (p.e.drop_threshold) {
-            const unsigned long long index = (unsigned long long)m * p.N + n;
-            const uint32_t mask = drop_mask<32>(key, index, p.e.drop_threshold);
+            const uint32_t mask = drop_mask<32>(key, (unsigned long long)index, p.e.drop_threshold);
 #pragma unroll
             for (int j = 0; j < 32; j++) f[j] = mask >> j & 1u ? f[j] * p.e.drop_scale : 0.f;
         }
         if (p.residual && row_ok) {
-            const __nv_bfloat16* res = p.residual + (long long)m * p.N + n;
-            if (p.vec_ok) {             // N a multiple of 8
 #pragma unroll
-                for (int ch = 0; ch < 4; ch++)
-                    if (full || n + ch * 8 < p.N) {
-                        const uint4 rv = __ldg(reinterpret_cast<const uint4*>(res + ch * 8));
-                        const __nv_bfloat162* h2 = reinterpret_cast<const __nv_bfloat162*>(&rv);
-#pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            f[ch * 8 + e * 2] += __low2float(h2[e]);
-                            f[ch * 8 + e * 2 + 1] += __high2float(h2[e]);
-                        }
-                    }
-            } else {
-#pragma unroll
-                for (int j = 0; j < 32; j++)
-                    if (n + j < p.N) f[j] += __bfloat162float(res[j]);
-            }
+            for (int j = 0; j < 32; j++)
+                if (n + j < p.N) f[j] += __bfloat162float(p.residual[index + j]);
         }
-        gm_stage32(slab, lane, f);
+        gm_stage32(stage, lane, f);
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) {
-            if (m0w < p.M) {
-                if (p.e.pre) tma_store_tile_2d(p.tmap_pre, smem_u32(slab + 2048), n, m0w);
-                if (aligned) tma_store_tile_2d(p.tmap_c, smem_u32(slab), n, m0w);
-            }
+        if (elect_one()) {
+            if (m0w < p.M && p.e.pre) tma_store_tile_2d(p.tmap_pre, smem_u32(stage + 2048), n, m0w);
             bulk_commit_group();
         }
-        if (!aligned) {
-            // rows of an odd width: lane = column, one row after the other, so that a store covers 64 consecutive bytes
-            __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(p.c) + (long long)m0w * p.ldc + n + lane;
-            const int rows = p.M - m0w < 32 ? p.M - m0w : 32;
-            for (int r = 0; r < rows; r++)
-                if (n + lane < p.N)
-                    out[r * p.ldc] = *reinterpret_cast<const __nv_bfloat16*>(slab + r * 64 + (((lane >> 3) ^ ((r >> 1) & 3)) << 4) + (lane & 7) * 2);
-            __syncwarp();
-        }
+        // lane = column, one row after the other, so that a store covers 64 consecutive bytes
+        __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(p.c) + (long long)m0w * p.ldc + n + lane;
+        const int rows = p.M - m0w < 32 ? p.M - m0w : 32;
+#pragma unroll 4
+        for (int r = 0; r < rows; r++)
+            if (n + lane < p.N)
+                out[r * p.ldc] = *reinterpret_cast<const __nv_bfloat16*>(stage + r * 64 + (((lane >> 3) ^ ((r >> 1) & 3)) << 4) + (lane & 7) * 2);
+        __syncwarp();
     }
 }
 
@@ -178,42 +254,101 @@ __device__ __forceinline__ void gm_epilogue_lse(const GemmParams& p, uint32_t t_
 }
 
 // C = (softmax - onehot(label)) * coefficient, the probabilities from this product's logits and the row's logsumexp.
-template <int BN>
+template <int COLS>
 __device__ __forceinline__ void gm_epilogue_dlogits(const GemmParams& p, uint32_t t_row, int m, int m0w, int n0, int lane, uint8_t* stage,
                                                     uint32_t& turn) {
     constexpr float kLog2e = 1.4426950408889634f;
     const bool row_ok = m < p.M;
     const float2 row = row_ok ? p.e.row[m] : make_float2(0.f, 0.f);
     const long long at = row_ok ? p.e.target[m] - p.e.col0 - n0 : -1;
-    const int label = at >= 0 && at < BN ? (int)at : -1;
+    const int label = at >= 0 && at < COLS ? (int)at : -1;
 #pragma unroll 1
-    for (int c0 = 0; c0 < BN; c0 += 32) {
+    for (int c0 = 0; c0 < COLS; c0 += 32) {
         const int n = n0 + c0;
         if (n >= p.N) break;            // warp-uniform
         float f[32];
         gm_load32(t_row + c0, f);
 #pragma unroll
-        for (int j = 0; j < 32; j++) {
-            float e;
-            asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(fmaf(f[j], kLog2e, -row.x)));
-            f[j] = e;
+        for (int j = 0; j < 32; j += 2) {
+            float e0, e1;
+            split_f32x2(fma_f32x2(f32x2(f[j], f[j + 1]), f32x2(kLog2e, kLog2e), f32x2(-row.x, -row.x)), e0, e1);
+            asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e0) : "f"(e0));
+            asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e1) : "f"(e1));
+            split_f32x2(mul_f32x2(f32x2(e0, e1), f32x2(row.y, row.y)), f[j], f[j + 1]);
         }
         if (__any_sync(0xffffffffu, label >= c0 && label < c0 + 32)) {
 #pragma unroll
-            for (int j = 0; j < 32; j++) f[j] -= label == c0 + j ? 1.f : 0.f;
+            for (int j = 0; j < 32; j++) f[j] -= label == c0 + j ? row.y : 0.f;
         }
+        if (__any_sync(0xffffffffu, row.y == 0.f)) {
 #pragma unroll
-        for (int j = 0; j < 32; j++) f[j] = row.y == 0.f ? 0.f : f[j] * row.y;
-        uint8_t* slab = stage + (turn & 1) * 4096;
-        if (lane == 0) bulk_wait_group_read<1>();
+            for (int j = 0; j < 32; j++) f[j] = row.y == 0.f ? 0.f : f[j];
+        }
+        uint8_t* slab = stage + (turn++ & 1) * 2048;
+        if (elect_one()) bulk_wait_group_read<1>();
         __syncwarp();
-        turn++;
         gm_stage32(slab, lane, f);
+        __syncwarp();
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) {
+        if (elect_one()) {
             if (m0w < p.M) tma_store_tile_2d(p.tmap_c, smem_u32(slab), n, m0w);
             bulk_commit_group();
+        }
+        __syncwarp();
+    }
+}
+
+// A dual launch's tiles: float32 accumulators plus the first product's addend (which may be its output), rounded to the output's type.
+template <int BN>
+__device__ __forceinline__ void gm_epilogue_dual(const GemmParamsDual& p, bool second, uint32_t t_row, int m, int m0w, int n0, int lane, uint8_t* stage,
+                                                 uint32_t& turn) {
+    const int M = second ? p.second.M : p.M, N = second ? p.second.N : p.N;
+    const bool out_f32 = second ? p.second.out_f32 : p.out_f32;
+    const unsigned char* map = second ? p.second.tmap_c : p.tmap_c;
+    const float* addend = second || m >= M || !p.e.addend ? nullptr : p.e.addend + (long long)m * N;
+#pragma unroll 1
+    for (int c0 = 0; c0 < BN; c0 += 32) {
+        const int n = n0 + c0;
+        if (n >= N) break;              // warp-uniform
+        float f[32];
+        gm_load32(t_row + c0, f);
+        if (addend) {                   // N is a multiple of 8
+#pragma unroll
+            for (int j = 0; j < 32; j += 4)
+                if (n + j < N) {
+                    const float4 a = *reinterpret_cast<const float4*>(addend + n + j);
+                    f[j] += a.x; f[j + 1] += a.y; f[j + 2] += a.z; f[j + 3] += a.w;
+                }
+        }
+        // 64 bfloat16 or 32 float32 columns a slab of 128-byte rows
+        const int half = out_f32 ? 0 : (c0 >> 5) & 1;
+        uint8_t* slab = stage + (turn & 1) * 4096;
+        if (half == 0) {
+            if (elect_one()) bulk_wait_group_read<1>();
+            __syncwarp();
+        }
+        uint8_t* row = slab + lane * 128;
+        if (out_f32) {
+#pragma unroll
+            for (int ch = 0; ch < 8; ch++)
+                *reinterpret_cast<float4*>(row + ((ch ^ (lane & 7)) << 4)) = make_float4(f[ch * 4], f[ch * 4 + 1], f[ch * 4 + 2], f[ch * 4 + 3]);
+        } else {
+#pragma unroll
+            for (int ch = 0; ch < 4; ch++)
+                *reinterpret_cast<uint4*>(row + (((half * 4 + ch) ^ (lane & 7)) << 4)) =
+                    make_uint4(gm_pack(f[ch * 8], f[ch * 8 + 1]), gm_pack(f[ch * 8 + 2], f[ch * 8 + 3]), gm_pack(f[ch * 8 + 4], f[ch * 8 + 5]),
+                               gm_pack(f[ch * 8 + 6], f[ch * 8 + 7]));
+        }
+        if (out_f32 || half == 1 || c0 + 32 >= BN || n + 32 >= N) {
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (elect_one()) {
+                if (m0w < M) tma_store_tile_2d(map, smem_u32(slab), n - half * 32, m0w);
+                bulk_commit_group();
+            }
+            __syncwarp();
+            turn++;
         }
     }
 }

@@ -71,6 +71,7 @@ __global__ void __launch_bounds__(LA_THREADS) dropout_kernel(const T* __restrict
     pdl_launch_dependents();
     DropKey key = {};
     if (threshold) key = drop_key(rng, site);
+    const uint32_t limit = drop_limit(threshold);
     const long long groups = (n + 7) / 8;
     for (long long g = (long long)blockIdx.x * blockDim.x + threadIdx.x; g < groups; g += (long long)gridDim.x * blockDim.x) {
         const long long i = g * 8;
@@ -91,7 +92,7 @@ __global__ void __launch_bounds__(LA_THREADS) dropout_kernel(const T* __restrict
         if (threshold) drop_bits(key, (unsigned long long)g, c);
 #pragma unroll
         for (int e = 0; e < 8; e++) {
-            v[e] = drop_keeps(c, e, threshold) ? v[e] * scale : 0.f;
+            v[e] = threshold == 0 || drop_keeps(c, e, limit) ? v[e] * scale : 0.f;
             if (residual) v[e] += r[e];
         }
         if (VEC && left == 8) {

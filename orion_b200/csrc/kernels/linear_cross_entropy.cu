@@ -20,44 +20,54 @@
 #include "gemm_call.h"
 #include "pdl.cuh"
 
+extern "C" int ob200_plan_sm_count(void);
+
 namespace ob200 {
 
 constexpr int CE_THREADS = 256;
 constexpr float CE_LOG2E = 1.4426950408889634f;
 
-// lse and loss of every row from its parts.  32 rows a CTA; group g of 8 joins parts g, g + 8, ..., then the groups are joined in order.
-__global__ void __launch_bounds__(CE_THREADS) ce_rows_kernel(const float2* __restrict__ part, const float* __restrict__ label_logit,
-                                                             const long long* __restrict__ target, float* __restrict__ loss,
-                                                             float* __restrict__ lse, int rows, int parts, int V, long long ignore_index) {
+// lse and loss of every row from its parts.  A CTA has 32 rows; group g of 32 takes parts g, g + 32, ..., eight at a time in registers
+// (the kernel is a few dependent steps long: their loads are one), then the groups are joined in order.
+__global__ void __launch_bounds__(1024) ce_rows_kernel(const float2* __restrict__ part, const float* __restrict__ label_logit,
+                                                       const long long* __restrict__ target, float* __restrict__ loss, float* __restrict__ lse,
+                                                       int rows, int parts, int V, long long ignore_index) {
     pdl_wait();
     pdl_launch_dependents();
-    __shared__ float2 sh[8][32];
+    __shared__ float2 sh[32][33];
     const int c = threadIdx.x & 31, g = threadIdx.x >> 5;
+    // A maximum of minus infinity has a sum of 0, or one that is not a number; it is weighed with 1, so that the latter stays.
+    auto weight = [](float top, float now) { return top == -INFINITY ? 1.f : exp2f((top - now) * CE_LOG2E); };
     for (int r0 = blockIdx.x * 32; r0 < rows; r0 += gridDim.x * 32) {
         const int r = r0 + c;
         float top = -INFINITY, sum = 0.f;
-        auto join = [&](float2 q) {
-            const float now = fmaxf(top, q.x);
-            if (now == -INFINITY) {   // nothing above minus infinity yet; a sum that is not a number stays one
-                sum += q.y;
-                return;
-            }
-            sum = (top == -INFINITY ? sum : sum * exp2f((top - now) * CE_LOG2E)) + (q.x == -INFINITY ? q.y : q.y * exp2f((q.x - now) * CE_LOG2E));
+        for (int t0 = g; t0 < parts; t0 += 256) {
+            float2 q[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) q[i] = r < rows && t0 + 32 * i < parts ? part[(long long)(t0 + 32 * i) * rows + r] : make_float2(-INFINITY, 0.f);
+            float now = top;
+#pragma unroll
+            for (int i = 0; i < 8; i++) now = fmaxf(now, q[i].x);
+            sum *= weight(top, now);
+#pragma unroll
+            for (int i = 0; i < 8; i++) sum += q[i].y * weight(q[i].x, now);
             top = now;
-        };
-        if (r < rows) {
-#pragma unroll 8
-            for (int t = g; t < parts; t += 8) join(part[(long long)t * rows + r]);
         }
         sh[g][c] = make_float2(top, sum);
         __syncthreads();
-        if (g == 0 && r < rows) {
+        // warp g joins the groups of row r0 + g: lane = group, in a fixed tree
+        float2 q = sh[c][g];
+        float now = q.x;
 #pragma unroll
-            for (int k = 1; k < 8; k++) join(sh[k][c]);
-            const float l = top + logf(sum);
-            const long long t = target[r];
-            lse[r] = l;
-            loss[r] = t == ignore_index ? 0.f : t >= 0 && t < V ? l - label_logit[r] : NAN;
+        for (int o = 16; o > 0; o >>= 1) now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, o));
+        float all = q.y * weight(q.x, now);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+        if (c == 0 && r0 + g < rows) {
+            const float l = now + logf(all);
+            const long long t = target[r0 + g];
+            lse[r0 + g] = l;
+            loss[r0 + g] = t == ignore_index ? 0.f : t >= 0 && t < V ? l - label_logit[r0 + g] : NAN;
         }
         __syncthreads();
     }
@@ -122,15 +132,36 @@ __global__ void __launch_bounds__(CE_THREADS) ce_prepare_kernel(const __nv_bfloa
     }
 }
 
-// Columns of the vocabulary a piece of the backward pass has: dl of a piece is about as large as the L2 cache, and no piece so narrow
-// that its products are small.
-static int ce_piece(long long rows, int V) {
-    long long v = (128LL << 20) / (2 * rows) / 256 * 256;
-    if (v < 2048) v = 2048;
-    const long long all = ((long long)V + 7) / 8 * 8;
-    if (v >= all) return (int)all;
-    const long long pieces = (V + v - 1) / v;
-    return (int)(((V + pieces - 1) / pieces + 255) / 256 * 256);
+// Columns of the vocabulary a piece of the backward pass has: dl of a piece takes at most 192 MB (and no piece is so narrow that its
+// products are small), and of the four fewest numbers of pieces the one whose 256 x 256 tiles fill the last rounds of the CTA pairs best,
+// counted in k-blocks of 64 and eight for a tile's way out.  8192 x 32000 x 1024: three pieces of 10752 columns, whose gradient products
+// are 296 tiles for 74 pairs, instead of four of 8192 (256 tiles: 3.46 rounds).
+static int ce_piece(long long rows, int V, int H, int sms) {
+    long long most = (192LL << 20) / (2 * rows) / 256 * 256;
+    if (most < 2048) most = 2048;
+    const long long all = ((long long)V + 7) / 8 * 8, pairs = sms / 2 > 0 ? sms / 2 : 1, fewest = (V + most - 1) / most;
+    if (fewest == 1 && rows <= 128) return (int)all;   // no pairs
+    const long long tiles_t = (rows + 255) / 256, tiles_h = (H + 255) / 256;
+    long long best = 0, best_cost = 0;
+    for (long long n = fewest; n < fewest + 4; n++) {
+        const long long v = n == 1 ? all : ((V + n - 1) / n + 255) / 256 * 256;
+        long long cost = 0;
+        for (long long v0 = 0; v0 < V; v0 += v) {
+            const long long nv = V - v0 < v ? V - v0 : v, tiles_v = (nv + 255) / 256;
+            const long long dx = tiles_t * tiles_h, dw = tiles_v * tiles_h, dx_cost = nv / 64 + 8, dw_cost = rows / 64 + 8;
+            cost += (tiles_t * tiles_v + pairs - 1) / pairs * (H / 64 + 8);
+            // a pair has every pairs-th unit, those of dx first
+            auto load = [&](long long pair) {
+                const long long a = dx > pair ? (dx - pair + pairs - 1) / pairs : 0, b = dx + dw > pair ? (dx + dw - pair + pairs - 1) / pairs - a : 0;
+                return a * dx_cost + b * dw_cost;
+            };
+            long long longest = 0;
+            for (long long pair = 0; pair < pairs; pair++) longest = load(pair) > longest ? load(pair) : longest;
+            cost += longest;
+        }
+        if (best == 0 || cost < best_cost) { best = v; best_cost = cost; }
+    }
+    return (int)best;
 }
 constexpr int CE_ROW_BLOCK = 65536;   // rows a forward pass has in its workspace at a time
 static size_t ce_round(size_t bytes) { return (bytes + 255) & ~(size_t)255; }
@@ -139,7 +170,7 @@ struct CeBackwardSpace {
     size_t row, kept, dl, acc, slabs, total;
     int piece;
     CeBackwardSpace(long long rows, int V, int H, bool want_dx, bool want_dw) {
-        piece = ce_piece(rows, V);
+        piece = ce_piece(rows, V, H, ob200_plan_sm_count());
         row = ce_round((size_t)rows * sizeof(float2));
         kept = want_dw ? ce_round((size_t)rows * H * 2) : 0;
         dl = ce_round((size_t)rows * piece * 2);
@@ -193,9 +224,9 @@ extern "C" int ob200_linear_cross_entropy_forward(const void* x, const void* w, 
         g.stream = stream;
         int rc = gemm_bf16_run(g);
         if (rc) return rc;
-        const int want = (n + 31) / 32, cap = num_ctas * 8;
-        OB200_ELASTIC_HBM(ce_rows_kernel, 8);
-        rc = launch_pdl(ce_rows_kernel, (unsigned)(want < cap ? want : cap), (unsigned)CE_THREADS, st, (const float2*)part, (const float*)label_logit,
+        const int want = (n + 31) / 32, cap = num_ctas * 2;
+        OB200_ELASTIC_HBM(ce_rows_kernel, 2);
+        rc = launch_pdl(ce_rows_kernel, (unsigned)(want < cap ? want : cap), 1024u, st, (const float2*)part, (const float*)label_logit,
                         target + r0, loss + r0, lse + r0, n, parts, V, ignore_index);
         if (rc) return rc;
     }
@@ -259,26 +290,27 @@ extern "C" int ob200_linear_cross_entropy_backward(const void* x, const void* w,
         g.b_mn = 1;
         g.N = H;
         g.ldc = H;
-        if (dx) {   // dx[t, h] += sum_v dl[t, v] w[v, h]
-            g.b = wp; g.ldb = ldw;
-            g.M = rows; g.K = nv;
-            g.epi = first ? GM_EPI_PLAIN : GM_EPI_ACC;
-            g.e.addend = first ? nullptr : acc;
-            g.out_f32 = last ? 0 : 1;
-            g.c = last ? dx : (void*)acc;
-            rc = gemm_bf16_run(g);
-            if (rc) return rc;
+        GemmCall gx = g, gw = g;
+        // dx[t, h] += sum_v dl[t, v] w[v, h]
+        gx.b = wp; gx.ldb = ldw;
+        gx.M = rows; gx.K = nv;
+        gx.epi = first ? GM_EPI_PLAIN : GM_EPI_ACC;
+        gx.e.addend = first ? nullptr : acc;
+        gx.out_f32 = last ? 0 : 1;
+        gx.c = last ? dx : (void*)acc;
+        // dw[v, h] = sum_t dl[t, v] x[t, h]
+        gw.a_mn = 1;
+        gw.b = kept; gw.ldb = H;
+        gw.M = nv; gw.K = rows;
+        gw.epi = GM_EPI_PLAIN;
+        gw.c = (__nv_bfloat16*)dw + (long long)v0 * H;
+        if (dx && dw && gemm_bf16_dual_fits(gx, gw)) {
+            rc = gemm_bf16_run_dual(gx, gw);
+        } else {
+            if (dx) rc = gemm_bf16_run(gx);
+            if (dw && !rc) rc = gemm_bf16_run(gw);
         }
-        if (dw) {   // dw[v, h] = sum_t dl[t, v] x[t, h]
-            g.a_mn = 1;
-            g.b = kept; g.ldb = H;
-            g.M = nv; g.K = rows;
-            g.epi = GM_EPI_PLAIN;
-            g.out_f32 = 0;
-            g.c = (__nv_bfloat16*)dw + (long long)v0 * H;
-            rc = gemm_bf16_run(g);
-            if (rc) return rc;
-        }
+        if (rc) return rc;
     }
     return 0;
 }

@@ -44,16 +44,17 @@ __device__ __forceinline__ void drop_bits(const DropKey& key, unsigned long long
     }
 }
 
-// Half e of a group is kept.
-__device__ __forceinline__ bool drop_keeps(const uint32_t (&c)[4], int e, uint32_t threshold) {
-    return ((c[e >> 1] >> ((e & 1) * 16)) & 0xFFFFu) >= threshold;
-}
+// Half e of a group is kept.  The halves are compared in the upper half of a word with limit = 65536 * threshold - 1 (threshold > 0; for
+// 65536, where nothing is kept, that is the largest word), so that the high one needs no shift.
+__device__ __forceinline__ uint32_t drop_limit(uint32_t threshold) { return (threshold << 16) - 1u; }
+__device__ __forceinline__ bool drop_keeps(const uint32_t (&c)[4], int e, uint32_t limit) { return ((e & 1) ? c[e >> 1] : c[e >> 1] << 16) > limit; }
 // The same as a mask, bit e for half e.
 __device__ __forceinline__ uint32_t drop_group_mask(const DropKey& key, unsigned long long group, uint32_t threshold) {
     uint32_t c[4], mask = 0;
     drop_bits(key, group, c);
+    const uint32_t limit = drop_limit(threshold);
 #pragma unroll
-    for (int e = 0; e < 8; e++) mask |= drop_keeps(c, e, threshold) ? 1u << e : 0u;
+    for (int e = 0; e < 8; e++) mask |= drop_keeps(c, e, limit) ? 1u << e : 0u;
     return mask;
 }
 
@@ -68,6 +69,16 @@ __device__ __forceinline__ uint32_t drop_mask(const DropKey& key, unsigned long 
     for (int i = 0; i < COUNT / 8; i++) bits |= (unsigned long long)drop_group_mask(key, g + i, threshold) << (8 * i);
     if (off) bits |= (unsigned long long)drop_group_mask(key, g + COUNT / 8, threshold) << COUNT;
     return (uint32_t)(bits >> off);
+}
+
+// f[j] = kept ? f[j] * scale : 0 for the 32 elements of groups `group` .. `group + 3`: four draws side by side, which share the keys.
+__device__ __forceinline__ void drop_apply32(const DropKey& key, unsigned long long group, uint32_t threshold, float scale, float (&f)[32]) {
+    uint32_t c[4][4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) drop_bits(key, group + i, c[i]);
+    const uint32_t limit = drop_limit(threshold);
+#pragma unroll
+    for (int j = 0; j < 32; j++) f[j] = drop_keeps(c[j >> 3], j & 7, limit) ? f[j] * scale : 0.f;
 }
 
 // A probability as the kernels use it.
