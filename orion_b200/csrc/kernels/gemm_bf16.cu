@@ -466,8 +466,8 @@ __global__ void __launch_bounds__(gm_threads(EPI), 1) gemm_bf16_kernel(const __g
                     if (slab_done) {
                         fence_proxy_async_smem();
                         __syncwarp();
-                        if (lane == 0 && m0w < p.M) {
-                            tma_store_tile_4d(p.tmap_c, smem_u32(slab), n - half * 32, m0w, bi, bo);
+                        if (lane == 0) {   // a warp whose rows are past the edge commits an empty group: the wait above counts slabs
+                            if (m0w < p.M) tma_store_tile_4d(p.tmap_c, smem_u32(slab), n - half * 32, m0w, bi, bo);
                             bulk_commit_group();
                         }
                         slab_i++;

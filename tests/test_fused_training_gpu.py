@@ -662,3 +662,17 @@ def test_through_the_c_abi(built):
         assert torch.equal(total, loss) and count.item() == 300
         for g, h in zip(K.linear_cross_entropy_backward(x, w, target, lse, torch.ones((), device="cuda"), count, num_ctas=21), want):
             assert torch.equal(g, h)
+
+
+@pytest.mark.parametrize("out_dtype", [torch.float32, BF])
+@pytest.mark.parametrize("M,N", [(2200, 2040), (264, 1000), (1040, 512)])
+def test_gemm_tiles_whose_lower_warps_are_past_the_edge(built, M, N, out_dtype):
+    """A warp with no rows in the last row of tiles must not run over the slab that its store of the tile before still reads: the same
+    bits time after time, from one CTA (all tiles in a row) and from all."""
+    from orion_b200 import kernels as K
+    torch.manual_seed(M)
+    a, b = torch.randn(M, 136, device="cuda").to(BF), torch.randn(N, 136, device="cuda").to(BF)
+    want = K.gemm_bf16(a, b, out_dtype=out_dtype)
+    for _ in range(60):
+        for ctas in (1, 7):
+            assert torch.equal(K.gemm_bf16(a, b, out_dtype=out_dtype, num_ctas=ctas), want)
