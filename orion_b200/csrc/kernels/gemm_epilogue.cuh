@@ -90,7 +90,7 @@ __device__ __forceinline__ bool gm_epilogue_act(const GemmParams& p, uint32_t t_
     const int cols = p.N - n0 < COLS ? p.N - n0 : COLS, act = p.e.act;
     const uint32_t threshold = p.e.drop_threshold;
     DropKey key = {};
-    if (threshold) key = drop_key(p.e.rng, p.e.site);
+    if (threshold) key = drop_key_warp(p.e.rng, p.e.site);
     unsigned long long group = ((unsigned long long)m * p.N + n0) >> 3;
     const __nv_bfloat16* bias = p.bias_bf16 ? p.bias_bf16 + n0 : nullptr;
 #pragma unroll 1
@@ -155,7 +155,7 @@ template <int COLS>
 __device__ __forceinline__ void gm_epilogue_act_any(const GemmParams& p, uint32_t t_row, int m, int m0w, int n0, int lane, uint8_t* stage) {
     const bool row_ok = m < p.M;
     DropKey key = {};
-    if (p.e.drop_threshold) key = drop_key(p.e.rng, p.e.site);
+    if (p.e.drop_threshold) key = drop_key_warp(p.e.rng, p.e.site);
 #pragma unroll 1
     for (int c0 = 0; c0 < COLS; c0 += 32) {
         const int n = n0 + c0;

@@ -70,7 +70,7 @@ __global__ void __launch_bounds__(LA_THREADS) dropout_kernel(const T* __restrict
     pdl_wait();
     pdl_launch_dependents();
     DropKey key = {};
-    if (threshold) key = drop_key(rng, site);
+    if (threshold) key = drop_key_warp(rng, site);
     const uint32_t limit = drop_limit(threshold);
     const long long groups = (n + 7) / 8;
     for (long long g = (long long)blockIdx.x * blockDim.x + threadIdx.x; g < groups; g += (long long)gridDim.x * blockDim.x) {
@@ -110,7 +110,7 @@ __global__ void __launch_bounds__(LA_THREADS) dropout_kernel(const T* __restrict
 // item is 256 columns of one range of rows; the ranges follow from the sizes alone, so the sums do not depend on the CTA count.
 // VEC: rows of dy are 16-byte multiples (an even width); rows of z and dz always are.
 template <bool VEC>
-__global__ void __launch_bounds__(LA_THREADS) act_backward_kernel(const __nv_bfloat16* __restrict__ dy, const __nv_bfloat16* __restrict__ pre,
+__global__ void __launch_bounds__(LA_THREADS, 3) act_backward_kernel(const __nv_bfloat16* __restrict__ dy, const __nv_bfloat16* __restrict__ pre,
                                                                   long long ld_pre, __nv_bfloat16* __restrict__ dz, long long ld_dz,
                                                                   float* __restrict__ partial, long long rows, int N, int ranges, int act,
                                                                   const long long* __restrict__ rng, uint32_t site, uint32_t threshold, float scale) {
@@ -120,7 +120,8 @@ __global__ void __launch_bounds__(LA_THREADS) act_backward_kernel(const __nv_bfl
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int col_tiles = (N + LA_COLS - 1) / LA_COLS;
     DropKey key = {};
-    if (threshold) key = drop_key(rng, site);
+    if (threshold) key = drop_key_warp(rng, site);
+    const uint32_t limit = drop_limit(threshold);
     for (int item = blockIdx.x; item < col_tiles * ranges; item += gridDim.x) {
         const int ct = item % col_tiles, range = item / col_tiles;
         const int col = ct * LA_COLS + lane * 8;
@@ -129,34 +130,47 @@ __global__ void __launch_bounds__(LA_THREADS) act_backward_kernel(const __nv_bfl
 #pragma unroll
         for (int e = 0; e < 8; e++) acc[e] = 0.f;
         if (col < N) {
-#pragma unroll 4
-            for (long long row = r0 + warp; row < r1; row += LA_ROWS) {
-                float d[8], z[8];
-                if (VEC) {
-                    Pack8<__nv_bfloat16>::load(dy + row * N + col, d);
-                } else {
+            // two rows under way at a time
+            for (long long row = r0 + warp; row < r1; row += 2 * LA_ROWS) {
+                float d[2][8], z[2][8];
 #pragma unroll
-                    for (int e = 0; e < 8; e++) d[e] = col + e < N ? __bfloat162float(dy[row * N + col + e]) : 0.f;
-                }
-                if (act) Pack8<__nv_bfloat16>::load(pre + row * ld_pre + col, z);
-                if (threshold) {
-                    const uint32_t mask = drop_mask<8>(key, (unsigned long long)row * N + col, threshold);
+                for (int u = 0; u < 2; u++) {
+                    const long long r = row + u * LA_ROWS < r1 ? row + u * LA_ROWS : row;
+                    if (VEC) {
+                        Pack8<__nv_bfloat16>::load(dy + r * N + col, d[u]);
+                    } else {
 #pragma unroll
-                    for (int e = 0; e < 8; e++) d[e] = mask >> e & 1u ? d[e] * scale : 0.f;
-                }
-                if (act == 2) {
-#pragma unroll
-                    for (int e = 0; e < 8; e++) {
-                        const float ex = gauss_exp(z[e]);
-                        d[e] *= gauss_cdf_with_exp(z[e], ex) + z[e] * 0.3989422804014327f * ex;
+                        for (int e = 0; e < 8; e++) d[u][e] = col + e < N ? __bfloat162float(dy[r * N + col + e]) : 0.f;
                     }
-                } else if (act == 1) {
-#pragma unroll
-                    for (int e = 0; e < 8; e++) d[e] = z[e] > 0.f ? d[e] : 0.f;
+                    if (act) Pack8<__nv_bfloat16>::load(pre + r * ld_pre + col, z[u]);
                 }
-                if (dz) Pack8<__nv_bfloat16>::store(dz + row * ld_dz + col, d);
 #pragma unroll
-                for (int e = 0; e < 8; e++) acc[e] += d[e];
+                for (int u = 0; u < 2; u++) {
+                    const long long r = row + u * LA_ROWS;
+                    if (r >= r1) break;
+                    if (threshold) {
+                        if (VEC) {
+                            uint32_t c[4];
+                            drop_bits(key, ((unsigned long long)r * N + col) >> 3, c);
+#pragma unroll
+                            for (int e = 0; e < 8; e++) d[u][e] = drop_keeps(c, e, limit) ? d[u][e] * scale : 0.f;
+                        } else {
+                            const uint32_t mask = drop_mask<8>(key, (unsigned long long)r * N + col, threshold);
+#pragma unroll
+                            for (int e = 0; e < 8; e++) d[u][e] = mask >> e & 1u ? d[u][e] * scale : 0.f;
+                        }
+                    }
+                    if (act == 2) {
+#pragma unroll
+                        for (int e = 0; e < 8; e += 2) gelu_slope_pair(d[u][e], d[u][e + 1], z[u][e], z[u][e + 1]);
+                    } else if (act == 1) {
+#pragma unroll
+                        for (int e = 0; e < 8; e++) d[u][e] = z[u][e] > 0.f ? d[u][e] : 0.f;
+                    }
+                    if (dz) Pack8<__nv_bfloat16>::store(dz + r * ld_dz + col, d[u]);
+#pragma unroll
+                    for (int e = 0; e < 8; e++) acc[e] += d[u][e];
+                }
             }
         }
         if (partial) {
@@ -236,7 +250,7 @@ extern "C" int ob200_dropout(const void* x, const void* residual, void* y, long 
 }
 
 extern "C" long long ob200_linear_act_workspace(int M, int N, int K) {
-    if (M <= 0 || N <= 0 || K <= 0) return 0;
+    if (M <= 0 || N <= 0 || K <= 0 || few_rows_fit(M, N, K)) return 0;
     return (long long)gemm_bf16_slab_bytes(M, N, K);
 }
 
@@ -268,7 +282,7 @@ extern "C" int ob200_linear_act_bf16(const void* x, const void* w, void* y, void
     g.slab_bytes = (size_t)workspace_bytes;
     g.num_ctas = num_ctas;
     g.stream = stream;
-    return gemm_bf16_run(g);
+    return few_rows_fit(M, N, K) ? few_rows_run(g) : gemm_bf16_run(g);
 }
 
 namespace {

@@ -27,24 +27,27 @@ namespace ob200 {
 constexpr int CE_THREADS = 256;
 constexpr float CE_LOG2E = 1.4426950408889634f;
 
-// lse and loss of every row from its parts.  A CTA has 32 rows; group g of 32 takes parts g, g + 32, ..., eight at a time in registers
-// (the kernel is a few dependent steps long: their loads are one), then the groups are joined in order.
+// lse and loss of every row from its parts.  A CTA has C rows; group g of G = 1024 / C takes parts g, g + G, ..., eight at a time in
+// registers (the kernel is a few dependent steps long: their loads are one), then the groups are joined in a fixed tree.  32 rows, or 4
+// where rows are few and their parts many.
+template <int C>
 __global__ void __launch_bounds__(1024) ce_rows_kernel(const float2* __restrict__ part, const float* __restrict__ label_logit,
                                                        const long long* __restrict__ target, float* __restrict__ loss, float* __restrict__ lse,
                                                        int rows, int parts, int V, long long ignore_index) {
     pdl_wait();
     pdl_launch_dependents();
-    __shared__ float2 sh[32][33];
-    const int c = threadIdx.x & 31, g = threadIdx.x >> 5;
+    constexpr int G = 1024 / C;
+    __shared__ float2 sh[G][C + 1];
+    const int c = threadIdx.x % C, g = threadIdx.x / C, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     // A maximum of minus infinity has a sum of 0, or one that is not a number; it is weighed with 1, so that the latter stays.
     auto weight = [](float top, float now) { return top == -INFINITY ? 1.f : exp2f((top - now) * CE_LOG2E); };
-    for (int r0 = blockIdx.x * 32; r0 < rows; r0 += gridDim.x * 32) {
+    for (int r0 = blockIdx.x * C; r0 < rows; r0 += gridDim.x * C) {
         const int r = r0 + c;
         float top = -INFINITY, sum = 0.f;
-        for (int t0 = g; t0 < parts; t0 += 256) {
+        for (int t0 = g; t0 < parts; t0 += 8 * G) {
             float2 q[8];
 #pragma unroll
-            for (int i = 0; i < 8; i++) q[i] = r < rows && t0 + 32 * i < parts ? part[(long long)(t0 + 32 * i) * rows + r] : make_float2(-INFINITY, 0.f);
+            for (int i = 0; i < 8; i++) q[i] = r < rows && t0 + G * i < parts ? part[(long long)(t0 + G * i) * rows + r] : make_float2(-INFINITY, 0.f);
             float now = top;
 #pragma unroll
             for (int i = 0; i < 8; i++) now = fmaxf(now, q[i].x);
@@ -55,19 +58,27 @@ __global__ void __launch_bounds__(1024) ce_rows_kernel(const float2* __restrict_
         }
         sh[g][c] = make_float2(top, sum);
         __syncthreads();
-        // warp g joins the groups of row r0 + g: lane = group, in a fixed tree
-        float2 q = sh[c][g];
-        float now = q.x;
+        if (warp < C && r0 + warp < rows) {   // warp w joins the groups of row r0 + w
+            float2 q[G / 32];
+            float now = -INFINITY, all = 0.f;
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, o));
-        float all = q.y * weight(q.x, now);
+            for (int i = 0; i < G / 32; i++) {
+                q[i] = sh[i * 32 + lane][warp];
+                now = fmaxf(now, q[i].x);
+            }
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
-        if (c == 0 && r0 + g < rows) {
-            const float l = now + logf(all);
-            const long long t = target[r0 + g];
-            lse[r0 + g] = l;
-            loss[r0 + g] = t == ignore_index ? 0.f : t >= 0 && t < V ? l - label_logit[r0 + g] : NAN;
+            for (int o = 16; o > 0; o >>= 1) now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, o));
+#pragma unroll
+            for (int i = 0; i < G / 32; i++) all += q[i].y * weight(q[i].x, now);
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+            if (lane == 0) {
+                const int row = r0 + warp;
+                const float l = now + logf(all);
+                const long long t = target[row];
+                lse[row] = l;
+                loss[row] = t == ignore_index ? 0.f : t >= 0 && t < V ? l - label_logit[row] : NAN;
+            }
         }
         __syncthreads();
     }
@@ -191,10 +202,14 @@ struct CeBackwardSpace {
 
 using namespace ob200;
 
+// Parts of a row that a forward pass writes; the workspace has room for those of either kernel.
+static int ce_parts(int rows, int V, int H) { return few_rows_fit(rows, V, H) ? few_rows_parts(V) : (V + 127) / 128; }
+
 extern "C" long long ob200_linear_cross_entropy_workspace(int rows, int V) {
     if (rows <= 0 || V <= 0) return 0;
     const long long block = rows < CE_ROW_BLOCK ? rows : CE_ROW_BLOCK;
-    return (long long)ce_round((size_t)block * ((V + 127) / 128) * sizeof(float2)) + block * (long long)sizeof(float);
+    const int a = ce_parts(rows, V, 1), b = (V + 127) / 128;
+    return (long long)ce_round((size_t)block * (a > b ? a : b) * sizeof(float2)) + block * (long long)sizeof(float);
 }
 
 // See include/orion_kernels.h.  -1: sizes or arguments, -2: alignment, -3: workspace too small, -4: no TMA descriptor.
@@ -206,7 +221,7 @@ extern "C" int ob200_linear_cross_entropy_forward(const void* x, const void* w, 
     if (((uintptr_t)x | (uintptr_t)w | (uintptr_t)workspace) % 16 || (ldx | ldw) % 8) return -2;
     if (workspace_bytes < ob200_linear_cross_entropy_workspace(rows, V) || (!workspace && rows > 0)) return -3;
     cudaStream_t st = (cudaStream_t)stream;
-    const int block = rows < CE_ROW_BLOCK ? rows : CE_ROW_BLOCK, parts = (V + 127) / 128;
+    const int block = rows < CE_ROW_BLOCK ? rows : CE_ROW_BLOCK, parts = ce_parts(rows, V, H);
     float2* part = (float2*)workspace;
     float* label_logit = (float*)((char*)workspace + ce_round((size_t)block * parts * sizeof(float2)));
     for (int r0 = 0; r0 < rows; r0 += CE_ROW_BLOCK) {
@@ -222,12 +237,19 @@ extern "C" int ob200_linear_cross_entropy_forward(const void* x, const void* w, 
         g.e.label_logit = label_logit;
         g.num_ctas = num_ctas;
         g.stream = stream;
-        int rc = gemm_bf16_run(g);
+        int rc = few_rows_fit(rows, V, H) ? few_rows_run(g) : gemm_bf16_run(g);
         if (rc) return rc;
-        const int want = (n + 31) / 32, cap = num_ctas * 2;
-        OB200_ELASTIC_HBM(ce_rows_kernel, 2);
-        rc = launch_pdl(ce_rows_kernel, (unsigned)(want < cap ? want : cap), 1024u, st, (const float2*)part, (const float*)label_logit,
-                        target + r0, loss + r0, lse + r0, n, parts, V, ignore_index);
+        const int per_cta = n <= 64 ? 4 : 32, want = (n + per_cta - 1) / per_cta, cap = num_ctas * 2;
+        const unsigned grid = (unsigned)(want < cap ? want : cap);
+        if (per_cta == 4) {
+            OB200_ELASTIC_HBM(ce_rows_kernel<4>, 2);
+            rc = launch_pdl(ce_rows_kernel<4>, grid, 1024u, st, (const float2*)part, (const float*)label_logit, target + r0, loss + r0, lse + r0, n, parts, V,
+                            ignore_index);
+        } else {
+            OB200_ELASTIC_HBM(ce_rows_kernel<32>, 2);
+            rc = launch_pdl(ce_rows_kernel<32>, grid, 1024u, st, (const float2*)part, (const float*)label_logit, target + r0, loss + r0, lse + r0, n, parts, V,
+                            ignore_index);
+        }
         if (rc) return rc;
     }
     if (!total) return 0;

@@ -38,9 +38,18 @@ int* status_word(int dev) {
         cached = it->second;
         return cached;
     }
+    // The first call on a device may come while some stream is being captured: allocating and clearing on a stream of its own
+    // concerns no capture, and the relaxed mode says so.
     int* p = nullptr;
-    if (cudaMalloc(&p, sizeof(int)) != cudaSuccess) return nullptr;
-    cudaMemset(p, 0, sizeof(int));
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    cudaStream_t own = nullptr;
+    bool ok = cudaMalloc(&p, sizeof(int)) == cudaSuccess;
+    ok = ok && cudaStreamCreateWithFlags(&own, cudaStreamNonBlocking) == cudaSuccess;
+    ok = ok && cudaMemsetAsync(p, 0, sizeof(int), own) == cudaSuccess && cudaStreamSynchronize(own) == cudaSuccess;
+    if (own) cudaStreamDestroy(own);
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    if (!ok) return nullptr;
     g_status[dev] = p;
     return p;
 }

@@ -14,7 +14,7 @@ namespace ob200 {
 // Launches a kernel that begins with pdl_wait() as a programmatic dependent of the kernel before it in the stream: launch and
 // set-up overlap that kernel's tail, about 2 us per launch of a chain of short kernels.  ORION_PDL=0: plain stream order.
 template <typename... KArgs, typename... Args>
-inline int launch_pdl(void (*kernel)(KArgs...), unsigned grid, unsigned block, cudaStream_t stream, Args... args) {
+inline int launch_pdl_smem(void (*kernel)(KArgs...), unsigned grid, unsigned block, size_t smem, cudaStream_t stream, Args... args) {
     static const bool pdl = [] {
         const char* e = getenv("ORION_PDL");
         return !(e && e[0] == '0');
@@ -23,6 +23,7 @@ inline int launch_pdl(void (*kernel)(KArgs...), unsigned grid, unsigned block, c
     memset(&cfg, 0, sizeof cfg);
     cfg.gridDim = dim3(grid);
     cfg.blockDim = dim3(block);
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -30,6 +31,10 @@ inline int launch_pdl(void (*kernel)(KArgs...), unsigned grid, unsigned block, c
     cfg.attrs = attr;
     cfg.numAttrs = pdl ? 1 : 0;
     return (int)cudaLaunchKernelEx(&cfg, kernel, (KArgs)args...);
+}
+template <typename... KArgs, typename... Args>
+inline int launch_pdl(void (*kernel)(KArgs...), unsigned grid, unsigned block, cudaStream_t stream, Args... args) {
+    return launch_pdl_smem(kernel, grid, block, 0, stream, args...);
 }
 
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }

@@ -24,6 +24,16 @@ __device__ __forceinline__ DropKey drop_key(const long long* rng, uint32_t site)
     const unsigned long long seed = (unsigned long long)rng[0], step = (unsigned long long)rng[1];
     return {(uint32_t)seed, (uint32_t)(seed >> 32), (uint32_t)step, (uint32_t)(step >> 32) << 16, site};
 }
+// The same for a converged warp: taken by shuffle the key is known to be the same in all lanes, and its rounds cost a warp's
+// arithmetic nothing.
+__device__ __forceinline__ DropKey drop_key_warp(const long long* rng, uint32_t site) {
+    DropKey k = drop_key(rng, site);
+    k.k0 = __shfl_sync(0xffffffffu, k.k0, 0);
+    k.k1 = __shfl_sync(0xffffffffu, k.k1, 0);
+    k.step = __shfl_sync(0xffffffffu, k.step, 0);
+    k.step_hi = __shfl_sync(0xffffffffu, k.step_hi, 0);
+    return k;
+}
 
 // The 128 bits of elements 8 * group .. 8 * group + 7.
 __device__ __forceinline__ void drop_bits(const DropKey& key, unsigned long long group, uint32_t (&c)[4]) {

@@ -150,6 +150,42 @@ def test_linear_act_gradients(ops, M, N, K, act, residual, p, bias):
             assert torch.equal(got.pop(0), dy)
 
 
+@pytest.mark.parametrize("M", [1, 8, 9, 16, 17, 32])
+@pytest.mark.parametrize("N,K", [(20000, 512), (20003, 1000), (2500, 4096), (1000, 5000), (9000, 40), (7, 8)])
+def test_linear_act_of_few_rows(ops, M, N, K):
+    """Single tokens: tiles of 8 and 16 rows of w, one and many of them for a CTA (the rings come round), reductions of one piece and
+    of several, ragged ends of each; the same bits from any CTA count."""
+    x, w, b, r = make(M, N, K, True, BF, M + N)
+    rng = rng_of(5, 6)
+    want, bound = expect(x, w, b, r, "gelu", 0.1, rng, 2)[:2]
+    y = ops.linear_act(x, w, b, r, "gelu", 0.1, rng, 2)
+    within(y, want, bound, "y")
+    for q in (100, 3):
+        ops.set_sm_quota(q)
+        again = ops.linear_act(x, w, b, r, "gelu", 0.1, rng, 2)
+        ops.set_sm_quota(0)
+        assert torch.equal(again, y)
+    # what a row of x holds beyond the others' concerns it alone
+    bad = x.clone()
+    bad[0] = float("nan")
+    y2 = ops.linear_act(bad, w, b, r)
+    assert y2[0].isnan().all() and torch.equal(y2[1:], ops.linear_act(x, w, b, r)[1:])
+
+
+@pytest.mark.parametrize("T", [1, 8, 13, 32])
+@pytest.mark.parametrize("V,H", [(32000, 1024), (20003, 200), (5000, 1536)])
+def test_loss_of_few_rows(ops, T, V, H):
+    torch.manual_seed(T + V)
+    x, w = torch.randn(T, H, device="cuda").to(BF), (torch.randn(V, H, device="cuda") * 2 / math.sqrt(H)).to(BF)
+    target = torch.randint(0, V, (T,), device="cuda")
+    target[0] = V - 1
+    out, _, _ = check_loss(ops, x, w, target, "none")
+    ops.set_sm_quota(5)
+    again = ops.linear_cross_entropy(x, w, target, reduction="none")
+    ops.set_sm_quota(0)
+    assert torch.equal(again, out)
+
+
 def test_linear_act_gradient_is_the_difference_quotient(ops):
     """f(w) = sum(y * dy) along d: without an activation f is linear, so the quotient over any step is the derivative; with GELU the
     remainder of the central quotient is h^2 / 6 of the third derivative, |gelu'''| <= 2.4.  Steps and values have few bits, so that

@@ -27,6 +27,7 @@ SHIM = """
 #define __device__
 #define __forceinline__ inline
 #define __host__
+static inline uint32_t __shfl_sync(uint32_t, uint32_t v, int) { return v; }
 %s
 extern "C" void bits(uint32_t* c, const uint32_t* k) {
     // a counter of four words as (group, step, site): the step's upper bits and the group's share word 1
@@ -160,7 +161,8 @@ def test_entry_points_refuse_bad_arguments_without_a_gpu(K):
 def test_backward_of_the_loss_takes_less_scratch_than_the_logits(K):
     L = K.lib()
     rows, V, H = 8192, 32000, 1024
-    assert L.ob200_linear_cross_entropy_backward_workspace(rows, V, H, 1, 1) < 0.4 * rows * V * 2
+    # gradients of a piece's logits (at most 192 MB), a copy of x in bfloat16 and dx in float32: under half of the 524 MB
+    assert L.ob200_linear_cross_entropy_backward_workspace(rows, V, H, 1, 1) < 0.5 * rows * V * 2
     assert L.ob200_linear_cross_entropy_workspace(rows, V) < 0.05 * rows * V * 2
 
 
