@@ -253,22 +253,22 @@ int ob200_adamw_f32(float* p, const float* g, float* m, float* v, long long n, f
  * kept share, where 16 bits of Philox4x32-10 (Salmon et al., SC'11) are at least round(65536 p); element i of the flattened y takes half
  * i % 8 of the four words at counter (low 32 bits of i / 8, bits 32..47 of i / 8 | bits 32..47 of step << 16, low 32 bits of step, site)
  * under the key seed.  rng points to (seed, step) in device memory, read when the kernel runs, so that a captured graph draws a new
- * mask when the step moves on; `site` tells the calls of one step apart.  pre (NULL: not wanted), rows ld_pre apart (a multiple of 8):
- * x . w^T + bias in bfloat16, which the backward pass of an activation needs.  workspace: the bytes that
+ * mask when the step moves on; `site` tells the calls of one step apart.  slope (NULL: not wanted), rows ld_slope apart (a multiple of
+ * 8): the activation's derivative at x . w^T + bias in bfloat16, which the backward pass multiplies by.  workspace: the bytes that
  * ob200_linear_act_workspace names (0: none), any contents, the call's own until it has run.
  * Returns -1 for bad arguments, -2 for misaligned pointers or strides, -3 for a workspace that is too small, -4 when a TMA descriptor
  * cannot be built.  Stands for the sgemm, bias, GELU, fused_dropout_kernel_vec and add rows of the reference's
  * benchmarking/model_kernels/bert_8_fb1 (src/scheduler/utils_sched.cpp:490-501; src/cuda_capture/intercept_temp.cpp:418-458). */
-int ob200_linear_act_bf16(const void* x, const void* w, void* y, void* pre, const void* bias, int bias_f32, const void* residual, int act,
-                          float p, const long long* rng, int site, int M, int N, int K, long long ldx, long long ldw, long long ld_pre,
+int ob200_linear_act_bf16(const void* x, const void* w, void* y, void* slope, const void* bias, int bias_f32, const void* residual, int act,
+                          float p, const long long* rng, int site, int M, int N, int K, long long ldx, long long ldw, long long ld_slope,
                           void* workspace, long long workspace_bytes, int num_ctas, void* stream);
 long long ob200_linear_act_workspace(int M, int N, int K);
-/* Its gradients: dz = dropout(dy) * act'(pre), dbias = column sums of dz (in a fixed order, in the bias's type), dx = dz . w,
- * dw = dz^T . x; dy [M, N], dx [M, K], dw [N, K] contiguous, 16-byte aligned; dx, dw, dbias may be NULL (not wanted); pre only with an
+/* Its gradients: dz = dropout(dy) * slope, dbias = column sums of dz (in a fixed order, in the bias's type), dx = dz . w,
+ * dw = dz^T . x; dy [M, N], dx [M, K], dw [N, K] contiguous, 16-byte aligned; dx, dw, dbias may be NULL (not wanted); slope only with an
  * activation.  The residual's gradient is dy. */
-int ob200_linear_act_backward_bf16(const void* dy, const void* pre, const void* x, const void* w, void* dx, void* dw, void* dbias,
+int ob200_linear_act_backward_bf16(const void* dy, const void* slope, const void* x, const void* w, void* dx, void* dw, void* dbias,
                                    int bias_f32, int act, float p, const long long* rng, int site, int M, int N, int K, long long ldx,
-                                   long long ldw, long long ld_pre, void* workspace, long long workspace_bytes, int num_ctas, void* stream);
+                                   long long ldw, long long ld_slope, void* workspace, long long workspace_bytes, int num_ctas, void* stream);
 long long ob200_linear_act_backward_workspace(int M, int N, int K, int act, float p, int want_dx, int want_dw, int want_dbias);
 
 /* y = dropout(x) [+ residual] over n contiguous elements with the mask above (dtype 0 float32, 1 bfloat16; residual may be NULL; y may

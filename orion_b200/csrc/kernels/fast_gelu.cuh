@@ -87,15 +87,27 @@ __device__ __forceinline__ void gelu_pair(float& a0, float& a1) {
     const uint64_t tail = gauss_tail_pair(f32x2(a0, a1), nx, e);
     split_f32x2(fma_f32x2(nx, tail, f32x2(fmaxf(a0, 0.f), fmaxf(a1, 0.f))), a0, a1);
 }
-// d *= Phi(a) + a * density(a)
-__device__ __forceinline__ void gelu_slope_pair(float& d0, float& d1, float a0, float a1) {
-    const uint64_t a = f32x2(a0, a1);
-    uint64_t e;
-    float s0, s1;
-    split_f32x2(gauss_tail_pair(a, gauss_clamp_pair(a0, a1), e), s0, s1);
-    const uint64_t cdf = f32x2(a0 >= 0.f ? 1.0f - s0 : s0, a1 >= 0.f ? 1.0f - s1 : s1);
+// The same with the slopes Phi(a) + a * density(a), from the exponential that is there.
+__device__ __forceinline__ void gelu_slope_pair(float& a0, float& a1, float& s0, float& s1) {
+    const uint64_t a = f32x2(a0, a1), nx = gauss_clamp_pair(a0, a1);
     constexpr float kDensity = 0.3989422804014327f;
-    split_f32x2(mul_f32x2(f32x2(d0, d1), fma_f32x2(mul_f32x2(a, f32x2(kDensity, kDensity)), e, cdf)), d0, d1);
+    uint64_t e;
+    const uint64_t tail = gauss_tail_pair(a, nx, e);
+    float t0, t1;
+    split_f32x2(tail, t0, t1);
+    const uint64_t cdf = f32x2(a0 >= 0.f ? 1.0f - t0 : t0, a1 >= 0.f ? 1.0f - t1 : t1);
+    split_f32x2(fma_f32x2(mul_f32x2(a, f32x2(kDensity, kDensity)), e, cdf), s0, s1);
+    split_f32x2(fma_f32x2(nx, tail, f32x2(fmaxf(a0, 0.f), fmaxf(a1, 0.f))), a0, a1);
+}
+// One value: act(a) and its slope; 0 none, 1 ReLU, 2 GELU.
+__device__ __forceinline__ float act_slope(float a, int act, float& slope) {
+    if (act == 2) {
+        float b = 0.f, unused;
+        gelu_slope_pair(a, b, slope, unused);
+        return a;
+    }
+    slope = act == 1 && !(a > 0.f) ? 0.f : 1.f;
+    return act == 1 ? fmaxf(a, 0.f) : a;
 }
 
 }  // namespace ob200

@@ -111,8 +111,11 @@ __device__ __forceinline__ void few_way_out(const FewRowsParams& p, const float 
 #pragma unroll
             for (int k = 0; k < WARPS; k++) z += red[k][r][m];
             z += add;
-            if (p.e.pre) p.e.pre[m * p.e.ld_pre + n] = __float2bfloat16_rn(z);
-            z = p.e.act == 2 ? z * gauss_cdf(z) : p.e.act == 1 ? fmaxf(z, 0.f) : z;
+            if (p.e.act) {
+                float slope;
+                z = act_slope(z, p.e.act, slope);
+                if (p.e.slope) p.e.slope[m * p.e.ld_slope + n] = __float2bfloat16_rn(slope);
+            }
             if (p.e.drop_threshold) {
                 uint32_t bits[4];
                 drop_bits(drop_key(p.e.rng, p.e.site), (unsigned long long)index >> 3, bits);

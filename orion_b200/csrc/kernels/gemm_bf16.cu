@@ -48,7 +48,7 @@ constexpr int GM_BM = 128;
 constexpr int GM_BK = 64;
 // Warp 0: TMA, warp 1: MMA + tensor memory, the others: epilogue.  Four of them, or sixteen (four for each 32 rows, each a share of the
 // columns) where a turn of the epilogue is a long chain of latencies: bias + GELU of 8192 x 4096 x 1024.
-__host__ __device__ constexpr int gm_epi_warps(int epi) { return epi == GM_EPI_ACT || epi == GM_EPI_ACT_ANY ? 16 : epi == GM_EPI_DLOGITS ? 8 : 4; }
+__host__ __device__ constexpr int gm_epi_warps(int epi) { return epi == GM_EPI_ACT || epi == GM_EPI_ACT_SLOPE || epi == GM_EPI_ACT_ANY ? 16 : epi == GM_EPI_DLOGITS ? 8 : 4; }
 __host__ __device__ constexpr int gm_threads(int epi) { return 64 + 32 * gm_epi_warps(epi); }
 constexpr int GM_A_BYTES = GM_BM * 128;
 
@@ -85,7 +85,7 @@ struct GemmParams {
     alignas(64) unsigned char tmap_a[128];
     alignas(64) unsigned char tmap_b[128];
     alignas(64) unsigned char tmap_c[128];
-    alignas(64) unsigned char tmap_pre[128];
+    alignas(64) unsigned char tmap_slope[128];
     alignas(64) unsigned char tmap_res[128];
 };
 
@@ -168,6 +168,7 @@ __device__ __forceinline__ GemmUnit gm_unit(const GemmParamsOf<EPI>& p, long lon
 template <int BN, int CG, int EPI>
 __global__ void __launch_bounds__(gm_threads(EPI), 1) gemm_bf16_kernel(const __grid_constant__ GemmParamsOf<EPI> p) {
     using C = GemmCfg<BN, CG, EPI>;
+    constexpr bool kSlope = EPI == GM_EPI_ACT_SLOPE, kAct = EPI == GM_EPI_ACT || kSlope;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     uint8_t* epi_smem = smem + C::STAGES * C::STAGE_BYTES;
@@ -184,7 +185,7 @@ __global__ void __launch_bounds__(gm_threads(EPI), 1) gemm_bf16_kernel(const __g
             mbar_init(&ctl->acc_full[a], 1);
             mbar_init(&ctl->acc_empty[a], gm_epi_warps(EPI) * CG);   // the epilogue warps of both CTAs
         }
-        if (EPI == GM_EPI_ACT)
+        if (kAct)
             for (int i = 0; i < 32; i++) mbar_init(&ctl->res_full[i >> 1][i & 1], 1);
         ctl->abort_flag = 0;
         fence_barrier_init();
@@ -338,12 +339,11 @@ __global__ void __launch_bounds__(gm_threads(EPI), 1) gemm_bf16_kernel(const __g
             const bool idle = part * kCols >= BN;   // a narrow tile has no columns for this warp
             const int m0w = (tm * CG + (int)rank) * GM_BM + q * 32;      // first row of this warp's 32
             bool ahead = false;
-            if constexpr (EPI == GM_EPI_ACT) if (!idle) ahead = gm_residual_ahead<kCols>(p, m0w, tn * BN + part * kCols, epi_smem + (warp - 2) * 4096, slab_i, ctl->res_full[warp - 2]);
+            if constexpr (kAct) if (!idle) ahead = gm_residual_ahead<kSlope>(p, m0w, tn * BN + part * kCols, epi_smem + (warp - 2) * 4096, slab_i, ctl->res_full[warp - 2]);
             if (!mbar_wait_warp(&ctl->acc_full[ab], use & 1u, abort_flag)) {
                 if (!*abort_flag) { ctl->abort_flag = 1; if (p.status) atomicExch(p.status, OB200_ERR_WAIT_TMEM_FULL); }
                 if (ahead) {   // the residual's copy must have landed before the CTA leaves
-                    const uint32_t s = p.e.pre ? 0 : slab_i & 1;
-                    mbar_wait_landed(&ctl->res_full[warp - 2][s], p.e.pre ? slab_i & 1 : (slab_i >> 1) & 1, clock64());
+                    mbar_wait_landed(&ctl->res_full[warp - 2][slab_i & 1], (slab_i >> 1) & 1, clock64());
                 }
                 break;
             }
@@ -352,10 +352,10 @@ __global__ void __launch_bounds__(gm_threads(EPI), 1) gemm_bf16_kernel(const __g
             const int n0 = tn * BN;
             const uint32_t t_row = tmem_base + ((uint32_t)(q * 32) << 16) + ab * BN;
             if (idle) {
-            } else if constexpr (EPI == GM_EPI_ACT || EPI == GM_EPI_ACT_ANY) {
+            } else if constexpr (kAct || EPI == GM_EPI_ACT_ANY) {
                 if (p.splits > 1) gm_epilogue_slab<kCols>(p, t_row + part * kCols, m, n0 + part * kCols, sp);
                 else if constexpr (EPI == GM_EPI_ACT_ANY) gm_epilogue_act_any<kCols>(p, t_row + part * kCols, m, m0w, n0 + part * kCols, lane, epi_smem + (warp - 2) * 4096);
-                else if (!gm_epilogue_act<kCols>(p, t_row + part * kCols, m, m0w, n0 + part * kCols, lane, epi_smem + (warp - 2) * 4096, slab_i, ctl->res_full[warp - 2], abort_flag)) {
+                else if (!gm_epilogue_act<kCols, kSlope>(p, t_row + part * kCols, m, m0w, n0 + part * kCols, lane, epi_smem + (warp - 2) * 4096, slab_i, ctl->res_full[warp - 2], abort_flag)) {
                     if (!*abort_flag) { ctl->abort_flag = 1; if (p.status) atomicExch(p.status, OB200_ERR_WAIT_FULL); }
                     break;
                 }
@@ -589,8 +589,11 @@ __global__ void __launch_bounds__(256) gemm_splitk_act_kernel(const float* __res
                 float a = f[j];
                 if (bias) a += bias[col];
                 if (bias_bf16) a += __bfloat162float(bias_bf16[col]);
-                if (e.pre) e.pre[m * e.ld_pre + col] = __float2bfloat16_rn(a);
-                a = e.act == 2 ? a * gauss_cdf(a) : e.act == 1 ? fmaxf(a, 0.f) : a;
+                if (e.act) {
+                    float slope;
+                    a = act_slope(a, e.act, slope);
+                    if (e.slope) e.slope[m * e.ld_slope + col] = __float2bfloat16_rn(slope);
+                }
                 if (e.drop_threshold) a = mask >> j & 1u ? a * e.drop_scale : 0.f;
                 if (residual) a += __bfloat162float(residual[i0 + j]);
                 f[j] = a;
@@ -639,15 +642,15 @@ static bool gm_make_map(unsigned char* out, const void* base, long long inner, l
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// Tensor map of a bfloat16 matrix [M, N] that is copied 32 rows x 32 columns at a time (64-byte rows, swizzled).
-static bool gm_make_slab_map(unsigned char* out, const void* base, int M, int N, long long ld) {
+// Tensor map of a bfloat16 matrix [M, N] that is copied 32 rows and 32 or 16 columns at a time (64- or 32-byte rows, swizzled).
+static bool gm_make_slab_map(unsigned char* out, const void* base, int M, int N, long long ld, int cols) {
     GmEncodeTiledFn enc = gm_encode_fn();
     if (!enc) return false;
     cuuint64_t dims[2] = {(cuuint64_t)N, (cuuint64_t)M};
     cuuint64_t strides[1] = {(cuuint64_t)ld * 2};
-    cuuint32_t box[2] = {32, 32}, steps[2] = {1, 1};
+    cuuint32_t box[2] = {(cuuint32_t)cols, 32}, steps[2] = {1, 1};
     return enc(reinterpret_cast<CUtensorMap*>(out), CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, box, steps,
-               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+               CU_TENSOR_MAP_INTERLEAVE_NONE, cols == 32 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
@@ -854,11 +857,12 @@ int gemm_bf16_run(const GemmCall& g) {
         const bool aligned = ((uintptr_t)c % 16 == 0) && (ldc * es) % 16 == 0 && (batch_inner == 1 || (c_si * es) % 16 == 0) &&
                              (batch_outer == 1 || (c_so * es) % 16 == 0);
         static const bool tma_off = [] { const char* e = getenv("ORION_GEMM_TMA_STORE"); return e && e[0] == '0'; }();
-        if (epi == GM_EPI_ACT || epi == GM_EPI_DLOGITS) {   // 32 rows x 32 columns a copy
-            if (epi == GM_EPI_ACT && (!aligned || g.bias || ((uintptr_t)g.bias_bf16 | (uintptr_t)residual) % 16)) epi = GM_EPI_ACT_ANY;
-            if (p.splits == 1 && ((epi != GM_EPI_ACT_ANY && !gm_make_slab_map(p.tmap_c, c, M, N, ldc)) ||
-                                  (epi == GM_EPI_ACT && residual && !gm_make_slab_map(p.tmap_res, residual, M, N, N)) ||
-                                  (g.e.pre && !gm_make_slab_map(p.tmap_pre, g.e.pre, M, N, g.e.ld_pre))))
+        if (epi == GM_EPI_ACT || epi == GM_EPI_DLOGITS) {   // by slabs of 32 rows
+            if (epi == GM_EPI_ACT) epi = !aligned || g.bias || ((uintptr_t)g.bias_bf16 | (uintptr_t)residual) % 16 ? GM_EPI_ACT_ANY : g.e.slope ? GM_EPI_ACT_SLOPE : GM_EPI_ACT;
+            const int slab_cols = epi == GM_EPI_ACT_SLOPE ? 16 : 32;
+            if (p.splits == 1 && ((epi != GM_EPI_ACT_ANY && !gm_make_slab_map(p.tmap_c, c, M, N, ldc, slab_cols)) ||
+                                  (epi != GM_EPI_ACT_ANY && residual && !gm_make_slab_map(p.tmap_res, residual, M, N, N, slab_cols)) ||
+                                  (g.e.slope && !gm_make_slab_map(p.tmap_slope, g.e.slope, M, N, g.e.ld_slope, slab_cols))))
                 return -4;
         } else if (epi != GM_EPI_LSE && aligned && !tma_off && p.splits == 1) {
             GmEncodeTiledFn enc = gm_encode_fn();
@@ -893,6 +897,7 @@ int gemm_bf16_run(const GemmCall& g) {
     switch (epi) {
         case GM_EPI_ACC: rc = gm_launch_tile<GM_EPI_ACC>(p, bn, cg, grid, st); break;
         case GM_EPI_ACT: rc = gm_launch_tile<GM_EPI_ACT>(p, bn, cg, grid, st); break;
+        case GM_EPI_ACT_SLOPE: rc = gm_launch_tile<GM_EPI_ACT_SLOPE>(p, bn, cg, grid, st); break;
         case GM_EPI_ACT_ANY: rc = gm_launch_tile<GM_EPI_ACT_ANY>(p, bn, cg, grid, st); break;
         case GM_EPI_LSE: return gm_launch_tile<GM_EPI_LSE>(p, bn, cg, grid, st);
         case GM_EPI_DLOGITS: return gm_launch_tile<GM_EPI_DLOGITS>(p, bn, cg, grid, st);
@@ -900,7 +905,7 @@ int gemm_bf16_run(const GemmCall& g) {
     }
     if (rc != 0 || p.splits == 1) return rc;
     const long long elems = batch_ll * M * N;
-    if (epi == GM_EPI_ACT || epi == GM_EPI_ACT_ANY) {
+    if (epi == GM_EPI_ACT || epi == GM_EPI_ACT_SLOPE || epi == GM_EPI_ACT_ANY) {
         long long blocks = ((elems + 7) / 8 + 255) / 256;
         if (blocks > 8LL * num_ctas) blocks = 8LL * num_ctas;
         OB200_ELASTIC_HBM(gemm_splitk_act_kernel, 8);

@@ -10,8 +10,9 @@ namespace ob200 {
 enum : int {
     GM_EPI_PLAIN = 0,    // C = alpha * A.B^T (+ bias) (+ bfloat16 residual)
     GM_EPI_ACC = 1,      // the same plus a float32 addend (which may be C itself)
-    GM_EPI_ACT = 2,      // C = residual + dropout(act(A.B^T + bias)), optionally A.B^T + bias beside it
+    GM_EPI_ACT = 2,      // C = residual + dropout(act(A.B^T + bias)), optionally the activation's slope beside it
     GM_EPI_ACT_ANY = 3,  // GM_EPI_ACT for widths, types and alignments that its vector accesses do not take (chosen by the launcher)
+    GM_EPI_ACT_SLOPE = 7,// GM_EPI_ACT with the slope (chosen by the launcher)
     GM_EPI_LSE = 4,      // no C: per row and 128 columns the maximum and the sum of exponentials, and the label's column
     GM_EPI_DLOGITS = 5,  // C = (exp(A.B^T - lse) - onehot(label)) * coefficient
     GM_EPI_DUAL = 6,     // two products of one launch, each plain (the first one with GM_EPI_ACC's addend)
@@ -26,8 +27,8 @@ struct GemmEpi {
     float drop_scale;
     const long long* rng;           // (seed, step), in device memory
     uint32_t site;
-    __nv_bfloat16* pre;             // optional: A.B^T + bias, rows ld_pre apart (a multiple of 8)
-    long long ld_pre;
+    __nv_bfloat16* slope;           // optional, with an activation: act'(A.B^T + bias), rows ld_slope apart (a multiple of 8)
+    long long ld_slope;
     // GM_EPI_LSE, GM_EPI_DLOGITS
     const long long* target;        // label of every row
     long long col0;                 // column of the vocabulary that column 0 of this product is

@@ -1,25 +1,26 @@
 // Epilogues of the bfloat16 GEMM (included by gemm_bf16.cu, inside its namespace): what a warp does with its 32 rows of a finished
 // tile in tensor memory, thread = row, 32 columns at a time.  Arithmetic is float32; an output is rounded to bfloat16 once, staged in
-// a swizzled slab of 32 rows x 64 bytes and written by a TMA store.  A warp has two such slabs: its turns alternate between them, or
-// the pre-activation has the second one and a turn waits until the stores of the turn before have read theirs.
+// a swizzled slab of 32 rows x 64 bytes and written by a TMA store.  A warp's turns alternate between two slabs.
 
 __device__ __forceinline__ uint32_t gm_pack(float a, float b) {
     const __nv_bfloat162 h2 = __floats2bfloat162_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&h2);
 }
 
-// 32 bfloat16 values of this thread's row into a slab of 64-byte rows, 64-byte swizzle (16-byte chunk index XOR (row / 2) % 4: eight
-// consecutive rows of one chunk fall into eight different bank groups).
-__device__ __forceinline__ void gm_stage32(uint8_t* slab, int lane, const float (&f)[32]) {
+// Byte of 16-byte chunk `ch` of this thread's row in a slab of 32 rows x W columns, in the swizzle of its tensor map (64 or 32 bytes
+// wide: eight consecutive rows of one chunk fall into eight different bank groups).
+template <int W>
+__device__ __forceinline__ int gm_slab_chunk(int lane, int ch) {
+    return W == 32 ? lane * 64 + ((ch ^ ((lane >> 1) & 3)) << 4) : lane * 32 + ((ch ^ ((lane >> 2) & 1)) << 4);
+}
+// W bfloat16 values of this thread's row into a slab.
+template <int W>
+__device__ __forceinline__ void gm_stage(uint8_t* slab, int lane, const float (&f)[W]) {
 #pragma unroll
-    for (int ch = 0; ch < 4; ch++) {
-        uint4 pk;
-        pk.x = gm_pack(f[ch * 8], f[ch * 8 + 1]);
-        pk.y = gm_pack(f[ch * 8 + 2], f[ch * 8 + 3]);
-        pk.z = gm_pack(f[ch * 8 + 4], f[ch * 8 + 5]);
-        pk.w = gm_pack(f[ch * 8 + 6], f[ch * 8 + 7]);
-        *reinterpret_cast<uint4*>(slab + lane * 64 + ((ch ^ ((lane >> 1) & 3)) << 4)) = pk;
-    }
+    for (int ch = 0; ch < W / 8; ch++)
+        *reinterpret_cast<uint4*>(slab + gm_slab_chunk<W>(lane, ch)) =
+            make_uint4(gm_pack(f[ch * 8], f[ch * 8 + 1]), gm_pack(f[ch * 8 + 2], f[ch * 8 + 3]), gm_pack(f[ch * 8 + 4], f[ch * 8 + 5]),
+                       gm_pack(f[ch * 8 + 6], f[ch * 8 + 7]));
 }
 
 // f += eight bfloat16 values (the upper halves of float32 ones).
@@ -32,12 +33,43 @@ __device__ __forceinline__ void gm_add8(float* f, uint4 v) {
 }
 
 // (Never issued ahead of its wait: the compiler takes the registers for filled and may move them.)
-__device__ __forceinline__ void gm_load32(uint32_t t_addr, float (&f)[32]) {
+__device__ __forceinline__ void gm_load(uint32_t t_addr, float (&f)[32]) {
     uint32_t v[32];
     tmem_ld_32x32(t_addr, v);
     tmem_ld_wait();
 #pragma unroll
     for (int j = 0; j < 32; j++) f[j] = __uint_as_float(v[j]);
+}
+__device__ __forceinline__ void gm_load(uint32_t t_addr, float (&f)[16]) {
+    uint32_t v[16];
+    tmem_ld_32x16(t_addr, v);
+    tmem_ld_wait();
+#pragma unroll
+    for (int j = 0; j < 16; j++) f[j] = __uint_as_float(v[j]);
+}
+
+// The activation of W values, and its slopes into a slab.
+template <int W>
+__device__ __forceinline__ void gm_act_slope(float (&f)[W], int act, uint8_t* slab, int lane) {
+#pragma unroll
+    for (int ch = 0; ch < W / 8; ch++) {
+        uint32_t w[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            float &a0 = f[ch * 8 + e * 2], &a1 = f[ch * 8 + e * 2 + 1];
+            float s0, s1;
+            if (act == 2) {
+                gelu_slope_pair(a0, a1, s0, s1);
+            } else {
+                s0 = a0 > 0.f ? 1.f : 0.f;
+                s1 = a1 > 0.f ? 1.f : 0.f;
+                a0 = fmaxf(a0, 0.f);
+                a1 = fmaxf(a1, 0.f);
+            }
+            w[e] = gm_pack(s0, s1);
+        }
+        *reinterpret_cast<uint4*>(slab + gm_slab_chunk<W>(lane, ch)) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
 }
 
 // Partial matrices of a product with split-K, as they are: the rest is gemm_splitk_act_kernel's.
@@ -69,24 +101,26 @@ __device__ __forceinline__ void gm_epilogue_slab(const GemmParams& p, uint32_t t
 // the arithmetic: no path for ragged widths, and the residual
 // brought into the slab that the output will leave from by a TMA load one turn ahead (read by the threads, each a row, it took 25 us of
 // 8192 x 4096; so 13).  The residual of the first turn is asked for before the accumulator is waited for (gm_residual_ahead).
-template <int COLS>
+// With the slope a turn has 16 columns instead of 32, so that a warp's 4 KB still are two turns of slabs and the registers suffice.
+template <bool SLOPE>
+constexpr int kActCols = SLOPE ? 16 : 32;
+template <bool SLOPE>
 __device__ __forceinline__ bool gm_residual_ahead(const GemmParams& p, int m0w, int n0, uint8_t* stage, uint32_t turn, uint64_t* bars) {
     if (!p.residual || p.splits > 1 || n0 >= p.N) return false;
     if (elect_one()) {
-        if (p.e.pre) bulk_wait_group_read<0>();
-        else bulk_wait_group_read<1>();
-        const uint32_t s = p.e.pre ? 0 : turn & 1;
-        mbar_arrive_expect_tx(&bars[s], 2048);
-        tma_load_tile_2d(smem_u32(stage + s * 2048), p.tmap_res, &bars[s], n0, m0w);
+        bulk_wait_group_read<1>();
+        mbar_arrive_expect_tx(&bars[turn & 1], kActCols<SLOPE> * 64);
+        tma_load_tile_2d(smem_u32(stage + (turn & 1) * 2048), p.tmap_res, &bars[turn & 1], n0, m0w);
     }
     __syncwarp();
     return true;
 }
-template <int COLS>
+template <int COLS, bool SLOPE>
 __device__ __forceinline__ bool gm_epilogue_act(const GemmParams& p, uint32_t t_row, int m, int m0w, int n0, int lane, uint8_t* stage, uint32_t& turn,
                                                 uint64_t* bars, volatile int* abort_flag) {
+    constexpr int W = kActCols<SLOPE>;
     if (n0 >= p.N) return true;
-    const bool has_pre = p.e.pre != nullptr, has_res = p.residual != nullptr;
+    const bool has_res = p.residual != nullptr;
     const int cols = p.N - n0 < COLS ? p.N - n0 : COLS, act = p.e.act;
     const uint32_t threshold = p.e.drop_threshold;
     DropKey key = {};
@@ -94,58 +128,57 @@ __device__ __forceinline__ bool gm_epilogue_act(const GemmParams& p, uint32_t t_
     unsigned long long group = ((unsigned long long)m * p.N + n0) >> 3;
     const __nv_bfloat16* bias = p.bias_bf16 ? p.bias_bf16 + n0 : nullptr;
 #pragma unroll 1
-    for (int c0 = 0; c0 < cols; c0 += 32) {
-        uint4 b[4];
+    for (int c0 = 0; c0 < cols; c0 += W, turn++) {
+        uint4 b[W / 8];
         if (bias) {
 #pragma unroll
-            for (int ch = 0; ch < 4; ch++)
+            for (int ch = 0; ch < W / 8; ch++)
                 if (c0 + ch * 8 < cols) b[ch] = __ldg(reinterpret_cast<const uint4*>(bias + c0 + ch * 8));
         }
-        float f[32];
-        gm_load32(t_row + c0, f);
+        float f[W];
+        gm_load(t_row + c0, f);
         if (bias) {
 #pragma unroll
-            for (int ch = 0; ch < 4; ch++) gm_add8(f + ch * 8, b[ch]);
+            for (int ch = 0; ch < W / 8; ch++) gm_add8(f + ch * 8, b[ch]);
         }
-        uint8_t* slab = has_pre ? stage : stage + (turn & 1) * 2048;
-        if (has_pre) {
-            if (elect_one()) bulk_wait_group_read<0>();
-            __syncwarp();
-            gm_stage32(stage + 2048, lane, f);
-        }
-        if (act == 2) {
+        uint8_t* slab = stage + (turn & 1) * 2048;
+        if (SLOPE) {
+            if (!has_res) {
+                if (elect_one()) bulk_wait_group_read<1>();   // the stores of two turns ago have read their slabs
+                __syncwarp();
+            }
+            gm_act_slope<W>(f, act, slab + 1024, lane);
+        } else if (act == 2) {
 #pragma unroll
-            for (int j = 0; j < 32; j += 2) gelu_pair(f[j], f[j + 1]);
+            for (int j = 0; j < W; j += 2) gelu_pair(f[j], f[j + 1]);
         } else if (act == 1) {
 #pragma unroll
-            for (int j = 0; j < 32; j++) f[j] = fmaxf(f[j], 0.f);
+            for (int j = 0; j < W; j++) f[j] = fmaxf(f[j], 0.f);
         }
         if (threshold) {
-            drop_apply32(key, group, threshold, p.e.drop_scale, f);
-            group += 4;
+            drop_apply<W>(key, group, threshold, p.e.drop_scale, f);
+            group += W / 8;
         }
         if (has_res) {
-            const uint32_t s = has_pre ? 0 : turn & 1, ph = has_pre ? turn & 1 : (turn >> 1) & 1;
-            if (!mbar_wait_warp(&bars[s], ph, abort_flag)) return false;
+            if (!mbar_wait_warp(&bars[turn & 1], (turn >> 1) & 1, abort_flag)) return false;
 #pragma unroll
-            for (int ch = 0; ch < 4; ch++) gm_add8(f + ch * 8, *reinterpret_cast<const uint4*>(slab + lane * 64 + ((ch ^ ((lane >> 1) & 3)) << 4)));
-        } else if (!has_pre) {
-            if (elect_one()) bulk_wait_group_read<1>();   // the store of two turns ago has read this slab
+            for (int ch = 0; ch < W / 8; ch++) gm_add8(f + ch * 8, *reinterpret_cast<const uint4*>(slab + gm_slab_chunk<W>(lane, ch)));
+        } else if (!SLOPE) {
+            if (elect_one()) bulk_wait_group_read<1>();
             __syncwarp();
         }
-        gm_stage32(slab, lane, f);
+        gm_stage<W>(slab, lane, f);
         fence_proxy_async_smem();
         __syncwarp();
-        turn++;
         if (elect_one()) {
             if (m0w < p.M) {
                 tma_store_tile_2d(p.tmap_c, smem_u32(slab), n0 + c0, m0w);
-                if (has_pre) tma_store_tile_2d(p.tmap_pre, smem_u32(stage + 2048), n0 + c0, m0w);
+                if (SLOPE) tma_store_tile_2d(p.tmap_slope, smem_u32(slab + 1024), n0 + c0, m0w);
             }
             bulk_commit_group();
         }
         __syncwarp();
-        if (c0 + 32 < cols) gm_residual_ahead<COLS>(p, m0w, n0 + c0 + 32, stage, turn, bars);
+        if (c0 + W < cols) gm_residual_ahead<SLOPE>(p, m0w, n0 + c0 + W, stage, turn + 1, bars);
     }
     return true;
 }
@@ -161,17 +194,18 @@ __device__ __forceinline__ void gm_epilogue_act_any(const GemmParams& p, uint32_
         const int n = n0 + c0;
         if (n >= p.N) break;            // warp-uniform
         float f[32];
-        gm_load32(t_row + c0, f);
+        gm_load(t_row + c0, f);
         const long long index = (long long)m * p.N + n;
         if (p.bias || p.bias_bf16) {
 #pragma unroll
             for (int j = 0; j < 32; j++)
                 if (n + j < p.N) f[j] += p.bias ? __ldg(p.bias + n + j) : __bfloat162float(p.bias_bf16[n + j]);
         }
-        if (elect_one()) bulk_wait_group_read<0>();   // the pre-activations of the turn before have left
+        if (elect_one()) bulk_wait_group_read<0>();   // the slopes of the turn before have left
         __syncwarp();
-        if (p.e.pre) gm_stage32(stage + 2048, lane, f);
-        if (p.e.act == 2) {
+        if (p.e.slope) {
+            gm_act_slope<32>(f, p.e.act, stage + 2048, lane);
+        } else if (p.e.act == 2) {
 #pragma unroll
             for (int j = 0; j < 32; j += 2) gelu_pair(f[j], f[j + 1]);
         } else if (p.e.act == 1) {
@@ -188,11 +222,11 @@ __device__ __forceinline__ void gm_epilogue_act_any(const GemmParams& p, uint32_
             for (int j = 0; j < 32; j++)
                 if (n + j < p.N) f[j] += __bfloat162float(p.residual[index + j]);
         }
-        gm_stage32(stage, lane, f);
+        gm_stage<32>(stage, lane, f);
         fence_proxy_async_smem();
         __syncwarp();
         if (elect_one()) {
-            if (m0w < p.M && p.e.pre) tma_store_tile_2d(p.tmap_pre, smem_u32(stage + 2048), n, m0w);
+            if (m0w < p.M && p.e.slope) tma_store_tile_2d(p.tmap_slope, smem_u32(stage + 2048), n, m0w);
             bulk_commit_group();
         }
         // lane = column, one row after the other, so that a store covers 64 consecutive bytes
@@ -201,7 +235,7 @@ __device__ __forceinline__ void gm_epilogue_act_any(const GemmParams& p, uint32_
 #pragma unroll 4
         for (int r = 0; r < rows; r++)
             if (n + lane < p.N)
-                out[r * p.ldc] = *reinterpret_cast<const __nv_bfloat16*>(stage + r * 64 + (((lane >> 3) ^ ((r >> 1) & 3)) << 4) + (lane & 7) * 2);
+                out[r * p.ldc] = *reinterpret_cast<const __nv_bfloat16*>(stage + gm_slab_chunk<32>(r, lane >> 3) + (lane & 7) * 2);
         __syncwarp();
     }
 }
@@ -219,7 +253,7 @@ __device__ __forceinline__ void gm_epilogue_lse(const GemmParams& p, uint32_t t_
         const int n = n0 + c0;
         if (n >= p.N) break;            // warp-uniform
         float f[32];
-        gm_load32(t_row + c0, f);
+        gm_load(t_row + c0, f);
         if (n + 32 > p.N) {
 #pragma unroll
             for (int j = 0; j < 32; j++)
@@ -267,7 +301,7 @@ __device__ __forceinline__ void gm_epilogue_dlogits(const GemmParams& p, uint32_
         const int n = n0 + c0;
         if (n >= p.N) break;            // warp-uniform
         float f[32];
-        gm_load32(t_row + c0, f);
+        gm_load(t_row + c0, f);
 #pragma unroll
         for (int j = 0; j < 32; j += 2) {
             float e0, e1;
@@ -287,7 +321,7 @@ __device__ __forceinline__ void gm_epilogue_dlogits(const GemmParams& p, uint32_
         uint8_t* slab = stage + (turn++ & 1) * 2048;
         if (elect_one()) bulk_wait_group_read<1>();
         __syncwarp();
-        gm_stage32(slab, lane, f);
+        gm_stage<32>(slab, lane, f);
         __syncwarp();
         fence_proxy_async_smem();
         __syncwarp();
@@ -312,7 +346,7 @@ __device__ __forceinline__ void gm_epilogue_dual(const GemmParamsDual& p, bool s
         const int n = n0 + c0;
         if (n >= N) break;              // warp-uniform
         float f[32];
-        gm_load32(t_row + c0, f);
+        gm_load(t_row + c0, f);
         if (addend) {                   // N is a multiple of 8
 #pragma unroll
             for (int j = 0; j < 32; j += 4)

@@ -65,7 +65,7 @@ struct Pack8<__nv_bfloat16> {
 // ------------------------------------------------------------------ dropout (+ residual)
 // A thread takes eight consecutive elements, one draw of the generator.  VEC: all pointers are 16-byte aligned.
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(LA_THREADS) dropout_kernel(const T* __restrict__ x, const T* __restrict__ residual, T* __restrict__ y, long long n,
+__global__ void __launch_bounds__(LA_THREADS, 6) dropout_kernel(const T* __restrict__ x, const T* __restrict__ residual, T* __restrict__ y, long long n,
                                                              const long long* __restrict__ rng, uint32_t site, uint32_t threshold, float scale) {
     pdl_wait();
     pdl_launch_dependents();
@@ -106,13 +106,13 @@ __global__ void __launch_bounds__(LA_THREADS) dropout_kernel(const T* __restrict
 }
 
 // ------------------------------------------------------------------ backward of bias, activation and dropout
-// dz = D(dy) * act'(z) (DZ; where nothing is behind the product dz is dy itself) and the column sums of dz per range of rows.  A work
+// dz = D(dy) * slope (where nothing is behind the product dz is dy itself) and the column sums of dz per range of rows.  A work
 // item is 256 columns of one range of rows; the ranges follow from the sizes alone, so the sums do not depend on the CTA count.
-// VEC: rows of dy are 16-byte multiples (an even width); rows of z and dz always are.
+// VEC: rows of dy are 16-byte multiples (an even width); rows of slope and dz always are.
 template <bool VEC>
-__global__ void __launch_bounds__(LA_THREADS, 3) act_backward_kernel(const __nv_bfloat16* __restrict__ dy, const __nv_bfloat16* __restrict__ pre,
-                                                                  long long ld_pre, __nv_bfloat16* __restrict__ dz, long long ld_dz,
-                                                                  float* __restrict__ partial, long long rows, int N, int ranges, int act,
+__global__ void __launch_bounds__(LA_THREADS, 4) act_backward_kernel(const __nv_bfloat16* __restrict__ dy, const __nv_bfloat16* __restrict__ slope,
+                                                                  long long ld_slope, __nv_bfloat16* __restrict__ dz, long long ld_dz,
+                                                                  float* __restrict__ partial, long long rows, int N, int ranges,
                                                                   const long long* __restrict__ rng, uint32_t site, uint32_t threshold, float scale) {
     pdl_wait();
     pdl_launch_dependents();
@@ -142,7 +142,7 @@ __global__ void __launch_bounds__(LA_THREADS, 3) act_backward_kernel(const __nv_
 #pragma unroll
                         for (int e = 0; e < 8; e++) d[u][e] = col + e < N ? __bfloat162float(dy[r * N + col + e]) : 0.f;
                     }
-                    if (act) Pack8<__nv_bfloat16>::load(pre + r * ld_pre + col, z[u]);
+                    if (slope) Pack8<__nv_bfloat16>::load(slope + r * ld_slope + col, z[u]);
                 }
 #pragma unroll
                 for (int u = 0; u < 2; u++) {
@@ -160,12 +160,9 @@ __global__ void __launch_bounds__(LA_THREADS, 3) act_backward_kernel(const __nv_
                             for (int e = 0; e < 8; e++) d[u][e] = mask >> e & 1u ? d[u][e] * scale : 0.f;
                         }
                     }
-                    if (act == 2) {
+                    if (slope) {
 #pragma unroll
-                        for (int e = 0; e < 8; e += 2) gelu_slope_pair(d[u][e], d[u][e + 1], z[u][e], z[u][e + 1]);
-                    } else if (act == 1) {
-#pragma unroll
-                        for (int e = 0; e < 8; e++) d[u][e] = z[u][e] > 0.f ? d[u][e] : 0.f;
+                        for (int e = 0; e < 8; e++) d[u][e] *= z[u][e];
                     }
                     if (dz) Pack8<__nv_bfloat16>::store(dz + r * ld_dz + col, d[u]);
 #pragma unroll
@@ -211,10 +208,10 @@ __global__ void __launch_bounds__(LA_THREADS) act_colsum_kernel(const float* __r
     }
 }
 
-// Ranges of rows of the backward pass: about four items for every SM, at least 32 rows each.
+// Ranges of rows of the backward pass: one round of items for four CTAs an SM where that is possible, at least 32 rows each.
 static int la_ranges(long long rows, int N, int sms) {
     const long long col_tiles = (N + LA_COLS - 1) / LA_COLS;
-    long long n = (4LL * sms + col_tiles - 1) / col_tiles, most = (rows + 31) / 32;
+    long long n = 4LL * sms / col_tiles, most = (rows + 31) / 32;
     if (n > most) n = most;
     return (int)(n < 1 ? 1 : n);
 }
@@ -233,12 +230,12 @@ extern "C" int ob200_dropout(const void* x, const void* residual, void* y, long 
     if (n == 0) return 0;
     if (!x || !y) return -1;
     const DropRate rate = drop_rate(p);
-    long long want = ((n + 7) / 8 + LA_THREADS - 1) / LA_THREADS, cap = (long long)num_ctas * 8 * grid_oversubscription();
+    long long want = ((n + 7) / 8 + LA_THREADS - 1) / LA_THREADS, cap = (long long)num_ctas * 6 * grid_oversubscription();
     const unsigned grid = (unsigned)(want < cap ? want : cap);
     const bool vec = (((uintptr_t)x | (uintptr_t)residual | (uintptr_t)y) % 16) == 0;
 #define OB200_DROP(T, VEC)                                                                                                                     \
     do {                                                                                                                                       \
-        OB200_ELASTIC_HBM((dropout_kernel<T, VEC>), 8);                                                                                        \
+        OB200_ELASTIC_HBM((dropout_kernel<T, VEC>), 6);                                                                                        \
         return launch_pdl(dropout_kernel<T, VEC>, grid, (unsigned)LA_THREADS, (cudaStream_t)stream, (const T*)x, (const T*)residual, (T*)y, n, \
                           rng, (uint32_t)site, rate.threshold, rate.scale);                                                                    \
     } while (0)
@@ -254,13 +251,13 @@ extern "C" long long ob200_linear_act_workspace(int M, int N, int K) {
     return (long long)gemm_bf16_slab_bytes(M, N, K);
 }
 
-extern "C" int ob200_linear_act_bf16(const void* x, const void* w, void* y, void* pre, const void* bias, int bias_f32, const void* residual, int act,
-                                     float p, const long long* rng, int site, int M, int N, int K, long long ldx, long long ldw, long long ld_pre,
+extern "C" int ob200_linear_act_bf16(const void* x, const void* w, void* y, void* slope, const void* bias, int bias_f32, const void* residual, int act,
+                                     float p, const long long* rng, int site, int M, int N, int K, long long ldx, long long ldw, long long ld_slope,
                                      void* workspace, long long workspace_bytes, int num_ctas, void* stream) {
     if (M < 0 || N < 0 || K <= 0 || act < 0 || act > 2 || !(p >= 0.f && p <= 1.f) || (p > 0.f && !rng) || num_ctas <= 0 || ldx < K || ldw < K) return -1;
     if (M == 0 || N == 0) return 0;
-    if (!x || !w || !y || (pre && (ld_pre < N || ld_pre % 8))) return -1;
-    if (((uintptr_t)x | (uintptr_t)w | (uintptr_t)y | (uintptr_t)pre | (uintptr_t)workspace) % 16 || (ldx | ldw) % 8) return -2;
+    if (!x || !w || !y || (slope && (ld_slope < N || ld_slope % 8 || !act))) return -1;
+    if (((uintptr_t)x | (uintptr_t)w | (uintptr_t)y | (uintptr_t)slope | (uintptr_t)workspace) % 16 || (ldx | ldw) % 8) return -2;
     if (workspace_bytes < ob200_linear_act_workspace(M, N, K) || (!workspace && workspace_bytes > 0)) return -3;
     const DropRate rate = drop_rate(p);
     GemmCall g;
@@ -276,8 +273,8 @@ extern "C" int ob200_linear_act_bf16(const void* x, const void* w, void* y, void
     g.e.drop_scale = rate.scale;
     g.e.rng = rng;
     g.e.site = (uint32_t)site;
-    g.e.pre = (__nv_bfloat16*)pre;
-    g.e.ld_pre = ld_pre;
+    g.e.slope = (__nv_bfloat16*)slope;
+    g.e.ld_slope = ld_slope;
     g.slabs = (float*)workspace;
     g.slab_bytes = (size_t)workspace_bytes;
     g.num_ctas = num_ctas;
@@ -304,13 +301,13 @@ extern "C" long long ob200_linear_act_backward_workspace(int M, int N, int K, in
     return (long long)LinearBackwardSpace(M, N, K, act, drop_rate(p).threshold, want_dx, want_dw, want_dbias).total;
 }
 
-extern "C" int ob200_linear_act_backward_bf16(const void* dy, const void* pre, const void* x, const void* w, void* dx, void* dw, void* dbias,
+extern "C" int ob200_linear_act_backward_bf16(const void* dy, const void* slope, const void* x, const void* w, void* dx, void* dw, void* dbias,
                                               int bias_f32, int act, float p, const long long* rng, int site, int M, int N, int K, long long ldx,
-                                              long long ldw, long long ld_pre, void* workspace, long long workspace_bytes, int num_ctas, void* stream) {
+                                              long long ldw, long long ld_slope, void* workspace, long long workspace_bytes, int num_ctas, void* stream) {
     if (M < 0 || N < 0 || K <= 0 || act < 0 || act > 2 || !(p >= 0.f && p <= 1.f) || (p > 0.f && !rng) || num_ctas <= 0 || ldx < K || ldw < K) return -1;
     if (M == 0 || N == 0) return 0;
-    if (!dy || (act && !pre) || (pre && (ld_pre < N || ld_pre % 8)) || (dx && !w) || (dw && !x)) return -1;
-    if (((uintptr_t)dy | (uintptr_t)pre | (uintptr_t)x | (uintptr_t)w | (uintptr_t)dx | (uintptr_t)dw | (uintptr_t)workspace) % 16 || (ldx | ldw) % 8)
+    if (!dy || (act && !slope) || (slope && (ld_slope < N || ld_slope % 8 || !act)) || (dx && !w) || (dw && !x)) return -1;
+    if (((uintptr_t)dy | (uintptr_t)slope | (uintptr_t)x | (uintptr_t)w | (uintptr_t)dx | (uintptr_t)dw | (uintptr_t)workspace) % 16 || (ldx | ldw) % 8)
         return -2;
     const DropRate rate = drop_rate(p);
     const LinearBackwardSpace space(M, N, K, act, rate.threshold, dx != nullptr, dw != nullptr, dbias != nullptr);
@@ -325,18 +322,18 @@ extern "C" int ob200_linear_act_backward_bf16(const void* dy, const void* pre, c
     const void* gz = dz ? (const void*)dz : dy;
     if ((dz && (dx || dw)) || partial) {
         const int ranges = la_ranges(M, N, ob200_plan_sm_count());
-        const long long items = (long long)ranges * ((N + LA_COLS - 1) / LA_COLS), cap = (long long)num_ctas * 8 * grid_oversubscription();
+        const long long items = (long long)ranges * ((N + LA_COLS - 1) / LA_COLS), cap = (long long)num_ctas * 4 * grid_oversubscription();
         const unsigned grid = (unsigned)(items < cap ? items : cap);
         __nv_bfloat16* out = dx || dw ? dz : nullptr;
         int rc;
         if (N % 8 == 0) {
-            OB200_ELASTIC_HBM(act_backward_kernel<true>, 8);
-            rc = launch_pdl(act_backward_kernel<true>, grid, (unsigned)LA_THREADS, st, (const __nv_bfloat16*)dy, (const __nv_bfloat16*)pre, ld_pre, out, ld_dz,
-                            partial, (long long)M, N, ranges, act, rng, (uint32_t)site, rate.threshold, rate.scale);
+            OB200_ELASTIC_HBM(act_backward_kernel<true>, 4);
+            rc = launch_pdl(act_backward_kernel<true>, grid, (unsigned)LA_THREADS, st, (const __nv_bfloat16*)dy, (const __nv_bfloat16*)slope, ld_slope, out, ld_dz,
+                            partial, (long long)M, N, ranges, rng, (uint32_t)site, rate.threshold, rate.scale);
         } else {
-            OB200_ELASTIC_HBM(act_backward_kernel<false>, 8);
-            rc = launch_pdl(act_backward_kernel<false>, grid, (unsigned)LA_THREADS, st, (const __nv_bfloat16*)dy, (const __nv_bfloat16*)pre, ld_pre, out,
-                            ld_dz, partial, (long long)M, N, ranges, act, rng, (uint32_t)site, rate.threshold, rate.scale);
+            OB200_ELASTIC_HBM(act_backward_kernel<false>, 4);
+            rc = launch_pdl(act_backward_kernel<false>, grid, (unsigned)LA_THREADS, st, (const __nv_bfloat16*)dy, (const __nv_bfloat16*)slope, ld_slope, out,
+                            ld_dz, partial, (long long)M, N, ranges, rng, (uint32_t)site, rate.threshold, rate.scale);
         }
         if (rc) return rc;
         if (partial) {

@@ -81,14 +81,15 @@ __device__ __forceinline__ uint32_t drop_mask(const DropKey& key, unsigned long 
     return (uint32_t)(bits >> off);
 }
 
-// f[j] = kept ? f[j] * scale : 0 for the 32 elements of groups `group` .. `group + 3`: four draws side by side, which share the keys.
-__device__ __forceinline__ void drop_apply32(const DropKey& key, unsigned long long group, uint32_t threshold, float scale, float (&f)[32]) {
-    uint32_t c[4][4];
+// f[j] = kept ? f[j] * scale : 0 for the W elements from group `group` on: draws side by side, which share the keys.
+template <int W>
+__device__ __forceinline__ void drop_apply(const DropKey& key, unsigned long long group, uint32_t threshold, float scale, float (&f)[W]) {
+    uint32_t c[W / 8][4];
 #pragma unroll
-    for (int i = 0; i < 4; i++) drop_bits(key, group + i, c[i]);
+    for (int i = 0; i < W / 8; i++) drop_bits(key, group + i, c[i]);
     const uint32_t limit = drop_limit(threshold);
 #pragma unroll
-    for (int j = 0; j < 32; j++) f[j] = drop_keeps(c[j >> 3], j & 7, limit) ? f[j] * scale : 0.f;
+    for (int j = 0; j < W; j++) f[j] = drop_keeps(c[j >> 3], j & 7, limit) ? f[j] * scale : 0.f;
 }
 
 // A probability as the kernels use it.

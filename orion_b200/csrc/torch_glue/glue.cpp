@@ -96,13 +96,13 @@ int ob200_cross_entropy_backward(const void* logits, const long long* target, co
                                  long long rows, int V, int dtype, void* stream);
 int ob200_adamw_multi(void* const* p, const void* const* g, void* const* m, void* const* v, const long long* n, int count, float lr,
                       float beta1, float beta2, float eps, float weight_decay, int step, int dtype, int num_ctas, void* stream);
-int ob200_linear_act_bf16(const void* x, const void* w, void* y, void* pre, const void* bias, int bias_f32, const void* residual, int act,
-                          float p, const long long* rng, int site, int M, int N, int K, long long ldx, long long ldw, long long ld_pre,
+int ob200_linear_act_bf16(const void* x, const void* w, void* y, void* slope, const void* bias, int bias_f32, const void* residual, int act,
+                          float p, const long long* rng, int site, int M, int N, int K, long long ldx, long long ldw, long long ld_slope,
                           void* workspace, long long workspace_bytes, int num_ctas, void* stream);
 long long ob200_linear_act_workspace(int M, int N, int K);
-int ob200_linear_act_backward_bf16(const void* dy, const void* pre, const void* x, const void* w, void* dx, void* dw, void* dbias,
+int ob200_linear_act_backward_bf16(const void* dy, const void* slope, const void* x, const void* w, void* dx, void* dw, void* dbias,
                                    int bias_f32, int act, float p, const long long* rng, int site, int M, int N, int K, long long ldx,
-                                   long long ldw, long long ld_pre, void* workspace, long long workspace_bytes, int num_ctas, void* stream);
+                                   long long ldw, long long ld_slope, void* workspace, long long workspace_bytes, int num_ctas, void* stream);
 long long ob200_linear_act_backward_workspace(int M, int N, int K, int act, float p, int want_dx, int want_dw, int want_dbias);
 int ob200_dropout(const void* x, const void* residual, void* y, long long n, float p, const long long* rng, int site, int dtype,
                   int num_ctas, void* stream);
@@ -875,9 +875,9 @@ struct LinearAct : public torch::autograd::Function<LinearAct> {
         }
         check_dropout("orion::linear_act", x, p, rng, site);
     }
-    // The output, and with `want_pre` the pre-activation in rows padded to a multiple of 8.
+    // The output, and with `want_slope` the activation's slope in rows padded to a multiple of 8.
     static at::Tensor run(const at::Tensor& x, const at::Tensor& w, const c10::optional<at::Tensor>& bias, const c10::optional<at::Tensor>& residual,
-                          int act, double p, const c10::optional<at::Tensor>& rng, int64_t site, bool want_pre, at::Tensor* pre) {
+                          int act, double p, const c10::optional<at::Tensor>& rng, int64_t site, bool want_slope, at::Tensor* slope) {
         c10::cuda::CUDAGuard guard(x.device());
         const int64_t K = w.size(1), N = w.size(0);
         auto shape = x.sizes().vec();
@@ -887,22 +887,22 @@ struct LinearAct : public torch::autograd::Function<LinearAct> {
         const at::Tensor xr = as_rows(x), wr = as_rows(w);
         const int64_t M = xr.size(0);
         const at::Tensor res = given(residual) ? residual->contiguous() : at::Tensor();
-        if (want_pre) *pre = at::empty({M, (N + 7) / 8 * 8}, x.options());
+        if (want_slope) *slope = at::empty({M, (N + 7) / 8 * 8}, x.options());
         const long long bytes = ob200_linear_act_workspace((int)M, (int)N, (int)K);
         const at::Tensor space = bytes ? workspace(bytes, x) : at::Tensor();
-        check(ob200_linear_act_bf16(xr.data_ptr(), wr.data_ptr(), y.data_ptr(), want_pre ? pre->data_ptr() : nullptr,
+        check(ob200_linear_act_bf16(xr.data_ptr(), wr.data_ptr(), y.data_ptr(), want_slope ? slope->data_ptr() : nullptr,
                                     given(bias) ? bias->data_ptr() : nullptr, given(bias) && bias->scalar_type() == at::kFloat ? 1 : 0,
                                     res.defined() ? res.data_ptr() : nullptr, act, (float)p, rng_ptr(rng, p), (int)site, (int)M, (int)N, (int)K,
-                                    xr.stride(0), wr.stride(0), want_pre ? pre->size(1) : 0, bytes ? space.data_ptr() : nullptr, bytes, quota(),
+                                    xr.stride(0), wr.stride(0), want_slope ? slope->size(1) : 0, bytes ? space.data_ptr() : nullptr, bytes, quota(),
                                     cur_stream()),
               "ob200_linear_act_bf16");
         return y;
     }
     static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w, const c10::optional<at::Tensor>& bias,
                               const c10::optional<at::Tensor>& residual, int64_t act, double p, const c10::optional<at::Tensor>& rng, int64_t site) {
-        at::Tensor pre;
-        at::Tensor y = run(x, w, bias, residual, (int)act, p, rng, site, act != 0, &pre);
-        ctx->save_for_backward({x, w, pre, p > 0.0 ? *rng : at::Tensor()});
+        at::Tensor slope;
+        at::Tensor y = run(x, w, bias, residual, (int)act, p, rng, site, act != 0, &slope);
+        ctx->save_for_backward({x, w, slope, p > 0.0 ? *rng : at::Tensor()});
         ctx->saved_data["act"] = act;
         ctx->saved_data["p"] = p;
         ctx->saved_data["site"] = site;
@@ -913,7 +913,7 @@ struct LinearAct : public torch::autograd::Function<LinearAct> {
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
         refuse_double_backward("orion::linear_act");
         auto saved = ctx->get_saved_variables();
-        const at::Tensor &x = saved[0], &w = saved[1], &pre = saved[2], &rng = saved[3];
+        const at::Tensor &x = saved[0], &w = saved[1], &slope = saved[2], &rng = saved[3];
         c10::cuda::CUDAGuard guard(x.device());
         const int act = (int)ctx->saved_data["act"].toInt(), bias = (int)ctx->saved_data["bias"].toInt();
         const double p = ctx->saved_data["p"].toDouble();
@@ -934,11 +934,11 @@ struct LinearAct : public torch::autograd::Function<LinearAct> {
             const at::Tensor dy = as_dense(grads[0]), xr = as_rows(x), wr = as_rows(w);
             const long long bytes = ob200_linear_act_backward_workspace((int)M, (int)N, (int)K, act, (float)p, want_dx, want_dw, want_db);
             const at::Tensor space = bytes ? workspace(bytes, x) : at::Tensor();
-            check(ob200_linear_act_backward_bf16(dy.data_ptr(), act ? pre.data_ptr() : nullptr, xr.data_ptr(), wr.data_ptr(),
+            check(ob200_linear_act_backward_bf16(dy.data_ptr(), act ? slope.data_ptr() : nullptr, xr.data_ptr(), wr.data_ptr(),
                                                  want_dx ? dx.data_ptr() : nullptr, want_dw ? dw.data_ptr() : nullptr, want_db ? db.data_ptr() : nullptr,
                                                  bias == 2 ? 1 : 0, act, (float)p, p > 0.0 ? (const long long*)rng.data_ptr<int64_t>() : nullptr,
                                                  (int)ctx->saved_data["site"].toInt(), (int)M, (int)N, (int)K, xr.stride(0), wr.stride(0),
-                                                 act ? pre.size(1) : 0, bytes ? space.data_ptr() : nullptr, bytes, quota(), cur_stream()),
+                                                 act ? slope.size(1) : 0, bytes ? space.data_ptr() : nullptr, bytes, quota(), cur_stream()),
                   "ob200_linear_act_backward_bf16");
             g_own_launches.fetch_add((want_dx ? 1 : 0) + (want_dw ? 1 : 0) + (want_db ? 1 : 0), std::memory_order_relaxed);
         }

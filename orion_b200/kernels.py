@@ -443,25 +443,25 @@ def _rows_ok(*tensors):
     return all(t.dim() == 2 and t.stride(1) == 1 and t.dtype == torch.bfloat16 for t in tensors)
 
 
-def linear_act(x, w, bias=None, residual=None, act="none", p=0.0, rng=None, site=0, want_pre=False, num_ctas=None):
+def linear_act(x, w, bias=None, residual=None, act="none", p=0.0, rng=None, site=0, want_slope=False, num_ctas=None):
     """residual + dropout(act(x . w^T + bias)) for bfloat16 x [M, K], w [N, K] (rows a multiple of 8 elements apart), bias bfloat16 or
-    float32; rng: int64 CUDA tensor (seed, step).  With `want_pre` also the pre-activation, in rows padded to a multiple of 8."""
+    float32; rng: int64 CUDA tensor (seed, step).  With `want_slope` also the activation's slope, in rows padded to a multiple of 8."""
     assert _rows_ok(x, w) and x.shape[1] == w.shape[1] and (residual is None or residual.is_contiguous())
     M, K = x.shape
     N = w.shape[0]
     y = torch.empty((M, N), device=x.device, dtype=x.dtype)
-    pre = torch.empty((M, (N + 7) // 8 * 8), device=x.device, dtype=x.dtype) if want_pre else None
+    slope = torch.empty((M, (N + 7) // 8 * 8), device=x.device, dtype=x.dtype) if want_slope else None
     n = lib().ob200_linear_act_workspace(M, N, K)
     space = torch.empty(n, device=x.device, dtype=torch.uint8) if n else None
-    _check(lib().ob200_linear_act_bf16(_ptr(x), _ptr(w), _ptr(y), _ptr(pre), _ptr(bias), int(bias is not None and bias.dtype == torch.float32),
+    _check(lib().ob200_linear_act_bf16(_ptr(x), _ptr(w), _ptr(y), _ptr(slope), _ptr(bias), int(bias is not None and bias.dtype == torch.float32),
                                        _ptr(residual), _ACTS[act], float(p), _ptr(rng), int(site), M, N, K, x.stride(0), w.stride(0),
-                                       pre.shape[1] if want_pre else 0, _ptr(space), n, num_ctas or sm_count(), _stream()),
+                                       slope.shape[1] if want_slope else 0, _ptr(space), n, num_ctas or sm_count(), _stream()),
            "ob200_linear_act_bf16")
-    return (y, pre) if want_pre else y
+    return (y, slope) if want_slope else y
 
 
-def linear_act_backward(dy, pre, x, w, bias_dtype=torch.bfloat16, act="none", p=0.0, rng=None, site=0, num_ctas=None):
-    """(dx, dw, dbias) of linear_act from dy [M, N] and what `want_pre` gave (None without an activation)."""
+def linear_act_backward(dy, slope, x, w, bias_dtype=torch.bfloat16, act="none", p=0.0, rng=None, site=0, num_ctas=None):
+    """(dx, dw, dbias) of linear_act from dy [M, N] and what `want_slope` gave (None without an activation)."""
     assert _rows_ok(x, w) and dy.is_contiguous() and dy.dtype == torch.bfloat16
     M, K = x.shape
     N = w.shape[0]
@@ -469,9 +469,9 @@ def linear_act_backward(dy, pre, x, w, bias_dtype=torch.bfloat16, act="none", p=
     db = torch.empty(N, device=x.device, dtype=bias_dtype)
     n = lib().ob200_linear_act_backward_workspace(M, N, K, _ACTS[act], float(p), 1, 1, 1)
     space = torch.empty(n, device=x.device, dtype=torch.uint8)
-    _check(lib().ob200_linear_act_backward_bf16(_ptr(dy), _ptr(pre), _ptr(x), _ptr(w), _ptr(dx), _ptr(dw), _ptr(db),
+    _check(lib().ob200_linear_act_backward_bf16(_ptr(dy), _ptr(slope), _ptr(x), _ptr(w), _ptr(dx), _ptr(dw), _ptr(db),
                                                 int(bias_dtype == torch.float32), _ACTS[act], float(p), _ptr(rng), int(site), M, N, K, x.stride(0),
-                                                w.stride(0), 0 if pre is None else pre.shape[1], _ptr(space), n, num_ctas or sm_count(), _stream()),
+                                                w.stride(0), 0 if slope is None else slope.shape[1], _ptr(space), n, num_ctas or sm_count(), _stream()),
            "ob200_linear_act_backward_bf16")
     return dx, dw, db
 

@@ -105,7 +105,7 @@ def test_linear_act_forward(ops, M, N, K, act, residual, p, bias):
     want, bound = expect(x, w, b, r, act, p, rng, 5)[:2]
     y = ops.linear_act(x, w, b, r, act, p, rng, 5)
     within(y, want, bound, "y")
-    # the same from any CTA count, and under grad mode, where the pre-activation is written beside it
+    # the same from any CTA count, and under grad mode, where the activation's slope is written beside it
     for n in (7, 1):
         ops.set_sm_quota(n)
         again = ops.linear_act(x, w, b, r, act, p, rng, 5)
@@ -127,9 +127,9 @@ def test_linear_act_gradients(ops, M, N, K, act, residual, p, bias):
         _, _, z, slope, m, z_err = expect(x, w, b, r, act, p, rng, 9)
         g = dy.double() * m
         dz = g * slope
-        # the derivative is taken at the rounded pre-activation: |gelu''| <= 0.8; near 0 a ReLU may fall on the other side
+        # the slope is kept rounded, taken at a float32 z: |gelu''| <= 0.8; near 0 a ReLU may fall on the other side
         if act == "gelu":
-            dz_err = g.abs() * (0.8 * (U * z.abs() + z_err) + 1e-6) + U * dz.abs()
+            dz_err = g.abs() * (U * slope.abs() + 0.8 * z_err + 1e-6) + U * dz.abs()
         elif act == "relu":
             dz_err = torch.where(z.abs() <= 2 * z_err, g.abs(), 0.0) + U * dz.abs()
         else:
@@ -686,9 +686,9 @@ def test_through_the_c_abi(built):
     y = ops.linear_act(x, w, b, r, "gelu", 0.1, rng, 6)
     want = torch.autograd.grad(y, leaves, dy)
     with torch.no_grad():
-        mine, pre = K.linear_act(x, w, b, r, "gelu", 0.1, rng, 6, want_pre=True, num_ctas=40)
+        mine, slope = K.linear_act(x, w, b, r, "gelu", 0.1, rng, 6, want_slope=True, num_ctas=40)
         assert torch.equal(mine, y)
-        for g, h in zip(K.linear_act_backward(dy, pre, x, w, torch.float32, "gelu", 0.1, rng, 6, num_ctas=33), want):
+        for g, h in zip(K.linear_act_backward(dy, slope, x, w, torch.float32, "gelu", 0.1, rng, 6, num_ctas=33), want):
             assert torch.equal(g, h)
         assert torch.equal(K.dropout(r, 0.3, rng, 1, num_ctas=3), ops.dropout(r, 0.3, rng, 1))
     loss = ops.linear_cross_entropy(x, w, target)

@@ -108,13 +108,13 @@ def test_entry_points_refuse_bad_arguments_without_a_gpu(K):
     L = K.lib()
     a = 1 << 20   # an aligned address that is never touched: every call below is refused before a launch
 
-    def act(x=a, w=a, y=a, pre=None, bias=None, act=0, p=0.0, rng=None, M=4, N=8, K=8, ldx=8, ldw=8, ld_pre=0, ws=None, nbytes=0, ctas=1):
-        return L.ob200_linear_act_bf16(x, w, y, pre, bias, 0, None, act, p, rng, 0, M, N, K, ldx, ldw, ld_pre, ws, nbytes, ctas, None)
+    def act(x=a, w=a, y=a, slope=None, bias=None, act=0, p=0.0, rng=None, M=4, N=8, K=8, ldx=8, ldw=8, ld_slope=0, ws=None, nbytes=0, ctas=1):
+        return L.ob200_linear_act_bf16(x, w, y, slope, bias, 0, None, act, p, rng, 0, M, N, K, ldx, ldw, ld_slope, ws, nbytes, ctas, None)
     nan = float("nan")
     for bad in (dict(act=3), dict(act=-1), dict(p=-0.1), dict(p=1.5), dict(p=nan), dict(p=0.5), dict(M=-1), dict(N=-1), dict(K=0), dict(ldx=4), dict(ldw=4),
-                dict(ctas=0), dict(x=None), dict(w=None), dict(y=None), dict(pre=a, ld_pre=4), dict(pre=a, ld_pre=12)):
+                dict(ctas=0), dict(x=None), dict(w=None), dict(y=None), dict(act=1, slope=a, ld_slope=4), dict(act=1, slope=a, ld_slope=12), dict(slope=a, ld_slope=8)):
         assert act(**bad) == -1, bad
-    for bad in (dict(x=a + 8), dict(w=a + 2), dict(y=a + 4), dict(ldx=12), dict(ldw=9), dict(pre=a + 8, ld_pre=8)):
+    for bad in (dict(x=a + 8), dict(w=a + 2), dict(y=a + 4), dict(ldx=12), dict(ldw=9), dict(act=1, slope=a + 8, ld_slope=8)):
         assert act(**bad) == -2, bad
     M, N, KK = 64, 1024, 4096
     need = L.ob200_linear_act_workspace(M, N, KK)
@@ -123,13 +123,13 @@ def test_entry_points_refuse_bad_arguments_without_a_gpu(K):
     assert act(M=M, N=N, K=KK, ldx=KK, ldw=KK, ws=None, nbytes=need) == -3
     assert act(M=0) == 0 and act(N=0) == 0
 
-    def back(dy=a, pre=None, x=a, w=a, dx=a, dw=a, db=None, act=0, p=0.0, rng=None, M=4, N=8, K=8, ldx=8, ldw=8, ld_pre=0, ws=a, nbytes=1 << 30):
-        return L.ob200_linear_act_backward_bf16(dy, pre, x, w, dx, dw, db, 0, act, p, rng, 0, M, N, K, ldx, ldw, ld_pre, ws, nbytes, 1, None)
-    for bad in (dict(act=2), dict(dy=None), dict(x=None), dict(w=None), dict(p=0.5), dict(act=2, pre=a, ld_pre=7), dict(K=0)):
+    def back(dy=a, slope=None, x=a, w=a, dx=a, dw=a, db=None, act=0, p=0.0, rng=None, M=4, N=8, K=8, ldx=8, ldw=8, ld_slope=0, ws=a, nbytes=1 << 30):
+        return L.ob200_linear_act_backward_bf16(dy, slope, x, w, dx, dw, db, 0, act, p, rng, 0, M, N, K, ldx, ldw, ld_slope, ws, nbytes, 1, None)
+    for bad in (dict(act=2), dict(dy=None), dict(x=None), dict(w=None), dict(p=0.5), dict(act=2, slope=a, ld_slope=7), dict(K=0)):
         assert back(**bad) == -1, bad
     for bad in (dict(dy=a + 2), dict(dx=a + 2), dict(dw=a + 8), dict(ldx=9)):
         assert back(**bad) == -2, bad
-    assert back(act=2, pre=a, ld_pre=8, nbytes=0) == -3 and back(db=a, ws=None) == -3
+    assert back(act=2, slope=a, ld_slope=8, nbytes=0) == -3 and back(db=a, ws=None) == -3
     assert back(M=0) == 0
 
     def drop(x=a, y=a, n=8, p=0.1, rng=a, dtype=1, ctas=1):
