@@ -254,7 +254,7 @@ int ob200_adamw_f32(float* p, const float* g, float* m, float* v, long long n, f
  * i % 8 of the four words at counter (low 32 bits of i / 8, bits 32..47 of i / 8 | bits 32..47 of step << 16, low 32 bits of step, site)
  * under the key seed.  rng points to (seed, step) in device memory, read when the kernel runs, so that a captured graph draws a new
  * mask when the step moves on; `site` tells the calls of one step apart.  slope (NULL: not wanted), rows ld_slope apart (a multiple of
- * 8): the activation's derivative at x . w^T + bias in bfloat16, which the backward pass multiplies by.  workspace: the bytes that
+ * 8): the activation's derivative at x . w^T + bias in float16, which the backward pass multiplies by.  workspace: the bytes that
  * ob200_linear_act_workspace names (0: none), any contents, the call's own until it has run.
  * Returns -1 for bad arguments, -2 for misaligned pointers or strides, -3 for a workspace that is too small, -4 when a TMA descriptor
  * cannot be built.  Stands for the sgemm, bias, GELU, fused_dropout_kernel_vec and add rows of the reference's

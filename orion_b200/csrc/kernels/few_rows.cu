@@ -114,7 +114,7 @@ __device__ __forceinline__ void few_way_out(const FewRowsParams& p, const float 
             if (p.e.act) {
                 float slope;
                 z = act_slope(z, p.e.act, slope);
-                if (p.e.slope) p.e.slope[m * p.e.ld_slope + n] = __float2bfloat16_rn(slope);
+                if (p.e.slope) p.e.slope[m * p.e.ld_slope + n] = __float2half_rn(slope);
             }
             if (p.e.drop_threshold) {
                 uint32_t bits[4];

@@ -424,7 +424,12 @@ __global__ void __launch_bounds__(gm_threads(EPI), 1) gemm_bf16_kernel(const __g
                     }
                 }
                 if constexpr (EPI == GM_EPI_ACC) {
-                    if (row_ok) {   // N a multiple of 4: no column of a vector is past the edge alone
+                    if (p.e.factor) {
+                        const float factor = __ldg(p.e.factor);
+#pragma unroll
+                        for (int j = 0; j < 32; j++) f[j] *= factor;
+                    }
+                    if (p.e.addend && row_ok) {   // N a multiple of 4: no column of a vector is past the edge alone
                         const float* add = p.e.addend + (long long)m * p.N + n;
 #pragma unroll
                         for (int j = 0; j < 32; j += 4)
@@ -530,10 +535,11 @@ __global__ void __launch_bounds__(gm_threads(EPI), 1) gemm_bf16_kernel(const __g
 __global__ void __launch_bounds__(256) gemm_splitk_finish_kernel(const float* __restrict__ slabs, void* c,
                                                                  const float* __restrict__ bias,
                                                                  const __nv_bfloat16* __restrict__ bias_bf16,
-                                                                 const __nv_bfloat16* __restrict__ residual, const float* addend, int splits, int batch, int nb_inner,
+                                                                 const __nv_bfloat16* __restrict__ residual, const float* addend, const float* factor, int splits, int batch, int nb_inner,
                                                                  int M, int N, long long ldc, long long c_si, long long c_so,
                                                                  int out_f32, float alpha) {
     const long long per_split = (long long)batch * M * N;
+    if (factor) alpha *= *factor;
     for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < per_split; i += (long long)gridDim.x * blockDim.x) {
         float acc = 0.f;
         for (int s = 0; s < splits; s++) acc += slabs[(long long)s * per_split + i];
@@ -592,7 +598,7 @@ __global__ void __launch_bounds__(256) gemm_splitk_act_kernel(const float* __res
                 if (e.act) {
                     float slope;
                     a = act_slope(a, e.act, slope);
-                    if (e.slope) e.slope[m * e.ld_slope + col] = __float2bfloat16_rn(slope);
+                    if (e.slope) e.slope[m * e.ld_slope + col] = __float2half_rn(slope);
                 }
                 if (e.drop_threshold) a = mask >> j & 1u ? a * e.drop_scale : 0.f;
                 if (residual) a += __bfloat162float(residual[i0 + j]);
@@ -915,7 +921,7 @@ int gemm_bf16_run(const GemmCall& g) {
     long long blocks = (elems + 255) / 256;
     if (blocks > 4LL * num_ctas) blocks = 4LL * num_ctas;
     OB200_ELASTIC_HBM(gemm_splitk_finish_kernel, 4);
-    gemm_splitk_finish_kernel<<<(int)blocks, 256, 0, st>>>(p.slabs, c, g.bias, p.bias_bf16, p.residual, epi == GM_EPI_ACC ? p.e.addend : nullptr, p.splits, p.batch,
+    gemm_splitk_finish_kernel<<<(int)blocks, 256, 0, st>>>(p.slabs, c, g.bias, p.bias_bf16, p.residual, epi == GM_EPI_ACC ? p.e.addend : nullptr, epi == GM_EPI_ACC ? p.e.factor : nullptr, p.splits, p.batch,
                                                            p.nb_inner, M, N, ldc, c_si, c_so, p.out_f32, g.alpha);
     return (int)cudaGetLastError();
 }

@@ -1,6 +1,7 @@
 // The bfloat16 GEMM (gemm_bf16.cu) as the other kernels of the library call it: one problem with one of several epilogues.
 #pragma once
 #include <cuda_bf16.h>
+#include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <stddef.h>
 #include <stdint.h>
@@ -9,7 +10,7 @@ namespace ob200 {
 
 enum : int {
     GM_EPI_PLAIN = 0,    // C = alpha * A.B^T (+ bias) (+ bfloat16 residual)
-    GM_EPI_ACC = 1,      // the same plus a float32 addend (which may be C itself)
+    GM_EPI_ACC = 1,      // the same with a factor from device memory and a float32 addend (which may be C itself)
     GM_EPI_ACT = 2,      // C = residual + dropout(act(A.B^T + bias)), optionally the activation's slope beside it
     GM_EPI_ACT_ANY = 3,  // GM_EPI_ACT for widths, types and alignments that its vector accesses do not take (chosen by the launcher)
     GM_EPI_ACT_SLOPE = 7,// GM_EPI_ACT with the slope (chosen by the launcher)
@@ -19,15 +20,16 @@ enum : int {
 };
 
 struct GemmEpi {
-    // GM_EPI_ACC
-    const float* addend;            // [M, N], rows N apart
+    // GM_EPI_ACC, GM_EPI_DUAL
+    const float* addend;            // [M, N], rows N apart, or null
+    const float* factor;            // optional: what the products are multiplied by, in device memory
     // GM_EPI_ACT
     int act;                        // 0 none, 1 ReLU, 2 GELU
     uint32_t drop_threshold;        // 0: no dropout
     float drop_scale;
     const long long* rng;           // (seed, step), in device memory
     uint32_t site;
-    __nv_bfloat16* slope;           // optional, with an activation: act'(A.B^T + bias), rows ld_slope apart (a multiple of 8)
+    __half* slope;                  // optional, with an activation: act'(A.B^T + bias), rows ld_slope apart (a multiple of 8)
     long long ld_slope;
     // GM_EPI_LSE, GM_EPI_DLOGITS
     const long long* target;        // label of every row

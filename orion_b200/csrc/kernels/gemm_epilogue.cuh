@@ -7,6 +7,13 @@ __device__ __forceinline__ uint32_t gm_pack(float a, float b) {
     return *reinterpret_cast<const uint32_t*>(&h2);
 }
 
+// Slopes are kept in float16: they lie between -0.13 and 1.13, and three more bits than bfloat16's keep what multiplies the gradient an
+// eighth as far off as the rounding of the product.
+__device__ __forceinline__ uint32_t gm_pack_half(float a, float b) {
+    const __half2 h2 = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h2);
+}
+
 // Byte of 16-byte chunk `ch` of this thread's row in a slab of 32 rows x W columns, in the swizzle of its tensor map (64 or 32 bytes
 // wide: eight consecutive rows of one chunk fall into eight different bank groups).
 template <int W>
@@ -66,7 +73,7 @@ __device__ __forceinline__ void gm_act_slope(float (&f)[W], int act, uint8_t* sl
                 a0 = fmaxf(a0, 0.f);
                 a1 = fmaxf(a1, 0.f);
             }
-            w[e] = gm_pack(s0, s1);
+            w[e] = gm_pack_half(s0, s1);
         }
         *reinterpret_cast<uint4*>(slab + gm_slab_chunk<W>(lane, ch)) = make_uint4(w[0], w[1], w[2], w[3]);
     }
@@ -333,7 +340,7 @@ __device__ __forceinline__ void gm_epilogue_dlogits(const GemmParams& p, uint32_
     }
 }
 
-// A dual launch's tiles: float32 accumulators plus the first product's addend (which may be its output), rounded to the output's type.
+// A dual launch's tiles: float32 accumulators times the factor, plus the first product's addend (which may be its output), rounded to the output's type.
 template <int BN>
 __device__ __forceinline__ void gm_epilogue_dual(const GemmParamsDual& p, bool second, uint32_t t_row, int m, int m0w, int n0, int lane, uint8_t* stage,
                                                  uint32_t& turn) {
@@ -341,12 +348,15 @@ __device__ __forceinline__ void gm_epilogue_dual(const GemmParamsDual& p, bool s
     const bool out_f32 = second ? p.second.out_f32 : p.out_f32;
     const unsigned char* map = second ? p.second.tmap_c : p.tmap_c;
     const float* addend = second || m >= M || !p.e.addend ? nullptr : p.e.addend + (long long)m * N;
+    const float factor = p.e.factor ? __ldg(p.e.factor) : 1.f;
 #pragma unroll 1
     for (int c0 = 0; c0 < BN; c0 += 32) {
         const int n = n0 + c0;
         if (n >= N) break;              // warp-uniform
         float f[32];
         gm_load(t_row + c0, f);
+#pragma unroll
+        for (int j = 0; j < 32; j++) f[j] *= factor;
         if (addend) {                   // N is a multiple of 8
 #pragma unroll
             for (int j = 0; j < 32; j += 4)

@@ -8,6 +8,7 @@
 // GELU, add and fused_dropout_kernel_vec rows of benchmarking/model_kernels/bert_8_fb1 behind its cudaLaunchKernel trap
 // (reference src/cuda_capture/intercept_temp.cpp:418-458).
 #include <cuda_bf16.h>
+#include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -62,6 +63,17 @@ struct Pack8<__nv_bfloat16> {
     __device__ static __nv_bfloat16 put(float x) { return __float2bfloat16_rn(x); }
 };
 
+__device__ __forceinline__ void load_half8(const __half* p, float (&v)[8]) {
+    const uint4 q = *reinterpret_cast<const uint4*>(p);
+    const __half2* h = reinterpret_cast<const __half2*>(&q);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const float2 f = __half22float2(h[i]);
+        v[2 * i] = f.x;
+        v[2 * i + 1] = f.y;
+    }
+}
+
 // ------------------------------------------------------------------ dropout (+ residual)
 // A thread takes eight consecutive elements, one draw of the generator.  VEC: all pointers are 16-byte aligned.
 template <typename T, bool VEC>
@@ -106,14 +118,15 @@ __global__ void __launch_bounds__(LA_THREADS, 6) dropout_kernel(const T* __restr
 }
 
 // ------------------------------------------------------------------ backward of bias, activation and dropout
-// dz = D(dy) * slope (where nothing is behind the product dz is dy itself) and the column sums of dz per range of rows.  A work
+// dz = D(dy) * slope without dropout's factor, which the products and the column sums take instead, so that dz is rounded only where a
+// slope made it inexact (where nothing is behind the product dz is dy itself), and the column sums of dz per range of rows.  A work
 // item is 256 columns of one range of rows; the ranges follow from the sizes alone, so the sums do not depend on the CTA count.
 // VEC: rows of dy are 16-byte multiples (an even width); rows of slope and dz always are.
 template <bool VEC>
-__global__ void __launch_bounds__(LA_THREADS, 4) act_backward_kernel(const __nv_bfloat16* __restrict__ dy, const __nv_bfloat16* __restrict__ slope,
+__global__ void __launch_bounds__(LA_THREADS, 4) act_backward_kernel(const __nv_bfloat16* __restrict__ dy, const __half* __restrict__ slope,
                                                                   long long ld_slope, __nv_bfloat16* __restrict__ dz, long long ld_dz,
                                                                   float* __restrict__ partial, long long rows, int N, int ranges,
-                                                                  const long long* __restrict__ rng, uint32_t site, uint32_t threshold, float scale) {
+                                                                  const long long* __restrict__ rng, uint32_t site, uint32_t threshold) {
     pdl_wait();
     pdl_launch_dependents();
     __shared__ float sh[LA_ROWS][LA_COLS];
@@ -142,7 +155,7 @@ __global__ void __launch_bounds__(LA_THREADS, 4) act_backward_kernel(const __nv_
 #pragma unroll
                         for (int e = 0; e < 8; e++) d[u][e] = col + e < N ? __bfloat162float(dy[r * N + col + e]) : 0.f;
                     }
-                    if (slope) Pack8<__nv_bfloat16>::load(slope + r * ld_slope + col, z[u]);
+                    if (slope) load_half8(slope + r * ld_slope + col, z[u]);
                 }
 #pragma unroll
                 for (int u = 0; u < 2; u++) {
@@ -153,11 +166,11 @@ __global__ void __launch_bounds__(LA_THREADS, 4) act_backward_kernel(const __nv_
                             uint32_t c[4];
                             drop_bits(key, ((unsigned long long)r * N + col) >> 3, c);
 #pragma unroll
-                            for (int e = 0; e < 8; e++) d[u][e] = drop_keeps(c, e, limit) ? d[u][e] * scale : 0.f;
+                            for (int e = 0; e < 8; e++) d[u][e] = drop_keeps(c, e, limit) ? d[u][e] : 0.f;
                         } else {
                             const uint32_t mask = drop_mask<8>(key, (unsigned long long)r * N + col, threshold);
 #pragma unroll
-                            for (int e = 0; e < 8; e++) d[u][e] = mask >> e & 1u ? d[u][e] * scale : 0.f;
+                            for (int e = 0; e < 8; e++) d[u][e] = mask >> e & 1u ? d[u][e] : 0.f;
                         }
                     }
                     if (slope) {
@@ -185,7 +198,7 @@ __global__ void __launch_bounds__(LA_THREADS, 4) act_backward_kernel(const __nv_
 
 // out[col] = sum over the ranges, in their order: thread (g, c) of 256 takes ranges g, g + 8, ..., then the eight sums are added.
 template <typename T>
-__global__ void __launch_bounds__(LA_THREADS) act_colsum_kernel(const float* __restrict__ partial, int ranges, int N, T* __restrict__ out) {
+__global__ void __launch_bounds__(LA_THREADS) act_colsum_kernel(const float* __restrict__ partial, int ranges, int N, float scale, T* __restrict__ out) {
     pdl_wait();
     pdl_launch_dependents();
     __shared__ float sh[8][32];
@@ -202,7 +215,7 @@ __global__ void __launch_bounds__(LA_THREADS) act_colsum_kernel(const float* __r
             float t = 0.f;
 #pragma unroll
             for (int k = 0; k < 8; k++) t += sh[k][c];
-            out[c0 + c] = Pack8<T>::put(t);
+            out[c0 + c] = Pack8<T>::put(t * scale);
         }
         __syncthreads();
     }
@@ -273,7 +286,7 @@ extern "C" int ob200_linear_act_bf16(const void* x, const void* w, void* y, void
     g.e.drop_scale = rate.scale;
     g.e.rng = rng;
     g.e.site = (uint32_t)site;
-    g.e.slope = (__nv_bfloat16*)slope;
+    g.e.slope = (__half*)slope;
     g.e.ld_slope = ld_slope;
     g.slabs = (float*)workspace;
     g.slab_bytes = (size_t)workspace_bytes;
@@ -320,6 +333,7 @@ extern "C" int ob200_linear_act_backward_bf16(const void* dy, const void* slope,
     float* partial = dbias ? (float*)at : nullptr;
     at += space.partial;
     const void* gz = dz ? (const void*)dz : dy;
+    const float factor = rate.threshold ? rate.scale : 1.f;
     if ((dz && (dx || dw)) || partial) {
         const int ranges = la_ranges(M, N, ob200_plan_sm_count());
         const long long items = (long long)ranges * ((N + LA_COLS - 1) / LA_COLS), cap = (long long)num_ctas * 4 * grid_oversubscription();
@@ -328,12 +342,12 @@ extern "C" int ob200_linear_act_backward_bf16(const void* dy, const void* slope,
         int rc;
         if (N % 8 == 0) {
             OB200_ELASTIC_HBM(act_backward_kernel<true>, 4);
-            rc = launch_pdl(act_backward_kernel<true>, grid, (unsigned)LA_THREADS, st, (const __nv_bfloat16*)dy, (const __nv_bfloat16*)slope, ld_slope, out, ld_dz,
-                            partial, (long long)M, N, ranges, rng, (uint32_t)site, rate.threshold, rate.scale);
+            rc = launch_pdl(act_backward_kernel<true>, grid, (unsigned)LA_THREADS, st, (const __nv_bfloat16*)dy, (const __half*)slope, ld_slope, out, ld_dz,
+                            partial, (long long)M, N, ranges, rng, (uint32_t)site, rate.threshold);
         } else {
             OB200_ELASTIC_HBM(act_backward_kernel<false>, 4);
-            rc = launch_pdl(act_backward_kernel<false>, grid, (unsigned)LA_THREADS, st, (const __nv_bfloat16*)dy, (const __nv_bfloat16*)slope, ld_slope, out,
-                            ld_dz, partial, (long long)M, N, ranges, rng, (uint32_t)site, rate.threshold, rate.scale);
+            rc = launch_pdl(act_backward_kernel<false>, grid, (unsigned)LA_THREADS, st, (const __nv_bfloat16*)dy, (const __half*)slope, ld_slope, out,
+                            ld_dz, partial, (long long)M, N, ranges, rng, (uint32_t)site, rate.threshold);
         }
         if (rc) return rc;
         if (partial) {
@@ -341,10 +355,10 @@ extern "C" int ob200_linear_act_backward_bf16(const void* dy, const void* slope,
             const unsigned blocks = (unsigned)(want < most ? want : most);
             if (bias_f32) {
                 OB200_ELASTIC_HBM(act_colsum_kernel<float>, 8);
-                rc = launch_pdl(act_colsum_kernel<float>, blocks, (unsigned)LA_THREADS, st, (const float*)partial, ranges, N, (float*)dbias);
+                rc = launch_pdl(act_colsum_kernel<float>, blocks, (unsigned)LA_THREADS, st, (const float*)partial, ranges, N, factor, (float*)dbias);
             } else {
                 OB200_ELASTIC_HBM(act_colsum_kernel<__nv_bfloat16>, 8);
-                rc = launch_pdl(act_colsum_kernel<__nv_bfloat16>, blocks, (unsigned)LA_THREADS, st, (const float*)partial, ranges, N, (__nv_bfloat16*)dbias);
+                rc = launch_pdl(act_colsum_kernel<__nv_bfloat16>, blocks, (unsigned)LA_THREADS, st, (const float*)partial, ranges, N, factor, (__nv_bfloat16*)dbias);
             }
             if (rc) return rc;
         }
@@ -358,6 +372,7 @@ extern "C" int ob200_linear_act_backward_bf16(const void* dy, const void* slope,
     g.lda = dz ? ld_dz : N;
     g.b_mn = 1;
     g.ldc = K;
+    g.alpha = factor;
     if (dx) {   // dx[m, k] = sum_n dz[m, n] w[n, k]: w is [reduction, columns] as it lies
         g.b = w; g.ldb = ldw; g.c = dx;
         g.M = M; g.N = K; g.K = N;

@@ -1,7 +1,7 @@
 // Softmax cross-entropy of logits x . w^T over a large vocabulary, and its gradients, without the logits:
 //
 //   loss[t] = lse[t] - l[t, target[t]],   l = x . w^T,   lse[t] = log sum_v exp(l[t, v])
-//   dl = (exp(l - lse) - onehot(target)) * c[t];   dx = dl . w;   dw = dl^T . x       c[t] = upstream gradient (/ rows that count)
+//   dl = exp(l - lse) - onehot(target);   dx = c dl . w;   dw = c dl^T . x       c = upstream gradient (/ rows that count)
 //
 // Forward: one GEMM whose epilogue keeps, of every row and 128 columns, the maximum and the sum of exponentials (gemm_bf16.cu,
 // GM_EPI_LSE), and a kernel that joins them: 2 T V H operations and V / 16 bytes a row instead of 2 V.  Backward, in pieces of the
@@ -121,20 +121,25 @@ __global__ void __launch_bounds__(1024) ce_total_kernel(const float* __restrict_
     }
 }
 
-// Per row (lse * log2(e), coefficient) for the epilogue, and a copy of x without the rows that do not count, whatever they hold (0 times
-// infinity would reach dw).  One warp a row.  A label outside the vocabulary makes the coefficient, and so the gradients, not a number.
+// Per row (lse * log2(e), coefficient) for the epilogue, the factor of both gradients, and a copy of x without the rows that do not count, whatever they hold (0 times
+// infinity would reach dw).  One warp a row.  An upstream gradient that is one number, and the mean's divisor, are the factor, which
+// the products of the rounded dl are multiplied by: in the coefficient they would make every row's largest term, the label's, off by
+// the same rounding.  A label outside the vocabulary makes the coefficient, and so the gradients, not a number.
 __global__ void __launch_bounds__(CE_THREADS) ce_prepare_kernel(const __nv_bfloat16* __restrict__ x, long long ldx, __nv_bfloat16* __restrict__ kept,
                                                                 const float* __restrict__ lse, const long long* __restrict__ target,
                                                                 const float* __restrict__ grad, int grad_per_row, const float* __restrict__ count,
-                                                                float2* __restrict__ row, long long rows, int V, int H, long long ignore_index) {
+                                                                float2* __restrict__ row, float* __restrict__ factor, long long rows, int V, int H,
+                                                                long long ignore_index) {
     pdl_wait();
     pdl_launch_dependents();
     const int lane = threadIdx.x & 31;
     for (long long r = (long long)blockIdx.x * (CE_THREADS / 32) + (threadIdx.x >> 5); r < rows; r += (long long)gridDim.x * (CE_THREADS / 32)) {
         const long long t = target[r];
-        const float g = (grad_per_row ? grad[r] : grad[0]) / (count ? *count : 1.f);
-        const float c = t == ignore_index ? 0.f : t >= 0 && t < V ? g : NAN;
-        if (lane == 0) row[r] = make_float2(lse[r] * CE_LOG2E, c);
+        const float c = t == ignore_index ? 0.f : t >= 0 && t < V ? (grad_per_row ? grad[r] : 1.f) : NAN;
+        if (lane == 0) {
+            row[r] = make_float2(lse[r] * CE_LOG2E, c);
+            if (r == 0) *factor = (grad_per_row ? 1.f : grad[0]) / (count ? *count : 1.f);
+        }
         if (kept) {
             const uint4* src = reinterpret_cast<const uint4*>(x + r * ldx);
             uint4* dst = reinterpret_cast<uint4*>(kept + r * H);
@@ -182,7 +187,7 @@ struct CeBackwardSpace {
     int piece;
     CeBackwardSpace(long long rows, int V, int H, bool want_dx, bool want_dw) {
         piece = ce_piece(rows, V, H, ob200_plan_sm_count());
-        row = ce_round((size_t)rows * sizeof(float2));
+        row = ce_round((size_t)rows * sizeof(float2) + sizeof(float));
         kept = want_dw ? ce_round((size_t)rows * H * 2) : 0;
         dl = ce_round((size_t)rows * piece * 2);
         acc = want_dx && piece < V ? ce_round((size_t)rows * H * sizeof(float)) : 0;
@@ -276,6 +281,7 @@ extern "C" int ob200_linear_cross_entropy_backward(const void* x, const void* w,
     cudaStream_t st = (cudaStream_t)stream;
     char* at = (char*)workspace;
     float2* row = (float2*)at;
+    float* factor = (float*)(row + rows);
     at += space.row;
     __nv_bfloat16* kept = dw ? (__nv_bfloat16*)at : nullptr;
     at += space.kept;
@@ -287,7 +293,7 @@ extern "C" int ob200_linear_cross_entropy_backward(const void* x, const void* w,
         const long long want = ((long long)rows + CE_THREADS / 32 - 1) / (CE_THREADS / 32), cap = (long long)num_ctas * 8;
         OB200_ELASTIC_HBM(ce_prepare_kernel, 8);
         const int rc = launch_pdl(ce_prepare_kernel, (unsigned)(want < cap ? want : cap), (unsigned)CE_THREADS, st, (const __nv_bfloat16*)x, ldx, kept, lse,
-                                  target, grad, grad_per_row, count, row, (long long)rows, V, H, ignore_index);
+                                  target, grad, grad_per_row, count, row, factor, (long long)rows, V, H, ignore_index);
         if (rc) return rc;
     }
     for (int v0 = 0; v0 < V; v0 += space.piece) {
@@ -316,15 +322,17 @@ extern "C" int ob200_linear_cross_entropy_backward(const void* x, const void* w,
         // dx[t, h] += sum_v dl[t, v] w[v, h]
         gx.b = wp; gx.ldb = ldw;
         gx.M = rows; gx.K = nv;
-        gx.epi = first ? GM_EPI_PLAIN : GM_EPI_ACC;
+        gx.epi = GM_EPI_ACC;
         gx.e.addend = first ? nullptr : acc;
+        gx.e.factor = factor;
         gx.out_f32 = last ? 0 : 1;
         gx.c = last ? dx : (void*)acc;
         // dw[v, h] = sum_t dl[t, v] x[t, h]
         gw.a_mn = 1;
         gw.b = kept; gw.ldb = H;
         gw.M = nv; gw.K = rows;
-        gw.epi = GM_EPI_PLAIN;
+        gw.epi = GM_EPI_ACC;
+        gw.e.factor = factor;
         gw.c = (__nv_bfloat16*)dw + (long long)v0 * H;
         if (dx && dw && gemm_bf16_dual_fits(gx, gw)) {
             rc = gemm_bf16_run_dual(gx, gw);

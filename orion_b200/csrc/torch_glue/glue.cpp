@@ -887,7 +887,7 @@ struct LinearAct : public torch::autograd::Function<LinearAct> {
         const at::Tensor xr = as_rows(x), wr = as_rows(w);
         const int64_t M = xr.size(0);
         const at::Tensor res = given(residual) ? residual->contiguous() : at::Tensor();
-        if (want_slope) *slope = at::empty({M, (N + 7) / 8 * 8}, x.options());
+        if (want_slope) *slope = at::empty({M, (N + 7) / 8 * 8}, x.options().dtype(at::kHalf));
         const long long bytes = ob200_linear_act_workspace((int)M, (int)N, (int)K);
         const at::Tensor space = bytes ? workspace(bytes, x) : at::Tensor();
         check(ob200_linear_act_bf16(xr.data_ptr(), wr.data_ptr(), y.data_ptr(), want_slope ? slope->data_ptr() : nullptr,

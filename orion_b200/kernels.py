@@ -450,7 +450,7 @@ def linear_act(x, w, bias=None, residual=None, act="none", p=0.0, rng=None, site
     M, K = x.shape
     N = w.shape[0]
     y = torch.empty((M, N), device=x.device, dtype=x.dtype)
-    slope = torch.empty((M, (N + 7) // 8 * 8), device=x.device, dtype=x.dtype) if want_slope else None
+    slope = torch.empty((M, (N + 7) // 8 * 8), device=x.device, dtype=torch.float16) if want_slope else None
     n = lib().ob200_linear_act_workspace(M, N, K)
     space = torch.empty(n, device=x.device, dtype=torch.uint8) if n else None
     _check(lib().ob200_linear_act_bf16(_ptr(x), _ptr(w), _ptr(y), _ptr(slope), _ptr(bias), int(bias is not None and bias.dtype == torch.float32),
