@@ -12,6 +12,10 @@ Transformer-XL is not reproduced.  Everything is bfloat16 with synthetic token i
 Inference runs on the orion kernels (tcgen05 GEMM and fused attention, LayerNorm, softmax, GELU), and so does
 training (ORION_PREPARE=1, the default): linear layers and attention with all their gradient products on the
 bfloat16 GEMM, LayerNorm / GELU / softmax / embedding / cross-entropy forward and backward, one-launch AdamW.
+ORION_FUSED_LINEAR=1 runs every linear layer with what follows it (bias, GELU, dropout, residual) as one launch, ORION_FUSED_LOSS=1
+computes the decoder's loss from the hidden states, without logits, and ORION_DROPOUT=p trains with dropout of the embeddings and
+of both residual branches, as the reference's clients do (reference benchmarking/model_kernels/bert_8_fb1, fused_dropout_kernel_vec); the
+masks are drawn from counters and never stored.  All three are off by default: recorded profiles have a row per launch.
 With ORION_PREPARE=0 training uses stock PyTorch modules, whose cuBLASLt / flash-attention / elementwise
 launches are captured and scheduled like any other op.
 """
@@ -31,6 +35,12 @@ FUSED_ATTENTION = os.environ.get("ORION_FUSED_ATTENTION", "1") == "1"
 # ORION_OWN_GEMM_TRAINING=0 leaves the GEMMs, the attention and the embeddings of the training clients on the stock kernels
 OWN_GEMM_TRAINING = os.environ.get("ORION_OWN_GEMM_TRAINING", "1") == "1"
 
+# linear layers of the text clients with their bias, GELU, dropout and residual in one launch; loss of the decoder without its logits
+FUSED_LINEAR = os.environ.get("ORION_FUSED_LINEAR", "0") == "1"
+FUSED_LOSS = os.environ.get("ORION_FUSED_LOSS", "0") == "1"
+# dropout probability of the training clients (embeddings and both residual branches)
+DROPOUT = float(os.environ.get("ORION_DROPOUT", "0"))
+
 BERT = dict(layers=12, hidden=768, heads=12, ffn=3072, vocab=30528, max_pos=512, seq=384)
 LM = dict(layers=16, hidden=1024, heads=16, ffn=4096, vocab=32000, seq=512)
 
@@ -46,10 +56,17 @@ def _f32(module, p):
     return hit[1]
 
 
+def _count_step(rng):
+    """(seed, step) of this forward pass, a copy that its backward pass can go by while the model counts on."""
+    rng[1:] += 1
+    return rng.clone()
+
+
 class BertLayer(nn.Module):
-    def __init__(self, h, heads, ffn):
+    def __init__(self, h, heads, ffn, dropout=0.0, site=0):
         super().__init__()
         self.heads = heads
+        self.dropout, self.site = dropout, site   # probability; number of the layer's first dropout in the model
         self.qkv = nn.Linear(h, 3 * h)
         self.out = nn.Linear(h, h)
         self.ln1 = nn.LayerNorm(h, eps=1e-12)
@@ -57,8 +74,18 @@ class BertLayer(nn.Module):
         self.fc2 = nn.Linear(ffn, h)
         self.ln2 = nn.LayerNorm(h, eps=1e-12)
 
-    def forward(self, x, causal=False):
+    def forward(self, x, causal=False, rng=None):
         b, s, h = x.shape
+        p = self.dropout if self.training else 0.0
+        if ORION_TRAIN_KERNELS and OWN_GEMM_TRAINING and x.is_cuda and self.training and x.dtype == torch.bfloat16 and (FUSED_LINEAR or p > 0.0):
+            # the same with bias, GELU, dropout and residual behind the products, not beside them
+            ops = torch.ops.orion
+            ctx = ops.attention_train(ops.linear_act(x, self.qkv.weight, self.qkv.bias), self.heads, 1.0 / math.sqrt(h // self.heads), causal)
+            x = ops.layernorm_train(ops.linear_act(ctx, self.out.weight, self.out.bias, x, "none", p, rng, self.site), self.ln1.weight,
+                                    self.ln1.bias, self.ln1.eps)
+            hid = ops.linear_act(x, self.fc1.weight, self.fc1.bias, None, "gelu")
+            return ops.layernorm_train(ops.linear_act(hid, self.fc2.weight, self.fc2.bias, x, "none", p, rng, self.site + 1), self.ln2.weight,
+                                       self.ln2.bias, self.ln2.eps)
         if ORION_TRAIN_KERNELS and OWN_GEMM_TRAINING and x.is_cuda and self.training and x.dtype == torch.bfloat16:
             # every op of the layer, forward and backward, on the orion kernels; residual adds ride in the GEMM epilogues
             ops = torch.ops.orion
@@ -73,11 +100,11 @@ class BertLayer(nn.Module):
         if ORION_TRAIN_KERNELS and x.is_cuda and self.training:
             # LayerNorm and bias + GELU, forward and backward, on the orion kernels (the GEMMs and the attention stay stock)
             ops = torch.ops.orion
-            x = ops.layernorm_train((x + self.out(ctx)).contiguous(), self.ln1.weight, self.ln1.bias, self.ln1.eps)
+            x = ops.layernorm_train((x + F.dropout(self.out(ctx), p)).contiguous(), self.ln1.weight, self.ln1.bias, self.ln1.eps)
             hid = ops.bias_gelu_train(F.linear(x, self.fc1.weight), self.fc1.bias)
-            return ops.layernorm_train((x + self.fc2(hid)).contiguous(), self.ln2.weight, self.ln2.bias, self.ln2.eps)
-        x = self.ln1(x + self.out(ctx))
-        return self.ln2(x + self.fc2(F.gelu(self.fc1(x))))
+            return ops.layernorm_train((x + F.dropout(self.fc2(hid), p)).contiguous(), self.ln2.weight, self.ln2.bias, self.ln2.eps)
+        x = self.ln1(x + F.dropout(self.out(ctx), p))
+        return self.ln2(x + F.dropout(self.fc2(F.gelu(self.fc1(x))), p))
 
     def forward_orion(self, x, causal=False):
         """Same math on the orion kernels (inference): x [B, S, H] bfloat16."""
@@ -85,6 +112,13 @@ class BertLayer(nn.Module):
         b, s, h = x.shape
         d = h // self.heads
         flat = x.reshape(b * s, h)
+        if FUSED_LINEAR and d == 64 and (s <= 384 or s % 8 == 0) and x.dtype == torch.bfloat16 and FUSED_ATTENTION:
+            attend = ops.attention if s <= 384 else ops.attention_long
+            ctx = attend(ops.linear_act(flat, self.qkv.weight, self.qkv.bias).view(b, s, 3 * h), self.heads, 1.0 / math.sqrt(d), causal)
+            attn = ops.linear_act(ctx, self.out.weight, self.out.bias, flat)
+            y = ops.layernorm(attn, _f32(self, self.ln1.weight), _f32(self, self.ln1.bias), self.ln1.eps)
+            out = ops.linear_act(ops.linear_act(y, self.fc1.weight, self.fc1.bias, None, "gelu"), self.fc2.weight, self.fc2.bias, y)
+            return ops.layernorm(out, _f32(self, self.ln2.weight), _f32(self, self.ln2.bias), self.ln2.eps).view(b, s, h)
         qkv = ops.linear(flat, self.qkv.weight, _f32(self, self.qkv.bias), False)
         if d == 64 and s <= 384 and x.dtype == torch.bfloat16 and FUSED_ATTENTION:
             # scores, softmax and the context product in one kernel, read straight from the projection's output
@@ -114,19 +148,23 @@ class BertQA(nn.Module):
         self.pos = nn.Embedding(cfg["max_pos"], h)
         self.typ = nn.Embedding(2, h)
         self.ln = nn.LayerNorm(h, eps=1e-12)
-        self.layers = nn.ModuleList([BertLayer(h, cfg["heads"], cfg["ffn"]) for _ in range(cfg["layers"])])
+        self.dropout = cfg.get("dropout", 0.0)
+        self.layers = nn.ModuleList([BertLayer(h, cfg["heads"], cfg["ffn"], self.dropout, 2 * i + 1) for i in range(cfg["layers"])])
         self.qa = nn.Linear(h, 2)
+        self.register_buffer("rng", torch.tensor([0, 0]), persistent=False)   # seed and step of the dropout masks
 
     def _own_training(self, ids):
         return ORION_TRAIN_KERNELS and OWN_GEMM_TRAINING and ids.is_cuda and self.training and self.word.weight.dtype == torch.bfloat16
 
-    def embed(self, ids):
+    def embed(self, ids, rng=None):
+        p = self.dropout if self.training else 0.0
         if self._own_training(ids):
             ops = torch.ops.orion
-            return ops.layernorm_train(ops.embedding_train(ids, self.word.weight, self.pos.weight, self.typ.weight), self.ln.weight,
-                                       self.ln.bias, self.ln.eps)
+            x = ops.layernorm_train(ops.embedding_train(ids, self.word.weight, self.pos.weight, self.typ.weight), self.ln.weight,
+                                    self.ln.bias, self.ln.eps)
+            return ops.dropout(x, p, rng, 0) if p > 0.0 else x
         pos = torch.arange(ids.shape[1], device=ids.device)
-        return self.ln(self.word(ids) + self.pos(pos)[None] + self.typ.weight[0])
+        return F.dropout(self.ln(self.word(ids) + self.pos(pos)[None] + self.typ.weight[0]), p)
 
     def forward(self, ids, orion=False):
         if orion and ids.is_cuda and self.word.weight.dtype == torch.bfloat16:
@@ -135,19 +173,24 @@ class BertQA(nn.Module):
             emb = ops.embedding_train(ids.contiguous(), self.word.weight, self.pos.weight, self.typ.weight)
             x = ops.layernorm(emb.view(b * s, -1), _f32(self, self.ln.weight), _f32(self, self.ln.bias), self.ln.eps).view(b, s, -1)
         else:
-            x = self.embed(ids)
+            rng = self._step(ids)
+            x = self.embed(ids, rng)
         for layer in self.layers:
-            x = layer.forward_orion(x) if orion else layer(x)
+            x = layer.forward_orion(x) if orion else layer(x, False, rng)
         return self.qa(x)   # [B, S, 2]: start / end logits
+
+    def _step(self, ids):
+        return _count_step(self.rng) if self.dropout > 0.0 and self._own_training(ids) else None
 
     def span_logits(self, ids):
         """Training on the orion kernels: the start / end logits as [2, B, S] (positions contiguous, the layout the
         loss reads), computed as qa.weight . x^T.  The head's bias is left out: it shifts all positions of a row alike,
         so the position softmax, the loss and every gradient are the same without it (its own gradient is zero)."""
         b, s = ids.shape
-        x = self.embed(ids)
+        rng = self._step(ids)
+        x = self.embed(ids, rng)
         for layer in self.layers:
-            x = layer(x)
+            x = layer(x, False, rng)
         return torch.ops.orion.linear_train(self.qa.weight, x.view(b * s, -1), None).view(2, b, s)
 
 
@@ -157,34 +200,64 @@ class DecoderLM(nn.Module):
         h = cfg["hidden"]
         self.word = nn.Embedding(cfg["vocab"], h)
         self.pos = nn.Embedding(cfg["seq"], h)
-        self.layers = nn.ModuleList([BertLayer(h, cfg["heads"], cfg["ffn"]) for _ in range(cfg["layers"])])
+        self.dropout = cfg.get("dropout", 0.0)
+        self.layers = nn.ModuleList([BertLayer(h, cfg["heads"], cfg["ffn"], self.dropout, 2 * i + 1) for i in range(cfg["layers"])])
         self.ln = nn.LayerNorm(h)
         self.head = nn.Linear(h, cfg["vocab"], bias=False)
+        self.register_buffer("rng", torch.tensor([0, 0]), persistent=False)   # seed and step of the dropout masks
 
-    def forward(self, ids, orion=False):
+    def hidden(self, ids, orion=False):
+        """What the vocabulary projection takes: [B, S, H], behind the last LayerNorm."""
+        p = self.dropout if self.training else 0.0
         if (not orion and ORION_TRAIN_KERNELS and OWN_GEMM_TRAINING and ids.is_cuda and self.training
                 and self.word.weight.dtype == torch.bfloat16):
             ops = torch.ops.orion
+            rng = _count_step(self.rng) if p > 0.0 else None
             x = ops.embedding_train(ids.contiguous(), self.word.weight, self.pos.weight)
+            if p > 0.0:
+                x = ops.dropout(x, p, rng, 0)
             for layer in self.layers:
-                x = layer(x, causal=True)
-            return ops.linear_train(ops.layernorm_train(x, self.ln.weight, self.ln.bias, self.ln.eps), self.head.weight, None)
+                x = layer(x, True, rng)
+            return ops.layernorm_train(x, self.ln.weight, self.ln.bias, self.ln.eps)
         if orion and ids.is_cuda and self.word.weight.dtype == torch.bfloat16:
             x = torch.ops.orion.embedding_train(ids.contiguous(), self.word.weight, self.pos.weight)
         else:
             pos = torch.arange(ids.shape[1], device=ids.device)
-            x = self.word(ids) + self.pos(pos)[None]
+            x = F.dropout(self.word(ids) + self.pos(pos)[None], p)
         if not orion:
             for layer in self.layers:
                 x = layer(x, causal=True)
-            return self.head(self.ln(x))
+            return self.ln(x)
         # inference on the orion kernels: causal softmax, final LayerNorm and the vocabulary projection included
-        ops = torch.ops.orion
         for layer in self.layers:
             x = layer.forward_orion(x, causal=True)
         b, s, h = x.shape
-        y = ops.layernorm(x.reshape(b * s, h), _f32(self, self.ln.weight), _f32(self, self.ln.bias), self.ln.eps)
-        return ops.linear(y, self.head.weight, None, False).view(b, s, -1)
+        return torch.ops.orion.layernorm(x.reshape(b * s, h), _f32(self, self.ln.weight), _f32(self, self.ln.bias), self.ln.eps).view(b, s, h)
+
+    def forward(self, ids, orion=False):
+        x = self.hidden(ids, orion)
+        if orion:
+            return torch.ops.orion.linear(x.view(-1, x.shape[-1]), self.head.weight, None, False).view(*ids.shape, -1)
+        if ORION_TRAIN_KERNELS and OWN_GEMM_TRAINING and ids.is_cuda and self.training and x.dtype == torch.bfloat16:
+            return torch.ops.orion.linear_train(x, self.head.weight, None)
+        return self.head(x)
+
+    def loss(self, ids, target):
+        """Mean cross-entropy of the next tokens `target` [B, S] (-100: not asked for), from the hidden states: on the orion kernels
+        neither the logits nor their gradient, 2 x B x S x vocabulary, are ever in memory."""
+        x = self.hidden(ids)
+        if x.is_cuda and x.dtype == torch.bfloat16 and ORION_TRAIN_KERNELS:
+            return torch.ops.orion.linear_cross_entropy(x, self.head.weight, target.contiguous())
+        return F.cross_entropy(self.head(x).float().flatten(0, 1), target.flatten())
+
+    def score(self, ids):
+        """Log-likelihood of every token given those before it, [B, S - 1] (a scoring request), without the logits."""
+        with torch.no_grad():
+            if ids.is_cuda and self.word.weight.dtype == torch.bfloat16:
+                target = F.pad(ids[:, 1:], (0, 1), value=-100)   # nothing follows the last token
+                return -torch.ops.orion.linear_cross_entropy(self.hidden(ids, orion=True), self.head.weight, target, reduction="none")[:, :-1]
+            logits = self.head(self.hidden(ids))[:, :-1].float()
+            return -F.cross_entropy(logits.flatten(0, 1), ids[:, 1:].flatten(), reduction="none").view(ids.shape[0], -1)
 
 
 def _adamw(params, lr):
@@ -203,7 +276,7 @@ def bert_loop(batchsize, train, num_iters, rps, uniform, dummy_data, local_rank,
     resident = os.environ.get("ORION_RESIDENT_INPUTS", "0") == "1"
 
     def build(device):
-        model = BertQA().to(device).to(torch.bfloat16)
+        model = BertQA(dict(BERT, dropout=DROPOUT)).to(device).to(torch.bfloat16)
         ids = _pinned(torch.randint(0, vocab, (batchsize, seq)))
         labels = _pinned(torch.randint(0, seq, (2, batchsize)))
         state = {"ids": ids.to(device, non_blocking=True), "lab": labels.to(device, non_blocking=True)}
@@ -244,7 +317,7 @@ def transformer_loop(batchsize, train, num_iters, rps, uniform, dummy_data, loca
     resident = os.environ.get("ORION_RESIDENT_INPUTS", "0") == "1"
 
     def build(device):
-        model = DecoderLM().to(device).to(torch.bfloat16)
+        model = DecoderLM(dict(LM, dropout=DROPOUT)).to(device).to(torch.bfloat16)
         tokens = _pinned(torch.randint(0, vocab, (batchsize, seq + 1)))
         state = {"tok": tokens.to(device, non_blocking=True)}
         if train:
@@ -255,6 +328,11 @@ def transformer_loop(batchsize, train, num_iters, rps, uniform, dummy_data, loca
                 if not resident:
                     state["tok"] = tokens.to(device, non_blocking=True)
                 opt.zero_grad()
+                if FUSED_LOSS:
+                    loss = model.loss(state["tok"][:, :-1], state["tok"][:, 1:])
+                    loss.backward()
+                    opt.step()
+                    return loss
                 logits = model(state["tok"][:, :-1])
                 if ORION_TRAIN_KERNELS:   # loss and its gradient straight from the bfloat16 logits, one pass each
                     loss = torch.ops.orion.cross_entropy(logits.reshape(-1, vocab), state["tok"][:, 1:].reshape(-1))
