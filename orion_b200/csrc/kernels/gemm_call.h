@@ -57,15 +57,18 @@ struct GemmCall {
     bool stream_slabs = false;      // split-K partial matrices in the stream's own scratch; otherwise in `slabs` (none: no split)
     float* slabs = nullptr;
     size_t slab_bytes = 0;
+    int splits = 0;                 // parts of the reduction; 0: by the plan
     int num_ctas = 0;
     void* stream = nullptr;
 };
 
 // 0, a cudaError_t, -1 (sizes), -2 (alignment), -4 (no TMA descriptor).
 int gemm_bf16_run(const GemmCall& call);
-// Two products in one launch of CTA pairs, so that the last round of tiles is one and not two: no batch, bias, residual or alpha; rows
-// of C 16-byte multiples.  `fits`: both are wide enough for 256 x 256 tiles and neither wants its reduction split.
-bool gemm_bf16_dual_fits(const GemmCall& first, const GemmCall& second);
+// Two products in one launch of CTA pairs, 256 x 256 tiles, so that the last round of tiles is one and not two: no batch, bias or residual,
+// one alpha, epilogue GM_EPI_ACC (the addend is the first one's), rows of C 16-byte multiples.  `splits`: into how many parts the first
+// one's reduction is cut for that, 0 where the products are too narrow.
+int gemm_bf16_dual_splits(const GemmCall& first, const GemmCall& second);
+size_t gemm_bf16_dual_slab_bytes(const GemmCall& first, const GemmCall& second);
 int gemm_bf16_run_dual(const GemmCall& first, const GemmCall& second);
 // Bytes of partial matrices that the split of such a product (plain or with GM_EPI_ACT) wants; 0 where it is not split.
 size_t gemm_bf16_slab_bytes(int M, int N, int K);

@@ -79,7 +79,7 @@ __device__ __forceinline__ void gm_act_slope(float (&f)[W], int act, uint8_t* sl
     }
 }
 
-// Partial matrices of a product with split-K, as they are: the rest is gemm_splitk_act_kernel's.
+// Partial matrices of a product with split-K, as they are: the rest is a second kernel's.
 template <int COLS>
 __device__ __forceinline__ void gm_epilogue_slab(const GemmParams& p, uint32_t t_row, int m, int n0, int sp) {
 #pragma unroll 1
@@ -348,7 +348,7 @@ __device__ __forceinline__ void gm_epilogue_dual(const GemmParamsDual& p, bool s
     const bool out_f32 = second ? p.second.out_f32 : p.out_f32;
     const unsigned char* map = second ? p.second.tmap_c : p.tmap_c;
     const float* addend = second || m >= M || !p.e.addend ? nullptr : p.e.addend + (long long)m * N;
-    const float factor = p.e.factor ? __ldg(p.e.factor) : 1.f;
+    const float factor = p.e.factor ? p.alpha * __ldg(p.e.factor) : p.alpha;
 #pragma unroll 1
     for (int c0 = 0; c0 < BN; c0 += 32) {
         const int n = n0 + c0;

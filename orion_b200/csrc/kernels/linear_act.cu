@@ -303,7 +303,12 @@ struct LinearBackwardSpace {
         dz = act || threshold || N % 8 ? la_round((size_t)M * ld * 2) : 0;
         partial = want_db ? la_round((size_t)la_ranges(M, N, ob200_plan_sm_count()) * N * sizeof(float)) : 0;
         const size_t a = want_dx ? gemm_bf16_slab_bytes((int)M, K, N) : 0, b = want_dw ? gemm_bf16_slab_bytes(N, K, (int)M) : 0;
-        slabs = la_round(a > b ? a : b);
+        GemmCall gx, gw;
+        gx.M = (int)M; gx.N = gw.N = K; gx.K = N;
+        gw.M = N; gw.K = (int)M;
+        const size_t both = want_dx && want_dw ? gemm_bf16_dual_slab_bytes(gx, gw) : 0;
+        slabs = a > b ? a : b;
+        slabs = la_round(both > slabs ? both : slabs);
         total = dz + partial + slabs;
     }
 };
@@ -373,17 +378,19 @@ extern "C" int ob200_linear_act_backward_bf16(const void* dy, const void* slope,
     g.b_mn = 1;
     g.ldc = K;
     g.alpha = factor;
-    if (dx) {   // dx[m, k] = sum_n dz[m, n] w[n, k]: w is [reduction, columns] as it lies
-        g.b = w; g.ldb = ldw; g.c = dx;
-        g.M = M; g.N = K; g.K = N;
-        const int rc = gemm_bf16_run(g);
+    GemmCall gx = g, gw = g;
+    // dx[m, k] = sum_n dz[m, n] w[n, k]: w is [reduction, columns] as it lies
+    gx.b = w; gx.ldb = ldw; gx.c = dx;
+    gx.M = M; gx.N = K; gx.K = N;
+    // dw[n, k] = sum_m dz[m, n] x[m, k]: both operands are [reduction, ...] as they lie
+    gw.a_mn = 1;
+    gw.b = x; gw.ldb = ldx; gw.c = dw;
+    gw.M = N; gw.N = K; gw.K = M;
+    if (dx && dw && gemm_bf16_dual_splits(gx, gw) > 0) return gemm_bf16_run_dual(gx, gw);
+    if (dx) {
+        const int rc = gemm_bf16_run(gx);
         if (rc) return rc;
     }
-    if (dw) {   // dw[n, k] = sum_m dz[m, n] x[m, k]: both operands are [reduction, ...] as they lie
-        g.a_mn = 1;
-        g.b = x; g.ldb = ldx; g.c = dw;
-        g.M = N; g.N = K; g.K = M;
-        return gemm_bf16_run(g);
-    }
+    if (dw) return gemm_bf16_run(gw);
     return 0;
 }

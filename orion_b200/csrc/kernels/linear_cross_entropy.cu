@@ -164,8 +164,13 @@ static int ce_piece(long long rows, int V, int H, int sms) {
         long long cost = 0;
         for (long long v0 = 0; v0 < V; v0 += v) {
             const long long nv = V - v0 < v ? V - v0 : v, tiles_v = (nv + 255) / 256;
-            const long long dx = tiles_t * tiles_h, dw = tiles_v * tiles_h, dx_cost = nv / 64 + 8, dw_cost = rows / 64 + 8;
-            cost += (tiles_t * tiles_v + pairs - 1) / pairs * (H / 64 + 8);
+            const long long work = tiles_t * tiles_h * (nv / 64) + tiles_v * tiles_h * (rows / 64), dw_cost = rows / 64 + 8;
+            const long long dx = tiles_t * tiles_h, dw = tiles_v * tiles_h, dx_cost = nv / 64 + 8;
+            cost += (tiles_t * tiles_v + pairs - 1) / pairs * (H / 64 + 8) + 16;   // and two launches more
+            if (2 * dx <= pairs) {   // few tiles: their reduction is split, and evens the load
+                cost += work / pairs + dw_cost / 2 + 16;
+                continue;
+            }
             // a pair has every pairs-th unit, those of dx first
             auto load = [&](long long pair) {
                 const long long a = dx > pair ? (dx - pair + pairs - 1) / pairs : 0, b = dx + dw > pair ? (dx + dw - pair + pairs - 1) / pairs - a : 0;
@@ -194,9 +199,13 @@ struct CeBackwardSpace {
         slabs = 0;
         const int last = V - (V - 1) / piece * piece;   // columns of the last piece
         for (int v : {piece < V ? piece : V, last}) {
+            GemmCall gx, gw;
+            gx.M = (int)rows; gx.N = gw.N = H; gx.K = v;
+            gw.M = v; gw.K = (int)rows;
             const size_t a = want_dx ? gemm_bf16_slab_bytes((int)rows, H, v) : 0, b = want_dw ? gemm_bf16_slab_bytes(v, H, (int)rows) : 0;
-            if (a > slabs) slabs = a;
-            if (b > slabs) slabs = b;
+            const size_t c = want_dx && want_dw ? gemm_bf16_dual_slab_bytes(gx, gw) : 0;
+            for (size_t n : {a, b, c})
+                if (n > slabs) slabs = n;
         }
         slabs = ce_round(slabs);
         total = row + kept + dl + acc + slabs;
@@ -334,7 +343,7 @@ extern "C" int ob200_linear_cross_entropy_backward(const void* x, const void* w,
         gw.epi = GM_EPI_ACC;
         gw.e.factor = factor;
         gw.c = (__nv_bfloat16*)dw + (long long)v0 * H;
-        if (dx && dw && gemm_bf16_dual_fits(gx, gw)) {
+        if (dx && dw && gemm_bf16_dual_splits(gx, gw) > 0) {
             rc = gemm_bf16_run_dual(gx, gw);
         } else {
             if (dx) rc = gemm_bf16_run(gx);
