@@ -1,5 +1,5 @@
-// Products of a few rows (single tokens of a few sequences) with a weight matrix, the epilogues of linear_act and of the loss without
-// logits behind them, in one launch:  z[m, n] = sum_k x[m, k] w[n, k],  m <= 32.
+// Products of a few rows (single tokens of a few sequences, a short prompt) with a weight matrix, the epilogues of linear_act and of the
+// loss without logits behind them, in one launch:  z[m, n] = sum_k x[m, k] w[n, k].
 //
 // Bound: reading w once.  Rows of w are the 16-row operand of mma.sync and the tokens its 8 columns, so that nothing is padded to a
 // 128-row tensor-memory tile whose way in and out takes longer than the whole product: 4096 x 1024 with bias and GELU 9.6 -> 4.8 us at one
@@ -76,21 +76,21 @@ __device__ __forceinline__ void few_put(float (&red)[16][LD], const float (&acc)
     }
 }
 
-// A tile's way out, by WARPS warps: the sums of the warps that shared the reduction are joined in their order, then either the epilogue of
+// A tile's way out, by WARPS warps, for tokens [first, first + tokens): the sums of the warps that shared the reduction are joined in their order, then either the epilogue of
 // linear_act, a thread an output, or, half a warp a token and a lane a row of w, the maximum, the sum of exponentials and the label's logit.
 template <int WARPS, int LD, bool LSE>
-__device__ __forceinline__ void few_way_out(const FewRowsParams& p, const float (*red)[16][LD], int tile, int id, int warp, int lane) {
+__device__ __forceinline__ void few_way_out(const FewRowsParams& p, const float (*red)[16][LD], int tile, int first, int tokens, int id, int warp, int lane) {
     const int n0 = tile * p.tile_rows;
     if constexpr (LSE) {
         const int r = lane & 15;
-        for (int m0 = warp * 2; m0 < p.M; m0 += 2 * WARPS) {
+        for (int m0 = warp * 2; m0 < tokens; m0 += 2 * WARPS) {
             const int m = m0 + (lane >> 4);
             float v = -INFINITY;
-            if (m < p.M && r < p.tile_rows && n0 + r < p.N) {
+            if (m < tokens && r < p.tile_rows && n0 + r < p.N) {
                 v = 0.f;
 #pragma unroll
                 for (int k = 0; k < WARPS; k++) v += red[k][r][m];
-                if (p.e.target[m] - n0 == r) p.e.label_logit[m] = v;
+                if (p.e.target[first + m] - n0 == r) p.e.label_logit[first + m] = v;
             }
             float top = v;
 #pragma unroll
@@ -98,13 +98,13 @@ __device__ __forceinline__ void few_way_out(const FewRowsParams& p, const float 
             float sum = exp2f((v - (top == -INFINITY ? 0.f : top)) * 1.4426950408889634f);
 #pragma unroll
             for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            if (r == 0 && m < p.M) p.e.part[(long long)tile * p.M + m] = make_float2(top, sum);
+            if (r == 0 && m < tokens) p.e.part[(long long)tile * p.M + first + m] = make_float2(top, sum);
         }
     } else {
-        for (int i = id; i < p.tile_rows * p.M; i += WARPS * 32) {
+        for (int i = id; i < p.tile_rows * tokens; i += WARPS * 32) {
             const int r = i % p.tile_rows, m = i / p.tile_rows, n = n0 + r;
             if (n >= p.N) continue;
-            const long long index = (long long)m * p.N + n;
+            const long long index = (long long)(first + m) * p.N + n;
             const float add = p.bias ? p.bias[n] : p.bias_bf16 ? __bfloat162float(p.bias_bf16[n]) : 0.f;
             const float res = p.residual ? __bfloat162float(p.residual[index]) : 0.f;
             float z = 0.f;
@@ -114,7 +114,7 @@ __device__ __forceinline__ void few_way_out(const FewRowsParams& p, const float 
             if (p.e.act) {
                 float slope;
                 z = act_slope(z, p.e.act, slope);
-                if (p.e.slope) p.e.slope[m * p.e.ld_slope + n] = __float2half_rn(slope);
+                if (p.e.slope) p.e.slope[(first + m) * p.e.ld_slope + n] = __float2half_rn(slope);
             }
             if (p.e.drop_threshold) {
                 uint32_t bits[4];
@@ -130,7 +130,8 @@ __device__ __forceinline__ void few_way_out(const FewRowsParams& p, const float 
 
 // ------------------------------------------------------------------ few tiles: straight to registers
 // Sixteen warps share a tile's reduction, four k-blocks of 32 (two of them for 32 tokens) under way in each.  There is no ring to fill and no copy to wait for, so
-// a launch of one or two tiles an SM is over sooner: 1024 x 4096 7.8 -> 5.4 us.
+// a launch of one or two tiles an SM is over sooner: 1024 x 4096 7.8 -> 5.9 us.  More than 32 tokens are groups of 32, each with tiles of
+// its own: w is then read from L2 once a group.
 template <int NT, bool LSE>
 __global__ void __launch_bounds__(FEW_CONSUMERS * 32, NT == 2 ? 1 : 2) few_tiles_kernel(const __grid_constant__ FewRowsParams p) {
     constexpr int LD = NT * 8 + 1, WARPS = FEW_CONSUMERS, DEPTH = NT == 4 ? 2 : 4;
@@ -141,10 +142,11 @@ __global__ void __launch_bounds__(FEW_CONSUMERS * 32, NT == 2 ? 1 : 2) few_tiles
     const int kblocks = (p.K + 31) / 32, kb0 = kblocks * warp / WARPS, kb1 = kblocks * (warp + 1) / WARPS;
     const int tiles = (p.N + p.tile_rows - 1) / p.tile_rows;
     const uint4 zero = make_uint4(0, 0, 0, 0);
-    for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+    for (int unit = blockIdx.x; unit < tiles * ((p.M + 31) / 32); unit += gridDim.x) {
+        const int tile = unit % tiles, first = unit / tiles * 32, tokens = p.M - first < 32 ? p.M - first : 32;
         const int r0 = tile * p.tile_rows + g, r1 = r0 + 8;
         const bool has0 = r0 < p.N, has1 = p.tile_rows == 16 && r1 < p.N;
-        const __nv_bfloat16 *w0 = p.w + (long long)r0 * p.ldw + t * 8, *w1 = w0 + 8 * p.ldw, *x0 = p.x + (long long)g * p.ldx + t * 8;
+        const __nv_bfloat16 *w0 = p.w + (long long)r0 * p.ldw + t * 8, *w1 = w0 + 8 * p.ldw, *x0 = p.x + (long long)(first + g) * p.ldx + t * 8;
         float acc[NT][4];
 #pragma unroll
         for (int i = 0; i < NT; i++) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
@@ -157,7 +159,7 @@ __global__ void __launch_bounds__(FEW_CONSUMERS * 32, NT == 2 ? 1 : 2) few_tiles
                 a[d][0] = in && has0 ? few_load(w0 + k) : zero;
                 a[d][1] = in && has1 ? few_load(w1 + k) : zero;
 #pragma unroll
-                for (int i = 0; i < NT; i++) b[d][i] = in && g + i * 8 < p.M ? __ldg(reinterpret_cast<const uint4*>(x0 + i * 8 * p.ldx + k)) : zero;
+                for (int i = 0; i < NT; i++) b[d][i] = in && g + i * 8 < tokens ? __ldg(reinterpret_cast<const uint4*>(x0 + i * 8 * p.ldx + k)) : zero;
             }
 #pragma unroll
             for (int d = 0; d < DEPTH; d++)
@@ -169,7 +171,7 @@ __global__ void __launch_bounds__(FEW_CONSUMERS * 32, NT == 2 ? 1 : 2) few_tiles
         }
         few_put(red[warp], acc, g, t);
         __syncthreads();
-        few_way_out<WARPS, LD, LSE>(p, red, tile, threadIdx.x, warp, lane);
+        few_way_out<WARPS, LD, LSE>(p, red, tile, first, tokens, threadIdx.x, warp, lane);
         __syncthreads();
     }
 }
@@ -288,22 +290,25 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_rows_kernel(const __grid_c
             few_put(red[group][kw], acc, g, t);
             meet();
             if (!ok) continue;
-            few_way_out<WARPS, LD, LSE>(p, red[group], tile, id, kw, lane);
+            few_way_out<WARPS, LD, LSE>(p, red[group], tile, 0, p.M, id, kw, lane);
         }
     }
 }
 
 // 16 rows of w a tile, or 8 where tiles of 16 would leave SMs without one.
-static int few_tile_rows(int N) { return (N + 15) / 16 >= ob200_plan_sm_count() ? 16 : 8; }
+static int few_tile_rows(int M, int N) { return (long long)(N + 15) / 16 * ((M + 31) / 32) >= ob200_plan_sm_count() ? 16 : 8; }
 
 // Whether a launch is of few tiles: all of them resident at once, two an SM.  By the sizes and the device, because it sets the order of
-// a sum.  32000 x 1024, one token: 15.6 us of single-token tiles straight to registers, 14.6 through the ring; 16 tokens 19.4 and 18.2.
-static bool few_tiles(int N) { return (N + few_tile_rows(N) - 1) / few_tile_rows(N) <= 2 * ob200_plan_sm_count(); }
+// a sum.  32000 x 1024, one token: 15.6 us straight to registers, 14.6 through the ring; 16 tokens 19.4 and 18.2.
+static bool few_tiles(int M, int N) {
+    const int rows = few_tile_rows(M, N);
+    return ((long long)N + rows - 1) / rows * ((M + 31) / 32) <= 2 * ob200_plan_sm_count();
+}
 
 struct FewPlan { int stages, bytes; };
 static FewPlan few_plan(int M, int N, int K) {
     const int nt = M <= 8 ? 1 : M <= 16 ? 2 : 4, boxes = (K + FEW_BOX - 1) / FEW_BOX;
-    const int fixed = FEW_CTL + FEW_CONSUMERS * 16 * (nt * 8 + 1) * 4 + boxes * nt * 8 * FEW_BOX * 2, stage_bytes = few_tile_rows(N) * FEW_CHUNK * 2;
+    const int fixed = FEW_CTL + FEW_CONSUMERS * 16 * (nt * 8 + 1) * 4 + boxes * nt * 8 * FEW_BOX * 2, stage_bytes = few_tile_rows(M, N) * FEW_CHUNK * 2;
     FewPlan f;
     const int room = FEW_SMEM - fixed, stages = room > 0 && K <= FEW_CHUNK * FEW_MAX_CHUNKS ? room / stage_bytes : 0;
     f.stages = (stages < FEW_MAX_STAGES ? stages : FEW_MAX_STAGES) / FEW_GROUPS;
@@ -329,15 +334,19 @@ static bool few_make_map(unsigned char* out, const void* base, int cols, int row
                       CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-bool few_rows_fit(int M, int N, int K) { return M > 0 && M <= FEW_MAX_ROWS && N > 0 && K > 0 && (few_tiles(N) || few_plan(M, N, K).stages >= 2); }
-int few_rows_parts(int V) { return (V + few_tile_rows(V) - 1) / few_tile_rows(V); }
+bool few_rows_fit(int M, int N, int K) {
+    if (M <= 0 || N <= 0 || K <= 0) return false;
+    return few_tiles(M, N) || (M <= FEW_MAX_ROWS && few_plan(M, N, K).stages >= 2);
+}
+int few_rows_parts(int M, int V) { return (V + few_tile_rows(M, V) - 1) / few_tile_rows(M, V); }
 
 template <int NT, bool LSE>
 static int few_launch(const FewRowsParams& p, int num_ctas, cudaStream_t stream) {
     const int tiles = (p.N + p.tile_rows - 1) / p.tile_rows;
-    if (few_tiles(p.N)) {
+    if (few_tiles(p.M, p.N)) {
+        const int units = tiles * ((p.M + 31) / 32);
         OB200_ELASTIC_HBM((few_tiles_kernel<NT, LSE>), 2);
-        return launch_pdl(few_tiles_kernel<NT, LSE>, (unsigned)(tiles < 2 * num_ctas ? tiles : 2 * num_ctas), FEW_CONSUMERS * 32u, stream, p);
+        return launch_pdl(few_tiles_kernel<NT, LSE>, (unsigned)(units < 2 * num_ctas ? units : 2 * num_ctas), FEW_CONSUMERS * 32u, stream, p);
     }
     static bool attr_set[64] = {};
     int dev = 0;
@@ -358,10 +367,10 @@ int few_rows_run(const GemmCall& g) {
     p.x = (const __nv_bfloat16*)g.a; p.w = (const __nv_bfloat16*)g.b;
     p.ldx = g.lda; p.ldw = g.ldb;
     p.M = g.M; p.N = g.N; p.K = g.K;
-    p.tile_rows = few_tile_rows(g.N);
+    p.tile_rows = few_tile_rows(g.M, g.N);
     p.chunks = (g.K + FEW_CHUNK - 1) / FEW_CHUNK;
     p.stages = few_plan(g.M, g.N, g.K).stages;
-    if (few_tiles(g.N)) p.status = nullptr;   // it waits for nothing
+    if (few_tiles(g.M, g.N)) p.status = nullptr;   // it waits for nothing
     else if (!few_make_map(p.tmap_x, g.a, g.K, g.M, g.lda, g.M <= 8 ? 8 : g.M <= 16 ? 16 : 32) || !few_make_map(p.tmap_w, g.b, g.K, g.N, g.ldb, p.tile_rows)) return -4;
     else p.status = ob200_status_word_for_current_device();
     p.bias = g.bias;

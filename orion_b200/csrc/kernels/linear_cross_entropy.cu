@@ -217,7 +217,7 @@ struct CeBackwardSpace {
 using namespace ob200;
 
 // Parts of a row that a forward pass writes; the workspace has room for those of either kernel.
-static int ce_parts(int rows, int V, int H) { return few_rows_fit(rows, V, H) ? few_rows_parts(V) : (V + 127) / 128; }
+static int ce_parts(int rows, int V, int H) { return few_rows_fit(rows, V, H) ? few_rows_parts(rows, V) : (V + 127) / 128; }
 
 extern "C" long long ob200_linear_cross_entropy_workspace(int rows, int V) {
     if (rows <= 0 || V <= 0) return 0;
