@@ -717,9 +717,17 @@ static bool gm_make_slab_map(unsigned char* out, const void* base, int M, int N,
 // bit) is the same for every quota.  Tile width and pairing do not touch the order; they are chosen again for a smaller quota, where
 // rounds are many and an odd CTA is lost to pairs (three CTAs, 3072 x 2304 x 768: 663 us in two, 348 in three).  With few CTAs at
 // work a pair's k-block gains 7 % more on a single CTA's than on the full device (seven CTAs, 8192 x 1024 x 1024: 201 us in six, 212).
+// Which splits a call may have.  GM_SPLIT_FILL is the rule above: few tiles are always cut until they fill the device.  GM_SPLIT_PRICED, of the
+// epilogues that are not GM_EPI_PLAIN, weighs every number of parts, none among them, with a second launch that costs 4 us: 256 x 4096 x
+// 1024 with bias and GELU, 64 tiles, 16.8 us in two parts and 9.3 in one.
+enum GemmSplit { GM_SPLIT_NEVER, GM_SPLIT_FILL, GM_SPLIT_PRICED };
+static GemmSplit gm_split_rule(int epi) {
+    return epi == GM_EPI_LSE || epi == GM_EPI_DLOGITS ? GM_SPLIT_NEVER : epi == GM_EPI_PLAIN ? GM_SPLIT_FILL : GM_SPLIT_PRICED;
+}
 struct GemmPlan { int bn, cg, splits, grid; };
 struct GemmTile { int bn, cg; double kblock_us, tile_us, tail_us, launch_us; };
-static GemmPlan gm_plan(int M, int N, int K, long long batch, int tri, int device_sms, int num_ctas, bool splittable = true) {
+static GemmPlan gm_plan(int M, int N, int K, long long batch, int tri, int device_sms, int num_ctas, GemmSplit rule = GM_SPLIT_FILL) {
+    const bool splittable = rule != GM_SPLIT_NEVER;
     static const GemmTile kNarrow = {64, 1, 0.44, 2.15, 1.0, 0.0};   // outputs of at most 64 columns
     static const GemmTile kTiles[] = {{128, 1, 0.44, 2.15, 1.0, 0.0}, {256, 1, 0.51, 3.0, 2.0, 0.0},
                                       {128, 2, 0.32, 2.15, 1.0, 1.3}, {256, 2, 0.45, 3.0, 2.0, 1.3}};
@@ -732,7 +740,7 @@ static GemmPlan gm_plan(int M, int N, int K, long long batch, int tri, int devic
         const double rounds = (double)((tiles_of(t.bn, t.cg) * splits + at_once - 1) / at_once);
         const double depth = (double)((kblocks + splits - 1) / splits) * t.kblock_us * (t.cg == 2 ? pair_relief : 1.0);
         const double us = t.launch_us + rounds * (depth > t.tile_us ? depth : t.tile_us) + t.tail_us;
-        return splits > 1 ? us + 6.0 + (double)splits * batch * M * N * 8.0 / 6e6 : us;
+        return splits > 1 ? us + (rule == GM_SPLIT_PRICED ? 4.0 : 6.0) + (double)splits * batch * M * N * 8.0 / 6e6 : us;
     };
     const bool may_split = tiles_of(list[0].bn, 1) * 2 <= device_sms && kblocks >= 8 && tri == 0 && splittable;
     GemmPlan pl = {0, 1, 1, 1};
@@ -747,8 +755,10 @@ static GemmPlan gm_plan(int M, int N, int K, long long batch, int tri, int devic
             if (sp > kblocks / 4) sp = kblocks / 4;
             if (sp > 16) sp = 16;
         }
-        const double us = price(t, (int)sp, at_once, 1.0);
-        if (pl.bn == 0 || us < best) { best = us; pl.bn = t.bn; pl.cg = t.cg; pl.splits = (int)sp; }
+        for (long long n = rule == GM_SPLIT_PRICED ? 1 : sp; n <= sp; n++) {
+            const double us = price(t, (int)n, at_once, 1.0);
+            if (pl.bn == 0 || us < best) { best = us; pl.bn = t.bn; pl.cg = t.cg; pl.splits = (int)n; }
+        }
     }
     if (num_ctas < device_sms) {
         pl.bn = 0;
@@ -826,9 +836,9 @@ extern "C" int ob200_plan_gemm_bf16(int M, int N, int K, long long batch, int tr
 
 namespace ob200 {
 
-size_t gemm_bf16_slab_bytes(int M, int N, int K) {
+size_t gemm_bf16_slab_bytes(int M, int N, int K, int epi) {
     const int sms = ob200_plan_sm_count();
-    const GemmPlan pl = gm_plan(M, N, K, 1, 0, sms, sms);
+    const GemmPlan pl = gm_plan(M, N, K, 1, 0, sms, sms, gm_split_rule(epi));
     return pl.splits > 1 ? (size_t)pl.splits * M * N * sizeof(float) : 0;
 }
 
@@ -885,7 +895,7 @@ int gemm_bf16_run(const GemmCall& g) {
     p.vec_ok = ((uintptr_t)c % 16 == 0) && ((uintptr_t)residual % 16 == 0) && (!residual || !out_f32) && (ldc % cal == 0) && (batch_inner == 1 || c_si % cal == 0) && (batch_outer == 1 || c_so % cal == 0);
     const int plan = ob200_plan_sm_count();
     p.kblocks = (K + GM_BK - 1) / GM_BK;
-    const GemmPlan pl = gm_plan(M, N, K, batch_ll, tri, plan, num_ctas, epi != GM_EPI_LSE && epi != GM_EPI_DLOGITS);
+    const GemmPlan pl = gm_plan(M, N, K, batch_ll, tri, plan, num_ctas, gm_split_rule(epi));
     const int bn = pl.bn, cg = pl.cg;
     int splits = g.splits > 0 ? g.splits : pl.splits;
     p.tiles_m = (M + cg * GM_BM - 1) / (cg * GM_BM);

@@ -70,8 +70,8 @@ int gemm_bf16_run(const GemmCall& call);
 int gemm_bf16_dual_splits(const GemmCall& first, const GemmCall& second);
 size_t gemm_bf16_dual_slab_bytes(const GemmCall& first, const GemmCall& second);
 int gemm_bf16_run_dual(const GemmCall& first, const GemmCall& second);
-// Bytes of partial matrices that the split of such a product (plain or with GM_EPI_ACT) wants; 0 where it is not split.
-size_t gemm_bf16_slab_bytes(int M, int N, int K);
+// Bytes of partial matrices that the split of a product with this epilogue wants; 0 where it is not split.
+size_t gemm_bf16_slab_bytes(int M, int N, int K, int epi);
 
 // The same for few rows (few_rows.cu; up to 32, more where all tiles are resident at once): GM_EPI_ACT, and GM_EPI_LSE with `few_rows_parts` parts a row instead of N / 128.
 bool few_rows_fit(int M, int N, int K);

@@ -261,7 +261,7 @@ extern "C" int ob200_dropout(const void* x, const void* residual, void* y, long 
 
 extern "C" long long ob200_linear_act_workspace(int M, int N, int K) {
     if (M <= 0 || N <= 0 || K <= 0 || few_rows_fit(M, N, K)) return 0;
-    return (long long)gemm_bf16_slab_bytes(M, N, K);
+    return (long long)gemm_bf16_slab_bytes(M, N, K, GM_EPI_ACT);
 }
 
 extern "C" int ob200_linear_act_bf16(const void* x, const void* w, void* y, void* slope, const void* bias, int bias_f32, const void* residual, int act,
@@ -302,7 +302,7 @@ struct LinearBackwardSpace {
         const long long ld = (N + 7) / 8 * 8;
         dz = act || threshold || N % 8 ? la_round((size_t)M * ld * 2) : 0;
         partial = want_db ? la_round((size_t)la_ranges(M, N, ob200_plan_sm_count()) * N * sizeof(float)) : 0;
-        const size_t a = want_dx ? gemm_bf16_slab_bytes((int)M, K, N) : 0, b = want_dw ? gemm_bf16_slab_bytes(N, K, (int)M) : 0;
+        const size_t a = want_dx ? gemm_bf16_slab_bytes((int)M, K, N, GM_EPI_ACC) : 0, b = want_dw ? gemm_bf16_slab_bytes(N, K, (int)M, GM_EPI_ACC) : 0;
         GemmCall gx, gw;
         gx.M = (int)M; gx.N = gw.N = K; gx.K = N;
         gw.M = N; gw.K = (int)M;
@@ -378,6 +378,7 @@ extern "C" int ob200_linear_act_backward_bf16(const void* dy, const void* slope,
     g.b_mn = 1;
     g.ldc = K;
     g.alpha = factor;
+    g.epi = GM_EPI_ACC;
     GemmCall gx = g, gw = g;
     // dx[m, k] = sum_n dz[m, n] w[n, k]: w is [reduction, columns] as it lies
     gx.b = w; gx.ldb = ldw; gx.c = dx;

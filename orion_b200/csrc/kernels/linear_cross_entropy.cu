@@ -202,7 +202,7 @@ struct CeBackwardSpace {
             GemmCall gx, gw;
             gx.M = (int)rows; gx.N = gw.N = H; gx.K = v;
             gw.M = v; gw.K = (int)rows;
-            const size_t a = want_dx ? gemm_bf16_slab_bytes((int)rows, H, v) : 0, b = want_dw ? gemm_bf16_slab_bytes(v, H, (int)rows) : 0;
+            const size_t a = want_dx ? gemm_bf16_slab_bytes((int)rows, H, v, GM_EPI_ACC) : 0, b = want_dw ? gemm_bf16_slab_bytes(v, H, (int)rows, GM_EPI_ACC) : 0;
             const size_t c = want_dx && want_dw ? gemm_bf16_dual_slab_bytes(gx, gw) : 0;
             for (size_t n : {a, b, c})
                 if (n > slabs) slabs = n;

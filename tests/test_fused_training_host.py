@@ -116,7 +116,7 @@ def test_entry_points_refuse_bad_arguments_without_a_gpu(K):
         assert act(**bad) == -1, bad
     for bad in (dict(x=a + 8), dict(w=a + 2), dict(y=a + 4), dict(ldx=12), dict(ldw=9), dict(act=1, slope=a + 8, ld_slope=8)):
         assert act(**bad) == -2, bad
-    M, N, KK = 64, 1024, 4096
+    M, N, KK = 600, 1024, 4096
     need = L.ob200_linear_act_workspace(M, N, KK)
     assert need > 0 and need % (4 * M * N) == 0
     assert act(M=M, N=N, K=KK, ldx=KK, ldw=KK, ws=a, nbytes=need - 1) == -3
