@@ -16,7 +16,7 @@
 // and SM): decoder feed-forward 8192 x 4096 x 1024 57.9 -> 50.3 us (1.37 PFLOP/s), vocabulary projection 8192 x 32000 x 1024
 // 505 -> 411 us.  Warp 0 issues TMA copies (4-D tensor maps:
 // inner, outer, batch_inner, batch_outer; out-of-range elements read as zero, so ragged M, N, K need no special path),
-// warp 1 issues tcgen05.mma kind::f16 into one of two tensor-memory accumulators, warps 2-5 drain the other one:
+// warp 1 issues tcgen05.mma kind::f16 into one of two tensor-memory accumulators, warps 2-5 (more for the epilogues that compute) drain the other one:
 // tcgen05.ld (one output row per thread), alpha / bias / residual in registers, 32 rows x 128 bytes staged in a swizzled
 // shared-memory slab per warp and written by a TMA store (two slabs per warp in flight; the tensor map clips ragged edges;
 // outputs whose rows are not 16-byte multiples take per-thread stores).  An MN-major operand is declared as such in the instruction
@@ -47,8 +47,10 @@ namespace ob200 {
 constexpr int GM_BM = 128;
 constexpr int GM_BK = 64;
 // Warp 0: TMA, warp 1: MMA + tensor memory, the others: epilogue.  Four of them, or sixteen (four for each 32 rows, each a share of the
-// columns) where a turn of the epilogue is a long chain of latencies: bias + GELU of 8192 x 4096 x 1024.
-__host__ __device__ constexpr int gm_epi_warps(int epi) { return epi == GM_EPI_ACT || epi == GM_EPI_ACT_SLOPE || epi == GM_EPI_ACT_ANY ? 16 : epi == GM_EPI_DLOGITS ? 8 : 4; }
+// columns) where a turn of the epilogue is a long chain of latencies: bias + GELU of 8192 x 4096 x 1024.  Eight for the loss: over a
+// short reduction the exponentials bound it (4096 x 16384 x 256: row maxima and sums 57 us in four warps, 44 in eight; over 1024 deep
+// no difference), and sixteen for its gradient take the stages that a deep one needs (2048 x 32000 x 1024: 475 us in eight, 486).
+__host__ __device__ constexpr int gm_epi_warps(int epi) { return epi == GM_EPI_ACT || epi == GM_EPI_ACT_SLOPE || epi == GM_EPI_ACT_ANY ? 16 : epi == GM_EPI_LSE || epi == GM_EPI_DLOGITS ? 8 : 4; }
 __host__ __device__ constexpr int gm_threads(int epi) { return 64 + 32 * gm_epi_warps(epi); }
 constexpr int GM_A_BYTES = GM_BM * 128;
 
@@ -344,7 +346,8 @@ __global__ void __launch_bounds__(gm_threads(EPI), 1) gemm_bf16_kernel(const __g
             if (w.skip) continue;
             const uint32_t ab = local & 1u, use = local >> 1;
             local++;
-            constexpr int kCols = BN * 4 / gm_epi_warps(EPI) < 32 ? 32 : BN * 4 / gm_epi_warps(EPI);   // columns of a tile that a warp takes
+            // columns of a tile that a warp takes; a row's maximum and sum are those of 128 columns in one warp
+            constexpr int kLeast = EPI == GM_EPI_LSE ? 128 : 32, kCols = BN * 4 / gm_epi_warps(EPI) < kLeast ? kLeast : BN * 4 / gm_epi_warps(EPI);
             const int part = (warp - 2) >> 2;
             const bool idle = part * kCols >= BN;   // a narrow tile has no columns for this warp
             const int m0w = (tm * CG + (int)rank) * GM_BM + q * 32;      // first row of this warp's 32
@@ -372,7 +375,7 @@ __global__ void __launch_bounds__(gm_threads(EPI), 1) gemm_bf16_kernel(const __g
             } else if constexpr (EPI == GM_EPI_DUAL) {
                 if (p.splits > 1 && !w.second) gm_epilogue_slab<BN>(p, t_row, m, n0, sp);
                 else gm_epilogue_dual<BN>(p, w.second, t_row, m, m0w, n0, lane, epi_smem + (warp - 2) * 8192, slab_i);
-            } else if constexpr (EPI == GM_EPI_LSE) gm_epilogue_lse<BN>(p, t_row, m, n0);
+            } else if constexpr (EPI == GM_EPI_LSE) gm_epilogue_lse<kCols>(p, t_row + part * kCols, m, n0 + part * kCols);
             else if constexpr (EPI == GM_EPI_DLOGITS) gm_epilogue_dlogits<kCols>(p, t_row + part * kCols, m, m0w, n0 + part * kCols, lane, epi_smem + (warp - 2) * 4096, slab_i);
             else {
             const bool to_slab = p.splits > 1;
@@ -1006,9 +1009,11 @@ static bool gm_make_c_map(unsigned char* out, const GemmCall& g) {
 // Whether two products run as one launch, and the split of the first one's reduction: 0 for no.  The fewest k-blocks of 64 on the CTA pair
 // that has most of them, eight added for a tile's way out, and for a split the second launch and its partial matrices at 0.45 us a
 // k-block and 6 TB/s.  Planned for the device, so that the order of the sums is the same for every CTA count.
+// Outputs of at most 128 columns have narrower tiles in launches of their own; one of 136 is better in one tile of 256 than in two of
+// 128 that read the other operand twice (gradient products of 6437 x 13042 x 136: 143 us in two launches, 77 in one).
 int gemm_bf16_dual_splits(const GemmCall& a, const GemmCall& b) {
     for (const GemmCall* g : {&a, &b})
-        if (g->M <= GM_BM || g->N < 256 || g->N % 8) return 0;
+        if (g->M <= GM_BM || g->N <= 128 || g->N % 8) return 0;
     const int pairs = ob200_plan_sm_count() / 2;
     if (pairs < 1) return 0;
     auto tiles = [](const GemmCall& g) { return (((long long)g.M + 255) / 256) * (((long long)g.N + 255) / 256); };

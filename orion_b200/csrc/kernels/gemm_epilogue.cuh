@@ -248,15 +248,15 @@ __device__ __forceinline__ void gm_epilogue_act_any(const GemmParams& p, uint32_
 }
 
 // Of every row and 128 columns the maximum and the sum of exponentials relative to it, and the logit of the row's label.
-template <int BN>
+template <int COLS>
 __device__ __forceinline__ void gm_epilogue_lse(const GemmParams& p, uint32_t t_row, int m, int n0) {
     constexpr float kLog2e = 1.4426950408889634f;
     const bool row_ok = m < p.M;
     const long long at = row_ok ? p.e.target[m] - p.e.col0 - n0 : -1;
-    const int label = at >= 0 && at < BN ? (int)at : -1;   // the label's column of this tile
+    const int label = at >= 0 && at < COLS ? (int)at : -1;   // the label's column of this warp's
     float top = -INFINITY, sum = 0.f;
 #pragma unroll 1
-    for (int c0 = 0; c0 < BN; c0 += 32) {
+    for (int c0 = 0; c0 < COLS; c0 += 32) {
         const int n = n0 + c0;
         if (n >= p.N) break;            // warp-uniform
         float f[32];
@@ -277,14 +277,19 @@ __device__ __forceinline__ void gm_epilogue_lse(const GemmParams& p, uint32_t t_
         const float now = fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), top);
         const float ref = now == -INFINITY ? 0.f : now * kLog2e;   // columns of minus infinity alone weigh nothing
         // nothing above minus infinity so far: a sum of 0, or not a number
-        float part[4] = {top == -INFINITY ? sum : sum * exp2f(top * kLog2e - ref), 0.f, 0.f, 0.f};
+        uint64_t part[2] = {f32x2(top == -INFINITY ? sum : sum * exp2f(top * kLog2e - ref), 0.f), f32x2(0.f, 0.f)};
 #pragma unroll
-        for (int j = 0; j < 32; j++) {
-            float e;
-            asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(fmaf(f[j], kLog2e, -ref)));
-            part[j & 3] += e;
+        for (int j = 0; j < 32; j += 2) {
+            float e0, e1;
+            split_f32x2(fma_f32x2(f32x2(f[j], f[j + 1]), f32x2(kLog2e, kLog2e), f32x2(-ref, -ref)), e0, e1);
+            asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e0) : "f"(e0));
+            asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e1) : "f"(e1));
+            part[j >> 1 & 1] = add_f32x2(part[j >> 1 & 1], f32x2(e0, e1));
         }
-        sum = (part[0] + part[1]) + (part[2] + part[3]);
+        float s0, s1, s2, s3;
+        split_f32x2(part[0], s0, s1);
+        split_f32x2(part[1], s2, s3);
+        sum = (s0 + s1) + (s2 + s3);
         top = now;
         if (((c0 + 32) & 127) == 0 || n + 32 >= p.N) {
             if (row_ok) p.e.part[(long long)(n >> 7) * p.M + m] = make_float2(top, sum);

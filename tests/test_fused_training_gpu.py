@@ -395,7 +395,7 @@ def check_loss(ops, x, w, target, reduction, upstream=None):
     return out.detach(), dx, dw
 
 
-LOSS_SIZES = [(1, 1, 8), (1, 1000, 64), (3, 7, 8), (16, 1000, 64), (130, 515, 72), (257, 2050, 136), (77, 30522, 64), (300, 128, 1024), (600, 4096, 200)]
+LOSS_SIZES = [(1, 1, 8), (1, 1000, 64), (3, 7, 8), (16, 1000, 64), (130, 515, 72), (257, 2050, 136), (77, 30522, 64), (300, 128, 1024), (600, 4096, 200), (2100, 5003, 248)]
 
 
 @pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
