@@ -286,7 +286,7 @@ int ob200_dropout(const void* x, const void* residual, void* y, long long n, flo
 int ob200_linear_cross_entropy_forward(const void* x, const void* w, const long long* target, float* loss, float* lse, float* total,
                                        float* count, int rows, int V, int H, long long ldx, long long ldw, long long ignore_index, int mean,
                                        void* workspace, long long workspace_bytes, int num_ctas, void* stream);
-long long ob200_linear_cross_entropy_workspace(int rows, int V);
+long long ob200_linear_cross_entropy_workspace(int rows, int V, int H);
 /* Its gradients in pieces of the vocabulary, dx [rows, H] and dw [V, H] contiguous bfloat16 (either may be NULL): logits of a piece are
  * computed again.  grad: the upstream gradient, one value or one per row (grad_per_row), divided by *count where count is given (the
  * mean).  Rows that do not count contribute nothing, whatever x holds there. */

@@ -83,12 +83,16 @@ struct GemmParams {
                              // 2 = A[m, k] is zero for k > m (reduction stops behind the tile's last row),
                              // 3 = A[m, k] is zero for k < m (reduction starts at the tile's first row)
     float alpha;
+    const int* live;         // packed rows: how many count, or null
+    int live_k;              // they are the reduction (of a dual launch's second product in any case)
+    int live_all;            // with as many as this the operand in tmap_all is taken, unpacked (0: never)
     GemmEpi e;               // of the epilogues other than GM_EPI_PLAIN
     alignas(64) unsigned char tmap_a[128];
     alignas(64) unsigned char tmap_b[128];
     alignas(64) unsigned char tmap_c[128];
     alignas(64) unsigned char tmap_slope[128];
     alignas(64) unsigned char tmap_res[128];
+    alignas(64) unsigned char tmap_all[128];
 };
 
 // The second product of a GM_EPI_DUAL launch; its tiles come behind the first one's.
@@ -137,10 +141,28 @@ __device__ __forceinline__ bool gm_tile_skipped(const GemmParams& p, int tm, int
     return p.tri == 1 && tn * BN > tm * GM_BM + GM_BM - 1;
 }
 
+// Packed rows: how many count, at least one (a reduction over none is one over a block of zeros).
+__host__ __device__ constexpr bool gm_packs(int epi) { return epi == GM_EPI_ACC || epi == GM_EPI_LSE || epi == GM_EPI_DLOGITS || epi == GM_EPI_DUAL; }
+template <int EPI>
+__device__ __forceinline__ int gm_live(const GemmParams& p) {
+    if constexpr (gm_packs(EPI)) {
+        if (p.live) {
+            const int n = *(const volatile int*)p.live;
+            return n > 1 ? n : 1;
+        }
+    }
+    return 0x7fffffff;
+}
+template <int EPI>
+__device__ __forceinline__ bool gm_unpacked(const GemmParams& p) {
+    if constexpr (gm_packs(EPI)) return p.live && p.live_all > 0 && *(const volatile int*)p.live == p.live_all;
+    return false;
+}
+
 // Work unit u: output tile (tm, tn) of problem b (bi, bo), k-blocks [kb0, kb1), split sp; `second`: of a dual launch's second product.
 struct GemmUnit { int sp, bi, bo, tm, tn, kb0, kb1; bool skip, second; };
-template <int BN, int EPI>
-__device__ __forceinline__ GemmUnit gm_unit(const GemmParamsOf<EPI>& p, long long u, int tiles_per_problem) {
+template <int BN, int CG, int EPI>
+__device__ __forceinline__ GemmUnit gm_unit(const GemmParamsOf<EPI>& p, long long u, int tiles_per_problem, int live) {
     GemmUnit w;
     w.second = false;
     if constexpr (EPI == GM_EPI_DUAL) {
@@ -154,12 +176,14 @@ __device__ __forceinline__ GemmUnit gm_unit(const GemmParamsOf<EPI>& p, long lon
             w.tn = t - w.tm * p.second.tiles_n;
             w.sp = w.kb0 = 0;
             w.kb1 = p.second.kblocks;
+            if ((live - 1) / GM_BK + 1 < w.kb1) w.kb1 = (live - 1) / GM_BK + 1;
         } else {
             const int t = (int)(u / p.splits);
             w.sp = (int)(u - (long long)t * p.splits);
             w.tm = t / p.tiles_n;
             w.tn = t - w.tm * p.tiles_n;
             gm_kb_range(p, w.sp, w.tm, w.kb0, w.kb1);
+            w.skip = (long long)w.tm * (CG * GM_BM) >= live;
         }
     } else {
         w.sp = (int)(u % p.splits);
@@ -171,6 +195,19 @@ __device__ __forceinline__ GemmUnit gm_unit(const GemmParamsOf<EPI>& p, long lon
         w.bo = b / p.nb_inner;
         w.skip = gm_tile_skipped<BN>(p, w.tm, w.tn);
         gm_kb_range(p, w.sp, w.tm, w.kb0, w.kb1);
+        if constexpr (gm_packs(EPI)) {
+            if (EPI == GM_EPI_ACC && p.live_k) {
+                const int blocks = (live - 1) / GM_BK + 1;
+                if (blocks < p.kblocks) {
+                    const int per_split = (blocks + p.splits - 1) / p.splits;
+                    w.kb0 = w.sp * per_split;
+                    w.kb1 = w.kb0 + per_split < blocks ? w.kb0 + per_split : blocks;
+                    if (w.kb0 >= w.kb1) { w.kb0 = p.kblocks; w.kb1 = w.kb0 + 1; }   // nothing left: a block behind the end, which reads as zeros
+                }
+            } else {
+                w.skip |= (long long)w.tm * (CG * GM_BM) >= live;
+            }
+        }
     }
     return w;
 }
@@ -222,6 +259,7 @@ __global__ void __launch_bounds__(gm_threads(EPI), 1) gemm_bf16_kernel(const __g
     tc_fence_after_sync();
     pdl_wait();
     if (tid == 0) pdl_launch_dependents();
+    const int live = gm_live<EPI>(p);
     const uint32_t tmem_base = ctl->tmem_base;
     volatile int* abort_flag = &ctl->abort_flag;
     const int tiles_per_problem = p.tiles_m * p.tiles_n;
@@ -233,14 +271,20 @@ __global__ void __launch_bounds__(gm_threads(EPI), 1) gemm_bf16_kernel(const __g
         int s = 0;
         uint32_t ph = 0;
         bool dead = false;
+        const bool unpacked = gm_unpacked<EPI>(p);
         for (long long u = blockIdx.x / CG; u < units && !dead; u += gridDim.x / CG) {
-            const GemmUnit w = gm_unit<BN, EPI>(p, u, tiles_per_problem);
+            const GemmUnit w = gm_unit<BN, CG, EPI>(p, u, tiles_per_problem, live);
             if (w.skip) continue;
             const int m0 = (w.tm * CG + (int)rank) * GM_BM, nb0 = w.tn * BN + (int)rank * (BN / CG);
             const unsigned char *map_a = p.tmap_a, *map_b = p.tmap_b;
             int a_mn = p.a_mn, b_mn = p.b_mn;
-            if constexpr (EPI == GM_EPI_DUAL)
-                if (w.second) { map_a = p.second.tmap_a; map_b = p.second.tmap_b; a_mn = p.second.a_mn; b_mn = p.second.b_mn; }
+            if constexpr (EPI == GM_EPI_DUAL) {
+                if (w.second) { map_a = p.second.tmap_a; map_b = unpacked ? p.tmap_all : p.second.tmap_b; a_mn = p.second.a_mn; b_mn = p.second.b_mn; }
+            } else if constexpr (EPI == GM_EPI_ACC) {
+                if (unpacked) map_b = p.tmap_all;
+            } else if constexpr (gm_packs(EPI)) {
+                if (unpacked) map_a = p.tmap_all;
+            }
             for (int kb = w.kb0; kb < w.kb1; kb++) {
                 if (!mbar_wait_warp(&ctl->empty[s], ph ^ 1u, abort_flag)) {
                     if (!*abort_flag) { ctl->abort_flag = 1; if (p.status) atomicExch(p.status, OB200_ERR_WAIT_EMPTY); }
@@ -288,7 +332,7 @@ __global__ void __launch_bounds__(gm_threads(EPI), 1) gemm_bf16_kernel(const __g
             uint32_t local = 0;
             bool dead = false;
             for (long long u = blockIdx.x / CG; u < units && !dead; u += gridDim.x / CG) {
-                const GemmUnit w = gm_unit<BN, EPI>(p, u, tiles_per_problem);
+                const GemmUnit w = gm_unit<BN, CG, EPI>(p, u, tiles_per_problem, live);
                 if (w.skip) continue;
                 int a_mn = p.a_mn, b_mn = p.b_mn;
                 if constexpr (EPI == GM_EPI_DUAL)
@@ -341,7 +385,7 @@ __global__ void __launch_bounds__(gm_threads(EPI), 1) gemm_bf16_kernel(const __g
         uint32_t local = 0;
         uint32_t slab_i = 0;
         for (long long u = blockIdx.x / CG; u < units; u += gridDim.x / CG) {
-            const GemmUnit w = gm_unit<BN, EPI>(p, u, tiles_per_problem);
+            const GemmUnit w = gm_unit<BN, CG, EPI>(p, u, tiles_per_problem, live);
             const int sp = w.sp, tm = w.tm, tn = w.tn, bi = w.bi, bo = w.bo;
             if (w.skip) continue;
             const uint32_t ab = local & 1u, use = local >> 1;
@@ -922,6 +966,17 @@ int gemm_bf16_run(const GemmCall& g) {
     const bool ok_b = b_mn ? gm_make_map(p.tmap_b, b, N, K, ldb, batch_inner, g.b_si, batch_outer, g.b_so, 64, GM_BK)
                            : gm_make_map(p.tmap_b, b, K, N, ldb, batch_inner, g.b_si, batch_outer, g.b_so, GM_BK, bn / cg);
     if (!ok_a || !ok_b) return -4;
+    if (g.live) {
+        if (!gm_packs(epi) || batch_ll != 1 || tri || (g.live_k && epi != GM_EPI_ACC)) return -1;
+        p.live = g.live;
+        p.live_k = g.live_k;
+        if (g.all) {   // the same boxes as the packed operand's
+            p.live_all = g.live_k ? K : M;
+            if (g.live_k ? !b_mn : epi == GM_EPI_ACC || a_mn) return -1;
+            if (!(g.live_k ? gm_make_map(p.tmap_all, g.all, N, K, g.ld_all, 1, 0, 1, 0, 64, GM_BK) : gm_make_map(p.tmap_all, g.all, K, M, g.ld_all, 1, 0, 1, 0, GM_BK, GM_BM)))
+                return -4;
+        }
+    }
     // C by TMA stores when its rows and batch offsets are 16-byte multiples (always true for the layouts of the clients)
     {
         const int es = out_f32 ? 4 : 2;
@@ -1081,6 +1136,15 @@ int gemm_bf16_run_dual(const GemmCall& a, const GemmCall& b) {
         !gm_make_c_map(p.second.tmap_c, b))
         return -4;
     p.c_tma = 1;
+    if (a.live) {   // rows of the first product, the reduction of the second
+        if (b.live != a.live || a.live_k || !b.live_k || a.M != b.K) return -1;
+        p.live = a.live;
+        if (b.all) {
+            p.live_all = b.K;
+            if (!b.b_mn) return -1;
+            if (!gm_make_map(p.tmap_all, b.all, b.N, b.K, b.ld_all, 1, 0, 1, 0, 64, GM_BK)) return -4;
+        }
+    }
     const long long tiles = (long long)p.tiles_m * p.tiles_n * splits + (long long)p.second.tiles_m * p.second.tiles_n;
     if (tiles > 0x3fffffffLL) return -1;
     const long long most = a.num_ctas / 2;

@@ -58,6 +58,13 @@ struct GemmCall {
     float* slabs = nullptr;
     size_t slab_bytes = 0;
     int splits = 0;                 // parts of the reduction; 0: by the plan
+    // Packed rows (GM_EPI_ACC, GM_EPI_LSE, GM_EPI_DLOGITS and both products of a dual launch): only the first *live rows of A count, or with
+    // live_k the first *live indices of the reduction.  Tiles and k-blocks behind them are left out (their outputs unwritten); *live may be
+    // 0.  `all`: what stands for the packed operand (A of the losses, B of a product with live_k) where *live is everything, M or K.
+    const int* live = nullptr;
+    int live_k = 0;
+    const void* all = nullptr;
+    long long ld_all = 0;
     int num_ctas = 0;
     void* stream = nullptr;
 };

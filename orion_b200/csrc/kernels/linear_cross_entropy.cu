@@ -13,6 +13,7 @@
 // (reference benchmarking/model_kernels/bert_8_fb1; src/scheduler/utils_sched.cpp:490-501).
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
+#include <limits.h>
 #include <math.h>
 #include <stdint.h>
 
@@ -24,18 +25,20 @@ extern "C" int ob200_plan_sm_count(void);
 
 namespace ob200 {
 
-constexpr int CE_THREADS = 256;
+constexpr int CE_THREADS = 256, CE_PACK_THREADS = 512;
 constexpr float CE_LOG2E = 1.4426950408889634f;
 
 // lse and loss of every row from its parts.  A CTA has C rows; group g of G = 1024 / C takes parts g, g + G, ..., eight at a time in
 // registers (the kernel is a few dependent steps long: their loads are one), then the groups are joined in a fixed tree.  32 rows, or 4
-// where rows are few and their parts many.
+// where rows are few and their parts many.  Packed rows (`order`): row r of the parts is row order[r], and those from *live on do not
+// count.
 template <int C>
 __global__ void __launch_bounds__(1024) ce_rows_kernel(const float2* __restrict__ part, const float* __restrict__ label_logit,
                                                        const long long* __restrict__ target, float* __restrict__ loss, float* __restrict__ lse,
-                                                       int rows, int parts, int V, long long ignore_index) {
+                                                       const int* order, const int* live, int rows, int parts, int V, long long ignore_index) {
     pdl_wait();
     pdl_launch_dependents();
+    const int counted = live ? *live : rows;
     constexpr int G = 1024 / C;
     __shared__ float2 sh[G][C + 1];
     const int c = threadIdx.x % C, g = threadIdx.x / C, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -47,7 +50,7 @@ __global__ void __launch_bounds__(1024) ce_rows_kernel(const float2* __restrict_
         for (int t0 = g; t0 < parts; t0 += 8 * G) {
             float2 q[8];
 #pragma unroll
-            for (int i = 0; i < 8; i++) q[i] = r < rows && t0 + G * i < parts ? part[(long long)(t0 + G * i) * rows + r] : make_float2(-INFINITY, 0.f);
+            for (int i = 0; i < 8; i++) q[i] = r < counted && t0 + G * i < parts ? part[(long long)(t0 + G * i) * rows + r] : make_float2(-INFINITY, 0.f);
             float now = top;
 #pragma unroll
             for (int i = 0; i < 8; i++) now = fmaxf(now, q[i].x);
@@ -73,11 +76,11 @@ __global__ void __launch_bounds__(1024) ce_rows_kernel(const float2* __restrict_
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
             if (lane == 0) {
-                const int row = r0 + warp;
-                const float l = now + logf(all);
-                const long long t = target[row];
-                lse[row] = l;
-                loss[row] = t == ignore_index ? 0.f : t >= 0 && t < V ? l - label_logit[row] : NAN;
+                const int row = r0 + warp, to = order ? order[row] : row;
+                const float l = row < counted ? now + logf(all) : 0.f;
+                const long long t = target[to];
+                lse[to] = l;
+                loss[to] = t == ignore_index ? 0.f : t >= 0 && t < V ? l - label_logit[row] : NAN;
             }
         }
         __syncthreads();
@@ -121,31 +124,103 @@ __global__ void __launch_bounds__(1024) ce_total_kernel(const float* __restrict_
     }
 }
 
-// Per row (lse * log2(e), coefficient) for the epilogue, the factor of both gradients, and a copy of x without the rows that do not count, whatever they hold (0 times
-// infinity would reach dw).  One warp a row.  An upstream gradient that is one number, and the mean's divisor, are the factor, which
-// the products of the rounded dl are multiplied by: in the coefficient they would make every row's largest term, the label's, off by
-// the same rounding.  A label outside the vocabulary makes the coefficient, and so the gradients, not a number.
-__global__ void __launch_bounds__(CE_THREADS) ce_prepare_kernel(const __nv_bfloat16* __restrict__ x, long long ldx, __nv_bfloat16* __restrict__ kept,
-                                                                const float* __restrict__ lse, const long long* __restrict__ target,
-                                                                const float* __restrict__ grad, int grad_per_row, const float* __restrict__ count,
-                                                                float2* __restrict__ row, float* __restrict__ factor, long long rows, int V, int H,
-                                                                long long ignore_index) {
+// Rows that count first, in their order, then the others from the last one down: what the products take instead of x, so that rows
+// that do not count (the prompt of an answer, the words that a masked model is not asked for) cost no products, and whatever they hold
+// (0 times infinity) reaches none.  A CTA has consecutive rows; it counts those before them and all of them itself, which reads the
+// targets once per CTA and saves a launch.  Where every row counts x is not copied: the products take x itself.  Rows that do not
+// count become zeros where the last 64-row block of a reduction reads them.
+// order: row of every slot, slot: slot of every row, or -1.  For the gradients also per slot the label and (lse * log2(e), coefficient), and
+// the factor of both: an upstream gradient that is one number, and the mean's divisor, multiply the products of the rounded dl; in the
+// coefficient they would make every row's largest term, the label's, off by the same rounding.  A label outside the vocabulary makes the
+// coefficient, and so the gradients, not a number.
+struct CePack {
+    const __nv_bfloat16* x;
+    const long long* target;
+    const float *lse, *grad, *count;   // gradients (lse null: the forward pass)
+    __nv_bfloat16* packed;
+    long long* label;
+    int *order, *slot, *live;          // order or slot may be null
+    float2* row;
+    float* factor;
+    long long ldx, ignore_index;
+    int rows, V, H, grad_per_row;
+};
+__global__ void __launch_bounds__(CE_PACK_THREADS) ce_pack_kernel(const CePack p) {
+    pdl_wait();
+    pdl_launch_dependents();
+    constexpr int W = CE_PACK_THREADS / 32;
+    __shared__ int sh_all[W], sh_before[W], sh_slot[CE_PACK_THREADS];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const long long chunk = ((long long)p.rows + gridDim.x - 1) / gridDim.x, r0 = chunk * blockIdx.x, r1 = r0 + chunk < p.rows ? r0 + chunk : p.rows;
+    int all = 0, before = 0;
+#pragma unroll 8
+    for (long long r = tid; r < p.rows; r += CE_PACK_THREADS) {
+        const int counts = p.target[r] != p.ignore_index;
+        all += counts;
+        before += r < r0 ? counts : 0;
+    }
+    all = __reduce_add_sync(0xffffffffu, all);
+    before = __reduce_add_sync(0xffffffffu, before);
+    if (lane == 0) { sh_all[warp] = all; sh_before[warp] = before; }
+    __syncthreads();
+    all = before = 0;
+    for (int w = 0; w < W; w++) { all += sh_all[w]; before += sh_before[w]; }
+    if (blockIdx.x == 0 && tid == 0) {
+        *p.live = all;
+        if (p.factor) *p.factor = (p.grad_per_row ? 1.f : p.grad[0]) / (p.count ? *p.count : 1.f);
+    }
+    const int zeros_to = ((all > 1 ? all : 1) + 63) / 64 * 64;
+    for (long long base = r0; base < r1; base += CE_PACK_THREADS) {
+        const long long r = base + tid;
+        const long long t = r < r1 ? p.target[r] : p.ignore_index;
+        const bool counts = t != p.ignore_index;
+        const uint32_t votes = __ballot_sync(0xffffffffu, counts);
+        __syncthreads();   // sh_all and sh_slot of the turn before have been read
+        if (lane == 0) sh_all[warp] = __popc(votes);
+        __syncthreads();
+        int rank = before + __popc(votes & ((1u << lane) - 1));
+        int taken = 0;
+        for (int w = 0; w < W; w++) {
+            if (w < warp) rank += sh_all[w];
+            taken += sh_all[w];
+        }
+        before += taken;
+        // a row that does not count is the (r - rank)-th of those
+        const int slot = counts ? rank : p.rows - 1 - (int)(r - rank);
+        sh_slot[tid] = counts ? slot : r < r1 && slot < zeros_to ? ~slot : INT_MIN;
+        if (r < r1) {
+            p.label[slot] = counts ? t : -1;
+            if (p.order) p.order[slot] = (int)r;
+            if (p.slot) p.slot[r] = counts ? slot : -1;
+            if (p.row) p.row[slot] = make_float2(p.lse[r] * CE_LOG2E, !counts ? 0.f : t >= 0 && t < p.V ? (p.grad_per_row ? p.grad[r] : 1.f) : NAN);
+        }
+        __syncthreads();
+        if (all == p.rows) continue;
+        for (int i = warp; i < CE_PACK_THREADS && base + i < r1; i += W) {
+            const int to = sh_slot[i];
+            if (to == INT_MIN) continue;
+            const uint4* src = reinterpret_cast<const uint4*>(p.x + (base + i) * p.ldx);
+            uint4* dst = reinterpret_cast<uint4*>(p.packed + (long long)(to < 0 ? ~to : to) * p.H);
+            for (int c = lane; c < p.H / 8; c += 32) dst[c] = to < 0 ? make_uint4(0, 0, 0, 0) : src[c];
+        }
+    }
+}
+// dx from its packed rows; zeros for the rows that do not count.  One warp a row.
+__global__ void __launch_bounds__(CE_THREADS) ce_unpack_kernel(const __nv_bfloat16* packed, const int* slot, __nv_bfloat16* __restrict__ dx, long long rows, int H) {
     pdl_wait();
     pdl_launch_dependents();
     const int lane = threadIdx.x & 31;
     for (long long r = (long long)blockIdx.x * (CE_THREADS / 32) + (threadIdx.x >> 5); r < rows; r += (long long)gridDim.x * (CE_THREADS / 32)) {
-        const long long t = target[r];
-        const float c = t == ignore_index ? 0.f : t >= 0 && t < V ? (grad_per_row ? grad[r] : 1.f) : NAN;
-        if (lane == 0) {
-            row[r] = make_float2(lse[r] * CE_LOG2E, c);
-            if (r == 0) *factor = (grad_per_row ? 1.f : grad[0]) / (count ? *count : 1.f);
-        }
-        if (kept) {
-            const uint4* src = reinterpret_cast<const uint4*>(x + r * ldx);
-            uint4* dst = reinterpret_cast<uint4*>(kept + r * H);
-            for (int i = lane; i < H / 8; i += 32) dst[i] = c == 0.f ? make_uint4(0, 0, 0, 0) : src[i];
-        }
+        const int from = slot[r];
+        const uint4* src = reinterpret_cast<const uint4*>(packed + (long long)from * H);
+        uint4* dst = reinterpret_cast<uint4*>(dx + r * H);
+        for (int c = lane; c < H / 8; c += 32) dst[c] = from < 0 ? make_uint4(0, 0, 0, 0) : src[c];
     }
+}
+static int ce_pack(const CePack& p, int num_ctas, cudaStream_t st) {
+    const long long want = ((long long)p.rows + 31) / 32, cap = (long long)num_ctas * 2;
+    OB200_ELASTIC_HBM(ce_pack_kernel, 2);
+    return launch_pdl(ce_pack_kernel, (unsigned)(want < cap ? want : cap), (unsigned)CE_PACK_THREADS, st, p);
 }
 
 // Columns of the vocabulary a piece of the backward pass has: dl of a piece takes at most 192 MB (and no piece is so narrow that its
@@ -189,14 +264,17 @@ constexpr int CE_ROW_BLOCK = 65536;   // rows a forward pass has in its workspac
 static size_t ce_round(size_t bytes) { return (bytes + 255) & ~(size_t)255; }
 
 struct CeBackwardSpace {
-    size_t row, kept, dl, acc, slabs, total;
+    size_t row, label, slot, packed, dl, acc, dx, slabs, total;
     int piece;
     CeBackwardSpace(long long rows, int V, int H, bool want_dx, bool want_dw) {
         piece = ce_piece(rows, V, H, ob200_plan_sm_count());
-        row = ce_round((size_t)rows * sizeof(float2) + sizeof(float));
-        kept = want_dw ? ce_round((size_t)rows * H * 2) : 0;
+        row = ce_round((size_t)rows * sizeof(float2) + 2 * sizeof(float));   // and the factor, and how many rows count
+        label = ce_round((size_t)rows * sizeof(long long));
+        slot = ce_round((size_t)rows * sizeof(int));
+        packed = ce_round((size_t)rows * H * 2);
         dl = ce_round((size_t)rows * piece * 2);
         acc = want_dx && piece < V ? ce_round((size_t)rows * H * sizeof(float)) : 0;
+        dx = want_dx ? packed : 0;
         slabs = 0;
         const int last = V - (V - 1) / piece * piece;   // columns of the last piece
         for (int v : {piece < V ? piece : V, last}) {
@@ -209,7 +287,7 @@ struct CeBackwardSpace {
                 if (n > slabs) slabs = n;
         }
         slabs = ce_round(slabs);
-        total = row + kept + dl + acc + slabs;
+        total = row + label + slot + packed + dl + acc + dx + slabs;
     }
 };
 
@@ -220,11 +298,25 @@ using namespace ob200;
 // Parts of a row that a forward pass writes; the workspace has room for those of either kernel.
 static int ce_parts(int rows, int V, int H) { return few_rows_fit(rows, V, H) ? few_rows_parts(rows, V) : (V + 127) / 128; }
 
-extern "C" long long ob200_linear_cross_entropy_workspace(int rows, int V) {
-    if (rows <= 0 || V <= 0) return 0;
-    const long long block = rows < CE_ROW_BLOCK ? rows : CE_ROW_BLOCK;
-    const int a = ce_parts(rows, V, 1), b = (V + 127) / 128;
-    return (long long)ce_round((size_t)block * (a > b ? a : b) * sizeof(float2)) + block * (long long)sizeof(float);
+// Whether a forward pass packs the rows that count: where it can spare a tile of 128.
+static bool ce_packs(int rows, int V, int H) { return rows > 128 && !few_rows_fit(rows, V, H); }
+
+struct CeForwardSpace {
+    size_t part, label_logit, packed, label, order, total;
+    CeForwardSpace(long long rows, int V, int H) {
+        const size_t block = (size_t)(rows < CE_ROW_BLOCK ? rows : CE_ROW_BLOCK);
+        const bool packs = ce_packs((int)rows, V, H);
+        part = ce_round(block * ce_parts((int)rows, V, H) * sizeof(float2));
+        label_logit = ce_round((block + 1) * sizeof(float));   // and how many rows count
+        packed = packs ? ce_round(block * H * 2) : 0;
+        label = packs ? ce_round(block * sizeof(long long)) : 0;
+        order = packs ? ce_round(block * sizeof(int)) : 0;
+        total = part + label_logit + packed + label + order;
+    }
+};
+extern "C" long long ob200_linear_cross_entropy_workspace(int rows, int V, int H) {
+    if (rows <= 0 || V <= 0 || H <= 0) return 0;
+    return (long long)CeForwardSpace(rows, V, H).total;
 }
 
 // See include/orion_kernels.h.  -1: sizes or arguments, -2: alignment, -3: workspace too small, -4: no TMA descriptor.
@@ -234,15 +326,28 @@ extern "C" int ob200_linear_cross_entropy_forward(const void* x, const void* w, 
     if (rows < 0 || V <= 0 || H <= 0 || ldx < H || ldw < H || num_ctas <= 0) return -1;
     if ((rows > 0 && (!x || !w || !target || !loss || !lse)) || (total && !count)) return -1;
     if (((uintptr_t)x | (uintptr_t)w | (uintptr_t)workspace) % 16 || (ldx | ldw) % 8) return -2;
-    if (workspace_bytes < ob200_linear_cross_entropy_workspace(rows, V) || (!workspace && rows > 0)) return -3;
+    if (H % 8) return -2;
+    if (workspace_bytes < ob200_linear_cross_entropy_workspace(rows, V, H) || (!workspace && rows > 0)) return -3;
     cudaStream_t st = (cudaStream_t)stream;
     const int block = rows < CE_ROW_BLOCK ? rows : CE_ROW_BLOCK, parts = ce_parts(rows, V, H);
-    float2* part = (float2*)workspace;
-    float* label_logit = (float*)((char*)workspace + ce_round((size_t)block * parts * sizeof(float2)));
+    const bool packs = ce_packs(rows, V, H);
+    const CeForwardSpace space(rows, V, H);
+    char* at = (char*)workspace;
+    float2* part = (float2*)at;
+    at += space.part;
+    float* label_logit = (float*)at;
+    int* live = (int*)(label_logit + block);
+    at += space.label_logit;
+    __nv_bfloat16* packed = (__nv_bfloat16*)at;
+    at += space.packed;
+    long long* label = (long long*)at;
+    at += space.label;
+    int* order = packs ? (int*)at : nullptr;
     for (int r0 = 0; r0 < rows; r0 += CE_ROW_BLOCK) {
         const int n = rows - r0 < CE_ROW_BLOCK ? rows - r0 : CE_ROW_BLOCK;
+        const __nv_bfloat16* xb = (const __nv_bfloat16*)x + (long long)r0 * ldx;
         GemmCall g;
-        g.a = (const __nv_bfloat16*)x + (long long)r0 * ldx;
+        g.a = xb;
         g.b = w;
         g.M = n; g.N = V; g.K = H;
         g.lda = ldx; g.ldb = ldw; g.ldc = V;
@@ -252,17 +357,33 @@ extern "C" int ob200_linear_cross_entropy_forward(const void* x, const void* w, 
         g.e.label_logit = label_logit;
         g.num_ctas = num_ctas;
         g.stream = stream;
-        int rc = few_rows_fit(rows, V, H) ? few_rows_run(g) : gemm_bf16_run(g);
+        int rc;
+        if (packs) {
+            CePack k = {};
+            k.x = xb; k.ldx = ldx;
+            k.target = target + r0;
+            k.ignore_index = ignore_index;
+            k.packed = packed; k.label = label; k.order = order; k.live = live;
+            k.rows = n; k.V = V; k.H = H;
+            if ((rc = ce_pack(k, num_ctas, st)) != 0) return rc;
+            g.a = packed; g.lda = H;
+            g.all = xb; g.ld_all = ldx;
+            g.live = live;
+            g.e.target = label;
+        }
+        rc = few_rows_fit(rows, V, H) ? few_rows_run(g) : gemm_bf16_run(g);
         if (rc) return rc;
         const int per_cta = n <= 64 ? 4 : 32, want = (n + per_cta - 1) / per_cta, cap = num_ctas * 2;
         const unsigned grid = (unsigned)(want < cap ? want : cap);
         if (per_cta == 4) {
             OB200_ELASTIC_HBM(ce_rows_kernel<4>, 2);
-            rc = launch_pdl(ce_rows_kernel<4>, grid, 1024u, st, (const float2*)part, (const float*)label_logit, target + r0, loss + r0, lse + r0, n, parts, V,
+            rc = launch_pdl(ce_rows_kernel<4>, grid, 1024u, st, (const float2*)part, (const float*)label_logit, target + r0, loss + r0, lse + r0, (const int*)order,
+                            (const int*)(packs ? live : nullptr), n, parts, V,
                             ignore_index);
         } else {
             OB200_ELASTIC_HBM(ce_rows_kernel<32>, 2);
-            rc = launch_pdl(ce_rows_kernel<32>, grid, 1024u, st, (const float2*)part, (const float*)label_logit, target + r0, loss + r0, lse + r0, n, parts, V,
+            rc = launch_pdl(ce_rows_kernel<32>, grid, 1024u, st, (const float2*)part, (const float*)label_logit, target + r0, loss + r0, lse + r0, (const int*)order,
+                            (const int*)(packs ? live : nullptr), n, parts, V,
                             ignore_index);
         }
         if (rc) return rc;
@@ -292,20 +413,29 @@ extern "C" int ob200_linear_cross_entropy_backward(const void* x, const void* w,
     char* at = (char*)workspace;
     float2* row = (float2*)at;
     float* factor = (float*)(row + rows);
+    int* live = (int*)(factor + 1);
     at += space.row;
-    __nv_bfloat16* kept = dw ? (__nv_bfloat16*)at : nullptr;
-    at += space.kept;
+    long long* label = (long long*)at;
+    at += space.label;
+    int* slot = (int*)at;
+    at += space.slot;
+    __nv_bfloat16* packed = (__nv_bfloat16*)at;
+    at += space.packed;
     __nv_bfloat16* dl = (__nv_bfloat16*)at;
     at += space.dl;
     float* acc = (float*)at;
     at += space.acc;
-    {
-        const long long want = ((long long)rows + CE_THREADS / 32 - 1) / (CE_THREADS / 32), cap = (long long)num_ctas * 8;
-        OB200_ELASTIC_HBM(ce_prepare_kernel, 8);
-        const int rc = launch_pdl(ce_prepare_kernel, (unsigned)(want < cap ? want : cap), (unsigned)CE_THREADS, st, (const __nv_bfloat16*)x, ldx, kept, lse,
-                                  target, grad, grad_per_row, count, row, factor, (long long)rows, V, H, ignore_index);
-        if (rc) return rc;
-    }
+    __nv_bfloat16* packed_dx = (__nv_bfloat16*)at;
+    at += space.dx;
+    CePack k = {};
+    k.x = (const __nv_bfloat16*)x; k.ldx = ldx;
+    k.target = target;
+    k.ignore_index = ignore_index;
+    k.lse = lse; k.grad = grad; k.grad_per_row = grad_per_row; k.count = count;
+    k.packed = packed; k.label = label; k.slot = slot; k.live = live; k.row = row; k.factor = factor;
+    k.rows = rows; k.V = V; k.H = H;
+    int rc = ce_pack(k, num_ctas, st);
+    if (rc) return rc;
     for (int v0 = 0; v0 < V; v0 += space.piece) {
         const int nv = V - v0 < space.piece ? V - v0 : space.piece;
         const bool first = v0 == 0, last = v0 + nv == V;
@@ -313,15 +443,16 @@ extern "C" int ob200_linear_cross_entropy_backward(const void* x, const void* w,
         GemmCall g;
         g.num_ctas = num_ctas;
         g.stream = stream;
-        g.a = x; g.b = wp; g.c = dl;
+        g.a = packed; g.b = wp; g.c = dl;
         g.M = rows; g.N = nv; g.K = H;
-        g.lda = ldx; g.ldb = ldw; g.ldc = space.piece;
+        g.lda = H; g.ldb = ldw; g.ldc = space.piece;
+        g.live = live;
+        g.all = x; g.ld_all = ldx;
         g.epi = GM_EPI_DLOGITS;
-        g.e.target = target;
+        g.e.target = label;
         g.e.col0 = v0;
         g.e.row = row;
-        int rc = gemm_bf16_run(g);
-        if (rc) return rc;
+        if ((rc = gemm_bf16_run(g)) != 0) return rc;
         g.slabs = (float*)at;
         g.slab_bytes = space.slabs;
         g.a = dl; g.lda = space.piece;
@@ -336,10 +467,12 @@ extern "C" int ob200_linear_cross_entropy_backward(const void* x, const void* w,
         gx.e.addend = first ? nullptr : acc;
         gx.e.factor = factor;
         gx.out_f32 = last ? 0 : 1;
-        gx.c = last ? dx : (void*)acc;
+        gx.all = nullptr;
+        gx.c = last ? (void*)packed_dx : (void*)acc;
         // dw[v, h] = sum_t dl[t, v] x[t, h]
         gw.a_mn = 1;
-        gw.b = kept; gw.ldb = H;
+        gw.live_k = 1;
+        gw.b = packed; gw.ldb = H;
         gw.M = nv; gw.K = rows;
         gw.epi = GM_EPI_ACC;
         gw.e.factor = factor;
@@ -352,5 +485,9 @@ extern "C" int ob200_linear_cross_entropy_backward(const void* x, const void* w,
         }
         if (rc) return rc;
     }
-    return 0;
+    if (!dx) return 0;
+    const long long want = ((long long)rows + CE_THREADS / 32 - 1) / (CE_THREADS / 32), cap = (long long)num_ctas * 8;
+    OB200_ELASTIC_HBM(ce_unpack_kernel, 8);
+    return launch_pdl(ce_unpack_kernel, (unsigned)(want < cap ? want : cap), (unsigned)CE_THREADS, st, (const __nv_bfloat16*)packed_dx, (const int*)slot,
+                      (__nv_bfloat16*)dx, (long long)rows, H);
 }

@@ -109,7 +109,7 @@ int ob200_dropout(const void* x, const void* residual, void* y, long long n, flo
 int ob200_linear_cross_entropy_forward(const void* x, const void* w, const long long* target, float* loss, float* lse, float* total,
                                        float* count, int rows, int V, int H, long long ldx, long long ldw, long long ignore_index, int mean,
                                        void* workspace, long long workspace_bytes, int num_ctas, void* stream);
-long long ob200_linear_cross_entropy_workspace(int rows, int V);
+long long ob200_linear_cross_entropy_workspace(int rows, int V, int H);
 int ob200_linear_cross_entropy_backward(const void* x, const void* w, const long long* target, const float* lse, const float* grad,
                                         int grad_per_row, const float* count, void* dx, void* dw, int rows, int V, int H, long long ldx,
                                         long long ldw, long long ignore_index, void* workspace, long long workspace_bytes, int num_ctas,
@@ -1027,7 +1027,7 @@ struct LinearCrossEntropy : public torch::autograd::Function<LinearCrossEntropy>
         const auto f32 = x.options().dtype(at::kFloat).memory_format(at::MemoryFormat::Contiguous);
         at::Tensor loss = at::empty(target.sizes(), f32), lse = at::empty({rows}, f32);
         at::Tensor total = reduction ? at::empty({}, f32) : at::Tensor(), count = reduction ? at::empty({}, f32) : at::Tensor();
-        const long long bytes = ob200_linear_cross_entropy_workspace((int)rows, (int)V);
+        const long long bytes = ob200_linear_cross_entropy_workspace((int)rows, (int)V, (int)H);
         const at::Tensor space = workspace(bytes, x);
         check(ob200_linear_cross_entropy_forward(rows ? xr.data_ptr() : nullptr, wr.data_ptr(), (const long long*)tc.data_ptr<int64_t>(),
                                                  loss.data_ptr<float>(), lse.data_ptr<float>(), reduction ? total.data_ptr<float>() : nullptr,

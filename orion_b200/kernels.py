@@ -79,7 +79,7 @@ def lib():
         L.ob200_linear_act_backward_workspace.argtypes = [c_int] * 4 + [c_float] + [c_int] * 3
         L.ob200_dropout.argtypes = [c_void_p] * 3 + [c_ll, c_float, c_void_p, c_int, c_int, c_int, c_void_p]
         L.ob200_linear_cross_entropy_forward.argtypes = [c_void_p] * 7 + [c_int] * 3 + [c_ll] * 3 + [c_int, c_void_p, c_ll, c_int, c_void_p]
-        L.ob200_linear_cross_entropy_workspace.argtypes = [c_int] * 2
+        L.ob200_linear_cross_entropy_workspace.argtypes = [c_int] * 3
         L.ob200_linear_cross_entropy_backward.argtypes = [c_void_p] * 5 + [c_int] + [c_void_p] * 3 + [c_int] * 3 + [c_ll] * 3 + [c_void_p, c_ll, c_int, c_void_p]
         L.ob200_linear_cross_entropy_backward_workspace.argtypes = [c_int] * 5
         for name in ("linear_act_bf16", "linear_act_backward_bf16", "dropout", "linear_cross_entropy_forward", "linear_cross_entropy_backward"):
@@ -492,7 +492,7 @@ def linear_cross_entropy(x, w, target, ignore_index=-100, mean=True, num_ctas=No
     V = w.shape[0]
     loss, lse = (torch.empty(rows, device=x.device, dtype=torch.float32) for _ in range(2))
     total, count = (torch.empty((), device=x.device, dtype=torch.float32) for _ in range(2))
-    n = lib().ob200_linear_cross_entropy_workspace(rows, V)
+    n = lib().ob200_linear_cross_entropy_workspace(rows, V, H)
     space = torch.empty(n, device=x.device, dtype=torch.uint8)
     _check(lib().ob200_linear_cross_entropy_forward(_ptr(x), _ptr(w), _ptr(target), _ptr(loss), _ptr(lse), _ptr(total), _ptr(count), rows, V, H,
                                                     x.stride(0), w.stride(0), ignore_index, int(mean), _ptr(space), n, num_ctas or sm_count(),

@@ -432,6 +432,42 @@ def test_loss_in_several_pieces_of_the_vocabulary(ops):
     assert torch.equal(torch.autograd.grad(b, w)[0], dw)
 
 
+@pytest.mark.parametrize("counted", [0, 1, 63, 64, 65, 128, 129, 300, 512, 513, 699, 700])
+@pytest.mark.parametrize("V,H", [(1000, 64), (5003, 136), (2050, 1024)])
+def test_loss_over_the_rows_that_count(ops, V, H, counted):
+    """Rows that count are packed for the products: none of them, a block, a tile, one more and one less; whatever the others hold; and the
+    same bits from any CTA count."""
+    T = 700
+    torch.manual_seed(V + counted)
+    x, w = torch.randn(T, H, device="cuda").to(BF), (torch.randn(V, H, device="cuda") * 2 / math.sqrt(H)).to(BF)
+    target = torch.randint(0, V, (T,), device="cuda")
+    out = torch.randperm(T, device="cuda")[counted:]
+    target[out] = -100
+    junk = x.clone()
+    junk[out] = float("nan")
+
+    def run(rows, reduction, g, q):
+        ops.set_sm_quota(q)
+        xl, wl = rows.clone().requires_grad_(True), w.clone().requires_grad_(True)
+        loss = ops.linear_cross_entropy(xl, wl, target, reduction=reduction)
+        dx, dw = torch.autograd.grad(loss, (xl, wl), g)
+        ops.set_sm_quota(0)
+        return loss.detach(), dx, dw
+
+    for reduction, g in (("mean", torch.tensor(1.0, device="cuda")), ("none", torch.randn(T, device="cuda"))):
+        want = check_loss(ops, x, w, target, reduction, g if reduction == "none" else 1.0)
+        for q in (0, 9, 1):
+            for a, b in zip(run(junk, reduction, g, q), want):
+                assert torch.equal(a, b)
+    # each gradient alone: the sums may be cut otherwise, two roundings of nearly the same number
+    xl, wl = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    both = torch.autograd.grad(ops.linear_cross_entropy(xl, wl, target, reduction="sum"), (xl, wl))
+    alone = (torch.autograd.grad(ops.linear_cross_entropy(xl, w, target, reduction="sum"), xl)[0],
+             torch.autograd.grad(ops.linear_cross_entropy(x, wl, target, reduction="sum"), wl)[0])
+    for a, b in zip(alone, both):
+        assert (a - b).abs().max().item() <= 2.0 ** -7 * b.abs().max().item()
+
+
 def test_more_rows_than_a_forward_pass_has_under_way(ops):
     T, V, H = 65536 + 130, 200, 16
     torch.manual_seed(2)
@@ -441,6 +477,13 @@ def test_more_rows_than_a_forward_pass_has_under_way(ops):
     out = ops.linear_cross_entropy(x, w, target, reduction="none")
     within(out, rows, 2 * delta + 2.0 ** -20 * (1 + lse.abs()) + 2.0 ** -23 * rows.abs(), "losses")
     within(ops.linear_cross_entropy(x, w, target), rows.mean(), (2 * delta + 2.0 ** -20 * (1 + lse.abs())).mean() + 2.0 ** -23 * rows.mean(), "mean")
+    # the second block of rows is packed by itself, the first one empty
+    target[:65536 + 7] = -100
+    out = ops.linear_cross_entropy(x, w, target, reduction="none")
+    assert not out[:65536 + 7].any()
+    within(out[65536 + 7:], rows[65536 + 7:], (2 * delta + 2.0 ** -20 * (1 + lse.abs()) + 2.0 ** -23 * rows.abs())[65536 + 7:], "losses")
+    target[:] = -100
+    assert ops.linear_cross_entropy(x, w, target).item() == 0
 
 
 def test_rows_that_do_not_count_and_labels_that_do_not_exist(ops):
