@@ -102,7 +102,28 @@ struct GemmSecond {
     alignas(64) unsigned char tmap_b[128];
     alignas(64) unsigned char tmap_c[128];
 };
-struct GemmParamsDual : GemmParams { GemmSecond second; };
+// How the first product of a dual launch is cut, in tiles of 256 x 256: the plan for all of its rows, from which that for the rows that
+// count follows on the device.
+struct GemmCutPlan { int M, tiles_n, kblocks, splits, per_split, second_tiles, second_kblocks, pairs; };
+struct GemmCut { int splits, per_split, rows; };   // rows of a partial matrix
+// With fewer rows than planned for its few tiles would keep few CTA pairs busy for long: as many parts as make a unit about a third of a
+// pair's share of all the work, as far as the scratch goes (the matrices of the planned split, one at least).  171 of 1143 rows,
+// 30522 x 768: 67 us for both products in the planned parts, 43 so.
+__host__ __device__ inline GemmCut gm_cut(const GemmCutPlan& c, int live) {
+    const int all = (c.M - 1) / 256 + 1, some = (live - 1) / 256 + 1;
+    if (some >= all) return {c.splits, c.per_split, c.M};
+    const int deep = (live - 1) / GM_BK + 1 < c.second_kblocks ? (live - 1) / GM_BK + 1 : c.second_kblocks;
+    const long long work = (long long)some * c.tiles_n * c.kblocks + (long long)c.second_tiles * (deep + 8), share = work / c.pairs + 1;
+    const long long room = (long long)c.splits * all / some;
+    long long parts = 3LL * c.kblocks / share;
+    if (parts > room) parts = room;
+    if (parts > c.kblocks / 4) parts = c.kblocks / 4;
+    if (parts > 32) parts = 32;
+    if (parts < 2) return {1, c.kblocks, some * 256};
+    const int per_split = (int)((c.kblocks + parts - 1) / parts);
+    return {(c.kblocks + per_split - 1) / per_split, per_split, some * 256};
+}
+struct GemmParamsDual : GemmParams { GemmSecond second; GemmCutPlan cut; };
 template <int EPI>
 using GemmParamsOf = std::conditional_t<EPI == GM_EPI_DUAL, GemmParamsDual, GemmParams>;
 
@@ -162,11 +183,11 @@ __device__ __forceinline__ bool gm_unpacked(const GemmParams& p) {
 // Work unit u: output tile (tm, tn) of problem b (bi, bo), k-blocks [kb0, kb1), split sp; `second`: of a dual launch's second product.
 struct GemmUnit { int sp, bi, bo, tm, tn, kb0, kb1; bool skip, second; };
 template <int BN, int CG, int EPI>
-__device__ __forceinline__ GemmUnit gm_unit(const GemmParamsOf<EPI>& p, long long u, int tiles_per_problem, int live) {
+__device__ __forceinline__ GemmUnit gm_unit(const GemmParamsOf<EPI>& p, long long u, int tiles_per_problem, int live, const GemmCut& cut) {
     GemmUnit w;
     w.second = false;
     if constexpr (EPI == GM_EPI_DUAL) {
-        const int first = tiles_per_problem * p.splits;
+        const long long first = (long long)tiles_per_problem * cut.splits;
         w.second = u >= first;
         w.bi = w.bo = 0;
         w.skip = false;
@@ -178,12 +199,12 @@ __device__ __forceinline__ GemmUnit gm_unit(const GemmParamsOf<EPI>& p, long lon
             w.kb1 = p.second.kblocks;
             if ((live - 1) / GM_BK + 1 < w.kb1) w.kb1 = (live - 1) / GM_BK + 1;
         } else {
-            const int t = (int)(u / p.splits);
-            w.sp = (int)(u - (long long)t * p.splits);
+            const int t = (int)(u / cut.splits);
+            w.sp = (int)(u - (long long)t * cut.splits);
             w.tm = t / p.tiles_n;
             w.tn = t - w.tm * p.tiles_n;
-            gm_kb_range(p, w.sp, w.tm, w.kb0, w.kb1);
-            w.skip = (long long)w.tm * (CG * GM_BM) >= live;
+            w.kb0 = w.sp * cut.per_split;
+            w.kb1 = w.kb0 + cut.per_split < p.kblocks ? w.kb0 + cut.per_split : p.kblocks;
         }
     } else {
         w.sp = (int)(u % p.splits);
@@ -262,8 +283,13 @@ __global__ void __launch_bounds__(gm_threads(EPI), 1) gemm_bf16_kernel(const __g
     const int live = gm_live<EPI>(p);
     const uint32_t tmem_base = ctl->tmem_base;
     volatile int* abort_flag = &ctl->abort_flag;
-    const int tiles_per_problem = p.tiles_m * p.tiles_n;
-    long long units = (long long)p.batch * tiles_per_problem * p.splits;
+    int tiles_per_problem = p.tiles_m * p.tiles_n;
+    GemmCut cut = {};
+    if constexpr (EPI == GM_EPI_DUAL) {
+        cut = gm_cut(p.cut, live);
+        if (live < p.M) tiles_per_problem = ((live - 1) / (CG * GM_BM) + 1) * p.tiles_n;
+    }
+    long long units = (long long)p.batch * tiles_per_problem * (EPI == GM_EPI_DUAL ? cut.splits : p.splits);
     if constexpr (EPI == GM_EPI_DUAL) units += p.second.tiles_m * p.second.tiles_n;
 
     if (warp == 0) {
@@ -273,7 +299,7 @@ __global__ void __launch_bounds__(gm_threads(EPI), 1) gemm_bf16_kernel(const __g
         bool dead = false;
         const bool unpacked = gm_unpacked<EPI>(p);
         for (long long u = blockIdx.x / CG; u < units && !dead; u += gridDim.x / CG) {
-            const GemmUnit w = gm_unit<BN, CG, EPI>(p, u, tiles_per_problem, live);
+            const GemmUnit w = gm_unit<BN, CG, EPI>(p, u, tiles_per_problem, live, cut);
             if (w.skip) continue;
             const int m0 = (w.tm * CG + (int)rank) * GM_BM, nb0 = w.tn * BN + (int)rank * (BN / CG);
             const unsigned char *map_a = p.tmap_a, *map_b = p.tmap_b;
@@ -332,7 +358,7 @@ __global__ void __launch_bounds__(gm_threads(EPI), 1) gemm_bf16_kernel(const __g
             uint32_t local = 0;
             bool dead = false;
             for (long long u = blockIdx.x / CG; u < units && !dead; u += gridDim.x / CG) {
-                const GemmUnit w = gm_unit<BN, CG, EPI>(p, u, tiles_per_problem, live);
+                const GemmUnit w = gm_unit<BN, CG, EPI>(p, u, tiles_per_problem, live, cut);
                 if (w.skip) continue;
                 int a_mn = p.a_mn, b_mn = p.b_mn;
                 if constexpr (EPI == GM_EPI_DUAL)
@@ -385,7 +411,7 @@ __global__ void __launch_bounds__(gm_threads(EPI), 1) gemm_bf16_kernel(const __g
         uint32_t local = 0;
         uint32_t slab_i = 0;
         for (long long u = blockIdx.x / CG; u < units; u += gridDim.x / CG) {
-            const GemmUnit w = gm_unit<BN, CG, EPI>(p, u, tiles_per_problem, live);
+            const GemmUnit w = gm_unit<BN, CG, EPI>(p, u, tiles_per_problem, live, cut);
             const int sp = w.sp, tm = w.tm, tn = w.tn, bi = w.bi, bo = w.bo;
             if (w.skip) continue;
             const uint32_t ab = local & 1u, use = local >> 1;
@@ -410,14 +436,14 @@ __global__ void __launch_bounds__(gm_threads(EPI), 1) gemm_bf16_kernel(const __g
             const uint32_t t_row = tmem_base + ((uint32_t)(q * 32) << 16) + ab * BN;
             if (idle) {
             } else if constexpr (kAct || EPI == GM_EPI_ACT_ANY) {
-                if (p.splits > 1) gm_epilogue_slab<kCols>(p, t_row + part * kCols, m, n0 + part * kCols, sp);
+                if (p.splits > 1) gm_epilogue_slab<kCols>(p, t_row + part * kCols, m, n0 + part * kCols, sp, p.M);
                 else if constexpr (EPI == GM_EPI_ACT_ANY) gm_epilogue_act_any<kCols>(p, t_row + part * kCols, m, m0w, n0 + part * kCols, lane, epi_smem + (warp - 2) * 4096);
                 else if (!gm_epilogue_act<kCols, kSlope>(p, t_row + part * kCols, m, m0w, n0 + part * kCols, lane, epi_smem + (warp - 2) * 4096, slab_i, ctl->res_full[warp - 2], abort_flag)) {
                     if (!*abort_flag) { ctl->abort_flag = 1; if (p.status) atomicExch(p.status, OB200_ERR_WAIT_FULL); }
                     break;
                 }
             } else if constexpr (EPI == GM_EPI_DUAL) {
-                if (p.splits > 1 && !w.second) gm_epilogue_slab<BN>(p, t_row, m, n0, sp);
+                if (cut.splits > 1 && !w.second) gm_epilogue_slab<BN>(p, t_row, m, n0, sp, cut.rows);
                 else gm_epilogue_dual<BN>(p, w.second, t_row, m, m0w, n0, lane, epi_smem + (warp - 2) * 8192, slab_i);
             } else if constexpr (EPI == GM_EPI_LSE) gm_epilogue_lse<kCols>(p, t_row + part * kCols, m, n0 + part * kCols);
             else if constexpr (EPI == GM_EPI_DLOGITS) gm_epilogue_dlogits<kCols>(p, t_row + part * kCols, m, m0w, n0 + part * kCols, lane, epi_smem + (warp - 2) * 4096, slab_i);
@@ -618,9 +644,15 @@ __global__ void __launch_bounds__(256) gemm_splitk_finish_kernel(const float* __
 // same additions in the same order, 13 -> 4 us for 1143 x 768 in five parts.
 template <typename T>
 __global__ void __launch_bounds__(256) gemm_splitk_finish4_kernel(const float* __restrict__ slabs, T* c, const float* addend, const float* factor, int splits,
-                                                                  int M, int N, long long ldc, float alpha) {
+                                                                  int M, int N, long long ldc, float alpha, const int* live, GemmCutPlan plan) {
     pdl_wait();
     pdl_launch_dependents();
+    if (live) {   // of a dual launch over packed rows: cut on the device
+        const GemmCut cut = gm_cut(plan, *live > 1 ? *live : 1);
+        if (cut.splits == 1) return;
+        splits = cut.splits;
+        M = cut.rows;
+    }
     const long long per_split = (long long)M * N, quads = per_split / 4;
     const int row = N / 4;
     if (factor) alpha *= *factor;
@@ -899,15 +931,15 @@ static int gm_launch_tile(const GemmParams& p, int bn, int cg, int grid, cudaStr
 }
 
 static int gm_finish4(const float* slabs, void* c, int out_f32, const float* addend, const float* factor, int splits, int M, int N, long long ldc, float alpha,
-                      int num_ctas, cudaStream_t st) {
+                      int num_ctas, cudaStream_t st, const int* live = nullptr, const GemmCutPlan& plan = {}) {
     const long long want = ((long long)M * N / 4 + 255) / 256, most = 8LL * num_ctas;
     const unsigned blocks = (unsigned)(want < most ? want : most);
     if (out_f32) {
         OB200_ELASTIC_HBM(gemm_splitk_finish4_kernel<float>, 8);
-        return launch_pdl(gemm_splitk_finish4_kernel<float>, blocks, 256u, st, slabs, (float*)c, addend, factor, splits, M, N, ldc, alpha);
+        return launch_pdl(gemm_splitk_finish4_kernel<float>, blocks, 256u, st, slabs, (float*)c, addend, factor, splits, M, N, ldc, alpha, live, plan);
     }
     OB200_ELASTIC_HBM(gemm_splitk_finish4_kernel<__nv_bfloat16>, 8);
-    return launch_pdl(gemm_splitk_finish4_kernel<__nv_bfloat16>, blocks, 256u, st, slabs, (__nv_bfloat16*)c, addend, factor, splits, M, N, ldc, alpha);
+    return launch_pdl(gemm_splitk_finish4_kernel<__nv_bfloat16>, blocks, 256u, st, slabs, (__nv_bfloat16*)c, addend, factor, splits, M, N, ldc, alpha, live, plan);
 }
 
 int gemm_bf16_run(const GemmCall& g) {
@@ -1088,9 +1120,9 @@ int gemm_bf16_dual_splits(const GemmCall& a, const GemmCall& b) {
     }
     return best;
 }
-size_t gemm_bf16_dual_slab_bytes(const GemmCall& a, const GemmCall& b) {
+size_t gemm_bf16_dual_slab_bytes(const GemmCall& a, const GemmCall& b, bool packed) {
     const int s = gemm_bf16_dual_splits(a, b);
-    return s > 1 ? (size_t)s * a.M * a.N * sizeof(float) : 0;
+    return s > 1 || (packed && s > 0 && a.M > 256) ? (size_t)s * a.M * a.N * sizeof(float) : 0;
 }
 
 int gemm_bf16_run_dual(const GemmCall& a, const GemmCall& b) {
@@ -1098,39 +1130,34 @@ int gemm_bf16_run_dual(const GemmCall& a, const GemmCall& b) {
     if (splits < 1) return -1;
     const int kblocks = (a.K + GM_BK - 1) / GM_BK, per_split = (kblocks + splits - 1) / splits;
     splits = (kblocks + per_split - 1) / per_split;   // every split owns at least one k-block
-    if (splits > 1 && (!a.slabs || (size_t)splits * a.M * a.N * sizeof(float) > a.slab_bytes)) return -3;
-    if (a.num_ctas < 2) {   // no pair: one after the other, the same sums
-        GemmCall one = a, two = b;
-        one.epi = two.epi = GM_EPI_ACC;
-        one.splits = splits;
-        two.splits = 1;
-        const int rc = gemm_bf16_run(one);
-        return rc ? rc : gemm_bf16_run(two);
-    }
+    const bool recut = a.live && a.M > 256;   // fewer rows may be cut into more parts
+    if ((splits > 1 || recut) && (!a.slabs || (size_t)splits * a.M * a.N * sizeof(float) > a.slab_bytes)) return -3;
+    const int cg = a.num_ctas < 2 ? 1 : 2, tile_m = cg * GM_BM;   // one CTA: tiles of 128 rows, the same sums
     GemmParamsDual p;
     memset(&p, 0, sizeof p);
     p.status = ob200_status_word_for_current_device();
     p.M = a.M; p.N = a.N; p.K = a.K;
     p.batch = p.nb_inner = 1;
     p.splits = splits;
-    p.slabs = splits > 1 ? a.slabs : nullptr;
+    p.slabs = splits > 1 || recut ? a.slabs : nullptr;
     p.out_f32 = a.out_f32 ? 1 : 0;
     p.a_mn = a.a_mn; p.b_mn = a.b_mn;
     p.alpha = a.alpha;
     p.e = a.e;
     p.kblocks = kblocks;
     p.kb_per_split = per_split;
-    p.tiles_m = (a.M + 2 * GM_BM - 1) / (2 * GM_BM);
+    p.tiles_m = (a.M - 1) / tile_m + 1;
     p.tiles_n = (a.N + 255) / 256;
     p.second.M = b.M; p.second.N = b.N;
     p.second.out_f32 = b.out_f32 ? 1 : 0;
     p.second.a_mn = b.a_mn; p.second.b_mn = b.b_mn;
     p.second.kblocks = (b.K + GM_BK - 1) / GM_BK;
-    p.second.tiles_m = (b.M + 2 * GM_BM - 1) / (2 * GM_BM);
+    p.second.tiles_m = (b.M - 1) / tile_m + 1;
     p.second.tiles_n = (b.N + 255) / 256;
-    auto operands = [](const GemmCall& g, unsigned char* ta, unsigned char* tb) {
+    p.cut = {a.M, p.tiles_n, kblocks, splits, per_split, (int)(((long long)b.M + 255) / 256) * p.second.tiles_n, p.second.kblocks, ob200_plan_sm_count() / 2};
+    auto operands = [cg](const GemmCall& g, unsigned char* ta, unsigned char* tb) {
         return (g.a_mn ? gm_make_map(ta, g.a, g.M, g.K, g.lda, 1, 0, 1, 0, 64, GM_BK) : gm_make_map(ta, g.a, g.K, g.M, g.lda, 1, 0, 1, 0, GM_BK, GM_BM)) &&
-               (g.b_mn ? gm_make_map(tb, g.b, g.N, g.K, g.ldb, 1, 0, 1, 0, 64, GM_BK) : gm_make_map(tb, g.b, g.K, g.N, g.ldb, 1, 0, 1, 0, GM_BK, 128));
+               (g.b_mn ? gm_make_map(tb, g.b, g.N, g.K, g.ldb, 1, 0, 1, 0, 64, GM_BK) : gm_make_map(tb, g.b, g.K, g.N, g.ldb, 1, 0, 1, 0, GM_BK, 256 / cg));
     };
     if (!operands(a, p.tmap_a, p.tmap_b) || !operands(b, p.second.tmap_a, p.second.tmap_b) || !gm_make_c_map(p.tmap_c, a) ||
         !gm_make_c_map(p.second.tmap_c, b))
@@ -1147,11 +1174,13 @@ int gemm_bf16_run_dual(const GemmCall& a, const GemmCall& b) {
     }
     const long long tiles = (long long)p.tiles_m * p.tiles_n * splits + (long long)p.second.tiles_m * p.second.tiles_n;
     if (tiles > 0x3fffffffLL) return -1;
-    const long long most = a.num_ctas / 2;
+    const long long most = a.num_ctas / cg;
     annotate_launch(1, 2.0 * ((double)a.M * a.N * a.K + (double)b.M * b.N * b.K), 2.0 * ((double)a.M * a.K + (double)a.K * a.N + (double)b.M * b.K + (double)b.K * b.N));
-    const int rc = gm_launch<256, 2, GM_EPI_DUAL>(p, (int)(tiles < most ? tiles : most) * 2, (cudaStream_t)a.stream);
-    if (rc || splits == 1) return rc;
-    return gm_finish4(p.slabs, a.c, a.out_f32, a.e.addend, a.e.factor, splits, a.M, a.N, a.ldc, a.alpha, a.num_ctas, (cudaStream_t)a.stream);
+    const int grid = (int)(tiles < most ? tiles : most) * cg;
+    const int rc = cg == 2 ? gm_launch<256, 2, GM_EPI_DUAL>(p, grid, (cudaStream_t)a.stream) : gm_launch<256, 1, GM_EPI_DUAL>(p, grid, (cudaStream_t)a.stream);
+    if (rc || (splits == 1 && !recut)) return rc;
+    return gm_finish4(p.slabs, a.c, a.out_f32, a.e.addend, a.e.factor, splits, a.M, a.N, a.ldc, a.alpha, a.num_ctas, (cudaStream_t)a.stream,
+                      a.live, p.cut);
 }
 
 }  // namespace ob200

@@ -75,7 +75,7 @@ int gemm_bf16_run(const GemmCall& call);
 // one alpha, epilogue GM_EPI_ACC (the addend is the first one's), rows of C 16-byte multiples.  `splits`: into how many parts the first
 // one's reduction is cut for that, 0 where the products are too narrow.
 int gemm_bf16_dual_splits(const GemmCall& first, const GemmCall& second);
-size_t gemm_bf16_dual_slab_bytes(const GemmCall& first, const GemmCall& second);
+size_t gemm_bf16_dual_slab_bytes(const GemmCall& first, const GemmCall& second, bool packed = false);
 int gemm_bf16_run_dual(const GemmCall& first, const GemmCall& second);
 // Bytes of partial matrices that the split of a product with this epilogue wants; 0 where it is not split.
 size_t gemm_bf16_slab_bytes(int M, int N, int K, int epi);

@@ -81,7 +81,7 @@ __device__ __forceinline__ void gm_act_slope(float (&f)[W], int act, uint8_t* sl
 
 // Partial matrices of a product with split-K, as they are: the rest is a second kernel's.
 template <int COLS>
-__device__ __forceinline__ void gm_epilogue_slab(const GemmParams& p, uint32_t t_row, int m, int n0, int sp) {
+__device__ __forceinline__ void gm_epilogue_slab(const GemmParams& p, uint32_t t_row, int m, int n0, int sp, int rows) {
 #pragma unroll 1
     for (int c0 = 0; c0 < COLS; c0 += 32) {
         const int n = n0 + c0;
@@ -89,8 +89,8 @@ __device__ __forceinline__ void gm_epilogue_slab(const GemmParams& p, uint32_t t
         uint32_t v[32];
         tmem_ld_32x32(t_row + c0, v);
         tmem_ld_wait();
-        if (m >= p.M) continue;
-        float* srow = p.slabs + ((long long)sp * p.M + m) * p.N + n;
+        if (m >= rows) continue;
+        float* srow = p.slabs + ((long long)sp * rows + m) * p.N + n;
         if (n + 32 <= p.N && (p.N & 3) == 0) {
 #pragma unroll
             for (int j = 0; j < 32; j += 4) *reinterpret_cast<uint4*>(srow + j) = make_uint4(v[j], v[j + 1], v[j + 2], v[j + 3]);

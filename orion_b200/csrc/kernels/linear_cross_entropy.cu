@@ -201,6 +201,7 @@ __global__ void __launch_bounds__(CE_PACK_THREADS) ce_pack_kernel(const CePack p
             if (to == INT_MIN) continue;
             const uint4* src = reinterpret_cast<const uint4*>(p.x + (base + i) * p.ldx);
             uint4* dst = reinterpret_cast<uint4*>(p.packed + (long long)(to < 0 ? ~to : to) * p.H);
+#pragma unroll 4
             for (int c = lane; c < p.H / 8; c += 32) dst[c] = to < 0 ? make_uint4(0, 0, 0, 0) : src[c];
         }
     }
@@ -214,11 +215,12 @@ __global__ void __launch_bounds__(CE_THREADS) ce_unpack_kernel(const __nv_bfloat
         const int from = slot[r];
         const uint4* src = reinterpret_cast<const uint4*>(packed + (long long)from * H);
         uint4* dst = reinterpret_cast<uint4*>(dx + r * H);
+#pragma unroll 4
         for (int c = lane; c < H / 8; c += 32) dst[c] = from < 0 ? make_uint4(0, 0, 0, 0) : src[c];
     }
 }
 static int ce_pack(const CePack& p, int num_ctas, cudaStream_t st) {
-    const long long want = ((long long)p.rows + 31) / 32, cap = (long long)num_ctas * 2;
+    const long long want = ((long long)p.rows + 15) / 16, cap = (long long)num_ctas * 2;
     OB200_ELASTIC_HBM(ce_pack_kernel, 2);
     return launch_pdl(ce_pack_kernel, (unsigned)(want < cap ? want : cap), (unsigned)CE_PACK_THREADS, st, p);
 }
@@ -282,7 +284,7 @@ struct CeBackwardSpace {
             gx.M = (int)rows; gx.N = gw.N = H; gx.K = v;
             gw.M = v; gw.K = (int)rows;
             const size_t a = want_dx ? gemm_bf16_slab_bytes((int)rows, H, v, GM_EPI_ACC) : 0, b = want_dw ? gemm_bf16_slab_bytes(v, H, (int)rows, GM_EPI_ACC) : 0;
-            const size_t c = want_dx && want_dw ? gemm_bf16_dual_slab_bytes(gx, gw) : 0;
+            const size_t c = want_dx && want_dw ? gemm_bf16_dual_slab_bytes(gx, gw, true) : 0;
             for (size_t n : {a, b, c})
                 if (n > slabs) slabs = n;
         }

@@ -432,12 +432,11 @@ def test_loss_in_several_pieces_of_the_vocabulary(ops):
     assert torch.equal(torch.autograd.grad(b, w)[0], dw)
 
 
-@pytest.mark.parametrize("counted", [0, 1, 63, 64, 65, 128, 129, 300, 512, 513, 699, 700])
-@pytest.mark.parametrize("V,H", [(1000, 64), (5003, 136), (2050, 1024)])
-def test_loss_over_the_rows_that_count(ops, V, H, counted):
-    """Rows that count are packed for the products: none of them, a block, a tile, one more and one less; whatever the others hold; and the
-    same bits from any CTA count."""
-    T = 700
+@pytest.mark.parametrize("T,V,H,counted", [(700, V, H, n) for V, H in ((1000, 64), (5003, 136), (2050, 1024)) for n in (0, 1, 63, 64, 65, 128, 129, 300, 512, 513, 699, 700)] +
+                         [(1143, 9000, 768, n) for n in (170, 257)] + [(5000, 24001, 136, n) for n in (0, 40, 600, 3000, 4999)] + [(2100, 20000, 264, 200)])
+def test_loss_over_the_rows_that_count(ops, T, V, H, counted):
+    """Rows that count are packed for the products: none of them, a block, a tile, one more and one less; whatever the others hold; few of
+    many, whose gradient products are cut otherwise; in two pieces of the vocabulary; and the same bits from any CTA count."""
     torch.manual_seed(V + counted)
     x, w = torch.randn(T, H, device="cuda").to(BF), (torch.randn(V, H, device="cuda") * 2 / math.sqrt(H)).to(BF)
     target = torch.randint(0, V, (T,), device="cuda")

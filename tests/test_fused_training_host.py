@@ -161,8 +161,9 @@ def test_entry_points_refuse_bad_arguments_without_a_gpu(K):
 def test_backward_of_the_loss_takes_less_scratch_than_the_logits(K):
     L = K.lib()
     rows, V, H = 8192, 32000, 1024
-    # gradients of a piece's logits (at most 192 MB), copies of x and dx in bfloat16 and dx in float32: under half of the 524 MB
-    assert L.ob200_linear_cross_entropy_backward_workspace(rows, V, H, 1, 1) < 0.5 * rows * V * 2
+    # gradients of a piece's logits (at most 192 MB), copies of x and dx in bfloat16, dx in float32 and a
+    # partial matrix of it: 176 + 2 x 17 + 2 x 34 MB of the 524
+    assert L.ob200_linear_cross_entropy_backward_workspace(rows, V, H, 1, 1) < 0.54 * rows * V * 2
     # eight bytes for 128 columns of a row, and a copy of x: 16.4 and 16.8 MB
     assert L.ob200_linear_cross_entropy_workspace(rows, V, H) < 0.07 * rows * V * 2
 
