@@ -14,7 +14,7 @@ training (ORION_PREPARE=1, the default): linear layers and attention with all th
 bfloat16 GEMM, LayerNorm / GELU / softmax / embedding / cross-entropy forward and backward, one-launch AdamW.
 ORION_FUSED_LINEAR=1 runs every linear layer with what follows it (bias, GELU, dropout, residual) as one launch, ORION_FUSED_LOSS=1
 computes the decoder's loss from the hidden states, without logits, and ORION_DROPOUT=p trains with dropout of the embeddings and
-of both residual branches, as the reference's clients do (reference benchmarking/model_kernels/bert_8_fb1, fused_dropout_kernel_vec); the
+of both residual branches, as the reference's clients do (reference benchmarking/model_kernels/bert_8_fb1, dropout rows); the
 masks are drawn from counters and never stored.  All three are off by default: recorded profiles have a row per launch.
 With ORION_PREPARE=0 training uses stock PyTorch modules, whose cuBLASLt / flash-attention / elementwise
 launches are captured and scheduled like any other op.

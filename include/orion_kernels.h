@@ -257,7 +257,7 @@ int ob200_adamw_f32(float* p, const float* g, float* m, float* v, long long n, f
  * 8): the activation's derivative at x . w^T + bias in float16, which the backward pass multiplies by.  workspace: the bytes that
  * ob200_linear_act_workspace names (0: none), any contents, the call's own until it has run.
  * Returns -1 for bad arguments, -2 for misaligned pointers or strides, -3 for a workspace that is too small, -4 when a TMA descriptor
- * cannot be built.  Stands for the sgemm, bias, GELU, fused_dropout_kernel_vec and add rows of the reference's
+ * cannot be built.  Stands for the sgemm, bias, GELU, dropout and add rows of the reference's
  * benchmarking/model_kernels/bert_8_fb1 (src/scheduler/utils_sched.cpp:490-501; src/cuda_capture/intercept_temp.cpp:418-458). */
 int ob200_linear_act_bf16(const void* x, const void* w, void* y, void* slope, const void* bias, int bias_f32, const void* residual, int act,
                           float p, const long long* rng, int site, int M, int N, int K, long long ldx, long long ldw, long long ld_slope,
@@ -272,17 +272,17 @@ int ob200_linear_act_backward_bf16(const void* dy, const void* slope, const void
 long long ob200_linear_act_backward_workspace(int M, int N, int K, int act, float p, int want_dx, int want_dw, int want_dbias);
 
 /* y = dropout(x) [+ residual] over n contiguous elements with the mask above (dtype 0 float32, 1 bfloat16; residual may be NULL; y may
- * be x): the gradient is the same call on dy.  Stands for fused_dropout_kernel_vec and its masked-scale backward kernel (reference
+ * be x): the gradient is the same call on dy.  Stands for the dropout kernel and its masked-scale backward kernel (reference
  * benchmarking/model_kernels/bert_8_fb1), without the stored mask. */
 int ob200_dropout(const void* x, const void* residual, void* y, long long n, float p, const long long* rng, int site, int dtype,
                   int num_ctas, void* stream);
 
 /* Softmax cross-entropy of the logits x . w^T over a vocabulary of V, without the logits (bfloat16 x [rows, H] and w [V, H], rows ldx / ldw
  * apart; H, ldx, ldw multiples of 8, 16-byte aligned; V any): loss[row] = lse[row] - logit of target[row], lse[row] = logsumexp; 0 for
- * a row whose target is ignore_index, not a number for any other target outside the vocabulary.  total (NULL: not wanted) receives
- * the sum of the losses, or with `mean` their mean over the rows that count (0 where none does), count their number (at least 1).  The
- * results do not depend on num_ctas.  Stands where the reference's clients launch the vocabulary projection's sgemm and the softmax /
- * nll_loss kernels (reference benchmarking/model_kernels/bert_8_fb1). */
+ * a row whose target is ignore_index (its lse is not specified; its products are left out where that saves a tile), not a number for any
+ * other target outside the vocabulary.  total (NULL: not wanted) receives the sum of the losses, or with `mean` their mean over the rows
+ * that count (0 where none does), count their number (at least 1).  The results do not depend on num_ctas.  Stands where the reference's
+ * clients launch the vocabulary projection's product and the softmax and loss kernels (reference benchmarking/model_kernels/bert_8_fb1). */
 int ob200_linear_cross_entropy_forward(const void* x, const void* w, const long long* target, float* loss, float* lse, float* total,
                                        float* count, int rows, int V, int H, long long ldx, long long ldw, long long ignore_index, int mean,
                                        void* workspace, long long workspace_bytes, int num_ctas, void* stream);

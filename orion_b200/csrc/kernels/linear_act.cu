@@ -5,7 +5,7 @@
 //
 // The products are gemm_bf16.cu's with the GM_EPI_ACT epilogue; here are the elementwise kernels.  No mask is stored: it is a function
 // of the element's index (philox.cuh) and drawn again in the backward pass.  The reference's clients launch these steps as the bias,
-// GELU, add and fused_dropout_kernel_vec rows of benchmarking/model_kernels/bert_8_fb1 behind its cudaLaunchKernel trap
+// GELU, add and dropout rows of benchmarking/model_kernels/bert_8_fb1 behind its cudaLaunchKernel trap
 // (reference src/cuda_capture/intercept_temp.cpp:418-458).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
