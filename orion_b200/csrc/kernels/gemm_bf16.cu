@@ -114,7 +114,7 @@ __host__ __device__ inline GemmCut gm_cut(const GemmCutPlan& c, int live) {
     if (some >= all) return {c.splits, c.per_split, c.M};
     const int deep = (live - 1) / GM_BK + 1 < c.second_kblocks ? (live - 1) / GM_BK + 1 : c.second_kblocks;
     const long long work = (long long)some * c.tiles_n * c.kblocks + (long long)c.second_tiles * (deep + 8), share = work / c.pairs + 1;
-    const long long room = (long long)c.splits * all / some;
+    const long long room = (long long)c.splits * c.M / (some * 256LL);
     long long parts = 3LL * c.kblocks / share;
     if (parts > room) parts = room;
     if (parts > c.kblocks / 4) parts = c.kblocks / 4;
