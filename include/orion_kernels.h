@@ -265,7 +265,7 @@ int ob200_linear_act_bf16(const void* x, const void* w, void* y, void* slope, co
 long long ob200_linear_act_workspace(int M, int N, int K);
 /* Its gradients: dz = dropout(dy) * slope, dbias = column sums of dz (in a fixed order, in the bias's type), dx = dz . w,
  * dw = dz^T . x; dy [M, N], dx [M, K], dw [N, K] contiguous, 16-byte aligned; dx, dw, dbias may be NULL (not wanted); slope only with an
- * activation.  The residual's gradient is dy. */
+ * activation.  The residual's gradient is dy.  With no rows (or no columns) dw and dbias (dx) are zeros. */
 int ob200_linear_act_backward_bf16(const void* dy, const void* slope, const void* x, const void* w, void* dx, void* dw, void* dbias,
                                    int bias_f32, int act, float p, const long long* rng, int site, int M, int N, int K, long long ldx,
                                    long long ldw, long long ld_slope, void* workspace, long long workspace_bytes, int num_ctas, void* stream);

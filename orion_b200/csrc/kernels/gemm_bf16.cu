@@ -1110,11 +1110,7 @@ int gemm_bf16_dual_splits(const GemmCall& a, const GemmCall& b) {
     for (int s = 1; s <= 16 && s <= ka; s++) {
         if (s > 1 && (ta * s > 2 * pairs || ka / s < 4)) break;
         const long long ua = ta * s, ca = (ka + s - 1) / s + 8, cb = kb + 8;
-        long long longest = 0;
-        for (long long p = 0; p < pairs && p < ua + tb; p++) {   // a pair has every pairs-th unit, those of the first product first
-            const long long na = ua > p ? (ua - p + pairs - 1) / pairs : 0, n = (ua + tb - p + pairs - 1) / pairs, cost = na * ca + (n - na) * cb;
-            if (cost > longest) longest = cost;
-        }
+        const long long longest = gemm_longest_share(pairs, ua, ca, tb, cb);
         const double cost = (double)longest + (s > 1 ? (3.0 + (double)s * a.M * a.N * 8.0 / 6e6) / 0.45 : 0.0);
         if (best_cost == 0.0 || cost < best_cost) { best = s; best_cost = cost; }
     }

@@ -71,6 +71,17 @@ struct GemmCall {
 
 // 0, a cudaError_t, -1 (sizes), -2 (alignment), -4 (no TMA descriptor).
 int gemm_bf16_run(const GemmCall& call);
+// Work of the CTA pair that has most of it: a pair takes every pairs-th unit, `a` of cost ca first, then `b` of cost cb.  What a pair gets
+// changes with its number at two places only.
+inline long long gemm_longest_share(long long pairs, long long a, long long ca, long long b, long long cb) {
+    long long longest = 0;
+    for (const long long p : {0LL, a % pairs, (a + b) % pairs}) {
+        const long long na = a > p ? (a - p - 1) / pairs + 1 : 0, n = a + b > p ? (a + b - p - 1) / pairs + 1 : 0, cost = na * ca + (n - na) * cb;
+        if (cost > longest) longest = cost;
+    }
+    return longest;
+}
+
 // Two products in one launch of CTA pairs, 256 x 256 tiles, so that the last round of tiles is one and not two: no batch, bias or residual,
 // one alpha, epilogue GM_EPI_ACC (the addend is the first one's), rows of C 16-byte multiples.  `splits`: into how many parts the first
 // one's reduction is cut for that, 0 where the products are too narrow.

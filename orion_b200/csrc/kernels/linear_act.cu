@@ -323,7 +323,13 @@ extern "C" int ob200_linear_act_backward_bf16(const void* dy, const void* slope,
                                               int bias_f32, int act, float p, const long long* rng, int site, int M, int N, int K, long long ldx,
                                               long long ldw, long long ld_slope, void* workspace, long long workspace_bytes, int num_ctas, void* stream) {
     if (M < 0 || N < 0 || K <= 0 || act < 0 || act > 2 || !(p >= 0.f && p <= 1.f) || (p > 0.f && !rng) || num_ctas <= 0 || ldx < K || ldw < K) return -1;
-    if (M == 0 || N == 0) return 0;
+    if (M == 0 || N == 0) {   // sums over nothing
+        cudaError_t e = cudaSuccess;
+        if (dx && M > 0) e = cudaMemsetAsync(dx, 0, (size_t)M * K * 2, (cudaStream_t)stream);
+        if (dw && N > 0 && e == cudaSuccess) e = cudaMemsetAsync(dw, 0, (size_t)N * K * 2, (cudaStream_t)stream);
+        if (dbias && N > 0 && e == cudaSuccess) e = cudaMemsetAsync(dbias, 0, (size_t)N * (bias_f32 ? 4 : 2), (cudaStream_t)stream);
+        return (int)e;
+    }
     if (!dy || (act && !slope) || (slope && (ld_slope < N || ld_slope % 8 || !act)) || (dx && !w) || (dw && !x)) return -1;
     if (((uintptr_t)dy | (uintptr_t)slope | (uintptr_t)x | (uintptr_t)w | (uintptr_t)dx | (uintptr_t)dw | (uintptr_t)workspace) % 16 || (ldx | ldw) % 8)
         return -2;

@@ -252,14 +252,7 @@ static int ce_piece(long long rows, int V, int H, int sms) {
                 cost += work / pairs + dw_cost / 2 + 16;
                 continue;
             }
-            // a pair has every pairs-th unit, those of dx first
-            auto load = [&](long long pair) {
-                const long long a = dx > pair ? (dx - pair + pairs - 1) / pairs : 0, b = dx + dw > pair ? (dx + dw - pair + pairs - 1) / pairs - a : 0;
-                return a * dx_cost + b * dw_cost;
-            };
-            long long longest = 0;
-            for (long long pair = 0; pair < pairs; pair++) longest = load(pair) > longest ? load(pair) : longest;
-            cost += longest;
+            cost += gemm_longest_share(pairs, dx, dx_cost, dw, dw_cost);
         }
         if (best == 0 || cost < best_cost) { best = v; best_cost = cost; }
     }

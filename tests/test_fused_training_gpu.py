@@ -743,6 +743,86 @@ def test_through_the_c_abi(built):
             assert torch.equal(g, h)
 
 
+@pytest.mark.parametrize("T,V,H,counted", [(1143, 9000, 768, 171), (1143, 9000, 768, 1143), (700, 5003, 136, 3), (5000, 24001, 136, 40), (300, 128, 1024, 100), (40, 515, 64, 20)])
+def test_calls_stay_inside_their_scratch_and_outputs(built, T, V, H, counted):
+    """Guard words behind the scratch and behind every output of the loss and of the linear layer stay as they were."""
+    from orion_b200 import kernels as K
+    L, guard = K.lib(), 1 << 20
+    torch.manual_seed(T + counted)
+    x, w = torch.randn(T, H, device="cuda").to(BF), torch.randn(V, H, device="cuda").to(BF)
+    target = torch.randint(0, V, (T,), device="cuda")
+    target[torch.randperm(T, device="cuda")[counted:]] = -100
+    spaces = []
+
+    def space(n):
+        t = torch.full((n + guard,), 0xA5, device="cuda", dtype=torch.uint8)
+        spaces.append((t, n))
+        return t
+    loss, lse, total, count, dx, dw = space(T * 4), space(T * 4), space(4), space(4), space(T * H * 2), space(V * H * 2)
+    one = torch.ones((), device="cuda")
+    n = L.ob200_linear_cross_entropy_workspace(T, V, H)
+    assert L.ob200_linear_cross_entropy_forward(*(K._ptr(t) for t in (x, w, target, loss, lse, total, count)), T, V, H, H, H, -100, 1, K._ptr(space(n)), n,
+                                                K.sm_count(), K._stream()) == 0
+    n = L.ob200_linear_cross_entropy_backward_workspace(T, V, H, 1, 1)
+    assert L.ob200_linear_cross_entropy_backward(*(K._ptr(t) for t in (x, w, target, lse, one)), 0, K._ptr(count), K._ptr(dx), K._ptr(dw), T, V, H, H, H,
+                                                 -100, K._ptr(space(n)), n, K.sm_count(), K._stream()) == 0
+    N = 515   # a linear layer of the same input
+    wl, bias, dy, rng = torch.randn(N, H, device="cuda").to(BF), torch.randn(N, device="cuda").to(BF), torch.randn(T, N, device="cuda").to(BF), rng_of(1, 2)
+    y, slope, dxl, dwl, db = space(T * N * 2), space(T * 520 * 2), space(T * H * 2), space(N * H * 2), space(N * 2)
+    n = L.ob200_linear_act_workspace(T, N, H)
+    assert L.ob200_linear_act_bf16(*(K._ptr(t) for t in (x, wl, y, slope, bias)), 0, None, 2, 0.1, K._ptr(rng), 0, T, N, H, H, H, 520, K._ptr(space(n)), n,
+                                   K.sm_count(), K._stream()) == 0
+    n = L.ob200_linear_act_backward_workspace(T, N, H, 2, 0.1, 1, 1, 1)
+    assert L.ob200_linear_act_backward_bf16(*(K._ptr(t) for t in (dy, slope, x, wl, dxl, dwl, db)), 0, 2, 0.1, K._ptr(rng), 0, T, N, H, H, H, 520,
+                                            K._ptr(space(n)), n, K.sm_count(), K._stream()) == 0
+    for t, n in spaces:
+        assert (t[n:] == 0xA5).all(), n
+
+
+def test_gradients_over_no_rows_are_zeros(built):
+    from orion_b200 import kernels as K
+    L = K.lib()
+    x, w, dy = torch.empty(0, 64, device="cuda", dtype=BF), torch.ones(40, 64, device="cuda", dtype=BF), torch.empty(0, 40, device="cuda", dtype=BF)
+    dw, db = torch.ones(40, 64, device="cuda", dtype=BF), torch.ones(40, device="cuda")
+    assert L.ob200_linear_act_backward_bf16(K._ptr(dy), None, K._ptr(x), K._ptr(w), None, K._ptr(dw), K._ptr(db), 1, 0, 0.0, None, 0, 0, 40, 64, 64, 64, 0,
+                                            None, 0, K.sm_count(), K._stream()) == 0
+    assert not dw.any() and not db.any()
+    dx = torch.ones(5, 64, device="cuda", dtype=BF)
+    assert L.ob200_linear_act_backward_bf16(K._ptr(dy), None, K._ptr(x), K._ptr(w), K._ptr(dx), None, None, 1, 0, 0.0, None, 0, 5, 0, 64, 64, 64, 0,
+                                            None, 0, K.sm_count(), K._stream()) == 0
+    assert not dx.any()
+
+
+def test_a_captured_loss_counts_its_rows_anew_at_each_replay(ops):
+    """How many rows count is read on the device: a graph captured with one number of them is right for every other."""
+    T, V, H = 900, 5003, 264
+    torch.manual_seed(4)
+    x, w = torch.randn(T, H, device="cuda").to(BF).requires_grad_(True), (torch.randn(V, H, device="cuda") / 8).to(BF).requires_grad_(True)
+    labels, target = torch.randint(0, V, (T,), device="cuda"), torch.empty(T, device="cuda", dtype=torch.long)
+    target.copy_(labels)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        torch.autograd.grad(ops.linear_cross_entropy(x, w, target), (x, w))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=s):
+        loss = ops.linear_cross_entropy(x, w, target)
+        out = [loss.detach()] + list(torch.autograd.grad(loss, (x, w)))
+        del loss
+    for counted in (900, 1, 0, 257, 256, 899, 64, 900):
+        target.copy_(labels)
+        target[torch.randperm(T, device="cuda")[counted:]] = -100
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        eager = ops.linear_cross_entropy(x, w, target)
+        want = [eager.detach()] + list(torch.autograd.grad(eager, (x, w)))
+        for a, b in zip(out, want):
+            assert torch.equal(a, b), counted
+        del eager
+
+
 @pytest.mark.parametrize("out_dtype", [torch.float32, BF])
 @pytest.mark.parametrize("M,N", [(2200, 2040), (264, 1000), (1040, 512)])
 def test_gemm_tiles_whose_lower_warps_are_past_the_edge(built, M, N, out_dtype):

@@ -130,7 +130,7 @@ def test_entry_points_refuse_bad_arguments_without_a_gpu(K):
     for bad in (dict(dy=a + 2), dict(dx=a + 2), dict(dw=a + 8), dict(ldx=9)):
         assert back(**bad) == -2, bad
     assert back(act=2, slope=a, ld_slope=8, nbytes=0) == -3 and back(db=a, ws=None) == -3
-    assert back(M=0) == 0
+    assert back(M=0, dw=None) == 0   # dw, a sum over nothing, would be zeroed
 
     def drop(x=a, y=a, n=8, p=0.1, rng=a, dtype=1, ctas=1):
         return L.ob200_dropout(x, None, y, n, p, rng, 0, dtype, ctas, None)
