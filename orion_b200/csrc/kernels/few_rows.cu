@@ -76,8 +76,9 @@ __device__ __forceinline__ void few_put(float (&red)[16][LD], const float (&acc)
     }
 }
 
-// A tile's way out, by WARPS warps, for tokens [first, first + tokens): the sums of the warps that shared the reduction are joined in their order, then either the epilogue of
-// linear_act, a thread an output, or, half a warp a token and a lane a row of w, the maximum, the sum of exponentials and the label's logit.
+// A tile's way out, by WARPS warps, for tokens [first, first + tokens): the sums of the warps that shared the reduction are joined in
+// their order, then either the epilogue of linear_act, a thread an output, or, half a warp a token and a lane a row of w, the maximum,
+// the sum of exponentials and the label's logit.
 template <int WARPS, int LD, bool LSE>
 __device__ __forceinline__ void few_way_out(const FewRowsParams& p, const float (*red)[16][LD], int tile, int first, int tokens, int id, int warp, int lane) {
     const int n0 = tile * p.tile_rows;
@@ -370,9 +371,12 @@ int few_rows_run(const GemmCall& g) {
     p.tile_rows = few_tile_rows(g.M, g.N);
     p.chunks = (g.K + FEW_CHUNK - 1) / FEW_CHUNK;
     p.stages = few_plan(g.M, g.N, g.K).stages;
-    if (few_tiles(g.M, g.N)) p.status = nullptr;   // it waits for nothing
-    else if (!few_make_map(p.tmap_x, g.a, g.K, g.M, g.lda, g.M <= 8 ? 8 : g.M <= 16 ? 16 : 32) || !few_make_map(p.tmap_w, g.b, g.K, g.N, g.ldb, p.tile_rows)) return -4;
-    else p.status = ob200_status_word_for_current_device();
+    p.status = nullptr;
+    if (!few_tiles(g.M, g.N)) {   // the other kernel copies by TMA, and waits
+        const int box = g.M <= 8 ? 8 : g.M <= 16 ? 16 : 32;
+        if (!few_make_map(p.tmap_x, g.a, g.K, g.M, g.lda, box) || !few_make_map(p.tmap_w, g.b, g.K, g.N, g.ldb, p.tile_rows)) return -4;
+        p.status = ob200_status_word_for_current_device();
+    }
     p.bias = g.bias;
     p.bias_bf16 = (const __nv_bfloat16*)g.bias_bf16;
     p.residual = (const __nv_bfloat16*)g.residual;

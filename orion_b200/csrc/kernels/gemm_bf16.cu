@@ -50,7 +50,10 @@ constexpr int GM_BK = 64;
 // columns) where a turn of the epilogue is a long chain of latencies: bias + GELU of 8192 x 4096 x 1024.  Eight for the loss: over a
 // short reduction the exponentials bound it (4096 x 16384 x 256: row maxima and sums 57 us in four warps, 44 in eight; over 1024 deep
 // no difference), and sixteen for its gradient take the stages that a deep one needs (2048 x 32000 x 1024: 475 us in eight, 486).
-__host__ __device__ constexpr int gm_epi_warps(int epi) { return epi == GM_EPI_ACT || epi == GM_EPI_ACT_SLOPE || epi == GM_EPI_ACT_ANY ? 16 : epi == GM_EPI_LSE || epi == GM_EPI_DLOGITS ? 8 : 4; }
+__host__ __device__ constexpr int gm_epi_warps(int epi) {
+    if (epi == GM_EPI_ACT || epi == GM_EPI_ACT_SLOPE || epi == GM_EPI_ACT_ANY) return 16;
+    return epi == GM_EPI_LSE || epi == GM_EPI_DLOGITS ? 8 : 4;
+}
 __host__ __device__ constexpr int gm_threads(int epi) { return 64 + 32 * gm_epi_warps(epi); }
 constexpr int GM_A_BYTES = GM_BM * 128;
 
@@ -58,8 +61,9 @@ constexpr int GM_A_BYTES = GM_BM * 128;
 template <int BN, int CG, int EPI>
 struct GemmCfg {
     static constexpr int STAGE_BYTES = GM_A_BYTES + BN / CG * 128;
-    static constexpr int STAGES = gm_epi_warps(EPI) == 16 ? (STAGE_BYTES == 49152 ? 3 : STAGE_BYTES == 32768 ? 5 : 6) : STAGE_BYTES == 49152 ? 4 : STAGE_BYTES == 32768 ? 6 : 8;
-    static constexpr int EPI_BYTES = gm_epi_warps(EPI) == 16 ? 16 * 4096 : 32768;   // per epilogue warp two slabs of 32 rows x 64 (x 128) bytes for the TMA stores
+    static constexpr bool WIDE = gm_epi_warps(EPI) == 16;
+    static constexpr int STAGES = STAGE_BYTES == 49152 ? (WIDE ? 3 : 4) : STAGE_BYTES == 32768 ? (WIDE ? 5 : 6) : WIDE ? 6 : 8;
+    static constexpr int EPI_BYTES = WIDE ? 16 * 4096 : 32768;   // per epilogue warp two slabs of 32 rows x 64 (x 128) bytes for the TMA stores
     static constexpr int SMEM = STAGES * STAGE_BYTES + EPI_BYTES + 1024 + 512;   // + alignment, barriers
     static constexpr int TMEM_COLS = 2 * BN < 32 ? 32 : 2 * BN;
 };
@@ -408,6 +412,7 @@ __global__ void __launch_bounds__(gm_threads(EPI), 1) gemm_bf16_kernel(const __g
     } else {
         // ------------------------------------------------------------ epilogue: thread = output row
         const int q = warp & 3;                       // tensor-memory lane group this warp may read
+        uint8_t* stage = epi_smem + (warp - 2) * (C::EPI_BYTES / gm_epi_warps(EPI));   // this warp's slabs
         uint32_t local = 0;
         uint32_t slab_i = 0;
         for (long long u = blockIdx.x / CG; u < units; u += gridDim.x / CG) {
@@ -422,7 +427,9 @@ __global__ void __launch_bounds__(gm_threads(EPI), 1) gemm_bf16_kernel(const __g
             const bool idle = part * kCols >= BN;   // a narrow tile has no columns for this warp
             const int m0w = (tm * CG + (int)rank) * GM_BM + q * 32;      // first row of this warp's 32
             bool ahead = false;
-            if constexpr (kAct) if (!idle) ahead = gm_residual_ahead<kSlope>(p, m0w, tn * BN + part * kCols, epi_smem + (warp - 2) * 4096, slab_i, ctl->res_full[warp - 2]);
+            if constexpr (kAct) {
+                if (!idle) ahead = gm_residual_ahead<kSlope>(p, m0w, tn * BN + part * kCols, stage, slab_i, ctl->res_full[warp - 2]);
+            }
             if (!mbar_wait_warp(&ctl->acc_full[ab], use & 1u, abort_flag)) {
                 if (!*abort_flag) { ctl->abort_flag = 1; if (p.status) atomicExch(p.status, OB200_ERR_WAIT_TMEM_FULL); }
                 if (ahead) {   // the residual's copy must have landed before the CTA leaves
@@ -434,19 +441,21 @@ __global__ void __launch_bounds__(gm_threads(EPI), 1) gemm_bf16_kernel(const __g
             const int m = m0w + lane;
             const int n0 = tn * BN;
             const uint32_t t_row = tmem_base + ((uint32_t)(q * 32) << 16) + ab * BN;
+            const uint32_t t_part = t_row + part * kCols;
+            const int n_part = n0 + part * kCols;
             if (idle) {
             } else if constexpr (kAct || EPI == GM_EPI_ACT_ANY) {
-                if (p.splits > 1) gm_epilogue_slab<kCols>(p, t_row + part * kCols, m, n0 + part * kCols, sp, p.M);
-                else if constexpr (EPI == GM_EPI_ACT_ANY) gm_epilogue_act_any<kCols>(p, t_row + part * kCols, m, m0w, n0 + part * kCols, lane, epi_smem + (warp - 2) * 4096);
-                else if (!gm_epilogue_act<kCols, kSlope>(p, t_row + part * kCols, m, m0w, n0 + part * kCols, lane, epi_smem + (warp - 2) * 4096, slab_i, ctl->res_full[warp - 2], abort_flag)) {
+                if (p.splits > 1) gm_epilogue_slab<kCols>(p, t_part, m, n_part, sp, p.M);
+                else if constexpr (EPI == GM_EPI_ACT_ANY) gm_epilogue_act_any<kCols>(p, t_part, m, m0w, n_part, lane, stage);
+                else if (!gm_epilogue_act<kCols, kSlope>(p, t_part, m, m0w, n_part, lane, stage, slab_i, ctl->res_full[warp - 2], abort_flag)) {
                     if (!*abort_flag) { ctl->abort_flag = 1; if (p.status) atomicExch(p.status, OB200_ERR_WAIT_FULL); }
                     break;
                 }
             } else if constexpr (EPI == GM_EPI_DUAL) {
                 if (cut.splits > 1 && !w.second) gm_epilogue_slab<BN>(p, t_row, m, n0, sp, cut.rows);
-                else gm_epilogue_dual<BN>(p, w.second, t_row, m, m0w, n0, lane, epi_smem + (warp - 2) * 8192, slab_i);
-            } else if constexpr (EPI == GM_EPI_LSE) gm_epilogue_lse<kCols>(p, t_row + part * kCols, m, n0 + part * kCols);
-            else if constexpr (EPI == GM_EPI_DLOGITS) gm_epilogue_dlogits<kCols>(p, t_row + part * kCols, m, m0w, n0 + part * kCols, lane, epi_smem + (warp - 2) * 4096, slab_i);
+                else gm_epilogue_dual<BN>(p, w.second, t_row, m, m0w, n0, lane, stage, slab_i);
+            } else if constexpr (EPI == GM_EPI_LSE) gm_epilogue_lse<kCols>(p, t_part, m, n_part);
+            else if constexpr (EPI == GM_EPI_DLOGITS) gm_epilogue_dlogits<kCols>(p, t_part, m, m0w, n_part, lane, stage, slab_i);
             else {
             const bool to_slab = p.splits > 1;
             const bool row_ok = m < p.M;
@@ -529,7 +538,7 @@ __global__ void __launch_bounds__(gm_threads(EPI), 1) gemm_bf16_kernel(const __g
                     // stores), then one TMA store per slab: 64 bfloat16 or 32 float32 columns.  Two slabs alternate; before a
                     // slab is rewritten the store issued from it two slabs ago must have read it.
                     const int half = p.out_f32 ? 0 : ((c0 >> 5) & 1);
-                    uint8_t* slab = epi_smem + (warp - 2) * 8192 + (slab_i & 1) * 4096;
+                    uint8_t* slab = stage + (slab_i & 1) * 4096;
                     if (half == 0) {
                         if (lane == 0) bulk_wait_group_read<1>();
                         __syncwarp();
@@ -620,7 +629,8 @@ __global__ void __launch_bounds__(gm_threads(EPI), 1) gemm_bf16_kernel(const __g
 __global__ void __launch_bounds__(256) gemm_splitk_finish_kernel(const float* __restrict__ slabs, void* c,
                                                                  const float* __restrict__ bias,
                                                                  const __nv_bfloat16* __restrict__ bias_bf16,
-                                                                 const __nv_bfloat16* __restrict__ residual, const float* addend, const float* factor, int splits, int batch, int nb_inner,
+                                                                 const __nv_bfloat16* __restrict__ residual, const float* addend,
+                                                                 const float* factor, int splits, int batch, int nb_inner,
                                                                  int M, int N, long long ldc, long long c_si, long long c_so,
                                                                  int out_f32, float alpha) {
     const long long per_split = (long long)batch * M * N;
@@ -976,7 +986,7 @@ int gemm_bf16_run(const GemmCall& g) {
     p.kblocks = (K + GM_BK - 1) / GM_BK;
     const GemmPlan pl = gm_plan(M, N, K, batch_ll, tri, plan, num_ctas, gm_split_rule(epi));
     const int bn = pl.bn, cg = pl.cg;
-    int splits = g.splits > 0 ? g.splits : pl.splits;
+    int splits = pl.splits;
     p.tiles_m = (M + cg * GM_BM - 1) / (cg * GM_BM);
     p.tiles_n = (N + bn - 1) / bn;
     const long long tiles = batch_ll * p.tiles_m * p.tiles_n;
@@ -1005,7 +1015,8 @@ int gemm_bf16_run(const GemmCall& g) {
         if (g.all) {   // the same boxes as the packed operand's
             p.live_all = g.live_k ? K : M;
             if (g.live_k ? !b_mn : epi == GM_EPI_ACC || a_mn) return -1;
-            if (!(g.live_k ? gm_make_map(p.tmap_all, g.all, N, K, g.ld_all, 1, 0, 1, 0, 64, GM_BK) : gm_make_map(p.tmap_all, g.all, K, M, g.ld_all, 1, 0, 1, 0, GM_BK, GM_BM)))
+            if (!(g.live_k ? gm_make_map(p.tmap_all, g.all, N, K, g.ld_all, 1, 0, 1, 0, 64, GM_BK)
+                           : gm_make_map(p.tmap_all, g.all, K, M, g.ld_all, 1, 0, 1, 0, GM_BK, GM_BM)))
                 return -4;
         }
     }
@@ -1016,7 +1027,8 @@ int gemm_bf16_run(const GemmCall& g) {
                              (batch_outer == 1 || (c_so * es) % 16 == 0);
         static const bool tma_off = [] { const char* e = getenv("ORION_GEMM_TMA_STORE"); return e && e[0] == '0'; }();
         if (epi == GM_EPI_ACT || epi == GM_EPI_DLOGITS) {   // by slabs of 32 rows
-            if (epi == GM_EPI_ACT) epi = !aligned || g.bias || ((uintptr_t)g.bias_bf16 | (uintptr_t)residual) % 16 ? GM_EPI_ACT_ANY : g.e.slope ? GM_EPI_ACT_SLOPE : GM_EPI_ACT;
+            if (epi == GM_EPI_ACT && (!aligned || g.bias || ((uintptr_t)g.bias_bf16 | (uintptr_t)residual) % 16)) epi = GM_EPI_ACT_ANY;
+            else if (epi == GM_EPI_ACT && g.e.slope) epi = GM_EPI_ACT_SLOPE;
             const int slab_cols = epi == GM_EPI_ACT_SLOPE ? 16 : 32;
             if (p.splits == 1 && ((epi != GM_EPI_ACT_ANY && !gm_make_slab_map(p.tmap_c, c, M, N, ldc, slab_cols)) ||
                                   (epi != GM_EPI_ACT_ANY && residual && !gm_make_slab_map(p.tmap_res, residual, M, N, N, slab_cols)) ||
@@ -1076,7 +1088,8 @@ int gemm_bf16_run(const GemmCall& g) {
     long long blocks = (elems + 255) / 256;
     if (blocks > 4LL * num_ctas) blocks = 4LL * num_ctas;
     OB200_ELASTIC_HBM(gemm_splitk_finish_kernel, 4);
-    gemm_splitk_finish_kernel<<<(int)blocks, 256, 0, st>>>(p.slabs, c, g.bias, p.bias_bf16, p.residual, epi == GM_EPI_ACC ? p.e.addend : nullptr, epi == GM_EPI_ACC ? p.e.factor : nullptr, p.splits, p.batch,
+    gemm_splitk_finish_kernel<<<(int)blocks, 256, 0, st>>>(p.slabs, c, g.bias, p.bias_bf16, p.residual, epi == GM_EPI_ACC ? p.e.addend : nullptr,
+                                                           epi == GM_EPI_ACC ? p.e.factor : nullptr, p.splits, p.batch,
                                                            p.nb_inner, M, N, ldc, c_si, c_so, p.out_f32, g.alpha);
     return (int)cudaGetLastError();
 }
@@ -1171,7 +1184,8 @@ int gemm_bf16_run_dual(const GemmCall& a, const GemmCall& b) {
     const long long tiles = (long long)p.tiles_m * p.tiles_n * splits + (long long)p.second.tiles_m * p.second.tiles_n;
     if (tiles > 0x3fffffffLL) return -1;
     const long long most = a.num_ctas / cg;
-    annotate_launch(1, 2.0 * ((double)a.M * a.N * a.K + (double)b.M * b.N * b.K), 2.0 * ((double)a.M * a.K + (double)a.K * a.N + (double)b.M * b.K + (double)b.K * b.N));
+    annotate_launch(1, 2.0 * ((double)a.M * a.N * a.K + (double)b.M * b.N * b.K),
+                    2.0 * ((double)a.M * a.K + (double)a.K * a.N + (double)b.M * b.K + (double)b.K * b.N));
     const int grid = (int)(tiles < most ? tiles : most) * cg;
     const int rc = cg == 2 ? gm_launch<256, 2, GM_EPI_DUAL>(p, grid, (cudaStream_t)a.stream) : gm_launch<256, 1, GM_EPI_DUAL>(p, grid, (cudaStream_t)a.stream);
     if (rc || (splits == 1 && !recut)) return rc;

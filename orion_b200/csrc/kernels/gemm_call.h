@@ -57,7 +57,6 @@ struct GemmCall {
     bool stream_slabs = false;      // split-K partial matrices in the stream's own scratch; otherwise in `slabs` (none: no split)
     float* slabs = nullptr;
     size_t slab_bytes = 0;
-    int splits = 0;                 // parts of the reduction; 0: by the plan
     // Packed rows (GM_EPI_ACC, GM_EPI_LSE, GM_EPI_DLOGITS and both products of a dual launch): only the first *live rows of A count, or with
     // live_k the first *live indices of the reduction.  Tiles and k-blocks behind them are left out (their outputs unwritten); *live may be
     // 0.  `all`: what stands for the packed operand (A of the losses, B of a product with live_k) where *live is everything, M or K.
@@ -91,7 +90,8 @@ int gemm_bf16_run_dual(const GemmCall& first, const GemmCall& second);
 // Bytes of partial matrices that the split of a product with this epilogue wants; 0 where it is not split.
 size_t gemm_bf16_slab_bytes(int M, int N, int K, int epi);
 
-// The same for few rows (few_rows.cu; up to 32, more where all tiles are resident at once): GM_EPI_ACT, and GM_EPI_LSE with `few_rows_parts` parts a row instead of N / 128.
+// The same for few rows (few_rows.cu; up to 32, more where all tiles are resident at once): GM_EPI_ACT, and GM_EPI_LSE with
+// `few_rows_parts` parts a row instead of N / 128.
 bool few_rows_fit(int M, int N, int K);
 int few_rows_parts(int M, int V);
 int few_rows_run(const GemmCall& call);

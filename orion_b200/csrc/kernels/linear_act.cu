@@ -369,7 +369,8 @@ extern "C" int ob200_linear_act_backward_bf16(const void* dy, const void* slope,
                 rc = launch_pdl(act_colsum_kernel<float>, blocks, (unsigned)LA_THREADS, st, (const float*)partial, ranges, N, factor, (float*)dbias);
             } else {
                 OB200_ELASTIC_HBM(act_colsum_kernel<__nv_bfloat16>, 8);
-                rc = launch_pdl(act_colsum_kernel<__nv_bfloat16>, blocks, (unsigned)LA_THREADS, st, (const float*)partial, ranges, N, factor, (__nv_bfloat16*)dbias);
+                rc = launch_pdl(act_colsum_kernel<__nv_bfloat16>, blocks, (unsigned)LA_THREADS, st, (const float*)partial, ranges, N, factor,
+                                (__nv_bfloat16*)dbias);
             }
             if (rc) return rc;
         }

@@ -210,7 +210,8 @@ __global__ void __launch_bounds__(CE_PACK_THREADS) ce_pack_kernel(const CePack p
     }
 }
 // dx from its packed rows; zeros for the rows that do not count.  One warp a row.
-__global__ void __launch_bounds__(CE_THREADS) ce_unpack_kernel(const __nv_bfloat16* packed, const int* slot, __nv_bfloat16* __restrict__ dx, long long rows, int H) {
+__global__ void __launch_bounds__(CE_THREADS) ce_unpack_kernel(const __nv_bfloat16* packed, const int* slot, __nv_bfloat16* __restrict__ dx,
+                                                               long long rows, int H) {
     pdl_wait();
     pdl_launch_dependents();
     const int lane = threadIdx.x & 31;
