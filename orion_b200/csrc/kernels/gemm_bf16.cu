@@ -1109,14 +1109,17 @@ static bool gm_make_c_map(unsigned char* out, const GemmCall& g) {
 // Whether two products run as one launch, and the split of the first one's reduction: 0 for no.  The fewest k-blocks of 64 on the CTA pair
 // that has most of them, eight added for a tile's way out, and for a split the second launch and its partial matrices at 0.45 us a
 // k-block and 6 TB/s.  Planned for the device, so that the order of the sums is the same for every CTA count.
-// Outputs of at most 128 columns have narrower tiles in launches of their own; one of 136 is better in one tile of 256 than in two of
+// A first product of at most 128 rows (then the second one's reduction has two blocks at most, and its tiles' way out is all there is) runs
+// in single CTAs: 16 x 512 x 512 with GELU, all launches of
+// both directions, 18.7 -> 14.4 us, loss over 128 x 32000 x 1024 100 -> 92.  Otherwise pairs:
+// outputs of at most 128 columns have narrower tiles in launches of their own; one of 136 is better in one tile of 256 than in two of
 // 128 that read the other operand twice (gradient products of 6437 x 13042 x 136: 143 us in two launches, 77 in one).
+static int gm_dual_ctas(const GemmCall& a) { return a.M <= GM_BM ? 1 : 2; }
 int gemm_bf16_dual_splits(const GemmCall& a, const GemmCall& b) {
-    for (const GemmCall* g : {&a, &b})
-        if (g->M <= GM_BM || g->N <= 128 || g->N % 8) return 0;
-    const int pairs = ob200_plan_sm_count() / 2;
-    if (pairs < 1) return 0;
-    auto tiles = [](const GemmCall& g) { return (((long long)g.M + 255) / 256) * (((long long)g.N + 255) / 256); };
+    const int cg = gm_dual_ctas(a), pairs = ob200_plan_sm_count() / cg;   // or single CTAs
+    if (pairs < 1 || a.N % 8 || b.N % 8) return 0;
+    if (cg == 2 && (b.M <= GM_BM || a.N <= 128 || b.N <= 128)) return 0;
+    auto tiles = [cg](const GemmCall& g) { return (((long long)g.M - 1) / (cg * GM_BM) + 1) * (((long long)g.N + 255) / 256); };
     const long long ta = tiles(a), tb = tiles(b), ka = (a.K + 63) / 64, kb = (b.K + 63) / 64;
     int best = 1;
     double best_cost = 0.0;
@@ -1141,7 +1144,7 @@ int gemm_bf16_run_dual(const GemmCall& a, const GemmCall& b) {
     splits = (kblocks + per_split - 1) / per_split;   // every split owns at least one k-block
     const bool recut = a.live && a.M > 256;   // fewer rows may be cut into more parts
     if ((splits > 1 || recut) && (!a.slabs || (size_t)splits * a.M * a.N * sizeof(float) > a.slab_bytes)) return -3;
-    const int cg = a.num_ctas < 2 ? 1 : 2, tile_m = cg * GM_BM;   // one CTA: tiles of 128 rows, the same sums
+    const int cg = a.num_ctas < 2 ? 1 : gm_dual_ctas(a), tile_m = cg * GM_BM;   // one CTA: tiles of 128 rows, the same sums
     GemmParamsDual p;
     memset(&p, 0, sizeof p);
     p.status = ob200_status_word_for_current_device();

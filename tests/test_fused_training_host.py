@@ -129,7 +129,7 @@ def test_entry_points_refuse_bad_arguments_without_a_gpu(K):
         assert back(**bad) == -1, bad
     for bad in (dict(dy=a + 2), dict(dx=a + 2), dict(dw=a + 8), dict(ldx=9)):
         assert back(**bad) == -2, bad
-    assert back(act=2, slope=a, ld_slope=8, nbytes=0) == -3 and back(db=a, ws=None) == -3
+    assert back(act=2, slope=a, ld_slope=8, nbytes=0) == -3 and back(db=a, M=200, ws=None) == -3
     assert back(M=0, dw=None) == 0   # dw, a sum over nothing, would be zeroed
 
     def drop(x=a, y=a, n=8, p=0.1, rng=a, dtype=1, ctas=1):
