@@ -81,7 +81,7 @@ inline long long gemm_longest_share(long long pairs, long long a, long long ca, 
     return longest;
 }
 
-// Two products in one launch of CTA pairs, 256 x 256 tiles, so that the last round of tiles is one and not two: no batch, bias or residual,
+// Two products in one launch of CTA pairs, 256 x 256 tiles (of single CTAs, 128 x 256, where the first one has 128 rows at most), so that the last round of tiles is one and not two: no batch, bias or residual,
 // one alpha, epilogue GM_EPI_ACC (the addend is the first one's), rows of C 16-byte multiples.  `splits`: into how many parts the first
 // one's reduction is cut for that, 0 where the products are too narrow.
 int gemm_bf16_dual_splits(const GemmCall& first, const GemmCall& second);

@@ -29,6 +29,7 @@ extern "C" int ob200_plan_sm_count(void);
 namespace ob200 {
 
 constexpr int CE_THREADS = 256, CE_PACK_THREADS = 512;
+constexpr int CE_IN_PLACE = 128;   // rows of one tile: fewer of them cost the same
 constexpr float CE_LOG2E = 1.4426950408889634f;
 
 // lse and loss of every row from its parts.  A CTA has C rows; group g of G = 1024 / C takes parts g, g + G, ..., eight at a time in
@@ -131,7 +132,8 @@ __global__ void __launch_bounds__(1024) ce_total_kernel(const float* __restrict_
 // that do not count (the prompt of an answer, the words that a masked model is not asked for) cost no products, and whatever they hold
 // (0 times infinity) reaches none.  A CTA has consecutive rows; it counts those before them and all of them itself, which reads the
 // targets once per CTA and saves a launch.  Where every row counts x is not copied: the products take x itself.  Rows that do not
-// count become zeros where the last 64-row block of a reduction reads them.
+// count become zeros where the last 64-row block of a reduction reads them.  Up to 128 rows, one tile, there is nothing to spare and the
+// rows stay in place, which saves the gradients' way back (ce_unpack_kernel; 64 x 1000 x 64 with gradients 91 -> 86 us on the host).
 // order: row of every slot, slot: slot of every row, or -1.  For the gradients also per slot the label and (lse * log2(e), coefficient), and
 // the factor of both: an upstream gradient that is one number, and the mean's divisor, multiply the products of the rounded dl; in the
 // coefficient they would make every row's largest term, the label's, off by the same rounding.  A label outside the vocabulary makes the
@@ -147,6 +149,7 @@ struct CePack {
     float* factor;
     long long ldx, ignore_index;
     int rows, V, H, grad_per_row;
+    int in_place;                      // every row keeps its place, those that do not count become zeros
 };
 __global__ void __launch_bounds__(CE_PACK_THREADS) ce_pack_kernel(const CePack p) {
     pdl_wait();
@@ -189,8 +192,8 @@ __global__ void __launch_bounds__(CE_PACK_THREADS) ce_pack_kernel(const CePack p
         }
         before += taken;
         // a row that does not count is the (r - rank)-th of those
-        const int slot = counts ? rank : p.rows - 1 - (int)(r - rank);
-        sh_slot[tid] = counts ? slot : r < r1 && slot < zeros_to ? ~slot : INT_MIN;
+        const int slot = p.in_place ? (int)r : counts ? rank : p.rows - 1 - (int)(r - rank);
+        sh_slot[tid] = counts ? slot : r < r1 && (p.in_place || slot < zeros_to) ? ~slot : INT_MIN;
         if (r < r1) {
             p.label[slot] = counts ? t : -1;
             if (p.order) p.order[slot] = (int)r;
@@ -198,7 +201,7 @@ __global__ void __launch_bounds__(CE_PACK_THREADS) ce_pack_kernel(const CePack p
             if (p.row) p.row[slot] = make_float2(p.lse[r] * CE_LOG2E, !counts ? 0.f : t >= 0 && t < p.V ? (p.grad_per_row ? p.grad[r] : 1.f) : NAN);
         }
         __syncthreads();
-        if (all == p.rows) continue;
+        if (all == p.rows && !p.in_place) continue;
         for (int i = warp; i < CE_PACK_THREADS && base + i < r1; i += W) {
             const int to = sh_slot[i];
             if (to == INT_MIN) continue;
@@ -273,7 +276,7 @@ struct CeBackwardSpace {
         packed = ce_round((size_t)rows * H * 2);
         dl = ce_round((size_t)rows * piece * 2);
         acc = want_dx && piece < V ? ce_round((size_t)rows * H * sizeof(float)) : 0;
-        dx = want_dx ? packed : 0;
+        dx = want_dx && rows > CE_IN_PLACE ? packed : 0;
         slabs = 0;
         const int last = V - (V - 1) / piece * piece;   // columns of the last piece
         for (int v : {piece < V ? piece : V, last}) {
@@ -297,8 +300,8 @@ using namespace ob200;
 // Parts of a row that a forward pass writes; the workspace has room for those of either kernel.
 static int ce_parts(int rows, int V, int H) { return few_rows_fit(rows, V, H) ? few_rows_parts(rows, V) : (V + 127) / 128; }
 
-// Whether a forward pass packs the rows that count: where it can spare a tile of 128.
-static bool ce_packs(int rows, int V, int H) { return rows > 128 && !few_rows_fit(rows, V, H); }
+// Whether a forward pass packs the rows that count: where it can spare a tile.
+static bool ce_packs(int rows, int V, int H) { return rows > CE_IN_PLACE && !few_rows_fit(rows, V, H); }
 
 struct CeForwardSpace {
     size_t part, label_logit, packed, label, order, total;
@@ -433,6 +436,8 @@ extern "C" int ob200_linear_cross_entropy_backward(const void* x, const void* w,
     k.lse = lse; k.grad = grad; k.grad_per_row = grad_per_row; k.count = count;
     k.packed = packed; k.label = label; k.slot = slot; k.live = live; k.row = row; k.factor = factor;
     k.rows = rows; k.V = V; k.H = H;
+    const bool packs = rows > CE_IN_PLACE;
+    k.in_place = !packs;
     int rc = ce_pack(k, num_ctas, st);
     if (rc) return rc;
     for (int v0 = 0; v0 < V; v0 += space.piece) {
@@ -445,8 +450,9 @@ extern "C" int ob200_linear_cross_entropy_backward(const void* x, const void* w,
         g.a = packed; g.b = wp; g.c = dl;
         g.M = rows; g.N = nv; g.K = H;
         g.lda = H; g.ldb = ldw; g.ldc = space.piece;
-        g.live = live;
-        g.all = x; g.ld_all = ldx;
+        g.live = packs ? live : nullptr;
+        g.all = packs ? x : nullptr;
+        g.ld_all = ldx;
         g.epi = GM_EPI_DLOGITS;
         g.e.target = label;
         g.e.col0 = v0;
@@ -467,10 +473,10 @@ extern "C" int ob200_linear_cross_entropy_backward(const void* x, const void* w,
         gx.e.factor = factor;
         gx.out_f32 = last ? 0 : 1;
         gx.all = nullptr;
-        gx.c = last ? (void*)packed_dx : (void*)acc;
+        gx.c = !last ? (void*)acc : packs ? (void*)packed_dx : dx;
         // dw[v, h] = sum_t dl[t, v] x[t, h]
         gw.a_mn = 1;
-        gw.live_k = 1;
+        gw.live_k = packs;
         gw.b = packed; gw.ldb = H;
         gw.M = nv; gw.K = rows;
         gw.epi = GM_EPI_ACC;
@@ -484,7 +490,7 @@ extern "C" int ob200_linear_cross_entropy_backward(const void* x, const void* w,
         }
         if (rc) return rc;
     }
-    if (!dx) return 0;
+    if (!dx || !packs) return 0;
     const long long want = ((long long)rows + CE_THREADS / 32 - 1) / (CE_THREADS / 32), cap = (long long)num_ctas * 8;
     OB200_ELASTIC_HBM(ce_unpack_kernel, 8);
     return launch_pdl(ce_unpack_kernel, (unsigned)(want < cap ? want : cap), (unsigned)CE_THREADS, st, (const __nv_bfloat16*)packed_dx, (const int*)slot,
