@@ -81,9 +81,10 @@ inline long long gemm_longest_share(long long pairs, long long a, long long ca, 
     return longest;
 }
 
-// Two products in one launch of CTA pairs, 256 x 256 tiles (of single CTAs, 128 x 256, where the first one has 128 rows at most), so that the last round of tiles is one and not two: no batch, bias or residual,
-// one alpha, epilogue GM_EPI_ACC (the addend is the first one's), rows of C 16-byte multiples.  `splits`: into how many parts the first
-// one's reduction is cut for that, 0 where the products are too narrow.
+// Two products in one launch of CTA pairs, 256 x 256 tiles (of single CTAs, 128 x 256, where the first one has at most 128 rows), so that
+// the last round of tiles is one and not two: no batch, bias or residual, one alpha, epilogue GM_EPI_ACC (the addend is the first one's),
+// rows of C 16-byte multiples.  `splits`: into how many parts the first one's reduction is cut for that, 0 where the products are too
+// narrow.  `packed`: with `live`, whose rows may be cut into more parts.
 int gemm_bf16_dual_splits(const GemmCall& first, const GemmCall& second);
 size_t gemm_bf16_dual_slab_bytes(const GemmCall& first, const GemmCall& second, bool packed = false);
 int gemm_bf16_run_dual(const GemmCall& first, const GemmCall& second);
