@@ -99,6 +99,14 @@ __device__ __forceinline__ void gelu_slope_pair(float& a0, float& a1, float& s0,
     split_f32x2(fma_f32x2(mul_f32x2(a, f32x2(kDensity, kDensity)), e, cdf), s0, s1);
     split_f32x2(fma_f32x2(nx, tail, f32x2(fmaxf(a0, 0.f), fmaxf(a1, 0.f))), a0, a1);
 }
+// max(a, 0) and its slope.  What is not a number stays one in both, as behind GELU: fmaxf would give 0, and a step that has diverged
+// would look healthy behind the layer.
+__device__ __forceinline__ float relu(float a) {
+    float r;
+    asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(r) : "f"(a));
+    return r;
+}
+__device__ __forceinline__ float relu_slope(float a) { return a > 0.f ? 1.f : a <= 0.f ? 0.f : a; }
 // One value: act(a) and its slope; 0 none, 1 ReLU, 2 GELU.
 __device__ __forceinline__ float act_slope(float a, int act, float& slope) {
     if (act == 2) {
@@ -106,8 +114,8 @@ __device__ __forceinline__ float act_slope(float a, int act, float& slope) {
         gelu_slope_pair(a, b, slope, unused);
         return a;
     }
-    slope = act == 1 && !(a > 0.f) ? 0.f : 1.f;
-    return act == 1 ? fmaxf(a, 0.f) : a;
+    slope = act == 1 ? relu_slope(a) : 1.f;
+    return act == 1 ? relu(a) : a;
 }
 
 }  // namespace ob200

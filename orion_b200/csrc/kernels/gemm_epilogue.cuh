@@ -68,10 +68,10 @@ __device__ __forceinline__ void gm_act_slope(float (&f)[W], int act, uint8_t* sl
             if (act == 2) {
                 gelu_slope_pair(a0, a1, s0, s1);
             } else {
-                s0 = a0 > 0.f ? 1.f : 0.f;
-                s1 = a1 > 0.f ? 1.f : 0.f;
-                a0 = fmaxf(a0, 0.f);
-                a1 = fmaxf(a1, 0.f);
+                s0 = relu_slope(a0);
+                s1 = relu_slope(a1);
+                a0 = relu(a0);
+                a1 = relu(a1);
             }
             w[e] = gm_pack_half(s0, s1);
         }
@@ -160,7 +160,7 @@ __device__ __forceinline__ bool gm_epilogue_act(const GemmParams& p, uint32_t t_
             for (int j = 0; j < W; j += 2) gelu_pair(f[j], f[j + 1]);
         } else if (act == 1) {
 #pragma unroll
-            for (int j = 0; j < W; j++) f[j] = fmaxf(f[j], 0.f);
+            for (int j = 0; j < W; j++) f[j] = relu(f[j]);
         }
         if (threshold) {
             drop_apply<W>(key, group, threshold, p.e.drop_scale, f);
@@ -217,7 +217,7 @@ __device__ __forceinline__ void gm_epilogue_act_any(const GemmParams& p, uint32_
             for (int j = 0; j < 32; j += 2) gelu_pair(f[j], f[j + 1]);
         } else if (p.e.act == 1) {
 #pragma unroll
-            for (int j = 0; j < 32; j++) f[j] = fmaxf(f[j], 0.f);
+            for (int j = 0; j < 32; j++) f[j] = relu(f[j]);
         }
         if (p.e.drop_threshold) {
             const uint32_t mask = drop_mask<32>(key, (unsigned long long)index, p.e.drop_threshold);

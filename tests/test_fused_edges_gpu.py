@@ -1,0 +1,54 @@
+"""The fused linear layer, counter-based dropout and the loss without logits where values and calls are at their edges: numbers that are not
+numbers, tails, certain answers, derivatives of other kinds, SM quotas.  u = 2^-8 is half a step of bfloat16."""
+import math
+
+import pytest
+import torch
+
+from tests.test_fused_training_gpu import BF, U, act64, rng_of, within
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ops(built):
+    from orion_b200 import torch_ops
+    return torch_ops.load()
+
+
+@pytest.fixture(autouse=True)
+def status(built):
+    yield
+    from orion_b200 import kernels
+    assert kernels.read_status() == 0
+
+
+# few rows straight to registers and through the ring, tiles, a split reduction, odd widths of each
+PATHS = [(3, 64, 64), (16, 20000, 512), (600, 1024, 4096), (600, 1023, 4096), (300, 1000, 2056), (2050, 520, 72), (130, 73, 136), (33, 250, 4104), (5, 257, 1024)]
+
+
+@pytest.mark.parametrize("act", ["none", "relu", "gelu"])
+@pytest.mark.parametrize("M,N,K", PATHS)
+def test_not_a_number_stays_one_behind_every_activation(ops, M, N, K, act):
+    """A row of x, a row of w and an entry of the bias that are not numbers: every output that they reach is none either and the others are
+    what they were; so with the gradients, whose dz is none there: rows of dx, rows of dw and entries of the bias's."""
+    torch.manual_seed(M + N)
+    x, w, b = torch.randn(M, K, device="cuda").to(BF), (torch.randn(N, K, device="cuda") / math.sqrt(K)).to(BF), torch.randn(N, device="cuda").to(BF)
+    dy = torch.randn(M, N, device="cuda").to(BF)
+    clean = ops.linear_act(x, w, b, None, act)
+    row, col, entry = M // 2, N // 3, N - 1
+    for what in ("x", "w", "bias"):
+        bad = {"x": x.clone(), "w": w.clone(), "bias": b.clone()}
+        bad[what][row if what == "x" else col if what == "w" else entry] = float("nan")
+        hit = torch.zeros(M, N, dtype=torch.bool, device="cuda")
+        hit[row if what == "x" else slice(None), slice(None) if what == "x" else col if what == "w" else entry] = True
+        leaves = [bad[k].requires_grad_(True) for k in ("x", "w", "bias")]
+        for y in (ops.linear_act(*(t.detach() for t in leaves), None, act), ops.linear_act(*leaves, None, act)):
+            assert torch.equal(y.isnan(), hit) and torch.equal(y[~hit], clean[~hit])
+        if act == "none":   # dz is dy, whatever z holds
+            continue
+        dx, dw, db = torch.autograd.grad(y, leaves, dy)
+        rows, cols = hit.any(1), hit.any(0)
+        assert dx[rows].isnan().all() and dw[cols].isnan().all() and torch.equal(db.isnan(), cols)
+        if what == "bias":   # x and w are sound: nothing else is touched
+            assert not dw[~cols].isnan().any()
