@@ -833,6 +833,13 @@ at::Tensor as_dense(const at::Tensor& t) {
 }
 at::Tensor workspace(int64_t bytes, const at::Tensor& like) { return at::empty({bytes}, like.options().dtype(at::kByte)); }
 bool given(const c10::optional<at::Tensor>& t) { return t.has_value() && t->defined(); }
+// Whether something looks on: a backward pass, or a forward-mode derivative, whose tangent needs no requires_grad.  The autograd function
+// refuses the latter; passing it by would leave the output without a tangent, which reads as a derivative of zero.
+bool differentiated(std::initializer_list<const at::Tensor*> tensors) {
+    for (const at::Tensor* t : tensors)
+        if (t && t->defined() && ((at::GradMode::is_enabled() && t->requires_grad()) || t->_fw_grad(/*level=*/0).defined())) return true;
+    return false;
+}
 // The gradients are plain results, not functions of the inputs: a second derivative would silently be missing a term.
 void refuse_double_backward(const char* op) {
     TORCH_CHECK(!at::GradMode::is_enabled(), op, " cannot be differentiated twice (create_graph=True)");
@@ -953,9 +960,7 @@ at::Tensor linear_act_op(const at::Tensor& x, const at::Tensor& w, const c10::op
 }
 at::Tensor linear_act_autograd(const at::Tensor& x, const at::Tensor& w, const c10::optional<at::Tensor>& bias, const c10::optional<at::Tensor>& residual,
                                c10::string_view act, double p, const c10::optional<at::Tensor>& rng, int64_t site) {
-    const bool grad = at::GradMode::is_enabled() &&
-                      (x.requires_grad() || w.requires_grad() || (given(bias) && bias->requires_grad()) || (given(residual) && residual->requires_grad()));
-    if (!grad) return linear_act_op(x, w, bias, residual, act, p, rng, site);
+    if (!differentiated({&x, &w, given(bias) ? &*bias : nullptr, given(residual) ? &*residual : nullptr})) return linear_act_op(x, w, bias, residual, act, p, rng, site);
     const int code = LinearAct::act_code(act);
     LinearAct::check_args(x, w, bias, residual, p, rng, site);
     return LinearAct::apply(x, w, bias, residual, code, p, rng, site);

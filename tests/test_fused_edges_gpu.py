@@ -52,3 +52,22 @@ def test_not_a_number_stays_one_behind_every_activation(ops, M, N, K, act):
         assert dx[rows].isnan().all() and dw[cols].isnan().all() and torch.equal(db.isnan(), cols)
         if what == "bias":   # x and w are sound: nothing else is touched
             assert not dw[~cols].isnan().any()
+
+
+def test_forward_mode_derivatives_are_refused(ops):
+    """A tangent may not vanish: whichever argument carries one, in grad mode or not, the call is refused."""
+    import torch.autograd.forward_ad as fw
+    torch.manual_seed(1)
+    x, w, b, r = (torch.randn(*s, device="cuda").to(BF) for s in ((8, 64), (16, 64), (16,), (8, 16)))
+    target, rng = torch.zeros(8, dtype=torch.int64, device="cuda"), rng_of(1, 2)
+    calls = [(lambda x, w, b, r: ops.linear_act(x, w, b, r, "gelu"), 4), (lambda x, w, b, r: ops.dropout(x, 0.5, rng), 1),
+             (lambda x, w, b, r: ops.linear_cross_entropy(x, w, target), 2)]
+    with fw.dual_level():
+        for call, n in calls:
+            for i in range(n):
+                args = [x, w, b, r]
+                args[i] = fw.make_dual(args[i], torch.ones_like(args[i]))
+                for grad in (True, False):
+                    with torch.set_grad_enabled(grad), pytest.raises(RuntimeError, match="jvp|forward"):
+                        call(*args)
+    assert ops.linear_act(x, w, b, r, "gelu").shape == (8, 16)
