@@ -449,6 +449,8 @@ __global__ void __launch_bounds__(gm_threads(EPI), 1) gemm_bf16_kernel(const __g
                 else if constexpr (EPI == GM_EPI_ACT_ANY) gm_epilogue_act_any<kCols>(p, t_part, m, m0w, n_part, lane, stage);
                 else if (!gm_epilogue_act<kCols, kSlope>(p, t_part, m, m0w, n_part, lane, stage, slab_i, ctl->res_full[warp - 2], abort_flag)) {
                     if (!*abort_flag) { ctl->abort_flag = 1; if (p.status) atomicExch(p.status, OB200_ERR_WAIT_FULL); }
+                    // as above: the slab that it gave up waiting for
+                    mbar_wait_landed(&ctl->res_full[warp - 2][slab_i & 1], (slab_i >> 1) & 1, clock64());
                     break;
                 }
             } else if constexpr (EPI == GM_EPI_DUAL) {
