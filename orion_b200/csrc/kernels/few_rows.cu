@@ -133,8 +133,10 @@ __device__ __forceinline__ void few_way_out(const FewRowsParams& p, const float 
 // Sixteen warps share a tile's reduction, four k-blocks of 32 (two of them for 32 tokens) under way in each.  There is no ring to fill and no copy to wait for, so
 // a launch of one or two tiles an SM is over sooner: 1024 x 4096 7.8 -> 5.9 us.  More than 32 tokens are groups of 32, each with tiles of
 // its own: w is then read from L2 once a group.
+// CTAs an SM: what the launch bound, the quota's cut and the grid go by.  One of 9 to 16 tokens has the registers of two (110 a thread).
+constexpr int few_resident(int nt) { return nt == 2 ? 1 : 2; }
 template <int NT, bool LSE>
-__global__ void __launch_bounds__(FEW_CONSUMERS * 32, NT == 2 ? 1 : 2) few_tiles_kernel(const __grid_constant__ FewRowsParams p) {
+__global__ void __launch_bounds__(FEW_CONSUMERS * 32, few_resident(NT)) few_tiles_kernel(const __grid_constant__ FewRowsParams p) {
     constexpr int LD = NT * 8 + 1, WARPS = FEW_CONSUMERS, DEPTH = NT == 4 ? 2 : 4;
     __shared__ float red[WARPS][16][LD];
     pdl_wait();
@@ -299,8 +301,9 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_rows_kernel(const __grid_c
 // 16 rows of w a tile, or 8 where tiles of 16 would leave SMs without one.
 static int few_tile_rows(int M, int N) { return (long long)(N + 15) / 16 * ((M + 31) / 32) >= ob200_plan_sm_count() ? 16 : 8; }
 
-// Whether a launch is of few tiles: all of them resident at once, two an SM.  By the sizes and the device, because it sets the order of
-// a sum.  32000 x 1024, one token: 15.6 us straight to registers, 14.6 through the ring; 16 tokens 19.4 and 18.2.
+// Whether a launch is of few tiles: two an SM, which are resident at once but for 9 to 16 tokens, whose CTAs take them one after the other
+// (4096 x 1024, 256 tiles: 6.5 us in 148 CTAs, 7.0 in 256).  By the sizes and the device, because it sets the order of a sum.
+// 32000 x 1024, one token: 15.6 us straight to registers, 14.6 through the ring; 16 tokens 19.4 and 18.2.
 static bool few_tiles(int M, int N) {
     const int rows = few_tile_rows(M, N);
     return ((long long)N + rows - 1) / rows * ((M + 31) / 32) <= 2 * ob200_plan_sm_count();
@@ -345,9 +348,9 @@ template <int NT, bool LSE>
 static int few_launch(const FewRowsParams& p, int num_ctas, cudaStream_t stream) {
     const int tiles = (p.N + p.tile_rows - 1) / p.tile_rows;
     if (few_tiles(p.M, p.N)) {
-        const int units = tiles * ((p.M + 31) / 32);
-        OB200_ELASTIC_HBM((few_tiles_kernel<NT, LSE>), 2);
-        return launch_pdl(few_tiles_kernel<NT, LSE>, (unsigned)(units < 2 * num_ctas ? units : 2 * num_ctas), FEW_CONSUMERS * 32u, stream, p);
+        const int units = tiles * ((p.M + 31) / 32), most = few_resident(NT) * num_ctas;
+        OB200_ELASTIC_HBM((few_tiles_kernel<NT, LSE>), few_resident(NT));
+        return launch_pdl(few_tiles_kernel<NT, LSE>, (unsigned)(units < most ? units : most), FEW_CONSUMERS * 32u, stream, p);
     }
     static bool attr_set[64] = {};
     int dev = 0;

@@ -688,7 +688,7 @@ __global__ void __launch_bounds__(256) gemm_splitk_finish4_kernel(const float* _
 
 // The same for GM_EPI_ACT: bias, activation, dropout and residual behind the sum.  A thread takes eight elements of the flattened
 // output, the unit of the dropout's counter; partial matrices lie elems apart, so they are read in vectors where that allows it.
-__global__ void __launch_bounds__(256) gemm_splitk_act_kernel(const float* __restrict__ slabs, __nv_bfloat16* __restrict__ c,
+__global__ void __launch_bounds__(256, 6) gemm_splitk_act_kernel(const float* __restrict__ slabs, __nv_bfloat16* __restrict__ c,
                                                               const float* __restrict__ bias, const __nv_bfloat16* __restrict__ bias_bf16,
                                                               const __nv_bfloat16* __restrict__ residual, int splits, int M, int N, GemmEpi e) {
     pdl_wait();
@@ -1079,8 +1079,8 @@ int gemm_bf16_run(const GemmCall& g) {
     const long long elems = batch_ll * M * N;
     if (epi == GM_EPI_ACT || epi == GM_EPI_ACT_SLOPE || epi == GM_EPI_ACT_ANY) {
         long long blocks = ((elems + 7) / 8 + 255) / 256;
-        if (blocks > 8LL * num_ctas) blocks = 8LL * num_ctas;
-        OB200_ELASTIC_HBM(gemm_splitk_act_kernel, 8);
+        if (blocks > 6LL * num_ctas) blocks = 6LL * num_ctas;
+        OB200_ELASTIC_HBM(gemm_splitk_act_kernel, 6);
         return launch_pdl(gemm_splitk_act_kernel, (unsigned)blocks, 256u, st, (const float*)p.slabs, (__nv_bfloat16*)c, p.bias, p.bias_bf16, p.residual,
                           p.splits, M, N, p.e);
     }

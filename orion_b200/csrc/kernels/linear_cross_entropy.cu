@@ -34,8 +34,8 @@ constexpr float CE_LOG2E = 1.4426950408889634f;
 
 // lse and loss of every row from its parts.  A CTA has C rows; group g of G = 1024 / C takes parts g, g + G, ..., eight at a time in
 // registers (the kernel is a few dependent steps long: their loads are one), then the groups are joined in a fixed tree.  32 rows, or 4
-// where rows are few and their parts many.  Packed rows (`order`): row r of the parts is row order[r], and those from *live on do not
-// count.
+// where rows are few and their parts many.  1024 threads of 64 registers: one CTA an SM.  Packed rows (`order`): row r of the parts is
+// row order[r], and those from *live on do not count.
 template <int C>
 __global__ void __launch_bounds__(1024) ce_rows_kernel(const float2* __restrict__ part, const float* __restrict__ label_logit,
                                                        const long long* __restrict__ target, float* __restrict__ loss, float* __restrict__ lse,
@@ -375,15 +375,15 @@ extern "C" int ob200_linear_cross_entropy_forward(const void* x, const void* w, 
         }
         rc = few_rows_fit(rows, V, H) ? few_rows_run(g) : gemm_bf16_run(g);
         if (rc) return rc;
-        const int per_cta = n <= 64 ? 4 : 32, want = (n + per_cta - 1) / per_cta, cap = num_ctas * 2;
-        const unsigned grid = (unsigned)(want < cap ? want : cap);
+        const int per_cta = n <= 64 ? 4 : 32, want = (n + per_cta - 1) / per_cta;
+        const unsigned grid = (unsigned)(want < num_ctas ? want : num_ctas);
         if (per_cta == 4) {
-            OB200_ELASTIC_HBM(ce_rows_kernel<4>, 2);
+            OB200_ELASTIC_HBM(ce_rows_kernel<4>, 1);
             rc = launch_pdl(ce_rows_kernel<4>, grid, 1024u, st, (const float2*)part, (const float*)label_logit, target + r0, loss + r0, lse + r0, (const int*)order,
                             (const int*)(packs ? live : nullptr), n, parts, V,
                             ignore_index);
         } else {
-            OB200_ELASTIC_HBM(ce_rows_kernel<32>, 2);
+            OB200_ELASTIC_HBM(ce_rows_kernel<32>, 1);
             rc = launch_pdl(ce_rows_kernel<32>, grid, 1024u, st, (const float2*)part, (const float*)label_logit, target + r0, loss + r0, lse + r0, (const int*)order,
                             (const int*)(packs ? live : nullptr), n, parts, V,
                             ignore_index);
