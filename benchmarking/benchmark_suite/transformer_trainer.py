@@ -15,7 +15,7 @@ bfloat16 GEMM, LayerNorm / GELU / softmax / embedding / cross-entropy forward an
 ORION_FUSED_LINEAR=1 runs every linear layer with what follows it (bias, GELU, dropout, residual) as one launch, ORION_FUSED_LOSS=1
 computes the decoder's loss from the hidden states, without logits, and ORION_DROPOUT=p trains with dropout of the embeddings and
 of both residual branches, as the reference's clients do (reference benchmarking/model_kernels/bert_8_fb1, dropout rows); the
-masks are drawn from counters and never stored.  All three are off by default: recorded profiles have a row per launch.
+masks are drawn from counters and never stored; ORION_DROPOUT_SEED names their seed.  All three are off by default: recorded profiles have a row per launch.
 With ORION_PREPARE=0 training uses stock PyTorch modules, whose cuBLASLt / flash-attention / elementwise
 launches are captured and scheduled like any other op.
 """
@@ -38,8 +38,9 @@ OWN_GEMM_TRAINING = os.environ.get("ORION_OWN_GEMM_TRAINING", "1") == "1"
 # linear layers of the text clients with their bias, GELU, dropout and residual in one launch; loss of the decoder without its logits
 FUSED_LINEAR = os.environ.get("ORION_FUSED_LINEAR", "0") == "1"
 FUSED_LOSS = os.environ.get("ORION_FUSED_LOSS", "0") == "1"
-# dropout probability of the training clients (embeddings and both residual branches)
+# dropout probability of the training clients (embeddings and both residual branches), and the seed of a run's masks (default: torch's)
 DROPOUT = float(os.environ.get("ORION_DROPOUT", "0"))
+DROPOUT_SEED = os.environ.get("ORION_DROPOUT_SEED")
 
 BERT = dict(layers=12, hidden=768, heads=12, ffn=3072, vocab=30528, max_pos=512, seq=384)
 LM = dict(layers=16, hidden=1024, heads=16, ffn=4096, vocab=32000, seq=512)
@@ -54,6 +55,21 @@ def _f32(module, p):
         hit = (p._version, p.detach().float(), p.data_ptr())
         cache[id(p)] = hit
     return hit[1]
+
+
+def _dropout_state(module, cfg):
+    """`rng`, the seed and the step of the model's dropout masks.  The seed is cfg["dropout_seed"], or drawn from torch's generator, so that
+    masks follow torch.manual_seed and no two models share theirs."""
+    p, seed = cfg.get("dropout", 0.0), cfg.get("dropout_seed")
+    if seed is None:
+        seed = int(torch.randint(2 ** 62, ())) if p > 0.0 else 0   # without dropout nothing is drawn
+    module.register_buffer("rng", torch.tensor([seed, 0]), persistent=False)
+
+
+def _client_seed(tid, local_rank):
+    """A client's own masks: the run's seed with the process's rank and the client's number in it."""
+    base = int(DROPOUT_SEED) if DROPOUT_SEED else torch.initial_seed()
+    return (base + (int(os.environ.get("RANK", local_rank)) << 40) + (tid << 52)) % 2 ** 62
 
 
 def _count_step(rng):
@@ -151,7 +167,7 @@ class BertQA(nn.Module):
         self.dropout = cfg.get("dropout", 0.0)
         self.layers = nn.ModuleList([BertLayer(h, cfg["heads"], cfg["ffn"], self.dropout, 2 * i + 1) for i in range(cfg["layers"])])
         self.qa = nn.Linear(h, 2)
-        self.register_buffer("rng", torch.tensor([0, 0]), persistent=False)   # seed and step of the dropout masks
+        _dropout_state(self, cfg)
 
     def _own_training(self, ids):
         return ORION_TRAIN_KERNELS and OWN_GEMM_TRAINING and ids.is_cuda and self.training and self.word.weight.dtype == torch.bfloat16
@@ -204,7 +220,7 @@ class DecoderLM(nn.Module):
         self.layers = nn.ModuleList([BertLayer(h, cfg["heads"], cfg["ffn"], self.dropout, 2 * i + 1) for i in range(cfg["layers"])])
         self.ln = nn.LayerNorm(h)
         self.head = nn.Linear(h, cfg["vocab"], bias=False)
-        self.register_buffer("rng", torch.tensor([0, 0]), persistent=False)   # seed and step of the dropout masks
+        _dropout_state(self, cfg)
 
     def hidden(self, ids, orion=False):
         """What the vocabulary projection takes: [B, S, H], behind the last LayerNorm."""
@@ -276,7 +292,7 @@ def bert_loop(batchsize, train, num_iters, rps, uniform, dummy_data, local_rank,
     resident = os.environ.get("ORION_RESIDENT_INPUTS", "0") == "1"
 
     def build(device):
-        model = BertQA(dict(BERT, dropout=DROPOUT)).to(device).to(torch.bfloat16)
+        model = BertQA(dict(BERT, dropout=DROPOUT, dropout_seed=_client_seed(tid, local_rank))).to(device).to(torch.bfloat16)
         ids = _pinned(torch.randint(0, vocab, (batchsize, seq)))
         labels = _pinned(torch.randint(0, seq, (2, batchsize)))
         state = {"ids": ids.to(device, non_blocking=True), "lab": labels.to(device, non_blocking=True)}
@@ -317,7 +333,7 @@ def transformer_loop(batchsize, train, num_iters, rps, uniform, dummy_data, loca
     resident = os.environ.get("ORION_RESIDENT_INPUTS", "0") == "1"
 
     def build(device):
-        model = DecoderLM(dict(LM, dropout=DROPOUT)).to(device).to(torch.bfloat16)
+        model = DecoderLM(dict(LM, dropout=DROPOUT, dropout_seed=_client_seed(tid, local_rank))).to(device).to(torch.bfloat16)
         tokens = _pinned(torch.randint(0, vocab, (batchsize, seq + 1)))
         state = {"tok": tokens.to(device, non_blocking=True)}
         if train:

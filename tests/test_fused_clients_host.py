@@ -1,0 +1,52 @@
+"""The language clients' dropout state, loss and scores as far as the CPU goes."""
+import math
+
+import pytest
+import torch
+
+from benchmarking.benchmark_suite import transformer_trainer as tt
+
+SMALL = dict(layers=1, hidden=64, heads=2, ffn=128, vocab=96, seq=16, max_pos=16)
+
+
+def build(kind, **more):
+    return getattr(tt, kind)(dict(tt.BERT if kind == "BertQA" else tt.LM, **SMALL, **more))
+
+
+@pytest.mark.parametrize("kind", ["BertQA", "DecoderLM"])
+def test_masks_have_seeds_of_their_own(kind):
+    """The seed follows torch.manual_seed, no two models of a process have the same one, and a configuration may name it."""
+    def seed(**more):
+        rng = build(kind, dropout=0.1, **more).rng
+        assert rng.dtype == torch.int64 and rng.shape == (2,) and rng[1] == 0
+        return int(rng[0])
+    torch.manual_seed(1)
+    a, b = seed(), seed()
+    torch.manual_seed(1)
+    assert seed() == a != b
+    torch.manual_seed(2)
+    assert seed() not in (a, b)
+    assert seed(dropout_seed=77) == 77
+
+
+@pytest.mark.parametrize("kind", ["BertQA", "DecoderLM"])
+def test_a_model_without_dropout_draws_no_seed(kind):
+    """What is drawn behind it, a client's token ids say, stays what it was."""
+    torch.manual_seed(3)
+    plain = build(kind)
+    after = torch.get_rng_state()
+    torch.manual_seed(3)
+    named = build(kind, dropout=0.1, dropout_seed=5)
+    assert torch.equal(torch.get_rng_state(), after)
+    assert all(torch.equal(p, q) for p, q in zip(plain.parameters(), named.parameters()))
+
+
+def test_clients_and_ranks_have_different_masks(monkeypatch):
+    monkeypatch.delenv("RANK", raising=False)
+    torch.manual_seed(42)   # what every client starts with
+    seeds = [tt._client_seed(tid, rank) for tid in range(8) for rank in range(8)]
+    assert len(set(seeds)) == 64 and all(0 <= s < 2 ** 62 for s in seeds)
+    monkeypatch.setenv("RANK", "11")
+    assert tt._client_seed(0, 0) not in seeds
+    monkeypatch.setattr(tt, "DROPOUT_SEED", "123456789")
+    assert tt._client_seed(0, 0) != tt._client_seed(1, 0) and tt._client_seed(0, 0) not in seeds
