@@ -15,7 +15,8 @@ bfloat16 GEMM, LayerNorm / GELU / softmax / embedding / cross-entropy forward an
 ORION_FUSED_LINEAR=1 runs every linear layer with what follows it (bias, GELU, dropout, residual) as one launch, ORION_FUSED_LOSS=1
 computes the decoder's loss from the hidden states, without logits, and ORION_DROPOUT=p trains with dropout of the embeddings and
 of both residual branches, as the reference's clients do (reference benchmarking/model_kernels/bert_8_fb1, dropout rows); the
-masks are drawn from counters and never stored; ORION_DROPOUT_SEED names their seed.  All three are off by default: recorded profiles have a row per launch.
+masks are drawn from counters and never stored; ORION_DROPOUT_SEED names their seed.  All three are off by default: recorded profiles
+have a row per launch.
 With ORION_PREPARE=0 training uses stock PyTorch modules, whose cuBLASLt / flash-attention / elementwise
 launches are captured and scheduled like any other op.
 """
@@ -57,13 +58,22 @@ def _f32(module, p):
     return hit[1]
 
 
+def _fit_checkpoint(model, state, prefix, *_):
+    """A checkpoint of a model without dropout has no `rng`, and a model without dropout takes none."""
+    if model.dropout > 0.0:
+        state.setdefault(prefix + "rng", model.rng)
+    else:
+        state.pop(prefix + "rng", None)
+
+
 def _dropout_state(module, cfg):
     """`rng`, the seed and the step of the model's dropout masks.  The seed is cfg["dropout_seed"], or drawn from torch's generator, so that
     masks follow torch.manual_seed and no two models share theirs."""
     p, seed = cfg.get("dropout", 0.0), cfg.get("dropout_seed")
     if seed is None:
         seed = int(torch.randint(2 ** 62, ())) if p > 0.0 else 0   # without dropout nothing is drawn
-    module.register_buffer("rng", torch.tensor([seed, 0]), persistent=False)
+    module.register_buffer("rng", torch.tensor([seed, 0]), persistent=p > 0.0)   # a checkpoint goes on with the step that it stopped at
+    module.register_load_state_dict_pre_hook(_fit_checkpoint)
 
 
 def _client_seed(tid, local_rank):

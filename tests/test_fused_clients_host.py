@@ -1,5 +1,5 @@
 """The language clients' dropout state, loss and scores as far as the CPU goes."""
-import math
+import pickle
 
 import pytest
 import torch
@@ -50,3 +50,25 @@ def test_clients_and_ranks_have_different_masks(monkeypatch):
     assert tt._client_seed(0, 0) not in seeds
     monkeypatch.setattr(tt, "DROPOUT_SEED", "123456789")
     assert tt._client_seed(0, 0) != tt._client_seed(1, 0) and tt._client_seed(0, 0) not in seeds
+
+
+@pytest.mark.parametrize("kind", ["BertQA", "DecoderLM"])
+def test_a_checkpoint_goes_on_with_its_masks(kind):
+    """Seed and step are in the checkpoint of a model with dropout; checkpoints of models with and without fit each other."""
+    model, other, plain = build(kind, dropout=0.1), build(kind, dropout=0.1), build(kind)
+    model.rng[1] = 1234567
+    state = model.state_dict()
+    assert not torch.equal(other.rng, model.rng)
+    other.load_state_dict(state)
+    assert torch.equal(other.rng, model.rng) and other.rng.data_ptr() != model.rng.data_ptr()
+    assert "rng" not in plain.state_dict()
+    plain.load_state_dict(state)
+    assert not plain.rng.any() and "rng" in state                   # the caller's dictionary is as it was
+    before = other.rng.clone()
+    other.load_state_dict(plain.state_dict())
+    assert torch.equal(other.rng, before)
+    # a whole model, and one inside a larger module
+    assert torch.equal(pickle.loads(pickle.dumps(model)).rng, model.rng)
+    outer, again = (torch.nn.Sequential(build(kind, dropout=0.1)) for _ in range(2))
+    again.load_state_dict(outer.state_dict())
+    assert torch.equal(again[0].rng, outer[0].rng)
