@@ -269,12 +269,13 @@ class DecoderLM(nn.Module):
         return self.head(x)
 
     def loss(self, ids, target):
-        """Mean cross-entropy of the next tokens `target` [B, S] (-100: not asked for), from the hidden states: on the orion kernels
-        neither the logits nor their gradient, 2 x B x S x vocabulary, are ever in memory."""
+        """Mean cross-entropy of the next tokens `target` [B, S] (-100: not asked for; 0 where none is), from the hidden states: on the
+        orion kernels neither the logits nor their gradient, 2 x B x S x vocabulary, are ever in memory."""
         x = self.hidden(ids)
         if x.is_cuda and x.dtype == torch.bfloat16 and ORION_TRAIN_KERNELS:
             return torch.ops.orion.linear_cross_entropy(x, self.head.weight, target.contiguous())
-        return F.cross_entropy(self.head(x).float().flatten(0, 1), target.flatten())
+        total = F.cross_entropy(self.head(x).float().flatten(0, 1), target.flatten(), reduction="sum")
+        return total / (target != -100).sum().clamp(min=1)
 
     def score(self, ids):
         """Log-likelihood of every token given those before it, [B, S - 1] (a scoring request), without the logits."""

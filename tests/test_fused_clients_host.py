@@ -72,3 +72,17 @@ def test_a_checkpoint_goes_on_with_its_masks(kind):
     outer, again = (torch.nn.Sequential(build(kind, dropout=0.1)) for _ in range(2))
     again.load_state_dict(outer.state_dict())
     assert torch.equal(again[0].rng, outer[0].rng)
+
+
+def test_loss_of_no_tokens_is_zero_on_the_stock_path_too():
+    """As on the orion kernels: a step whose targets are all masked has no loss and no gradient.  With targets the mean is torch's."""
+    import torch.nn.functional as F
+    torch.manual_seed(4)
+    model = build("DecoderLM")
+    ids, target = torch.randint(0, 96, (2, 16)), torch.randint(0, 96, (2, 16))
+    target[0, 5:] = -100
+    want = F.cross_entropy(model(ids).flatten(0, 1), target.flatten())
+    assert abs(model.loss(ids, target) - want) <= 16 * 2.0 ** -23 * want   # 21 terms in another order, each rounding half of 2^-23
+    loss = model.loss(ids, torch.full_like(target, -100))
+    loss.backward()
+    assert loss.item() == 0 and not any(p.grad.any() for p in model.parameters() if p.grad is not None)
