@@ -182,8 +182,8 @@ class BertQA(nn.Module):
     def _own_training(self, ids):
         return ORION_TRAIN_KERNELS and OWN_GEMM_TRAINING and ids.is_cuda and self.training and self.word.weight.dtype == torch.bfloat16
 
-    def embed(self, ids, rng=None):
-        p = self.dropout if self.training else 0.0
+    def embed(self, ids, rng=None, orion=False):
+        p = self.dropout if self.training and not orion else 0.0   # a request (orion) drops nothing
         if self._own_training(ids):
             ops = torch.ops.orion
             x = ops.layernorm_train(ops.embedding_train(ids, self.word.weight, self.pos.weight, self.typ.weight), self.ln.weight,
@@ -199,8 +199,8 @@ class BertQA(nn.Module):
             emb = ops.embedding_train(ids.contiguous(), self.word.weight, self.pos.weight, self.typ.weight)
             x = ops.layernorm(emb.view(b * s, -1), _f32(self, self.ln.weight), _f32(self, self.ln.bias), self.ln.eps).view(b, s, -1)
         else:
-            rng = self._step(ids)
-            x = self.embed(ids, rng)
+            rng = None if orion else self._step(ids)
+            x = self.embed(ids, rng, orion)
         for layer in self.layers:
             x = layer.forward_orion(x) if orion else layer(x, False, rng)
         return self.qa(x)   # [B, S, 2]: start / end logits
@@ -233,8 +233,8 @@ class DecoderLM(nn.Module):
         _dropout_state(self, cfg)
 
     def hidden(self, ids, orion=False):
-        """What the vocabulary projection takes: [B, S, H], behind the last LayerNorm."""
-        p = self.dropout if self.training else 0.0
+        """What the vocabulary projection takes: [B, S, H], behind the last LayerNorm.  A request (orion) drops nothing."""
+        p = self.dropout if self.training and not orion else 0.0
         if (not orion and ORION_TRAIN_KERNELS and OWN_GEMM_TRAINING and ids.is_cuda and self.training
                 and self.word.weight.dtype == torch.bfloat16):
             ops = torch.ops.orion
@@ -283,7 +283,12 @@ class DecoderLM(nn.Module):
             if ids.is_cuda and self.word.weight.dtype == torch.bfloat16:
                 target = F.pad(ids[:, 1:], (0, 1), value=-100)   # nothing follows the last token
                 return -torch.ops.orion.linear_cross_entropy(self.hidden(ids, orion=True), self.head.weight, target, reduction="none")[:, :-1]
-            logits = self.head(self.hidden(ids))[:, :-1].float()
+            modes = [(m, m.training) for m in self.modules()]   # the stock path's request: without dropout, whatever mode the model is in
+            try:
+                logits = self.eval().head(self.hidden(ids))[:, :-1].float()
+            finally:
+                for m, mode in modes:
+                    m.training = mode
             return -F.cross_entropy(logits.flatten(0, 1), ids[:, 1:].flatten(), reduction="none").view(ids.shape[0], -1)
 
 

@@ -86,3 +86,17 @@ def test_loss_of_no_tokens_is_zero_on_the_stock_path_too():
     loss = model.loss(ids, torch.full_like(target, -100))
     loss.backward()
     assert loss.item() == 0 and not any(p.grad.any() for p in model.parameters() if p.grad is not None)
+
+
+def test_requests_drop_nothing():
+    """Scores, and embeddings of a request, are the same in training mode as in evaluation; the modes stay what they were."""
+    torch.manual_seed(5)
+    ids = torch.randint(0, 96, (2, 16))
+    model = build("DecoderLM", dropout=0.5)
+    want = model.eval().score(ids)
+    model.train()
+    model.ln.eval()
+    assert torch.equal(model.score(ids), want) and model.training and model.layers[0].training and not model.ln.training
+    assert not torch.equal(model(ids), model(ids))
+    bert = build("BertQA", dropout=0.5).train()
+    assert torch.equal(bert.embed(ids, orion=True), bert.embed(ids, orion=True)) and not torch.equal(bert.embed(ids), bert.embed(ids))
