@@ -232,11 +232,11 @@ static int ce_pack(const CePack& p, int num_ctas, cudaStream_t st) {
     return launch_pdl(ce_pack_kernel, (unsigned)(want < cap ? want : cap), (unsigned)CE_PACK_THREADS, st, p);
 }
 
-// Columns of the vocabulary a piece of the backward pass has: dl of a piece takes at most 192 MB (and no piece is so narrow that its
-// products are small), and of the four fewest numbers of pieces the one whose 256 x 256 tiles fill the last rounds of the CTA pairs best,
-// counted in k-blocks of 64 and eight for a tile's way out.  8192 x 32000 x 1024: three pieces of 10752 columns, whose gradient products
-// are 296 tiles for 74 pairs, instead of four of 8192 (256 tiles: 3.46 rounds).  Rows of dl start on 128-byte lines: 6437 x 13042 x 136 with
-// gradients 228 us without, 209 with.
+// Columns of the vocabulary a piece of the backward pass has: dl of a piece takes at most 192 MB, or 4 KB a row where that is more (2048
+// columns, so that its products are not small: from 49153 rows on), and of the four fewest numbers of pieces the one whose 256 x 256
+// tiles fill the last rounds of the CTA pairs best, counted in k-blocks of 64 and eight for a tile's way out.  8192 x 32000 x 1024: three
+// pieces of 10752 columns, whose gradient products are 296 tiles for 74 pairs, instead of four of 8192 (256 tiles: 3.46 rounds).  Rows of
+// dl start on 128-byte lines: 6437 x 13042 x 136 with gradients 228 us without, 209 with.
 static int ce_piece(long long rows, int V, int H, int sms) {
     long long most = (192LL << 20) / (2 * rows) / 256 * 256;
     if (most < 2048) most = 2048;
