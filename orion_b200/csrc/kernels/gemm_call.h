@@ -36,7 +36,7 @@ struct GemmEpi {
     long long col0;                 // column of the vocabulary that column 0 of this product is
     float2* part;                   // GM_EPI_LSE: [ceil(N / 128)][M] (maximum, sum of exp(x - maximum)) of 128 columns
     float* label_logit;             // GM_EPI_LSE: [M], written where the label is one of the columns
-    const float2* row;              // GM_EPI_DLOGITS: [M] (lse * log2(e), coefficient); a coefficient of zero gives zeros whatever else the row holds
+    const float2* row;              // GM_EPI_DLOGITS: [M] (logsumexp, coefficient); a coefficient of zero gives zeros whatever else the row holds
 };
 
 struct GemmCall {

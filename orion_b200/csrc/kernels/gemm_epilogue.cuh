@@ -247,14 +247,20 @@ __device__ __forceinline__ void gm_epilogue_act_any(const GemmParams& p, uint32_
     }
 }
 
+// 2^(ref - x log2(e)) for ref = x log2(e) as float32 rounds it; the multiply-add takes the difference exactly.
+__device__ __forceinline__ float gm_ref_error(float x, float ref) { return exp2f(-fmaf(x, 1.4426950408889634f, -ref)); }
+
 // Of every row and 128 columns the maximum and the sum of exponentials relative to it, and the logit of the row's label.
+//
+// Exponents are one multiply-add against a reference rounded to float32, 2^(x log2(e) - ref), and so off by what the rounding took from it,
+// up to 2^-24 of the maximum's exponent.  That is one factor for all columns: gm_ref_error, once a row, takes it out of the sum.
 template <int COLS>
 __device__ __forceinline__ void gm_epilogue_lse(const GemmParams& p, uint32_t t_row, int m, int n0) {
     constexpr float kLog2e = 1.4426950408889634f;
     const bool row_ok = m < p.M;
     const long long at = row_ok ? p.e.target[m] - p.e.col0 - n0 : -1;
     const int label = at >= 0 && at < COLS ? (int)at : -1;   // the label's column of this warp's
-    float top = -INFINITY, sum = 0.f;
+    float top = -INFINITY, sum = 0.f, ref = 0.f;
 #pragma unroll 1
     for (int c0 = 0; c0 < COLS; c0 += 32) {
         const int n = n0 + c0;
@@ -275,9 +281,10 @@ __device__ __forceinline__ void gm_epilogue_lse(const GemmParams& p, uint32_t t_
 #pragma unroll
         for (int j = 4; j < 32; j++) mx[j & 3] = fmaxf(mx[j & 3], f[j]);
         const float now = fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), top);
-        const float ref = now == -INFINITY ? 0.f : now * kLog2e;   // columns of minus infinity alone weigh nothing
+        const float was = ref;
+        ref = now == -INFINITY ? 0.f : __fmul_rn(now, kLog2e);   // columns of minus infinity alone weigh nothing
         // nothing above minus infinity so far: a sum of 0, or not a number
-        uint64_t part[2] = {f32x2(top == -INFINITY ? sum : sum * exp2f(top * kLog2e - ref), 0.f), f32x2(0.f, 0.f)};
+        uint64_t part[2] = {f32x2(top == -INFINITY ? sum : sum * exp2f(was - ref), 0.f), f32x2(0.f, 0.f)};
 #pragma unroll
         for (int j = 0; j < 32; j += 2) {
             float e0, e1;
@@ -292,20 +299,21 @@ __device__ __forceinline__ void gm_epilogue_lse(const GemmParams& p, uint32_t t_
         sum = (s0 + s1) + (s2 + s3);
         top = now;
         if (((c0 + 32) & 127) == 0 || n + 32 >= p.N) {
-            if (row_ok) p.e.part[(long long)(n >> 7) * p.M + m] = make_float2(top, sum);
+            if (row_ok) p.e.part[(long long)(n >> 7) * p.M + m] = make_float2(top, top == -INFINITY ? sum : sum * gm_ref_error(top, ref));
             top = -INFINITY;
             sum = 0.f;
         }
     }
 }
 
-// C = (softmax - onehot(label)) * coefficient, the probabilities from this product's logits and the row's logsumexp.
+// C = (softmax - onehot(label)) * coefficient, the probabilities from this product's logits and the row's logsumexp (see gm_ref_error).
 template <int COLS>
 __device__ __forceinline__ void gm_epilogue_dlogits(const GemmParams& p, uint32_t t_row, int m, int m0w, int n0, int lane, uint8_t* stage,
                                                     uint32_t& turn) {
     constexpr float kLog2e = 1.4426950408889634f;
     const bool row_ok = m < p.M;
     const float2 row = row_ok ? p.e.row[m] : make_float2(0.f, 0.f);
+    const float ref = __fmul_rn(row.x, kLog2e), scale = row.y * gm_ref_error(row.x, ref);
     const long long at = row_ok ? p.e.target[m] - p.e.col0 - n0 : -1;
     const int label = at >= 0 && at < COLS ? (int)at : -1;
 #pragma unroll 1
@@ -317,10 +325,10 @@ __device__ __forceinline__ void gm_epilogue_dlogits(const GemmParams& p, uint32_
 #pragma unroll
         for (int j = 0; j < 32; j += 2) {
             float e0, e1;
-            split_f32x2(fma_f32x2(f32x2(f[j], f[j + 1]), f32x2(kLog2e, kLog2e), f32x2(-row.x, -row.x)), e0, e1);
+            split_f32x2(fma_f32x2(f32x2(f[j], f[j + 1]), f32x2(kLog2e, kLog2e), f32x2(-ref, -ref)), e0, e1);
             asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e0) : "f"(e0));
             asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e1) : "f"(e1));
-            split_f32x2(mul_f32x2(f32x2(e0, e1), f32x2(row.y, row.y)), f[j], f[j + 1]);
+            split_f32x2(mul_f32x2(f32x2(e0, e1), f32x2(scale, scale)), f[j], f[j + 1]);
         }
         if (__any_sync(0xffffffffu, label >= c0 && label < c0 + 32)) {
 #pragma unroll

@@ -81,10 +81,12 @@ __global__ void __launch_bounds__(1024) ce_rows_kernel(const float2* __restrict_
             for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
             if (lane == 0) {
                 const int row = r0 + warp, to = order ? order[row] : row;
-                const float l = row < counted ? now + logf(all) : 0.f;
+                // The maximum itself weighs 1 but for roundings.  The loss is taken from the maximum, not from lse, whose rounding would be
+                // all that is left of the loss of a row that is sure.
+                const float log_sum = logf(all < 1.f && now > -INFINITY ? 1.f : all);
                 const long long t = target[to];
-                lse[to] = l;
-                loss[to] = t == ignore_index ? 0.f : t >= 0 && t < V ? l - label_logit[row] : NAN;
+                lse[to] = row < counted ? now + log_sum : 0.f;
+                loss[to] = t == ignore_index ? 0.f : t >= 0 && t < V ? (now - label_logit[row]) + log_sum : NAN;
             }
         }
         __syncthreads();
@@ -134,7 +136,7 @@ __global__ void __launch_bounds__(1024) ce_total_kernel(const float* __restrict_
 // targets once per CTA and saves a launch.  Where every row counts x is not copied: the products take x itself.  Rows that do not
 // count become zeros where the last 64-row block of a reduction reads them.  Up to 128 rows, one tile, there is nothing to spare and the
 // rows stay in place, which saves the gradients' way back (ce_unpack_kernel; 64 x 1000 x 64 with gradients 91 -> 86 us on the host).
-// order: row of every slot, slot: slot of every row, or -1.  For the gradients also per slot the label and (lse * log2(e), coefficient), and
+// order: row of every slot, slot: slot of every row, or -1.  For the gradients also per slot the label and (logsumexp, coefficient), and
 // the factor of both: an upstream gradient that is one number, and the mean's divisor, multiply the products of the rounded dl; in the
 // coefficient they would make every row's largest term, the label's, off by the same rounding.  A label outside the vocabulary makes the
 // coefficient, and so the gradients, not a number.
@@ -198,7 +200,7 @@ __global__ void __launch_bounds__(CE_PACK_THREADS) ce_pack_kernel(const CePack p
             p.label[slot] = counts ? t : -1;
             if (p.order) p.order[slot] = (int)r;
             if (p.slot) p.slot[r] = counts ? slot : -1;
-            if (p.row) p.row[slot] = make_float2(p.lse[r] * CE_LOG2E, !counts ? 0.f : t >= 0 && t < p.V ? (p.grad_per_row ? p.grad[r] : 1.f) : NAN);
+            if (p.row) p.row[slot] = make_float2(p.lse[r], !counts ? 0.f : t >= 0 && t < p.V ? (p.grad_per_row ? p.grad[r] : 1.f) : NAN);
         }
         __syncthreads();
         if (all == p.rows && !p.in_place) continue;

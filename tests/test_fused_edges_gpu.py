@@ -71,3 +71,33 @@ def test_forward_mode_derivatives_are_refused(ops):
                     with torch.set_grad_enabled(grad), pytest.raises(RuntimeError, match="jvp|forward"):
                         call(*args)
     assert ops.linear_act(x, w, b, r, "gelu").shape == (8, 16)
+
+
+@pytest.mark.parametrize("T", [3, 20, 100, 128, 300, 700])
+@pytest.mark.parametrize("V", [200, 5003])
+@pytest.mark.parametrize("base", [0.0, 8192.0, -8192.0])
+def test_losses_next_to_large_logits_and_of_rows_that_are_sure(ops, T, V, base):
+    """Logits that float32 holds exactly (multiples of 1/16 about `base`), so that only the loss's own arithmetic is off: of a weighted mean
+    of V exponentials the exponents' rounding, 2^-24 of a distance to the maximum of at most some 15 where it weighs, 2^-22 of an
+    exponential and some 40 float32 additions, 2^-18 in all, whatever the logits' size; and the result's rounding.  Half of the
+    rows are sure: losses next to zero, none below it."""
+    torch.manual_seed(V + T)
+    H = 64
+    w = (torch.randint(-8, 9, (V, H), device="cuda") / 16).to(BF)
+    w[:, :16] = base / 16
+    x = torch.ones(T, H, device="cuda").to(BF)
+    target = torch.randint(0, V, (T,), device="cuda")
+    # row t has the answer of its label's first free column: a unit 12 above there for the sure half
+    x[:, 16:32] = 0
+    w[:, 16:32] = 0
+    label = torch.arange(0, T, 2, device="cuda")
+    target[label] = V // 2
+    w[V // 2, 16] = 24
+    x[label, 16] = 1
+    target[T // 2 + 1:T // 2 + 3] = -100
+    counts = target != -100
+    logits = x.double() @ w.double().T
+    want = torch.where(counts, torch.logsumexp(logits, 1) - logits.gather(1, target.clamp(0)[:, None])[:, 0], 0.0)
+    got = ops.linear_cross_entropy(x, w, target, reduction="none")
+    within(got, want, 2.0 ** -18 + 2.0 ** -23 * want.abs(), "loss")
+    assert (got >= 0).all()
