@@ -8,7 +8,8 @@ __device__ __forceinline__ uint32_t gm_pack(float a, float b) {
 }
 
 // Slopes are kept in float16: they lie between -0.13 and 1.13, and three more bits than bfloat16's keep what multiplies the gradient an
-// eighth as far off as the rounding of the product.
+// eighth as far off as the rounding of the product.  Below 2^-14 (behind GELU, arguments below -4.5) they have an absolute error of
+// 2^-25; keeping the argument in bfloat16 instead would move them by up to 7 % there.
 __device__ __forceinline__ uint32_t gm_pack_half(float a, float b) {
     const __half2 h2 = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&h2);

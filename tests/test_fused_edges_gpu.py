@@ -101,3 +101,23 @@ def test_losses_next_to_large_logits_and_of_rows_that_are_sure(ops, T, V, base):
     got = ops.linear_cross_entropy(x, w, target, reduction="none")
     within(got, want, 2.0 ** -18 + 2.0 ** -23 * want.abs(), "loss")
     assert (got >= 0).all()
+
+
+@pytest.mark.parametrize("M,N", [(1, 8), (9, 16), (32, 8), (2000, 40), (2000, 33)])
+def test_gelu_of_far_negative_values_is_relatively_exact(ops, M, N):
+    """z is given exactly (a row of x with one entry, a column of ones), so that only GELU and the output's rounding are off: 0.16 % down to
+    -5.6, 2.5 % of what is smaller than 6e-8 (fast_gelu.cuh), and half a step of bfloat16.  The slope, in float16: half a step
+    relatively and 2^-25, and 3e-7 of the evaluation."""
+    from orion_b200 import kernels as K
+    z = -torch.logspace(-2, math.log10(12), M, device="cuda", dtype=torch.float64).to(BF)
+    x, w = torch.zeros(M, 8, device="cuda", dtype=BF), torch.zeros(N, 8, device="cuda", dtype=BF)
+    x[:, 0], w[:, 0] = z, 1
+    zd = z.double()
+    cdf = 0.5 * torch.special.erfc(-zd / math.sqrt(2))
+    want = (zd * cdf)[:, None].expand(M, N)
+    y, slope = K.linear_act(x, w, act="gelu", want_slope=True)
+    bound = (U + torch.where(zd >= -5.6, 1.6e-3, 0.025))[:, None] * want.abs()
+    for got in (y, ops.linear_act(x, w, act="gelu")):
+        assert ((got.double() - want).abs() <= bound).all()
+    s = (cdf + zd * torch.exp(-0.5 * zd * zd) / math.sqrt(2 * math.pi))[:, None].expand(M, N)
+    within(slope[:, :N], s, 2.0 ** -11 * s.abs() + 2.0 ** -25 + 3e-7, "slope")
