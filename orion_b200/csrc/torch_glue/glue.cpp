@@ -907,8 +907,10 @@ struct LinearAct : public torch::autograd::Function<LinearAct> {
     }
     static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w, const c10::optional<at::Tensor>& bias,
                               const c10::optional<at::Tensor>& residual, int64_t act, double p, const c10::optional<at::Tensor>& rng, int64_t site) {
+        // the residual's gradient alone, dy, needs no slope
+        const bool through = x.requires_grad() || w.requires_grad() || (given(bias) && bias->requires_grad());
         at::Tensor slope;
-        at::Tensor y = run(x, w, bias, residual, (int)act, p, rng, site, act != 0, &slope);
+        at::Tensor y = run(x, w, bias, residual, (int)act, p, rng, site, act != 0 && through, &slope);
         ctx->save_for_backward({x, w, slope, p > 0.0 ? *rng : at::Tensor()});
         ctx->saved_data["act"] = act;
         ctx->saved_data["p"] = p;

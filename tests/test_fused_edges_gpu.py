@@ -121,3 +121,22 @@ def test_gelu_of_far_negative_values_is_relatively_exact(ops, M, N):
         assert ((got.double() - want).abs() <= bound).all()
     s = (cdf + zd * torch.exp(-0.5 * zd * zd) / math.sqrt(2 * math.pi))[:, None].expand(M, N)
     within(slope[:, :N], s, 2.0 ** -11 * s.abs() + 2.0 ** -25 + 3e-7, "slope")
+
+
+def test_a_gradient_of_the_residual_alone_keeps_no_slope(ops):
+    """Memory of the call: the output alone; with a gradient of any other argument the slope, as large, beside it."""
+    torch.manual_seed(2)
+    M, N, K = 512, 1024, 64
+    x, w, b, r = torch.randn(M, K, device="cuda").to(BF), torch.randn(N, K, device="cuda").to(BF), torch.randn(N, device="cuda").to(BF), torch.randn(M, N, device="cuda").to(BF)
+    dy = torch.randn(M, N, device="cuda").to(BF)
+    want = ops.linear_act(x, w, b, r, "gelu")
+    for i, copies in ((0, 2), (1, 2), (2, 2), (3, 1)):
+        args = [t.detach().clone() for t in (x, w, b, r)]
+        args[i].requires_grad_(True)
+        before = torch.cuda.memory_allocated()
+        y = ops.linear_act(*args, "gelu")
+        assert torch.cuda.memory_allocated() - before == copies * M * N * 2
+        assert torch.equal(y.detach(), want)
+        g, = torch.autograd.grad(y, args[i], dy)
+        assert g.shape == args[i].shape and (i < 3 or torch.equal(g, dy))
+        del y, g
