@@ -279,7 +279,7 @@ extern "C" int ob200_linear_act_bf16(const void* x, const void* w, void* y, void
     if (M < 0 || N < 0 || K <= 0 || act < 0 || act > 2 || !(p >= 0.f && p <= 1.f) || (p > 0.f && !rng) || num_ctas <= 0 || ldx < K || ldw < K) return -1;
     if (M == 0 || N == 0) return 0;
     if (!x || !w || !y || (slope && (ld_slope < N || ld_slope % 8 || !act))) return -1;
-    if (((uintptr_t)x | (uintptr_t)w | (uintptr_t)y | (uintptr_t)slope | (uintptr_t)workspace) % 16 || (ldx | ldw) % 8) return -2;
+    if (((uintptr_t)x | (uintptr_t)w | (uintptr_t)y | (uintptr_t)slope | (uintptr_t)workspace) % 16 || (K | ldx | ldw) % 8) return -2;
     if (workspace_bytes < ob200_linear_act_workspace(M, N, K) || (!workspace && workspace_bytes > 0)) return -3;
     const DropRate rate = drop_rate(p);
     GemmCall g;
@@ -341,7 +341,8 @@ extern "C" int ob200_linear_act_backward_bf16(const void* dy, const void* slope,
         return (int)e;
     }
     if (!dy || (act && !slope) || (slope && (ld_slope < N || ld_slope % 8 || !act)) || (dx && !w) || (dw && !x)) return -1;
-    if (((uintptr_t)dy | (uintptr_t)slope | (uintptr_t)x | (uintptr_t)w | (uintptr_t)dx | (uintptr_t)dw | (uintptr_t)workspace) % 16 || (ldx | ldw) % 8)
+    if (((uintptr_t)dy | (uintptr_t)slope | (uintptr_t)x | (uintptr_t)w | (uintptr_t)dx | (uintptr_t)dw | (uintptr_t)workspace) % 16 ||
+        (K | ldx | ldw) % 8)
         return -2;
     const DropRate rate = drop_rate(p);
     const LinearBackwardSpace space(M, N, K, act, rate.threshold, dx != nullptr, dw != nullptr, dbias != nullptr);
