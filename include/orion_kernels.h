@@ -248,7 +248,8 @@ int ob200_adamw_f32(float* p, const float* g, float* m, float* v, long long n, f
 
 /* y = residual + dropout(act(x . w^T + bias)) in one launch (bfloat16; float32 accumulation, rounded once): x [M, K] rows ldx apart,
  * w [N, K] rows ldw apart, y and residual [M, N] contiguous; K, ldx, ldw multiples of 8, pointers 16-byte aligned (residual and bias:
- * any), N any.  bias [N] float32 (bias_f32) or bfloat16, or NULL; residual may be NULL; act 0 none, 1 ReLU, 2 GELU (erf).
+ * any), N any, no size beyond 2^31 - 65536 (nor of the loss below).  bias [N] float32 (bias_f32) or bfloat16, or NULL; residual may be
+ * NULL; act 0 none, 1 ReLU, 2 GELU (erf); what is not a number stays one behind each.
  * Dropout with probability p (0: none), rounded to a multiple of 2^-16: an element is kept, and scaled by the exact reciprocal of the
  * kept share, where 16 bits of Philox4x32-10 (Salmon et al., SC'11) are at least round(65536 p); element i of the flattened y takes half
  * i % 8 of the four words at counter (low 32 bits of i / 8, bits 32..47 of i / 8 | bits 32..47 of step << 16, low 32 bits of step, site)

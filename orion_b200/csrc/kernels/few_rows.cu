@@ -311,10 +311,11 @@ static bool few_tiles(int M, int N) {
 
 struct FewPlan { int stages, bytes; };
 static FewPlan few_plan(int M, int N, int K) {
+    if (K > FEW_CHUNK * FEW_MAX_CHUNKS) return {0, 0};
     const int nt = M <= 8 ? 1 : M <= 16 ? 2 : 4, boxes = (K + FEW_BOX - 1) / FEW_BOX;
     const int fixed = FEW_CTL + FEW_CONSUMERS * 16 * (nt * 8 + 1) * 4 + boxes * nt * 8 * FEW_BOX * 2, stage_bytes = few_tile_rows(M, N) * FEW_CHUNK * 2;
     FewPlan f;
-    const int room = FEW_SMEM - fixed, stages = room > 0 && K <= FEW_CHUNK * FEW_MAX_CHUNKS ? room / stage_bytes : 0;
+    const int room = FEW_SMEM - fixed, stages = room > 0 ? room / stage_bytes : 0;
     f.stages = (stages < FEW_MAX_STAGES ? stages : FEW_MAX_STAGES) / FEW_GROUPS;
     f.bytes = fixed + FEW_GROUPS * f.stages * stage_bytes;
     return f;

@@ -8,6 +8,11 @@
 
 namespace ob200 {
 
+// Largest row count, width and reduction of the fused operators: positions are ints, and loops over blocks (65536 rows at most) and tiles
+// step past the last one before they stop.
+constexpr int GM_MOST_EXTENT = 0x7fffffff - 65535;
+inline bool gm_extents_fit(int M, int N, int K) { return M <= GM_MOST_EXTENT && N <= GM_MOST_EXTENT && K <= GM_MOST_EXTENT; }
+
 enum : int {
     GM_EPI_PLAIN = 0,    // C = alpha * A.B^T (+ bias) (+ bfloat16 residual)
     GM_EPI_ACC = 1,      // the same with a factor from device memory and a float32 addend (which may be C itself)

@@ -269,14 +269,16 @@ extern "C" int ob200_dropout(const void* x, const void* residual, void* y, long 
 }
 
 extern "C" long long ob200_linear_act_workspace(int M, int N, int K) {
-    if (M <= 0 || N <= 0 || K <= 0 || few_rows_fit(M, N, K)) return 0;
+    if (M <= 0 || N <= 0 || K <= 0 || !gm_extents_fit(M, N, K) || few_rows_fit(M, N, K)) return 0;
     return (long long)gemm_bf16_slab_bytes(M, N, K, GM_EPI_ACT);
 }
 
 extern "C" int ob200_linear_act_bf16(const void* x, const void* w, void* y, void* slope, const void* bias, int bias_f32, const void* residual, int act,
                                      float p, const long long* rng, int site, int M, int N, int K, long long ldx, long long ldw, long long ld_slope,
                                      void* workspace, long long workspace_bytes, int num_ctas, void* stream) {
-    if (M < 0 || N < 0 || K <= 0 || act < 0 || act > 2 || !(p >= 0.f && p <= 1.f) || (p > 0.f && !rng) || num_ctas <= 0 || ldx < K || ldw < K) return -1;
+    if (M < 0 || N < 0 || K <= 0 || act < 0 || act > 2 || !(p >= 0.f && p <= 1.f) || (p > 0.f && !rng) || num_ctas <= 0 || ldx < K || ldw < K ||
+        !gm_extents_fit(M, N, K))
+        return -1;
     if (M == 0 || N == 0) return 0;
     if (!x || !w || !y || (slope && (ld_slope < N || ld_slope % 8 || !act))) return -1;
     if (((uintptr_t)x | (uintptr_t)w | (uintptr_t)y | (uintptr_t)slope | (uintptr_t)workspace) % 16 || (K | ldx | ldw) % 8) return -2;
@@ -325,14 +327,16 @@ struct LinearBackwardSpace {
 }  // namespace
 
 extern "C" long long ob200_linear_act_backward_workspace(int M, int N, int K, int act, float p, int want_dx, int want_dw, int want_dbias) {
-    if (M <= 0 || N <= 0 || K <= 0 || !(p >= 0.f && p <= 1.f)) return 0;
+    if (M <= 0 || N <= 0 || K <= 0 || !gm_extents_fit(M, N, K) || !(p >= 0.f && p <= 1.f)) return 0;
     return (long long)LinearBackwardSpace(M, N, K, act, drop_rate(p).threshold, want_dx, want_dw, want_dbias).total;
 }
 
 extern "C" int ob200_linear_act_backward_bf16(const void* dy, const void* slope, const void* x, const void* w, void* dx, void* dw, void* dbias,
                                               int bias_f32, int act, float p, const long long* rng, int site, int M, int N, int K, long long ldx,
                                               long long ldw, long long ld_slope, void* workspace, long long workspace_bytes, int num_ctas, void* stream) {
-    if (M < 0 || N < 0 || K <= 0 || act < 0 || act > 2 || !(p >= 0.f && p <= 1.f) || (p > 0.f && !rng) || num_ctas <= 0 || ldx < K || ldw < K) return -1;
+    if (M < 0 || N < 0 || K <= 0 || act < 0 || act > 2 || !(p >= 0.f && p <= 1.f) || (p > 0.f && !rng) || num_ctas <= 0 || ldx < K || ldw < K ||
+        !gm_extents_fit(M, N, K))
+        return -1;
     if (M == 0 || N == 0) {   // sums over nothing
         cudaError_t e = cudaSuccess;
         if (dx && M > 0) e = cudaMemsetAsync(dx, 0, (size_t)M * K * 2, (cudaStream_t)stream);

@@ -319,7 +319,7 @@ struct CeForwardSpace {
     }
 };
 extern "C" long long ob200_linear_cross_entropy_workspace(int rows, int V, int H) {
-    if (rows <= 0 || V <= 0 || H <= 0) return 0;
+    if (rows <= 0 || V <= 0 || H <= 0 || !gm_extents_fit(rows, V, H)) return 0;
     return (long long)CeForwardSpace(rows, V, H).total;
 }
 
@@ -327,7 +327,7 @@ extern "C" long long ob200_linear_cross_entropy_workspace(int rows, int V, int H
 extern "C" int ob200_linear_cross_entropy_forward(const void* x, const void* w, const long long* target, float* loss, float* lse, float* total, float* count,
                                                   int rows, int V, int H, long long ldx, long long ldw, long long ignore_index, int mean, void* workspace,
                                                   long long workspace_bytes, int num_ctas, void* stream) {
-    if (rows < 0 || V <= 0 || H <= 0 || ldx < H || ldw < H || num_ctas <= 0) return -1;
+    if (rows < 0 || V <= 0 || H <= 0 || ldx < H || ldw < H || num_ctas <= 0 || !gm_extents_fit(rows, V, H)) return -1;
     if ((rows > 0 && (!x || !w || !target || !loss || !lse)) || (total && !count)) return -1;
     if (((uintptr_t)x | (uintptr_t)w | (uintptr_t)workspace) % 16 || (ldx | ldw) % 8) return -2;
     if (H % 8) return -2;
@@ -398,7 +398,7 @@ extern "C" int ob200_linear_cross_entropy_forward(const void* x, const void* w, 
 }
 
 extern "C" long long ob200_linear_cross_entropy_backward_workspace(int rows, int V, int H, int want_dx, int want_dw) {
-    if (rows <= 0 || V <= 0 || H <= 0) return 0;
+    if (rows <= 0 || V <= 0 || H <= 0 || !gm_extents_fit(rows, V, H)) return 0;
     return (long long)CeBackwardSpace(rows, V, H, want_dx, want_dw).total;
 }
 
@@ -406,7 +406,7 @@ extern "C" int ob200_linear_cross_entropy_backward(const void* x, const void* w,
                                                    int grad_per_row, const float* count, void* dx, void* dw, int rows, int V, int H, long long ldx,
                                                    long long ldw, long long ignore_index, void* workspace, long long workspace_bytes, int num_ctas,
                                                    void* stream) {
-    if (rows < 0 || V <= 0 || H <= 0 || ldx < H || ldw < H || num_ctas <= 0) return -1;
+    if (rows < 0 || V <= 0 || H <= 0 || ldx < H || ldw < H || num_ctas <= 0 || !gm_extents_fit(rows, V, H)) return -1;
     if (rows == 0) return dw ? (int)cudaMemsetAsync(dw, 0, (size_t)V * H * 2, (cudaStream_t)stream) : 0;
     if (!x || !w || !target || !lse || !grad) return -1;
     if (((uintptr_t)x | (uintptr_t)w | (uintptr_t)dx | (uintptr_t)dw | (uintptr_t)workspace) % 16 || (ldx | ldw) % 8 || H % 8) return -2;
@@ -442,10 +442,10 @@ extern "C" int ob200_linear_cross_entropy_backward(const void* x, const void* w,
     k.in_place = !packs;
     int rc = ce_pack(k, num_ctas, st);
     if (rc) return rc;
-    for (int v0 = 0; v0 < V; v0 += space.piece) {
-        const int nv = V - v0 < space.piece ? V - v0 : space.piece;
+    for (long long v0 = 0; v0 < V; v0 += space.piece) {
+        const int nv = V - v0 < space.piece ? (int)(V - v0) : space.piece;
         const bool first = v0 == 0, last = v0 + nv == V;
-        const __nv_bfloat16* wp = (const __nv_bfloat16*)w + (long long)v0 * ldw;
+        const __nv_bfloat16* wp = (const __nv_bfloat16*)w + v0 * ldw;
         GemmCall g;
         g.num_ctas = num_ctas;
         g.stream = stream;
@@ -483,7 +483,7 @@ extern "C" int ob200_linear_cross_entropy_backward(const void* x, const void* w,
         gw.M = nv; gw.K = rows;
         gw.epi = GM_EPI_ACC;
         gw.e.factor = factor;
-        gw.c = (__nv_bfloat16*)dw + (long long)v0 * H;
+        gw.c = (__nv_bfloat16*)dw + v0 * H;
         if (dx && dw && gemm_bf16_dual_splits(gx, gw) > 0) {
             rc = gemm_bf16_run_dual(gx, gw);
         } else {

@@ -819,6 +819,7 @@ at::Tensor linear_train_op(const at::Tensor& x, const at::Tensor& w, const c10::
 }
 
 // ------------------------------------------------------------------ fused linear layer, dropout, loss without logits
+constexpr int64_t kMostExtent = 0x7fffffff - 65535;   // of rows, widths and reductions (gemm_call.h)
 // `t` as rows of its last dimension: a view where the rows lie a multiple of 8 elements apart and 16-byte aligned (what a TMA copy
 // needs), else a copy.
 at::Tensor as_rows(const at::Tensor& t) {
@@ -870,7 +871,7 @@ struct LinearAct : public torch::autograd::Function<LinearAct> {
                         x.dim() >= 2 && w.dim() == 2 && x.size(-1) == w.size(1) && w.size(1) > 0 && w.size(1) % 8 == 0,
                     "orion::linear_act: bfloat16 CUDA tensors [..., K] x [N, K] with K a multiple of 8 expected");
         const int64_t N = w.size(0), M = x.numel() / w.size(1);
-        TORCH_CHECK(M <= 0x7fffffff && N <= 0x7fffffff && w.size(1) <= 0x7fffffff, "orion::linear_act: sizes beyond 2^31 - 1");
+        TORCH_CHECK(M <= kMostExtent && N <= kMostExtent && w.size(1) <= kMostExtent, "orion::linear_act: sizes beyond 2^31 - 65536");
         if (given(bias))
             TORCH_CHECK(dtype_code(*bias) >= 0 && bias->dim() == 1 && bias->numel() == N && bias->is_contiguous() && bias->device() == x.device(),
                         "orion::linear_act: bias has to be contiguous [N], bfloat16 or float32");
@@ -1020,8 +1021,8 @@ struct LinearCrossEntropy : public torch::autograd::Function<LinearCrossEntropy>
                     "orion::linear_cross_entropy: bfloat16 CUDA tensors [..., H] x [V, H] with H a multiple of 8 expected");
         TORCH_CHECK(target.scalar_type() == at::kLong && target.device() == x.device() && target.sizes() == x.sizes().slice(0, x.dim() - 1),
                     "orion::linear_cross_entropy: int64 targets of the input's shape without its last dimension expected");
-        TORCH_CHECK(target.numel() <= 0x7fffffff && w.size(0) <= 0x7fffffff && w.size(1) <= 0x7fffffff,
-                    "orion::linear_cross_entropy: sizes beyond 2^31 - 1");
+        TORCH_CHECK(target.numel() <= kMostExtent && w.size(0) <= kMostExtent && w.size(1) <= kMostExtent,
+                    "orion::linear_cross_entropy: sizes beyond 2^31 - 65536");
         const int code = reduction == "none" ? 0 : reduction == "sum" ? 1 : reduction == "mean" ? 2 : -1;
         TORCH_CHECK(code >= 0, "orion::linear_cross_entropy: reduction has to be none, sum or mean, got ", reduction);
         return code;
