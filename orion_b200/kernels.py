@@ -439,16 +439,36 @@ def adamw_(p, g, m, v, step, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01
 _ACTS = {"none": 0, "relu": 1, "gelu": 2}
 
 
-def _rows_ok(*tensors):
-    return all(t.dim() == 2 and t.stride(1) == 1 and t.dtype == torch.bfloat16 for t in tensors)
+def _rows_ok(x, w):
+    assert all(t.dim() == 2 and t.dtype == torch.bfloat16 and t.stride(1) == 1 for t in (x, w)), "bfloat16 matrices of dense rows expected"
+    assert x.shape[1] == w.shape[1], "x [M, K] and w [N, K] expected"
+
+
+def _here(*tensors):
+    """A kernel runs on the current device and takes any pointer for one of its own."""
+    assert all(t is None or t.is_cuda and t.get_device() == torch.cuda.current_device() for t in tensors), "CUDA tensors of the current device expected"
+
+
+def _dense(t, shape, dtypes, name):
+    assert t is None or (t.shape == torch.Size(shape) and t.dtype in dtypes and t.is_contiguous()), "%s: a contiguous tensor of shape %s expected" % (name, tuple(shape))
+
+
+def _rng_ok(p, rng, site):
+    assert 0 <= site < 2 ** 31, "a site between 0 and 2^31 - 1 expected"
+    assert p == 0 or rng is not None, "dropout needs rng"
+    _dense(rng, (2,), (torch.int64,), "rng")
 
 
 def linear_act(x, w, bias=None, residual=None, act="none", p=0.0, rng=None, site=0, want_slope=False, num_ctas=None):
     """residual + dropout(act(x . w^T + bias)) for bfloat16 x [M, K], w [N, K] (rows a multiple of 8 elements apart), bias bfloat16 or
     float32; rng: int64 CUDA tensor (seed, step).  With `want_slope` also the activation's slope, in rows padded to a multiple of 8."""
-    assert _rows_ok(x, w) and x.shape[1] == w.shape[1] and (residual is None or residual.is_contiguous())
+    _rows_ok(x, w)
     M, K = x.shape
     N = w.shape[0]
+    _dense(bias, (N,), (torch.bfloat16, torch.float32), "bias")
+    _dense(residual, (M, N), (torch.bfloat16,), "residual")
+    _rng_ok(p, rng, site)
+    _here(x, w, bias, residual, rng)
     y = torch.empty((M, N), device=x.device, dtype=x.dtype)
     slope = torch.empty((M, (N + 7) // 8 * 8), device=x.device, dtype=torch.float16) if want_slope else None
     n = lib().ob200_linear_act_workspace(M, N, K)
@@ -462,9 +482,14 @@ def linear_act(x, w, bias=None, residual=None, act="none", p=0.0, rng=None, site
 
 def linear_act_backward(dy, slope, x, w, bias_dtype=torch.bfloat16, act="none", p=0.0, rng=None, site=0, num_ctas=None):
     """(dx, dw, dbias) of linear_act from dy [M, N] and what `want_slope` gave (None without an activation)."""
-    assert _rows_ok(x, w) and dy.is_contiguous() and dy.dtype == torch.bfloat16
+    _rows_ok(x, w)
     M, K = x.shape
     N = w.shape[0]
+    _dense(dy, (M, N), (torch.bfloat16,), "dy")
+    _dense(slope, (M, (N + 7) // 8 * 8), (torch.float16,), "slope")
+    _rng_ok(p, rng, site)
+    assert bias_dtype in (torch.bfloat16, torch.float32), "the bias is bfloat16 or float32"
+    _here(dy, slope, x, w, rng)
     dx, dw = torch.empty((M, K), device=x.device, dtype=x.dtype), torch.empty((N, K), device=x.device, dtype=x.dtype)
     db = torch.empty(N, device=x.device, dtype=bias_dtype)
     n = lib().ob200_linear_act_backward_workspace(M, N, K, _ACTS[act], float(p), 1, 1, 1)
@@ -478,7 +503,10 @@ def linear_act_backward(dy, slope, x, w, bias_dtype=torch.bfloat16, act="none", 
 
 def dropout(x, p, rng=None, site=0, residual=None, num_ctas=None):
     """dropout(x) [+ residual] with the mask that linear_act draws for an output of this shape; x contiguous float32 / bfloat16."""
-    assert x.is_contiguous() and (residual is None or residual.is_contiguous() and residual.dtype == x.dtype and residual.shape == x.shape)
+    _dense(x, x.shape, (torch.float32, torch.bfloat16), "x")
+    _dense(residual, x.shape, (x.dtype,), "residual")
+    _rng_ok(p, rng, site)
+    _here(x, residual, rng)
     y = torch.empty_like(x)
     _check(lib().ob200_dropout(_ptr(x), _ptr(residual), _ptr(y), x.numel(), float(p), _ptr(rng), int(site), _dtype_code(x), num_ctas or sm_count(),
                                _stream()), "ob200_dropout")
@@ -487,9 +515,11 @@ def dropout(x, p, rng=None, site=0, residual=None, num_ctas=None):
 
 def linear_cross_entropy(x, w, target, ignore_index=-100, mean=True, num_ctas=None):
     """(total, loss per row, lse per row, rows that count) of the cross-entropy of x . w^T, x [rows, H], w [V, H] bfloat16, int64 targets."""
-    assert _rows_ok(x, w) and x.shape[1] == w.shape[1] and target.dtype == torch.int64 and target.is_contiguous()
+    _rows_ok(x, w)
     rows, H = x.shape
     V = w.shape[0]
+    _dense(target, (rows,), (torch.int64,), "target")
+    _here(x, w, target)
     loss, lse = (torch.empty(rows, device=x.device, dtype=torch.float32) for _ in range(2))
     total, count = (torch.empty((), device=x.device, dtype=torch.float32) for _ in range(2))
     n = lib().ob200_linear_cross_entropy_workspace(rows, V, H)
@@ -502,9 +532,14 @@ def linear_cross_entropy(x, w, target, ignore_index=-100, mean=True, num_ctas=No
 
 def linear_cross_entropy_backward(x, w, target, lse, grad, count=None, ignore_index=-100, num_ctas=None):
     """(dx, dw) from what linear_cross_entropy gave; grad: one value, or one per row; count: rows that count (the mean) or None."""
-    assert _rows_ok(x, w) and grad.dtype == torch.float32 and grad.is_contiguous() and target.is_contiguous()
+    _rows_ok(x, w)
     rows, H = x.shape
     V = w.shape[0]
+    _dense(target, (rows,), (torch.int64,), "target")
+    _dense(lse, (rows,), (torch.float32,), "lse")
+    _dense(grad, () if grad.dim() == 0 else (rows,), (torch.float32,), "grad")
+    _dense(count, (), (torch.float32,), "count")
+    _here(x, w, target, lse, grad, count)
     dx, dw = torch.empty((rows, H), device=x.device, dtype=x.dtype), torch.empty((V, H), device=x.device, dtype=x.dtype)
     n = lib().ob200_linear_cross_entropy_backward_workspace(rows, V, H, 1, 1)
     space = torch.empty(n, device=x.device, dtype=torch.uint8)
