@@ -140,3 +140,50 @@ def test_a_gradient_of_the_residual_alone_keeps_no_slope(ops):
         g, = torch.autograd.grad(y, args[i], dy)
         assert g.shape == args[i].shape and (i < 3 or torch.equal(g, dy))
         del y, g
+
+
+@pytest.fixture
+def one_thread():
+    """A quota belongs to the thread that sets it: backward passes in the calling thread, so that it holds for them too."""
+    torch.autograd.set_multithreading_enabled(False)
+    yield
+    torch.autograd.set_multithreading_enabled(True)
+
+
+def under_quotas(ops, quotas, run):
+    want = run()
+    for q in quotas:
+        ops.set_sm_quota(q)
+        got = run()
+        ops.set_sm_quota(0)
+        for a, b in zip(got, want):
+            assert torch.equal(a, b), q
+
+
+@pytest.mark.parametrize("M,N,K", [(16, 512, 512), (128, 520, 264), (300, 1000, 2056), (600, 1024, 4096), (2050, 520, 72), (1040, 73, 136), (33, 257, 1024)])
+def test_gradients_of_the_layer_have_the_same_bits_from_any_cta_count(ops, one_thread, M, N, K):
+    torch.manual_seed(M + K)
+    x, w, b = torch.randn(M, K, device="cuda").to(BF), (torch.randn(N, K, device="cuda") / math.sqrt(K)).to(BF), torch.randn(N, device="cuda").to(BF)
+    dy, rng = torch.randn(M, N, device="cuda").to(BF), rng_of(M, N)
+
+    def run():
+        leaves = [t.clone().requires_grad_(True) for t in (x, w, b)]
+        return torch.autograd.grad(ops.linear_act(*leaves, None, "gelu", 0.1, rng, 4), leaves, dy)
+    under_quotas(ops, (147, 31, 2, 1), run)
+
+
+@pytest.mark.parametrize("T,V,H", [(12, 2000, 512), (128, 5003, 136), (700, 5003, 136), (1143, 9000, 768), (5000, 24001, 136)])
+def test_gradients_of_the_loss_have_the_same_bits_from_any_cta_count(ops, one_thread, T, V, H):
+    """All rows count, most, few: the gradient products are cut on the device for the rows that do."""
+    torch.manual_seed(T + V)
+    x, w = torch.randn(T, H, device="cuda").to(BF), (torch.randn(V, H, device="cuda") * 2 / math.sqrt(H)).to(BF)
+    labels, out = torch.randint(0, V, (T,), device="cuda"), torch.randperm(T, device="cuda")
+    for counted in sorted({T, T - T // 4, T // 7, 1, 0}):
+        target = labels.clone()
+        target[out[counted:]] = -100
+
+        def run():
+            leaves = [t.clone().requires_grad_(True) for t in (x, w)]
+            loss = ops.linear_cross_entropy(*leaves, target)
+            return [loss.detach()] + list(torch.autograd.grad(loss, leaves))
+        under_quotas(ops, (147, 31, 2, 1), run)
