@@ -2,10 +2,11 @@
 // loss without logits behind them, in one launch:  z[m, n] = sum_k x[m, k] w[n, k].
 //
 // Bound: reading w once.  Rows of w are the 16-row operand of mma.sync and the tokens its 8 columns, so that nothing is padded to a
-// 128-row tensor-memory tile whose way in and out takes longer than the whole product: 4096 x 1024 with bias and GELU 9.6 -> 4.8 us at one
-// token, 10.0 -> 5.1 at sixteen.  A lane reads 16 bytes of two rows of w and of a row of x at the same k and gives the instruction
-// pairs of them as if they lay in its order: the order of a sum's terms is free, as long as both operands share it, so wide accesses
-// are all there is.  Warps share a tile's reduction and join their sums through shared memory in a fixed order.
+// 128-row tensor-memory tile whose way in and out takes longer than the whole product: 4096 x 1024 with bias and GELU, w from HBM,
+// launches back to back, 9.7 -> 4.6 us at one token, 9.8 -> 6.4 at sixteen, 11.8 -> 6.8 at 32.  A lane reads 16 bytes of two rows of w
+// and of a row of x at the same k and gives the instruction pairs of them as if they lay in its order: the order of a sum's terms is
+// free, as long as both operands share it, so wide accesses are all there is.  Warps share a tile's reduction and join their sums
+// through shared memory in a fixed order.
 // Two kernels: w straight to registers where an SM has a tile or two, and where it has many, through a ring of TMA copies.
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -131,7 +132,7 @@ __device__ __forceinline__ void few_way_out(const FewRowsParams& p, const float 
 
 // ------------------------------------------------------------------ few tiles: straight to registers
 // Sixteen warps share a tile's reduction, four k-blocks of 32 (two of them for 32 tokens) under way in each.  There is no ring to fill and no copy to wait for, so
-// a launch of one or two tiles an SM is over sooner: 1024 x 4096 7.8 -> 5.9 us.  More than 32 tokens are groups of 32, each with tiles of
+// a launch of one or two tiles an SM is over sooner: 1024 x 4096 at one token 7.6 -> 5.7 us, at sixteen 8.4 -> 6.1.  More than 32 tokens are groups of 32, each with tiles of
 // its own: w is then read from L2 once a group.
 // CTAs an SM: what the launch bound, the quota's cut and the grid go by.  One of 9 to 16 tokens has the registers of two (110 a thread).
 constexpr int few_resident(int nt) { return nt == 2 ? 1 : 2; }
@@ -302,8 +303,9 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_rows_kernel(const __grid_c
 static int few_tile_rows(int M, int N) { return (long long)(N + 15) / 16 * ((M + 31) / 32) >= ob200_plan_sm_count() ? 16 : 8; }
 
 // Whether a launch is of few tiles: two an SM, which are resident at once but for 9 to 16 tokens, whose CTAs take them one after the other
-// (4096 x 1024, 256 tiles: 6.5 us in 148 CTAs, 7.0 in 256).  By the sizes and the device, because it sets the order of a sum.
-// 32000 x 1024, one token: 15.6 us straight to registers, 14.6 through the ring; 16 tokens 19.4 and 18.2.
+// (4096 x 1024, 256 tiles: 6.4 us in 148 CTAs, 7.0 in 256).  By the sizes and the device, because it sets the order of a sum.
+// 32000 x 1024, one token: 25.7 us straight to registers, 14.7 through the ring; 16 tokens 35.9 and 18.1.  4096 x 1024: 4.6 and 4.9; 16
+// tokens 6.4 and 5.4.
 static bool few_tiles(int M, int N) {
     const int rows = few_tile_rows(M, N);
     return ((long long)N + rows - 1) / rows * ((M + 31) / 32) <= 2 * ob200_plan_sm_count();

@@ -191,7 +191,9 @@ __device__ __forceinline__ bool gm_epilogue_act(const GemmParams& p, uint32_t t_
     return true;
 }
 
-// The same for any width, alignment and type of the bias.
+// The same for any width, alignment and type of the bias, which costs: 8192 x 4095 x 1024 takes 86 us with a bias (8192 x 4096 x 1024: 52),
+// 100 with GELU (58), 181 with a residual (58), 216 with GELU, dropout and residual (79).  A thread reads its row's residual element by
+// element, 32 rows apart, and a turn waits for the stores of the one before.
 template <int COLS>
 __device__ __forceinline__ void gm_epilogue_act_any(const GemmParams& p, uint32_t t_row, int m, int m0w, int n0, int lane, uint8_t* stage) {
     const bool row_ok = m < p.M;

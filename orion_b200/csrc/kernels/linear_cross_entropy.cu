@@ -10,8 +10,9 @@
 // written and 4 read, 1.2 ps, and the memory.  dl is rounded to bfloat16 because the tensor cores take it so: an error of at most
 // 2^-9 of each term of dx and dw, as large as that of the rounded result.  dx adds up over the pieces in float32.
 // Rows that do not count are left out of every product, by a count that stays on the device (ce_pack_kernel).
-// The tensor core bounds it.  8192 x 32000 x 1024: forward 319 us (1.68 PFLOP/s), a third of the logits' gradient 121 (1.49), both gradient
-// products of a third 225 (1.60), alone and cold; back to back under the power limit 1.5 - 1.7 ms a step, 1.25 - 1.43 PFLOP/s.
+// The tensor core bounds it.  8192 x 32000 x 1024: forward 320 us (1.68 PFLOP/s), a third of the logits' gradient 121 (1.49), both gradient
+// products of a third 222 (1.63), alone and cold; back to back under the power limit 1.5 - 1.8 ms a step, 1.2 - 1.43 PFLOP/s.  With its
+// logits kept (linear_train and cross_entropy) the same step takes 1.41 ms where this takes 1.48, and 1000 MB beside its results, not 343.
 // It stands where the reference's clients launch the vocabulary projection's product and the softmax and loss rows behind it
 // (reference benchmarking/model_kernels/bert_8_fb1; src/scheduler/utils_sched.cpp:490-501).
 #include <cuda_bf16.h>
