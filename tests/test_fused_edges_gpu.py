@@ -187,3 +187,156 @@ def test_gradients_of_the_loss_have_the_same_bits_from_any_cta_count(ops, one_th
             loss = ops.linear_cross_entropy(*leaves, target)
             return [loss.detach()] + list(torch.autograd.grad(loss, leaves))
         under_quotas(ops, (147, 31, 2, 1), run)
+
+
+FIRST_CALLS = r"""
+import torch
+from orion_b200 import torch_ops, kernels
+ops = torch_ops.load()
+BF = torch.bfloat16
+randn = lambda *s: torch.randn(*s, device="cuda").to(BF)
+x, few, w, t = randn(600, 512), randn(8, 512), randn(20000, 512).requires_grad_(True), torch.randint(0, 20000, (600,), device="cuda")
+rng = torch.tensor([1, 2], device="cuda")
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):      # nothing of the library has run before
+    out = [ops.linear_act(few, w, None, None, "gelu").detach(), ops.linear_act(x, w[:1024], None, None, "relu", 0.1, rng).detach(), ops.dropout(x, 0.2, rng)]
+    loss = ops.linear_cross_entropy(x, w, t)
+    out += [loss.detach()] + list(torch.autograd.grad(loss, w))
+    del loss
+graph.replay()
+torch.cuda.synchronize()
+want = [ops.linear_act(few, w, None, None, "gelu"), ops.linear_act(x, w[:1024], None, None, "relu", 0.1, rng), ops.dropout(x, 0.2, rng)]
+loss = ops.linear_cross_entropy(x, w, t)
+want += [loss] + list(torch.autograd.grad(loss, w))
+assert all(torch.equal(a, b) for a, b in zip(out, want))
+assert kernels.read_status() == 0
+print("SAME")
+"""
+
+
+def test_the_first_call_of_a_process_may_be_captured(built):
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    run = subprocess.run([sys.executable, "-c", FIRST_CALLS], cwd=root, capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0 and "SAME" in run.stdout, run.stderr[-3000:]
+
+
+def test_two_threads_train_at_once(ops):
+    """Each with its own stream and quota: the results of a thread alone."""
+    import threading
+
+    def data(seed):
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        rn = lambda *s: torch.randn(*s, device="cuda", generator=g).to(BF)  # noqa: E731
+        return rn(600, 512), (rn(5003, 512).float() / 16).to(BF), rn(512, 512), torch.randint(0, 5003, (600,), device="cuda", generator=g)
+
+    def step(x, w, u, t, seed):
+        w, u = w.clone().requires_grad_(True), u.clone().requires_grad_(True)
+        h = ops.linear_act(x, u, None, x, "gelu", 0.1, rng_of(seed, 1), 3)
+        loss = ops.linear_cross_entropy(h, w, t)
+        return [loss.detach()] + list(torch.autograd.grad(loss, (w, u)))
+    inputs = [data(s) for s in range(2)]
+    want = [step(*inputs[s], s) for s in range(2)]
+    torch.cuda.synchronize()
+    got, errors = [[], []], []
+
+    def client(s):
+        try:
+            ops.set_sm_quota(40 + 60 * s)
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(15):
+                    got[s].append(step(*inputs[s], s))
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:   # shown in the test's thread
+            errors.append(e)
+    threads = [threading.Thread(target=client, args=(s,)) for s in range(2)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert not errors, errors
+    for s in range(2):
+        for run in got[s]:
+            assert all(torch.equal(a, b) for a, b in zip(run, want[s]))
+
+
+@pytest.mark.parametrize("M,N,K", [(8, 5000, 16384), (8, 5000, 16392), (40, 24, 40000), (1, 1, 8), (4097, 8, 8)])
+def test_long_reductions_and_thin_layers(ops, M, N, K):
+    """The ring's longest reduction, one piece more, a few-row launch of a reduction of any length, and the thinnest layer: bound as in
+    the other tests (accumulation (K + 8) 2^-23 of the magnitudes)."""
+    torch.manual_seed(K)
+    x, w = torch.randn(M, K, device="cuda").to(BF), (torch.randn(N, K, device="cuda") / math.sqrt(K)).to(BF)
+    z, mag = x.double() @ w.double().T, x.double().abs() @ w.double().abs().T
+    within(ops.linear_act(x, w), z, U * z.abs() + (K + 8) * 2.0 ** -23 * mag, "y")
+
+
+def test_the_same_tensor_as_input_and_residual_and_everything_dropped(ops):
+    torch.manual_seed(3)
+    n = 136
+    x, w, b = torch.randn(77, n, device="cuda").to(BF), torch.randn(n, n, device="cuda").to(BF), torch.randn(n, device="cuda").to(BF)
+    dy, rng = torch.randn(77, n, device="cuda").to(BF), rng_of(1, 1)
+    xs = x.clone().requires_grad_(True)
+    y = ops.linear_act(xs, w, b, xs, "relu")
+    a, r = x.clone().requires_grad_(True), x.clone().requires_grad_(True)
+    y2 = ops.linear_act(a, w, b, r, "relu")
+    ga, gr = torch.autograd.grad(y2, (a, r), dy)
+    assert torch.equal(y, y2) and torch.equal(torch.autograd.grad(y, xs, dy)[0], ga + gr)
+    # nothing is kept: the residual alone, and gradients of nothing
+    for act in ("none", "gelu"):
+        leaves = [t.clone().requires_grad_(True) for t in (x, w, b, x)]
+        y = ops.linear_act(*leaves, act, 1.0, rng)
+        assert torch.equal(y.detach(), x)
+        dx, dw, db, dr = torch.autograd.grad(y, leaves, dy)
+        assert not dx.any() and not dw.any() and not db.any() and torch.equal(dr, dy)
+
+
+@pytest.mark.parametrize("M,N,K", [(16, 512, 512), (300, 1000, 2056), (2050, 520, 72), (130, 73, 136)])
+def test_each_gradient_of_the_layer_alone(ops, M, N, K):
+    """The bias's is the same; dx and dw may have their sums cut otherwise: each off by (terms + 8) 2^-23 of their magnitudes, |dz| <= 1.13 |dy|
+    over the kept share, and by its rounding."""
+    torch.manual_seed(M)
+    x, w, b = torch.randn(M, K, device="cuda").to(BF), (torch.randn(N, K, device="cuda") / math.sqrt(K)).to(BF), torch.randn(N, device="cuda")
+    dy, rng = torch.randn(M, N, device="cuda").to(BF), rng_of(M, N)
+
+    def grads(want):
+        leaves = [t.clone().requires_grad_(i in want) for i, t in enumerate((x, w, b))]
+        y = ops.linear_act(*leaves, None, "gelu", 0.1, rng, 4)
+        return dict(zip(want, torch.autograd.grad(y, [leaves[i] for i in want], dy)))
+    together = grads((0, 1, 2))
+    d = 1.13 / 0.89 * dy.double().abs()
+    mags = ((N + 8) * 2.0 ** -23 * (d @ w.double().abs()), (M + 8) * 2.0 ** -23 * (d.T @ x.double().abs()))
+    for want in ((0,), (1,), (2,), (0, 1), (0, 2), (1, 2)):
+        for i, g in grads(want).items():
+            if i == 2:
+                assert torch.equal(g, together[2])
+            else:
+                within(g, together[i].double(), 2 * U * together[i].double().abs() + 2 * (1 + U) * mags[i], "xw"[i])
+
+
+def test_a_captured_loss_of_few_rows_counts_them_anew(ops):
+    """Up to 128 rows stay in place; which of them count is read at each replay."""
+    T, V, H = 100, 3001, 72
+    torch.manual_seed(4)
+    x, w = torch.randn(T, H, device="cuda").to(BF).requires_grad_(True), (torch.randn(V, H, device="cuda") / 8).to(BF).requires_grad_(True)
+    labels, target = torch.randint(0, V, (T,), device="cuda"), torch.zeros(T, device="cuda", dtype=torch.long)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        torch.autograd.grad(ops.linear_cross_entropy(x, w, target), (x, w))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=s):
+        loss = ops.linear_cross_entropy(x, w, target)
+        out = [loss.detach()] + list(torch.autograd.grad(loss, (x, w)))
+        del loss
+    for counted in (100, 1, 0, 37, 100):
+        target.copy_(labels)
+        target[torch.randperm(T, device="cuda")[counted:]] = -100
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        eager = ops.linear_cross_entropy(x, w, target)
+        want = [eager.detach()] + list(torch.autograd.grad(eager, (x, w)))
+        assert all(torch.equal(a, b) for a, b in zip(out, want)), counted
+        del eager
