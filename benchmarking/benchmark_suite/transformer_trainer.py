@@ -59,11 +59,11 @@ def _f32(module, p):
 
 
 def _fit_checkpoint(model, state, prefix, *_):
-    """A checkpoint of a model without dropout has no `rng`, and a model without dropout takes none."""
-    if model.dropout > 0.0:
-        state.setdefault(prefix + "rng", model.rng)
-    else:
+    """A checkpoint of a model built without dropout has no `rng`, and such a model takes none."""
+    if "rng" in model._non_persistent_buffers_set:
         state.pop(prefix + "rng", None)
+    else:
+        state.setdefault(prefix + "rng", model.rng)
 
 
 def _dropout_state(module, cfg):

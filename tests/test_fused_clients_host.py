@@ -67,6 +67,13 @@ def test_a_checkpoint_goes_on_with_its_masks(kind):
     before = other.rng.clone()
     other.load_state_dict(plain.state_dict())
     assert torch.equal(other.rng, before)
+    # dropout switched off or on afterwards changes nothing of that
+    plain.dropout, other.dropout = 0.1, 0.0
+    plain.load_state_dict(state)
+    plain.load_state_dict(plain.state_dict())
+    other.load_state_dict(plain.state_dict())
+    other.load_state_dict(state)
+    assert torch.equal(other.rng, model.rng)
     # a whole model, and one inside a larger module
     assert torch.equal(pickle.loads(pickle.dumps(model)).rng, model.rng)
     outer, again = (torch.nn.Sequential(build(kind, dropout=0.1)) for _ in range(2))
