@@ -289,9 +289,10 @@ int ob200_linear_cross_entropy_forward(const void* x, const void* w, const long 
                                        void* workspace, long long workspace_bytes, int num_ctas, void* stream);
 long long ob200_linear_cross_entropy_workspace(int rows, int V, int H);
 /* Its gradients in pieces of the vocabulary, dx [rows, H] and dw [V, H] contiguous bfloat16 (either may be NULL): logits of a piece are
- * computed again.  The workspace holds a piece's gradients of logits, max(192 MB, 4 KB a row) at most, copies of x and dx in
- * bfloat16, dx in float32 where there are several pieces, and partial matrices of the products.  grad: the upstream gradient, one value or one per row (grad_per_row), divided by *count where count is given (the
- * mean).  Rows that do not count contribute nothing, whatever x holds there. */
+ * computed again.  grad: the upstream gradient, one value or one per row (grad_per_row), divided by *count where count is given (the
+ * mean).  Rows that do not count contribute nothing, whatever x holds there.  The workspace holds a piece's gradients of logits,
+ * max(192 MB, 4 KB a row) at most, copies of x and dx in bfloat16, dx in float32 where there are several pieces, and partial matrices
+ * of the products. */
 int ob200_linear_cross_entropy_backward(const void* x, const void* w, const long long* target, const float* lse, const float* grad,
                                         int grad_per_row, const float* count, void* dx, void* dw, int rows, int V, int H, long long ldx,
                                         long long ldw, long long ignore_index, void* workspace, long long workspace_bytes, int num_ctas,

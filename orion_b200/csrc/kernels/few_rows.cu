@@ -131,10 +131,11 @@ __device__ __forceinline__ void few_way_out(const FewRowsParams& p, const float 
 }
 
 // ------------------------------------------------------------------ few tiles: straight to registers
-// Sixteen warps share a tile's reduction, four k-blocks of 32 (two of them for 32 tokens) under way in each.  There is no ring to fill and no copy to wait for, so
-// a launch of one or two tiles an SM is over sooner: 1024 x 4096 at one token 7.6 -> 5.7 us, at sixteen 8.4 -> 6.1.  More than 32 tokens are groups of 32, each with tiles of
-// its own: w is then read from L2 once a group.
-// CTAs an SM: what the launch bound, the quota's cut and the grid go by.  One of 9 to 16 tokens has the registers of two (110 a thread).
+// Sixteen warps share a tile's reduction, four k-blocks of 32 (two of them for 32 tokens) under way in each.  There is no ring to fill and
+// no copy to wait for, so a launch of one or two tiles an SM is over sooner: 1024 x 4096 at one token 7.6 -> 5.7 us, at sixteen 8.4 -> 6.1.
+// More than 32 tokens are groups of 32, each with tiles of its own: w is then read from L2 once a group.
+// few_resident: CTAs an SM, what the launch bound, the quota's cut and the grid go by.  One of 9 to 16 tokens has the registers of two
+// (110 a thread).
 constexpr int few_resident(int nt) { return nt == 2 ? 1 : 2; }
 template <int NT, bool LSE>
 __global__ void __launch_bounds__(FEW_CONSUMERS * 32, few_resident(NT)) few_tiles_kernel(const __grid_constant__ FewRowsParams p) {
