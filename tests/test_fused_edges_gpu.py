@@ -1,5 +1,6 @@
 """The fused linear layer, counter-based dropout and the loss without logits where values and calls are at their edges: numbers that are not
 numbers, tails, certain answers, derivatives of other kinds, SM quotas.  u = 2^-8 is half a step of bfloat16."""
+import gc
 import math
 
 import pytest
@@ -125,6 +126,7 @@ def test_gelu_of_far_negative_values_is_relatively_exact(ops, M, N):
 
 def test_a_gradient_of_the_residual_alone_keeps_no_slope(ops):
     """Memory of the call: the output alone; with a gradient of any other argument the slope, as large, beside it."""
+    gc.collect()   # nothing of the tests before is freed in between
     torch.manual_seed(2)
     M, N, K = 512, 1024, 64
     x, w, b, r = torch.randn(M, K, device="cuda").to(BF), torch.randn(N, K, device="cuda").to(BF), torch.randn(N, device="cuda").to(BF), torch.randn(M, N, device="cuda").to(BF)
