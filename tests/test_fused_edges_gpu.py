@@ -6,7 +6,7 @@ import math
 import pytest
 import torch
 
-from tests.test_fused_training_gpu import BF, U, act64, rng_of, within
+from tests.test_fused_training_gpu import BF, U, rng_of, within
 
 pytestmark = pytest.mark.gpu
 
